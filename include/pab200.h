@@ -360,6 +360,142 @@ int pab200_kv_append(const pab200_kv_append_args* args, void* stream);
 int pab200_decode_append(const pab200_decode_args* args, const pab200_kv_append_args* app,
                          void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---------------------------------------------------------- 4-bit page caches
+ * No counterpart in the reference, whose caches hold 16-bit rows.
+ *
+ * A 4-bit cache is an array of pages, each one (sequence, kv head)'s block of
+ * block_size tokens: the PAGES layout (a pool [num_blocks, num_kv_heads,
+ * page_bytes] is addressed with bt_page_mul = num_kv_heads, bt_page_add = 1),
+ * with pab200_int4_page_bytes() bytes per page instead of block_size rows.
+ * A row is cut into groups of 64 elements.  A group stores its minimum lo and
+ * a scale s = T((max - lo) / 15) in the rows' 16-bit type T, and for every
+ * element a code c = rint((x - lo) / s) in 0..15 (0 if s is 0), which stands
+ * for lo + s * c.  A group that holds a NaN or an infinity, or whose range
+ * overflows fp32, stands for NaN.  The order of the bytes in a page follows
+ * the decode's matrix fragments (csrc/int4.cuh). */
+
+/* Bytes of one page: block_size * head_size * 9 / 16.  0 for sizes that are
+ * not built (head_size 64, 128, 256; block_size 8, 16, 32, 64). */
+size_t pab200_int4_page_bytes(int32_t head_size, int32_t block_size);
+
+/* Rows that go into or come out of a 4-bit cache.  Addressing as in
+ * pab200_decode_args. */
+typedef struct pab200_int4_rows_args {
+  void* k_cache;             /* 4-bit pages, 16-byte aligned                   */
+  void* v_cache;
+  void* k_rows;              /* [num_tokens, num_kv_heads, head_size], dtype   */
+  void* v_rows;
+  int32_t* seqlens;
+  const int32_t* block_table;
+  const int32_t* cu_tokens;  /* [num_seqs + 1]: tokens cu[s] .. cu[s+1] - 1 are
+                                sequence s's; null: one token per sequence      */
+  uint32_t* status;          /* device word: PAB200_STATUS_* bits ORed in; may be null */
+
+  int32_t dtype;             /* of the rows, and of the scales in the pages    */
+  int32_t num_seqs, num_kv_heads, head_size, block_size, max_blocks;
+  int64_t num_pages, num_tokens;
+  int64_t row_stride_t, row_stride_h;          /* of k_rows / v_rows; head_size stride 1 */
+  int64_t seqlens_stride_b, seqlens_stride_h;  /* h stride 0 => per-seq length */
+  int64_t bt_stride_b, bt_stride_h, bt_stride_i;
+  int32_t bt_page_mul, bt_page_add;
+} pab200_int4_rows_args;
+
+/* Append to a 4-bit cache: token j of sequence s, kv head h, is quantised into
+ * row (L + j) % block_size of page page(s, h, (L + j) / block_size), L =
+ * seqlens(s, h).  With `increment` the lengths then grow by the number of the
+ * sequence's tokens that come before the first without a place (no page slot:
+ * PAB200_STATUS_APPEND_FULL; a page id out of range: PAB200_STATUS_BAD_PAGE_ID;
+ * a negative length: PAB200_STATUS_NEG_SEQLEN, nothing is written), a length
+ * shared by the heads (seqlens_stride_h == 0) by the least of theirs.  Tokens
+ * outside every [cu[s], cu[s+1]) are not read. */
+int pab200_kv_append_int4(const pab200_int4_rows_args* args, int32_t increment, void* stream);
+
+/* Read rows back: k_rows / v_rows token j of sequence s becomes lo + s * c,
+ * rounded to dtype (saturating), of position starts[s * starts_stride] + j (starts null: j);
+ * zeros at positions outside [0, seqlens(s, h)) and on pages out of range.
+ * Rows outside every [cu[s], cu[s+1]) are left as they are.  k_rows and v_rows
+ * 16-byte aligned, strides multiples of 8. */
+int pab200_kv_read_int4(const pab200_int4_rows_args* args, const int32_t* starts,
+                        int64_t starts_stride, void* stream);
+
+/* Decode over 4-bit caches: pab200_decode() with k_cache / v_cache holding
+ * 4-bit pages whose scales have q's type, layout PAGES.  The attention is that
+ * of the values lo + s * c, which are not rounded to dtype.  The call reads
+ * nothing before everything earlier on `stream` has finished. */
+size_t pab200_decode_int4_workspace_size(const pab200_decode_args* args);
+int pab200_decode_int4(const pab200_decode_args* args, void* workspace, size_t workspace_bytes,
+                       void* stream);
+
+/* ------------------------------------------------------- page-sparse decode
+ * No counterpart in the reference, which attends to every page.
+ *
+ * page_bounds is [num_pages][2][head_size]: the elementwise minimum and maximum
+ * of the keys of one (page, kv head).  num_pages and the page ids count
+ * (page, kv head) pairs: pages of the PAGES layout, or block * num_kv_heads + h
+ * of a pool of either layout (bounds_page_mul = num_kv_heads, bounds_page_add =
+ * 1). */
+typedef struct pab200_page_bounds_args {
+  void* page_bounds;         /* [num_pages, 2, head_size], dtype, 16-byte aligned */
+  const void* k_rows;        /* new keys [num_tokens, num_kv_heads, head_size] */
+  const int32_t* seqlens;    /* lengths BEFORE the new tokens; not changed     */
+  const int32_t* block_table;
+  const int32_t* cu_tokens;  /* as in pab200_int4_rows_args                    */
+  uint32_t* status;
+
+  int32_t dtype, num_seqs, num_kv_heads, head_size, block_size, max_blocks;
+  int64_t num_pages, num_tokens;
+  int64_t row_stride_t, row_stride_h;
+  int64_t seqlens_stride_b, seqlens_stride_h;
+  int64_t bt_stride_b, bt_stride_h, bt_stride_i;
+  int32_t bounds_page_mul, bounds_page_add;
+} pab200_page_bounds_args;
+
+/* Bounds of the pages that new tokens go to: a page whose first row is new
+ * starts afresh, any other page's bounds are widened.  NaNs stay NaN.  Tokens
+ * without a place are left out (status bits as in pab200_kv_append_int4). */
+int pab200_update_page_bounds(const pab200_page_bounds_args* args, void* stream);
+
+/* Selection of the pages of every (sequence, kv head) that a query attends to. */
+typedef struct pab200_select_args {
+  const void* q;             /* [num_seqs, num_q_heads, head_size], dtype      */
+  const void* page_bounds;
+  const int32_t* seqlens;
+  const int32_t* block_table;
+  int32_t* tables;           /* out [num_seqs, num_kv_heads, num_selected]     */
+  int32_t* selected_lens;    /* out [num_seqs, num_kv_heads]                   */
+  uint32_t* status;
+
+  int32_t dtype, num_seqs, num_q_heads, num_kv_heads, head_size, block_size, max_blocks;
+  int32_t num_selected, num_sink, num_recent;
+  int64_t num_pages;
+  int64_t q_stride_b, q_stride_h;
+  int64_t seqlens_stride_b, seqlens_stride_h;
+  int64_t bt_stride_b, bt_stride_h, bt_stride_i;
+  int32_t bounds_page_mul, bounds_page_add;
+} pab200_select_args;
+
+/* For n = ceil(L / block_size) pages: all of them if n <= num_selected; else
+ * the first num_sink, the last num_recent (>= 1), and of the others those with
+ * the highest score
+ *   u(page) = sum_g sum_d max(q[g, d] * min[d], q[g, d] * max[d]),
+ * g over the kv head's query group: no token of the page has a larger sum of
+ * raw scores.  Scores are summed in 64 bits and rounded to fp32; equal scores
+ * go to the lower page, a score that is NaN ranks first, a page id out of range
+ * last.  tables[s, h] receives the block-table entries of the kept pages in
+ * ascending page order (-1 behind them) and selected_lens[s, h] the number of
+ * their tokens: a block table and lengths for any decode entry point. */
+size_t pab200_select_pages_workspace_size(const pab200_select_args* args);
+int pab200_select_pages(const pab200_select_args* args, void* workspace, size_t workspace_bytes,
+                        void* stream);
+
+/* pab200_select_pages() and the decode over its tables in one call.  `args`
+ * is a decode call (q and sizes as in `sel`); its seqlens, block_table,
+ * max_blocks and their strides are replaced by the selection's. */
+size_t pab200_decode_sparse_workspace_size(const pab200_decode_args* args,
+                                           const pab200_select_args* sel);
+int pab200_decode_sparse(const pab200_decode_args* args, const pab200_select_args* sel,
+                         void* workspace, size_t workspace_bytes, void* stream);
+
 /* Copy the device status word of `workspace` (the PAB200_STATUS_* bits raised
  * by the most recent pab200_decode call on it) to *status_out.  Synchronises
  * `stream`. */

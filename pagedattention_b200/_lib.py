@@ -59,6 +59,16 @@ EXPORTED_SYMBOLS = (
     "pab200_exchange_buffer_destroy",
     "pab200_exchange_merge",
     "pab200_decode_exchange",
+    "pab200_int4_page_bytes",
+    "pab200_kv_append_int4",
+    "pab200_kv_read_int4",
+    "pab200_decode_int4_workspace_size",
+    "pab200_decode_int4",
+    "pab200_update_page_bounds",
+    "pab200_select_pages_workspace_size",
+    "pab200_select_pages",
+    "pab200_decode_sparse_workspace_size",
+    "pab200_decode_sparse",
     "pab200_read_status",
     "pab200_strerror",
     "pab200_last_error",
@@ -137,6 +147,44 @@ class DecodeArgs(ctypes.Structure):
     ]
 
 
+def _fields(*groups):
+    return [(name, t) for t, names in groups for name in names.split()]
+
+
+class Int4RowsArgs(ctypes.Structure):
+    """Mirror of ``pab200_int4_rows_args`` (field order and types must match)."""
+
+    _fields_ = _fields(
+        (ctypes.c_void_p, "k_cache v_cache k_rows v_rows seqlens block_table cu_tokens status"),
+        (ctypes.c_int32, "dtype num_seqs num_kv_heads head_size block_size max_blocks"),
+        (ctypes.c_int64, "num_pages num_tokens row_stride_t row_stride_h seqlens_stride_b "
+                         "seqlens_stride_h bt_stride_b bt_stride_h bt_stride_i"),
+        (ctypes.c_int32, "bt_page_mul bt_page_add"))
+
+
+class PageBoundsArgs(ctypes.Structure):
+    """Mirror of ``pab200_page_bounds_args`` (field order and types must match)."""
+
+    _fields_ = _fields(
+        (ctypes.c_void_p, "page_bounds k_rows seqlens block_table cu_tokens status"),
+        (ctypes.c_int32, "dtype num_seqs num_kv_heads head_size block_size max_blocks"),
+        (ctypes.c_int64, "num_pages num_tokens row_stride_t row_stride_h seqlens_stride_b "
+                         "seqlens_stride_h bt_stride_b bt_stride_h bt_stride_i"),
+        (ctypes.c_int32, "bounds_page_mul bounds_page_add"))
+
+
+class SelectArgs(ctypes.Structure):
+    """Mirror of ``pab200_select_args`` (field order and types must match)."""
+
+    _fields_ = _fields(
+        (ctypes.c_void_p, "q page_bounds seqlens block_table tables selected_lens status"),
+        (ctypes.c_int32, "dtype num_seqs num_q_heads num_kv_heads head_size block_size max_blocks "
+                         "num_selected num_sink num_recent"),
+        (ctypes.c_int64, "num_pages q_stride_b q_stride_h seqlens_stride_b seqlens_stride_h "
+                         "bt_stride_b bt_stride_h bt_stride_i"),
+        (ctypes.c_int32, "bounds_page_mul bounds_page_add"))
+
+
 class LibraryNotBuilt(RuntimeError):
     pass
 
@@ -204,6 +252,20 @@ def load() -> ctypes.CDLL:
         ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32, ctypes.c_int64, ctypes.c_void_p,
         ctypes.c_void_p]
     lib.pab200_decode_exchange.restype = ctypes.c_int
+    V, Z, I32, I64 = ctypes.c_void_p, ctypes.c_size_t, ctypes.c_int32, ctypes.c_int64
+    R, S = ctypes.POINTER(Int4RowsArgs), ctypes.POINTER(SelectArgs)
+    for name, res, args in (
+            ("pab200_int4_page_bytes", Z, [I32, I32]),
+            ("pab200_kv_append_int4", ctypes.c_int, [R, I32, V]),
+            ("pab200_kv_read_int4", ctypes.c_int, [R, V, I64, V]),
+            ("pab200_decode_int4_workspace_size", Z, [P]),
+            ("pab200_decode_int4", ctypes.c_int, [P, V, Z, V]),
+            ("pab200_update_page_bounds", ctypes.c_int, [ctypes.POINTER(PageBoundsArgs), V]),
+            ("pab200_select_pages_workspace_size", Z, [S]),
+            ("pab200_select_pages", ctypes.c_int, [S, V, Z, V]),
+            ("pab200_decode_sparse_workspace_size", Z, [P, S]),
+            ("pab200_decode_sparse", ctypes.c_int, [P, S, V, Z, V])):
+        getattr(lib, name).restype, getattr(lib, name).argtypes = res, args
     lib.pab200_read_status.argtypes = [ctypes.c_void_p, ctypes.POINTER(ctypes.c_uint32),
                                        ctypes.c_void_p]
     lib.pab200_read_status.restype = ctypes.c_int

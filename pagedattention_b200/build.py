@@ -12,14 +12,17 @@ import os
 import shutil
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PKG_DIR = Path(__file__).resolve().parent
 REPO_DIR = PKG_DIR.parent
 CSRC = PKG_DIR / "csrc"
 LIB_PATH = PKG_DIR / "libpab200.so"
-SOURCES = [CSRC / "pab200.cu"]
-HEADERS = [CSRC / "decode.cuh", CSRC / "ptx.cuh", REPO_DIR / "include" / "pab200.h"]
+OBJ_DIR = PKG_DIR / "build"
+SOURCES = [CSRC / "pab200.cu", CSRC / "int4_decode.cu", CSRC / "int4.cu", CSRC / "sparse.cu"]
+HEADERS = [CSRC / "decode.cuh", CSRC / "int4.cuh", CSRC / "ptx.cuh", CSRC / "tokens.cuh",
+           CSRC / "host.h", REPO_DIR / "include" / "pab200.h"]
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
@@ -31,16 +34,19 @@ def nvcc_path() -> str:
     return cand
 
 
-def nvcc_command(out: Path, verbose_ptxas: bool = False) -> list[str]:
+def compile_command(src: Path, obj: Path, verbose_ptxas: bool = False) -> list[str]:
     cmd = [
         nvcc_path(), *ARCH_FLAGS, "-O3", "-lineinfo", "-std=c++17",
-        "-shared", "-Xcompiler", "-fPIC,-fvisibility=hidden",
-        "-I", str(REPO_DIR / "include"), "-I", str(CSRC),
-        "-o", str(out), *map(str, SOURCES),
+        "-Xcompiler", "-fPIC,-fvisibility=hidden",
+        "-I", str(REPO_DIR / "include"), "-I", str(CSRC), "-c", str(src), "-o", str(obj),
     ]
     if verbose_ptxas:
         cmd += ["-Xptxas", "-v"]
     return cmd
+
+
+def link_command(objs: list[Path], out: Path) -> list[str]:
+    return [nvcc_path(), *ARCH_FLAGS, "-shared", "-o", str(out), *map(str, objs)]
 
 
 def is_stale() -> bool:
@@ -54,13 +60,29 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     """Compile the library if it is missing or older than its sources."""
     if not force and not is_stale():
         return LIB_PATH
+    OBJ_DIR.mkdir(exist_ok=True)
+    objs = [OBJ_DIR / (src.stem + ".o") for src in SOURCES]
+    headers = max(p.stat().st_mtime for p in HEADERS)
+
+    def run(cmd):
+        res = subprocess.run(cmd, capture_output=True, text=True)
+        if verbose or res.returncode != 0:
+            sys.stderr.write(res.stdout + res.stderr)
+        if res.returncode != 0:
+            raise RuntimeError(f"nvcc failed ({res.returncode}): {' '.join(cmd)}")
+
+    def compile_one(pair):
+        src, obj = pair
+        if (force or not obj.exists()
+                or obj.stat().st_mtime < max(headers, src.stat().st_mtime)):
+            part = obj.with_suffix(".o.tmp")
+            run(compile_command(src, part, verbose_ptxas=verbose))
+            os.replace(part, obj)
+
+    with ThreadPoolExecutor(len(SOURCES)) as pool:
+        list(pool.map(compile_one, zip(SOURCES, objs)))
     tmp = LIB_PATH.with_suffix(".so.tmp")
-    cmd = nvcc_command(tmp, verbose_ptxas=verbose)
-    res = subprocess.run(cmd, capture_output=True, text=True)
-    if verbose or res.returncode != 0:
-        sys.stderr.write(res.stdout + res.stderr)
-    if res.returncode != 0:
-        raise RuntimeError(f"nvcc failed ({res.returncode}): {' '.join(cmd)}")
+    run(link_command(objs, tmp))
     os.replace(tmp, LIB_PATH)
     return LIB_PATH
 

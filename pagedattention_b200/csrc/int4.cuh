@@ -1,0 +1,127 @@
+// The 4-bit page format and the register arithmetic on its codes.
+//
+// A row (one token of one kv head) is cut into groups of 64 elements; a group
+// holds its minimum `lo` and a scale s = T((hi - lo) / 15), both of the rows'
+// 16-bit type T, and a code c = rint((x - lo) / s) in 0..15 per element, which
+// stands for lo + s c.  A page of block_size rows is
+//
+//   codes   block_size x D/2 bytes
+//   pairs   block_size x D/64 (s, lo)
+//
+// that is block_size * D * 9/16 bytes, contiguous, a multiple of 16.
+//
+// Codes are stored as 32-bit words of 8 consecutive elements, element i in
+// nibble i / 2 + 4 (i % 2): the low nibbles of the word's two 16-bit halves are
+// elements 0 and 1, so that a mask and an OR give two neighbouring elements in
+// one 16-bit pair.  Where a word goes follows the fragments of the decode's
+// matrix instructions, so that every lane reads its codes of 8 tokens with one
+// contiguous, conflict-free load and no transpose:
+//   keys    row-major rows of D/2 bytes; within a row, chunk c of 4 holds the
+//           words of elements 16 c .. 16 c + 15 of every group (D/64 x 2 words)
+//   values  tiles of 8 tokens, 4 D bytes each: [octet o of 8][token pair of 4]
+//           [token parity of 2][group] words of elements 8 o .. 8 o + 7
+#pragma once
+
+#include <cstdint>
+
+#include "ptx.cuh"
+
+namespace pab {
+
+constexpr int kInt4Group = 64;
+
+// Bytes of one row: its codes and its (scale, minimum) pairs.
+__host__ __device__ constexpr int int4_row_bytes(int D) { return D / 2 + D / kInt4Group * 4; }
+
+// Byte offset in a page of the code word of elements 64 g + 8 o .. + 7 (group
+// g, octet o) of row r.
+__host__ __device__ __forceinline__ int int4_key_word(int D, int r, int g, int o) {
+  return r * (D / 2) + (o >> 1) * (D / 8) + g * 8 + (o & 1) * 4;
+}
+__host__ __device__ __forceinline__ int int4_value_word(int D, int r, int g, int o) {
+  return (r >> 3) * (4 * D) + (((o * 4 + ((r & 7) >> 1)) * 2 + (r & 1)) * (D / kInt4Group) + g) * 4;
+}
+// Byte offset in a page of `bs` rows of group g's (scale, minimum) of row r.
+__host__ __device__ __forceinline__ int int4_pair(int D, int bs, int r, int g) {
+  return bs * (D / 2) + (r * (D / kInt4Group) + g) * 4;
+}
+
+// Two 16-bit values of one register.
+template <typename T>
+__device__ __forceinline__ float2 unpack2(uint32_t x);
+template <>
+__device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t x) {
+  return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u));
+}
+template <>
+__device__ __forceinline__ float2 unpack2<__half>(uint32_t x) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&x));
+}
+
+// N consecutive 32-bit words of shared memory (aligned to min(N, 4) words).
+template <int N>
+__device__ __forceinline__ void ld_shared_words(uint32_t addr, uint32_t (&w)[N]) {
+  if constexpr (N == 1) {
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[0]) : "r"(addr));
+  } else if constexpr (N == 2) {
+    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(addr));
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i += 4)
+      asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+                   : "=r"(w[i]), "=r"(w[i + 1]), "=r"(w[i + 2]), "=r"(w[i + 3])
+                   : "r"(addr + i * 4));
+  }
+}
+
+// (x & mask) | bits, one instruction.
+__device__ __forceinline__ uint32_t and_or(uint32_t x, uint32_t mask, uint32_t bits) {
+  uint32_t y;
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(y) : "r"(x), "r"(mask), "r"(bits));
+  return y;
+}
+
+// Nibble m of both 16-bit halves of w, as the pair r[m] of exact values c - 8
+// (-8..7) of type T.  A nibble OR-ed into the low mantissa bits of a power of
+// two P reads as P + c; subtracting P + 8 is exact.  fp16 (10 mantissa bits)
+// also takes the nibble at bits 4..7 in place: 1024 + 16 c, times 1/16 minus
+// 72.  Centred codes keep the products small: a value is (lo + 8 s) + s (c - 8),
+// and the rounding of a probability to T is multiplied by |s (c - 8)|, about
+// |x|, instead of by s c, about the group's range.
+template <typename T>
+__device__ __forceinline__ void int4_widen(uint32_t w, uint32_t (&r)[4]);
+
+template <>
+__device__ __forceinline__ void int4_widen<__half>(uint32_t w, uint32_t (&r)[4]) {
+  const uint32_t v = w >> 8;
+  const __half2 base = __float2half2_rn(1032.f);
+  const __half2 sixteenth = __float2half2_rn(0.0625f), off = __float2half2_rn(-72.f);
+  const uint32_t t[4] = {and_or(w, 0x000f000fu, 0x64006400u), and_or(w, 0x00f000f0u, 0x64006400u),
+                         and_or(v, 0x000f000fu, 0x64006400u), and_or(v, 0x00f000f0u, 0x64006400u)};
+#pragma unroll
+  for (int m = 0; m < 4; ++m) {
+    const __half2 x = *reinterpret_cast<const __half2*>(&t[m]);
+    const __half2 y = m & 1 ? __hfma2(x, sixteenth, off) : __hsub2(x, base);
+    r[m] = *reinterpret_cast<const uint32_t*>(&y);
+  }
+}
+
+template <>
+__device__ __forceinline__ void int4_widen<__nv_bfloat16>(uint32_t w, uint32_t (&r)[4]) {
+  const __nv_bfloat162 base = __floats2bfloat162_rn(136.f, 136.f);
+#pragma unroll
+  for (int m = 0; m < 4; ++m) {
+    const uint32_t t = and_or(w >> (4 * m), 0x000f000fu, 0x43004300u);
+    const __nv_bfloat162 y = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&t), base);
+    r[m] = *reinterpret_cast<const uint32_t*>(&y);
+  }
+}
+
+// (scale, value of code 8) of a (scale, minimum) pair.
+template <typename T>
+__device__ __forceinline__ float2 int4_centre(uint32_t pair) {
+  const float2 f = unpack2<T>(pair);
+  return make_float2(f.x, fmaf(8.f, f.x, f.y));
+}
+
+}  // namespace pab

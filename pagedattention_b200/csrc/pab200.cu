@@ -17,18 +17,15 @@
 #include <cstring>
 #include <mutex>
 
-#include "decode.cuh"
-#include "pab200.h"
-
-#define PAB200_EXPORT extern "C" __attribute__((visibility("default")))
+#include "host.h"
 
 extern char** environ;  // the process environment (POSIX)
 
 namespace {
-
 thread_local char g_last_error[512] = "";
+}  // namespace
 
-int fail(int code, const char* fmt, ...) {
+int pabh::fail(int code, const char* fmt, ...) {
   va_list ap;
   va_start(ap, fmt);
   vsnprintf(g_last_error, sizeof(g_last_error), fmt, ap);
@@ -36,9 +33,19 @@ int fail(int code, const char* fmt, ...) {
   return code;
 }
 
-int cuda_fail(cudaError_t e, const char* what) {
+int pabh::cuda_fail(cudaError_t e, const char* what) {
   return fail(PAB200_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
 }
+
+using pabh::align256;
+using pabh::aligned;
+using pabh::cuda_fail;
+using pabh::device_sm_count_current;
+using pabh::fail;
+using pabh::KernelOps;
+using pabh::LaunchCfg;
+
+namespace {
 
 PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
   static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
@@ -69,12 +76,16 @@ int device_sm_count(int dev) {
   return sms[dev];
 }
 
-int device_sm_count_current() {
+}  // namespace
+
+int pabh::device_sm_count_current() {
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return 148;
   const int n = device_sm_count(dev);
   return n > 0 ? n : 148;
 }
+
+namespace {
 
 // Tuning variables (PAB200_*), read from the environment: one pass over
 // the environment per planned call collects the (usually zero) PAB200_
@@ -103,42 +114,9 @@ int env_int(const char* name, int fallback) {
 }
 
 // ------------------------------------------------------------------ kernels
-struct KernelOps {
-  void* fn;  // decode kernel (for attributes / occupancy)
-  cudaError_t (*launch)(dim3, dim3, size_t, cudaStream_t, bool, const CUtensorMap&,
-                        const CUtensorMap&, const pab::DecodeParams&);
-};
-
-// Launch configuration; `pdl` lets the grid start while the previous kernel
-// in the stream finishes (programmatic dependent launch): the kernel waits
-// with griddepcontrol.wait before it reads that kernel's output.
-struct LaunchCfg {
-  cudaLaunchConfig_t cfg{};
-  cudaLaunchAttribute attr[1];
-  LaunchCfg(dim3 grid, dim3 block, size_t smem, cudaStream_t s, bool pdl) {
-    cfg.gridDim = grid;
-    cfg.blockDim = block;
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = s;
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = pdl ? 1 : 0;
-  }
-};
-
-template <typename T, int D, int NT, int ST, bool CORE, bool PAIR, bool TC>
-cudaError_t launch_decode(dim3 grid, dim3 block, size_t smem, cudaStream_t s, bool pdl,
-                          const CUtensorMap& k, const CUtensorMap& v,
-                          const pab::DecodeParams& p) {
-  LaunchCfg lc(grid, block, smem, s, pdl);
-  return cudaLaunchKernelEx(&lc.cfg, pab::decode_kernel<T, D, NT, ST, CORE, PAIR, TC>, k, v, p);
-}
-
 template <typename T, int D, int NT, int ST, bool CORE = false, bool PAIR = false, bool TC = false>
 KernelOps ops_of() {
-  return KernelOps{reinterpret_cast<void*>(&pab::decode_kernel<T, D, NT, ST, CORE, PAIR, TC>),
-                   &launch_decode<T, D, NT, ST, CORE, PAIR, TC>};
+  return pabh::kernel_ops<&pab::decode_kernel<T, D, NT, ST, CORE, PAIR, TC>>();
 }
 
 template <typename T, int ST>
@@ -197,7 +175,7 @@ bool select_kernel(int dtype, int D, int nt, int st, bool core, bool pair, bool 
 struct Plan {
   KernelOps ops;
   int G, nt, st, wpc, depth, ctas_per_sm, grid, W;
-  bool core, pair, tc;
+  bool core, pair, tc, int4;
   size_t smem;
   int n_heads;
   int slot_floats;
@@ -205,19 +183,16 @@ struct Plan {
   size_t off_cum, off_wstart, off_claims, off_hseg, off_empty, off_part, ws_bytes;
 };
 
-size_t align256(size_t x) { return (x + 255) & ~size_t(255); }
-
-bool aligned(const void* p, size_t a) {
-  return (reinterpret_cast<uintptr_t>(p) % a) == 0;
-}
-
 // Checks shapes, sizes and (with check_pointers) pointers and alignment.
-int validate(const pab200_decode_args* a, bool check_pointers) {
+// `int4`: the caches hold 4-bit pages.
+int validate(const pab200_decode_args* a, bool check_pointers, bool int4) {
   if (!a) return fail(PAB200_ERR_INVALID_ARGUMENT, "args is null");
   if (a->dtype != PAB200_DTYPE_BF16 && a->dtype != PAB200_DTYPE_F16)
     return fail(PAB200_ERR_UNSUPPORTED, "dtype %d: q/k/v must be bf16 or f16", a->dtype);
   if (a->layout != PAB200_LAYOUT_PAGES && a->layout != PAB200_LAYOUT_NHD)
     return fail(PAB200_ERR_INVALID_ARGUMENT, "unknown cache layout %d", a->layout);
+  if (int4 && a->layout != PAB200_LAYOUT_PAGES)
+    return fail(PAB200_ERR_UNSUPPORTED, "4-bit caches have the PAGES layout");
   if (a->num_seqs < 1 || a->num_kv_heads < 1 || a->num_q_heads < 1)
     return fail(PAB200_ERR_INVALID_ARGUMENT, "num_seqs, num_q_heads, num_kv_heads must be >= 1");
   if (a->num_q_heads % a->num_kv_heads != 0)
@@ -355,9 +330,9 @@ int choose_geometry(const KernelOps& ops, int dev, int depth, size_t stage, bool
 // tail-chunk count per warp (m_max) is lowered until the workspace fits it
 // (SIZE_MAX for a caller workspace, which is sized to the plan instead).
 int make_plan(const pab200_decode_args* a, Plan* pl, size_t scratch_cap,
-              bool check_pointers = true) {
+              bool check_pointers = true, bool int4 = false) {
   refresh_env();
-  int rc = validate(a, check_pointers);
+  int rc = validate(a, check_pointers, int4);
   if (rc) return rc;
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -366,6 +341,7 @@ int make_plan(const pab200_decode_args* a, Plan* pl, size_t scratch_cap,
   if (sms <= 0) return fail(PAB200_ERR_CUDA, "cannot query the SM count of device %d", dev);
 
   const int D = a->head_size, bs = a->block_size;
+  pl->int4 = int4;
   pl->G = a->num_q_heads / a->num_kv_heads;
   pl->nt = pl->G <= 8 ? 1 : (pl->G <= 16 ? 2 : 4);
   // Groups of 17-32 query heads that one warp cannot hold (D = 128): two
@@ -377,7 +353,8 @@ int make_plan(const pab200_decode_args* a, Plan* pl, size_t scratch_cap,
   // tcgen05 path (PAB200_TC=1): groups of 9-32 query heads at D = 64, on
   // the 5th-generation tensor cores with TMEM accumulators; two warps per
   // ring, 64-token stages.
-  pl->tc = pl->G > 8 && pl->G <= 32 && D == 64 && bs <= 64 && env_int("PAB200_TC", 0) != 0;
+  pl->tc = !int4 && pl->G > 8 && pl->G <= 32 && D == 64 && bs <= 64 &&
+           env_int("PAB200_TC", 0) != 0;
   if (pl->tc) pl->pair = true;
   if (pl->pair) pl->nt = 2;
   // Tokens per ring stage: a power of two >= block_size.
@@ -385,21 +362,23 @@ int make_plan(const pab200_decode_args* a, Plan* pl, size_t scratch_cap,
   if ((pl->st != 16 && pl->st != 32 && pl->st != 64) || pl->st < bs)
     return fail(PAB200_ERR_INVALID_ARGUMENT, "PAB200_ST must be 16, 32 or 64 and >= block_size");
   const int nh = D / 64;
-  if (2 * (pl->st / bs) * nh > 32)
+  if (!int4 && 2 * (pl->st / bs) * nh > 32)
     return fail(PAB200_ERR_UNSUPPORTED, "block_size %d with head_size %d needs > 32 copies per stage", bs, D);
   // Arithmetic: tensor-core MMA by default; the CUDA-core variant
   // (PAB200_CORE=1) exists for query groups of at most 4 heads, 32-token
   // stages and D <= 128.
-  pl->core = env_int("PAB200_CORE", 0) != 0 && pl->G <= pab::kCoreMaxG && pl->st == 32 && D <= 128;
+  pl->core = !int4 && env_int("PAB200_CORE", 0) != 0 && pl->G <= pab::kCoreMaxG && pl->st == 32 && D <= 128;
   if (pl->tc) pl->core = false;
-  if (!select_kernel(a->dtype, D, pl->nt, pl->st, pl->core, pl->pair, pl->tc, &pl->ops))
+  if (int4 ? !pabh::select_int4_kernel(a->dtype, D, pl->nt, pl->st, pl->pair, &pl->ops)
+           : !select_kernel(a->dtype, D, pl->nt, pl->st, pl->core, pl->pair, pl->tc, &pl->ops))
     return fail(PAB200_ERR_UNSUPPORTED, "no kernel for head_size %d, group %d", D, pl->G);
 
   // Each warp owns a private ring of `depth` stages.  Throughput grows with
   // resident warps (each warp's stage loop is latency-bound), so the default
   // is a 2-deep ring and as many warps as ~200 KB of shared memory per SM
   // holds (6 warps at 16 KiB stages).
-  const size_t stage = size_t(4) * pl->st * D;  // K + V bytes of one stage
+  const size_t stage =  // K + V bytes of one stage
+      int4 ? size_t(2) * pl->st * pab::int4_row_bytes(D) : size_t(4) * pl->st * D;
   // The tcgen05 path computes the scores of the next stage while the warps
   // work on the current one, so it needs a third stage in flight.
   int depth = env_int("PAB200_DEPTH", pl->tc ? 3 : 2);
@@ -612,9 +591,14 @@ cudaError_t launch_exchange(const pab::ExchangeParams& p, int out_dtype, int fus
 // One decode call planned as `pl`; with `app`, the planner first appends the
 // step's tokens; with `exchange`, the call ends in the fused exchange + merge
 // of a context split across GPUs instead of the reduce kernel.
+// `after_inputs`: the planner is launched without programmatic dependence, so
+// that everything before it on the stream, the writer of this call's tables
+// and lengths among it, has finished before the planner or the decode grid
+// reads anything.
 int decode_impl(const pab200_decode_args* a, const Plan& pl, const pab::AppendParams* app,
                 void* workspace, size_t workspace_bytes, void* stream,
-                pab::ExchangeParams* exchange = nullptr, int exchange_dtype = 0) {
+                pab::ExchangeParams* exchange = nullptr, int exchange_dtype = 0,
+                bool after_inputs = false) {
   int rc = PAB200_OK;
   if (!workspace || workspace_bytes < pl.ws_bytes)
     return fail(PAB200_ERR_WORKSPACE, "workspace of %zu bytes needed, %zu given", pl.ws_bytes,
@@ -679,20 +663,23 @@ int decode_impl(const pab200_decode_args* a, const Plan& pl, const pab::AppendPa
     p.app.status = p.status;  // append bits land in the call's status word
   }
 
+  p.k_pages = static_cast<const uint8_t*>(a->k_cache);
+  p.v_pages = static_cast<const uint8_t*>(a->v_cache);
   CUtensorMap kmap, vmap;
-  if (a->num_pages > 0) {
+  if (a->num_pages > 0 && !pl.int4) {
     if ((rc = encode_cache_map(a, a->k_cache, &kmap))) return rc;
     if ((rc = encode_cache_map(a, a->v_cache, &vmap))) return rc;
   } else {
-    // No pages: every sequence is empty, the planner writes all outputs and
-    // the decode kernel exits before touching the maps.
+    // 4-bit pages are copied without maps.  No pages: every sequence is
+    // empty, and the decode kernel exits before touching the maps.
     kmap = CUtensorMap{};
     vmap = CUtensorMap{};
   }
 
   const bool pdl = env_int("PAB200_PDL", 1) != 0;
-  cudaError_t e = a->dtype == PAB200_DTYPE_BF16 ? launch_plan<__nv_bfloat16>(p, s, pdl)
-                                                 : launch_plan<__half>(p, s, pdl);
+  const bool pdl_plan = pdl && !after_inputs;
+  cudaError_t e = a->dtype == PAB200_DTYPE_BF16 ? launch_plan<__nv_bfloat16>(p, s, pdl_plan)
+                                                 : launch_plan<__half>(p, s, pdl_plan);
   if (e != cudaSuccess) return cuda_fail(e, "plan kernel launch");
   if (a->event_before) {
     e = cudaEventRecord(static_cast<cudaEvent_t>(a->event_before), s);
@@ -732,6 +719,29 @@ PAB200_EXPORT int pab200_decode(const pab200_decode_args* a, void* workspace,
   const int rc = make_plan(a, &pl, SIZE_MAX);
   if (rc) return rc;
   return decode_impl(a, pl, nullptr, workspace, workspace_bytes, stream);
+}
+
+int pabh::decode_after(const pab200_decode_args* a, void* workspace, size_t workspace_bytes,
+                       void* stream) {
+  Plan pl;
+  const int rc = make_plan(a, &pl, SIZE_MAX);
+  if (rc) return rc;
+  return decode_impl(a, pl, nullptr, workspace, workspace_bytes, stream, nullptr, 0, true);
+}
+
+// ------------------------------------------------------------- 4-bit pages
+PAB200_EXPORT size_t pab200_decode_int4_workspace_size(const pab200_decode_args* args) {
+  Plan pl;
+  if (make_plan(args, &pl, SIZE_MAX, true, true) != PAB200_OK) return 0;
+  return pl.ws_bytes;
+}
+
+PAB200_EXPORT int pab200_decode_int4(const pab200_decode_args* a, void* workspace,
+                                     size_t workspace_bytes, void* stream) {
+  Plan pl;
+  const int rc = make_plan(a, &pl, SIZE_MAX, true, true);
+  if (rc) return rc;
+  return decode_impl(a, pl, nullptr, workspace, workspace_bytes, stream, nullptr, 0, true);
 }
 
 // ---------------------------------------------------------------- no-alloc

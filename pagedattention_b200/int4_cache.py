@@ -1,0 +1,256 @@
+"""4-bit page caches: append, read-back and decode attention.
+
+The reference's caches hold 16-bit rows (src/common.py:1-14) and it has no
+counterpart.  A 4-bit cache is a uint8 tensor of pages, one per (sequence, kv
+head)'s block of ``block_size`` tokens, ``int4_page_bytes(head_size,
+block_size)`` bytes each: a pool (num_blocks, num_kv_heads, page_bytes) with
+block tables (num_seqs, max_blocks), or pages (num_pages, page_bytes) with
+per-head block tables (num_seqs, num_kv_heads, max_blocks).  ``int4_cache``
+allocates a pool.
+
+Rows are quantised in groups of 64 elements: minimum lo and scale s = T((max -
+lo) / 15) in the rows' 16-bit type T, codes rint((x - lo) / s) in 0..15.  A
+group stands for lo + s * code; a group with a NaN or an infinity for NaN.  A
+page takes 9/32 of the bytes of its 16-bit rows.
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import _lib
+from .kernel_b200 import (_DTYPES, _append_status_word, _as_int32, _check_device,
+                          _current_stream_handle, _fill_common, _keep_workspace, _raise_for)
+
+_HEAD_SIZES = (64, 128, 256)
+_BLOCK_SIZES = (8, 16, 32, 64)
+
+
+def int4_page_bytes(head_size: int, block_size: int) -> int:
+    """Bytes of one page of a 4-bit cache (block_size * head_size * 9 / 16)."""
+    if head_size not in _HEAD_SIZES or block_size not in _BLOCK_SIZES:
+        raise ValueError(f"head_size must be one of {_HEAD_SIZES} and block_size one of "
+                         f"{_BLOCK_SIZES}, got {head_size} and {block_size}")
+    return block_size * head_size * 9 // 16
+
+
+def int4_cache(num_blocks, num_kv_heads, block_size, head_size, device="cuda"):
+    """Two zeroed 4-bit pools (num_blocks, num_kv_heads, page_bytes): keys and
+    values."""
+    shape = (num_blocks, num_kv_heads, int4_page_bytes(head_size, block_size))
+    return tuple(torch.zeros(shape, dtype=torch.uint8, device=device) for _ in range(2))
+
+
+def _check_caches(key_cache, value_cache, block_table, head_size, block_size, num_seqs,
+                  num_kv_heads):
+    """Checks of the caches and their table; returns (table, page count, kv
+    heads, bt_page_mul, bt_page_add, max_blocks, table strides)."""
+    if key_cache.dtype != torch.uint8 or value_cache.dtype != torch.uint8:
+        raise TypeError("4-bit caches must be uint8 tensors")
+    if tuple(key_cache.shape) != tuple(value_cache.shape):
+        raise ValueError("key_cache and value_cache shapes differ")
+    if not (key_cache.is_contiguous() and value_cache.is_contiguous()):
+        raise ValueError("key_cache and value_cache must be contiguous")
+    if key_cache.shape[-1] != int4_page_bytes(head_size, block_size):
+        raise ValueError(f"pages of {key_cache.shape[-1]} bytes, head_size {head_size} and "
+                         f"block_size {block_size} need {int4_page_bytes(head_size, block_size)}")
+    bt = _as_int32(block_table, "block_table")
+    if key_cache.dim() == 3:
+        nb, heads, _ = key_cache.shape
+        num_pages, mul, add = nb * heads, heads, 1
+    elif key_cache.dim() == 2:
+        if bt.dim() != 3:
+            raise ValueError("a 2-D (per-head page) cache needs a block table "
+                             "(num_seqs, num_kv_heads, max_blocks)")
+        num_pages, heads, mul, add = key_cache.shape[0], bt.shape[1], 1, 0
+    else:
+        raise ValueError(f"unsupported 4-bit cache rank {key_cache.dim()}")
+    if num_kv_heads is not None and heads != num_kv_heads:
+        raise ValueError(f"cache has {heads} kv heads, the rows {num_kv_heads}")
+    if bt.dim() == 3 and tuple(bt.shape[:2]) == (num_seqs, heads):
+        strides, maxb = bt.stride(), bt.shape[2]
+    elif bt.dim() == 2 and bt.shape[0] == num_seqs:
+        strides, maxb = (bt.stride(0), 0, bt.stride(1)), bt.shape[1]
+    else:
+        raise ValueError("block table must be (num_seqs, max_blocks) or "
+                         "(num_seqs, num_kv_heads, max_blocks)")
+    return bt, num_pages, heads, mul, add, maxb, strides
+
+
+def _length_strides(lens, num_seqs, heads, name):
+    if lens.dim() == 1 and lens.shape[0] == num_seqs:
+        return lens.stride(0), 0
+    if lens.dim() == 2 and tuple(lens.shape) == (num_seqs, heads):
+        return lens.stride()
+    raise ValueError(f"{name} must be (num_seqs,) or (num_seqs, num_kv_heads)")
+
+
+def _check_offsets(cu, num_seqs, name):
+    """Token offsets: an int32 tensor (num_seqs + 1,), or None."""
+    if cu is None:
+        return None
+    if cu.dtype != torch.int32:
+        raise TypeError(f"{name} must be int32")
+    if cu.dim() != 1 or cu.shape[0] != num_seqs + 1 or not cu.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous (num_seqs + 1,) tensor")
+    return cu
+
+
+def _rows_args(key_cache, value_cache, k, v, lens, block_table, cu, block_size, what):
+    """The arguments append and read-back share."""
+    if k.dim() != 3 or tuple(k.shape) != tuple(v.shape):
+        raise ValueError(f"{what} must be (num_tokens, num_kv_heads, head_size)")
+    if k.dtype not in _DTYPES or v.dtype != k.dtype:
+        raise TypeError(f"{what} must share one dtype, bfloat16 or float16")
+    if k.stride(2) != 1 or v.stride(2) != 1 or k.stride() != v.stride():
+        raise ValueError(f"{what} must share strides, contiguous in head_size")
+    N, Hkv, D = k.shape
+    B = lens.shape[0]
+    bt, num_pages, _, mul, add, maxb, bts = _check_caches(key_cache, value_cache, block_table, D,
+                                                          block_size, B, Hkv)
+    lsb, lsh = _length_strides(lens, B, Hkv, "cache_seqlens")
+    if cu is None and N != B:
+        raise ValueError(f"{N} tokens for {B} sequences need token offsets")
+    tensors = [key_cache, value_cache, k, v, lens, bt] + ([] if cu is None else [cu])
+    device = _check_device(*tensors)
+    a = _lib.Int4RowsArgs()
+    a.k_cache, a.v_cache = key_cache.data_ptr(), value_cache.data_ptr()
+    a.k_rows, a.v_rows = k.data_ptr(), v.data_ptr()
+    a.seqlens, a.block_table = lens.data_ptr(), bt.data_ptr()
+    a.cu_tokens = None if cu is None else cu.data_ptr()
+    a.status = _append_status_word(device).data_ptr()
+    a.dtype, a.num_seqs, a.num_kv_heads = _DTYPES[k.dtype], B, Hkv
+    a.head_size, a.block_size, a.max_blocks = D, block_size, maxb
+    a.num_pages, a.num_tokens = num_pages, N
+    a.row_stride_t, a.row_stride_h = k.stride(0), k.stride(1)
+    a.seqlens_stride_b, a.seqlens_stride_h = lsb, lsh
+    a.bt_stride_b, a.bt_stride_h, a.bt_stride_i = bts
+    a.bt_page_mul, a.bt_page_add = mul, add
+    return a, device, bt
+
+
+def kv_append_int4(key_cache, value_cache, k_new, v_new, cache_seqlens, block_table, block_size,
+                   cu_new=None, increment=True):
+    """Quantise new tokens into a 4-bit cache, in place.
+
+    The 4-bit form of ``kv_append``, for one token per sequence or for ragged
+    runs of them (prompts).  k_new, v_new: (num_tokens, num_kv_heads,
+    head_size), bfloat16 or float16.  ``cu_new``: int32 (num_seqs + 1,), tokens
+    cu_new[s] .. cu_new[s+1] - 1 belong to sequence s; None: one token per
+    sequence.  cache_seqlens: int32 (num_seqs,) or (num_seqs, num_kv_heads), the
+    lengths L before the call; token j goes to position L + j and, with
+    ``increment``, L grows in place by the tokens written.  Tokens from the
+    first one without a page slot or with an invalid page id are not counted,
+    and a bit read by ``kv_append_status`` is set.
+    """
+    if cache_seqlens.dtype != torch.int32:
+        raise TypeError("cache_seqlens must be int32 (it is updated in place)")
+    cu = _check_offsets(cu_new, cache_seqlens.shape[0], "cu_new")
+    a, device, keep = _rows_args(key_cache, value_cache, k_new, v_new, cache_seqlens, block_table,
+                                 cu, block_size, "k_new and v_new")
+    lib = _lib.load()
+    with torch.cuda.device(device):
+        rc = lib.pab200_kv_append_int4(ctypes.byref(a), 1 if increment else 0,
+                                       _current_stream_handle(device))
+    _raise_for(lib, rc, "pab200_kv_append_int4")
+    del keep
+
+
+def kv_read_int4(key_cache, value_cache, block_table, cache_seqlens, block_size, head_size, dtype,
+                 starts=None, cu_out=None, num_tokens=None, out=None):
+    """Read tokens of a 4-bit cache back as 16-bit rows.
+
+    Returns (k, v), each (num_tokens, num_kv_heads, head_size) of ``dtype``, the
+    type the tokens were appended in.  Rows cu_out[s] .. cu_out[s+1] - 1 are
+    positions starts[s], starts[s] + 1, ... of sequence s (``starts`` None: from
+    0); ``cu_out`` int32 (num_seqs + 1,) with ``num_tokens`` rows in all, or
+    None: one row per sequence.  Positions at or past cache_seqlens and pages
+    with an invalid id read as zeros.  ``out``: a (k, v) pair to fill; rows
+    behind cu_out's last are left as they were.
+    """
+    if dtype not in _DTYPES:
+        raise TypeError(f"dtype must be bfloat16 or float16, got {dtype}")
+    lens = _as_int32(cache_seqlens, "cache_seqlens")
+    B = lens.shape[0]
+    cu = _check_offsets(cu_out, B, "cu_out")
+    if out is None:
+        if cu is not None and num_tokens is None:
+            raise ValueError("cu_out needs num_tokens (or out)")
+        n = B if cu is None else int(num_tokens)
+        heads = key_cache.shape[1] if key_cache.dim() == 3 else block_table.shape[1]
+        make = torch.empty if cu is None else torch.zeros   # rows in no sequence are not written
+        out = tuple(make((n, heads, head_size), dtype=dtype, device=key_cache.device)
+                    for _ in range(2))
+    k, v = out
+    if k.dtype != dtype or k.dim() != 3 or k.shape[2] != head_size:
+        raise ValueError("out must be a pair of (num_tokens, num_kv_heads, head_size) of dtype")
+    if starts is not None:
+        starts = _as_int32(starts, "starts")
+        if starts.dim() != 1 or starts.shape[0] != B:
+            raise ValueError("starts must be (num_seqs,)")
+        _check_device(key_cache, starts)
+    a, device, keep = _rows_args(key_cache, value_cache, k, v, lens, block_table, cu, block_size,
+                                 "out")
+    lib = _lib.load()
+    with torch.cuda.device(device):
+        rc = lib.pab200_kv_read_int4(ctypes.byref(a), None if starts is None else starts.data_ptr(),
+                                     0 if starts is None else starts.stride(0),
+                                     _current_stream_handle(device))
+    _raise_for(lib, rc, "pab200_kv_read_int4")
+    del keep
+    return k, v
+
+
+def paged_attention_int4(out, query, key_cache, value_cache, block_tables, context_lens, scale,
+                         block_size, num_splits=0):
+    """In-place paged decode over 4-bit caches: ``paged_attention`` with the
+    caches of ``kv_append_int4``, appended in query's dtype.
+
+    out, query: (num_seqs, num_q_heads, head_size); block_tables (num_seqs,
+    max_blocks) or, per kv head, (num_seqs, num_kv_heads, max_blocks);
+    context_lens (num_seqs,) or (num_seqs, num_kv_heads).  Query groups as for
+    ``paged_attention``.
+    """
+    if query.dim() != 3:
+        raise ValueError("query must be (num_seqs, num_q_heads, head_size)")
+    if query.dtype not in _DTYPES:
+        raise TypeError(f"query must be bfloat16 or float16, got {query.dtype}")
+    if query.stride(2) != 1:
+        raise ValueError("query must be contiguous in head_size")
+    if out.shape != query.shape or out.dtype != query.dtype:
+        raise ValueError("out must match query in shape and dtype")
+    if out.stride(2) != 1:
+        raise ValueError("out must be contiguous in head_size")
+    if num_splits < 0:
+        raise ValueError("num_splits must be >= 0")
+    B, Hq, D = query.shape
+    bt, num_pages, Hkv, mul, add, maxb, bts = _check_caches(key_cache, value_cache, block_tables, D,
+                                                            block_size, B, None)
+    if Hq % Hkv != 0:
+        raise ValueError(f"num_q_heads {Hq} is not a multiple of num_kv_heads {Hkv}")
+    lens = _as_int32(context_lens, "context_lens")
+    lsb, lsh = _length_strides(lens, B, Hkv, "context_lens")
+    device = _check_device(query, out, key_cache, value_cache, bt, lens)
+    if B == 0:
+        return
+    args = _lib.DecodeArgs()
+    _fill_common(args, q=query, k_cache=key_cache, v_cache=value_cache, lens=lens, bt=bt,
+                 dtype=query.dtype, B=B, Hq=Hq, Hkv=Hkv, D=D, bs=block_size, num_pages=num_pages,
+                 scale=scale, num_splits=num_splits)
+    args.layout, args.max_blocks, args.out = _lib.LAYOUT_PAGES, maxb, out.data_ptr()
+    args.q_stride_b, args.q_stride_h = query.stride(0), query.stride(1)
+    args.out_stride_b, args.out_stride_h = out.stride(0), out.stride(1)
+    args.seqlens_stride_b, args.seqlens_stride_h = lsb, lsh
+    args.bt_stride_b, args.bt_stride_h, args.bt_stride_i = bts
+    args.bt_page_mul, args.bt_page_add = mul, add
+    lib = _lib.load()
+    with torch.cuda.device(device):
+        need = lib.pab200_decode_int4_workspace_size(ctypes.byref(args))
+        if need == 0:
+            raise ValueError(f"pab200_decode_int4: {lib.pab200_last_error().decode()}")
+        ws = torch.empty(need, dtype=torch.uint8, device=device)
+        stream = _current_stream_handle(device)
+        rc = lib.pab200_decode_int4(ctypes.byref(args), ws.data_ptr(), need, stream)
+    _raise_for(lib, rc, "pab200_decode_int4")
+    _keep_workspace(device, ws, stream)

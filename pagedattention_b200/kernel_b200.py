@@ -178,6 +178,18 @@ def _launch(lib, args, device, append=None, exchange=None) -> int:
     return rc
 
 
+def _raise_for(lib, rc, what) -> None:
+    """ValueError for refused arguments, RuntimeError for other failures."""
+    if rc in (_lib.ERR_INVALID_ARGUMENT, _lib.ERR_UNSUPPORTED, _lib.ERR_ALIGNMENT):
+        raise ValueError(f"{what}: {_lib.error_text(lib, rc)}")
+    _lib.check(lib, rc, what)
+
+
+def _keep_workspace(device, ws, stream_handle) -> None:
+    """The workspace whose status word ``read_status`` reports next."""
+    _last_ws[device.index] = (ws, stream_handle)
+
+
 def _fill_common(args, *, q, k_cache, v_cache, lens, bt, dtype, B, Hq, Hkv, D, bs,
                  num_pages, scale, num_splits):
     args.q = q.data_ptr()

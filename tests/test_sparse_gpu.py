@@ -1,0 +1,326 @@
+"""Key bounds, page selection and page-sparse decode on a GPU: bounds and
+selected pages exactly, attention against the dense call over the same pages."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import pagedattention_b200 as pa
+from oracle import pages as op
+from pagedattention_b200 import _lib
+from tests.test_int4_gpu import check_attention, half_step, tables
+
+pytestmark = pytest.mark.gpu
+BF, HF = torch.bfloat16, torch.float16
+
+
+def expect_bounds(bounds, k, lens, bt, bs, cu, per_head):
+    """Restatement on CPU copies, in place.  bounds (P, 2, D) by page id."""
+    Hkv = k.shape[1]
+    for s in range(lens.shape[0]):
+        a, b = (s, s + 1) if cu is None else (int(cu[s]), int(cu[s + 1]))
+        for h in range(Hkv):
+            L = int(lens[s, h] if lens.dim() == 2 else lens[s])
+            for j in range(b - a):
+                i = (L + j) // bs
+                if L < 0 or i >= bt.shape[-1]:
+                    continue
+                e = int(bt[s, h, i] if bt.dim() == 3 else bt[s, i])
+                pid = e if per_head else e * Hkv + h
+                if pid < 0 or pid >= bounds.shape[0]:
+                    continue
+                x = k[a + j, h]
+                if (L + j) % bs == 0:
+                    bounds[pid, 0] = bounds[pid, 1] = x
+                else:
+                    bounds[pid, 0] = torch.minimum(bounds[pid, 0], x)
+                    bounds[pid, 1] = torch.maximum(bounds[pid, 1], x)
+
+
+@pytest.mark.parametrize("dt,D,bs,Hkv,lens,new,per_head", [
+    (BF, 128, 16, 8, [0, 15, 16, 100], None, False),
+    (HF, 64, 8, 1, [0, 7, 3, 61], [1, 20, 0, 33], False),
+    (BF, 256, 32, 2, [5, 0], [70, 1], True),
+    (HF, 128, 64, 3, [63, 1, 0, 64], [2, 200, 65, 64], False),
+    (BF, 64, 16, 5, [0], [513], True),
+])
+@pytest.mark.parametrize("off", [0, 1])
+def test_bounds_exact(cuda_device, dt, D, bs, Hkv, lens, new, per_head, off):
+    g = torch.Generator().manual_seed(D)
+    lens = torch.tensor(lens, dtype=torch.int32)
+    B = lens.numel()
+    n = torch.ones(B, dtype=torch.int32) if new is None else torch.tensor(new, dtype=torch.int32)
+    cu = None
+    if new is not None:
+        cu = torch.zeros(B + 1, dtype=torch.int32)
+        cu[1:] = torch.cumsum(n, 0)
+    total = lens + n
+    bt, pool = tables(total[:, None].expand(B, Hkv).contiguous() if per_head else total, bs)
+    P = pool if per_head else pool * Hkv
+    N = int(n.sum()) + (0 if cu is None else 2)
+    flat = torch.randn((N, Hkv * D + 8), generator=g).to(dt)
+    k = flat[:, off:off + Hkv * D].unflatten(1, (Hkv, D))
+    kd = flat.to(cuda_device)[:, off:off + Hkv * D].unflatten(1, (Hkv, D))
+    k[0, 0, 3] = kd[0, 0, 3] = float("nan")
+    bounds = torch.randn((P, 2, D), generator=g).to(dt)
+    bd = bounds.to(cuda_device).view((P, 2, D) if per_head else (pool, Hkv, 2, D))
+    ld = lens.to(cuda_device)
+    pa.kv_append_status()
+    pa.update_page_bounds(bd, kd, ld, bt.to(cuda_device), bs,
+                          cu_new=None if cu is None else cu.to(cuda_device))
+    assert pa.kv_append_status() == 0
+    expect_bounds(bounds, k, lens, bt, bs, cu, per_head)
+    assert torch.equal(torch.nan_to_num(bd.cpu().view(P, 2, D), nan=99.0),
+                       torch.nan_to_num(bounds, nan=99.0))
+    assert torch.equal(ld.cpu(), lens)
+
+
+def test_bounds_places_that_do_not_exist(cuda_device):
+    dt, D, bs, Hkv = BF, 64, 8, 2
+    lens = torch.tensor([30, 4, -2, 0], dtype=torch.int32)
+    cu = torch.tensor([0, 5, 25, 28, 37], dtype=torch.int32)
+    bt = torch.tensor([[0, 1, 2, 3], [4, 99, 5, 6], [7, 8, 9, 10], [11, -1, 12, 13]], dtype=torch.int32)
+    g = torch.Generator().manual_seed(1)
+    k = torch.randn((37, Hkv, D), generator=g).to(dt)
+    bounds = torch.randn((28, 2, D), generator=g).to(dt)
+    bd = bounds.to(cuda_device).view(14, Hkv, 2, D)
+    pa.kv_append_status()
+    pa.update_page_bounds(bd, k.to(cuda_device), lens.to(cuda_device), bt.to(cuda_device), bs,
+                          cu_new=cu.to(cuda_device))
+    assert pa.kv_append_status() == (_lib.STATUS_APPEND_FULL | _lib.STATUS_BAD_PAGE_ID
+                                     | _lib.STATUS_NEG_SEQLEN)
+    expect_bounds(bounds, k, lens, bt, bs, cu, False)
+    assert torch.equal(bd.cpu().view(28, 2, D), bounds)
+
+
+# --------------------------------------------------------------- selection
+
+def expect_select(q, bounds, bt, lens, bs, keep, sink, recent, Hkv, per_head):
+    B, Hq, _ = q.shape
+    G = Hq // Hkv
+    tabs = torch.full((B, Hkv, keep), -1, dtype=torch.int32)
+    out = torch.zeros((B, Hkv), dtype=torch.int32)
+    cap = bt.shape[-1] * bs
+    for s in range(B):
+        for h in range(Hkv):
+            L = int(lens[s, h] if lens.dim() == 2 else lens[s])
+            L = min(max(L, 0), cap)
+            n = (L + bs - 1) // bs
+            row = bt[s, h] if bt.dim() == 3 else bt[s]
+            ids = [int(e) if per_head else int(e) * Hkv + h for e in row[:n]]
+            b, bad = np.zeros((n, 2, q.shape[2])), set()
+            for i, pid in enumerate(ids):
+                if 0 <= pid < bounds.shape[0]:
+                    b[i] = bounds[pid].double().numpy()
+                else:
+                    bad.add(i)
+            got = op.select(q[s, h * G:(h + 1) * G].double().numpy(), b, n, keep, sink, recent, bad)
+            tabs[s, h, :len(got)] = row[torch.tensor(got, dtype=torch.long)]
+            out[s, h] = (len(got) - 1) * bs + L - (n - 1) * bs if n else 0
+    return tabs, out
+
+
+SELECT = [  # dtype, D, G, Hkv, bs, lens, keep, sink, recent
+    (BF, 128, 4, 2, 16, [1000, 0, 1, 333, 128, 129], 8, 1, 1),
+    (HF, 64, 8, 1, 8, [5000, 63, 64, 65], 8, 0, 1),
+    (BF, 256, 2, 3, 32, [700, 2000], 5, 2, 2),
+    (HF, 128, 1, 2, 64, [4097, 260], 4, 3, 1),       # nothing left to choose
+    (BF, 64, 32, 1, 8, [9000], 300, 1, 4),
+    (HF, 128, 3, 5, 16, [17, 600], 1, 0, 1),         # only the last page
+    (BF, 128, 8, 1, 8, [20000], 1030, 1, 1),
+]
+
+
+@pytest.mark.parametrize("dt,D,G,Hkv,bs,lens,keep,sink,recent", SELECT)
+@pytest.mark.parametrize("per_head", [False, True])
+def test_select_exact(cuda_device, dt, D, G, Hkv, bs, lens, keep, sink, recent, per_head):
+    g = torch.Generator().manual_seed(keep + D)
+    lens = torch.tensor(lens, dtype=torch.int32)
+    B = lens.numel()
+    ll = lens[:, None].expand(B, Hkv).contiguous() if per_head else lens
+    bt, pool = tables(ll, bs)
+    P = pool if per_head else pool * Hkv
+    x = torch.randn((P, 2, D), generator=g).to(dt)
+    bounds = torch.stack((x.amin(1), x.amax(1)), 1)
+    q = torch.randn((B, G * Hkv, D), generator=g).to(dt)
+    bd = bounds.to(cuda_device).view((P, 2, D) if per_head else (pool, Hkv, 2, D))
+    pa.kv_append_status()
+    tabs, out = pa.select_pages(q.to(cuda_device), bd, bt.to(cuda_device), ll.to(cuda_device), bs, keep,
+                                num_sink=sink, num_recent=recent)
+    assert pa.kv_append_status() == 0
+    want, wl = expect_select(q, bounds, bt, ll, bs, keep, sink, recent, Hkv, per_head)
+    assert torch.equal(out.cpu(), wl)
+    assert torch.equal(tabs.cpu(), want)
+
+
+def test_select_ties_nan_and_bad_pages(cuda_device):
+    """Equal scores go to the lower page, NaN ranks first, bad ids last; -0 is +0."""
+    dt, D, G, Hkv, bs = BF, 64, 2, 1, 8
+    n, keep = 400, 50
+    bounds = torch.zeros((n, 2, D), dtype=dt)
+    bounds[::2, 1, 0] = 1.0                          # two scores in all
+    bounds[1::4, 0, 1], bounds[1::4, 1, 1] = -0.0, -0.0
+    bounds[100] = float("nan")
+    bounds[301] = float("nan")
+    bounds[200:203, 1, 0] = 5.0
+    q = torch.zeros((1, G, D), dtype=dt)
+    q[:, :, 0] = 1.0
+    bt = torch.arange(n, dtype=torch.int32)[None].clone()
+    bt[0, 7], bt[0, 11] = -3, 10 ** 6
+    lens = torch.tensor([n * bs - 3], dtype=torch.int32)
+    for keep in (50, 4, 380, 399):
+        pa.kv_append_status()
+        tabs, out = pa.select_pages(q.to(cuda_device), bounds.to(cuda_device).view(n, 1, 2, D),
+                                    bt.to(cuda_device), lens.to(cuda_device), bs, keep)
+        assert pa.kv_append_status() == _lib.STATUS_BAD_PAGE_ID
+        want, wl = expect_select(q, bounds, bt, lens, bs, keep, 1, 1, Hkv, False)
+        assert torch.equal(out.cpu(), wl) and torch.equal(tabs.cpu(), want)
+
+
+def test_select_lengths_out_of_range(cuda_device):
+    dt, D, bs = HF, 64, 8
+    g = torch.Generator().manual_seed(0)
+    bounds = torch.randn((20, 2, D), generator=g).to(dt).sort(1).values
+    q = torch.randn((2, 2, D), generator=g).to(dt)
+    bt = torch.arange(20, dtype=torch.int32).view(2, 10)
+    lens = torch.tensor([-1, 10 ** 6], dtype=torch.int32)
+    pa.kv_append_status()
+    tabs, out = pa.select_pages(q.to(cuda_device), bounds.view(20, 1, 2, D).to(cuda_device),
+                                bt.to(cuda_device), lens.to(cuda_device), bs, 4)
+    assert pa.kv_append_status() == _lib.STATUS_NEG_SEQLEN | _lib.STATUS_SEQLEN_CLAMP
+    want, wl = expect_select(q, bounds, bt, lens, bs, 4, 1, 1, 1, False)
+    assert torch.equal(out.cpu(), wl) and torch.equal(tabs.cpu(), want)
+
+
+# --------------------------------------------------------- sparse attention
+
+@pytest.mark.parametrize("dt,D,G,Hkv,bs,lens,keep,layout", [
+    (BF, 128, 4, 2, 16, [1000, 0, 1, 333, 128, 129], 8, "HND"),
+    (HF, 64, 8, 1, 8, [3000, 63], 16, "HND"),
+    (HF, 128, 8, 2, 32, [1500, 40], 7, "NHD"),
+    (BF, 256, 2, 1, 64, [3000], 3, "NHD"),
+    (BF, 128, 32, 1, 16, [900], 12, "HND"),
+])
+def test_sparse_attention(cuda_device, dt, D, G, Hkv, bs, lens, keep, layout):
+    g = torch.Generator().manual_seed(D + G)
+    lens = torch.tensor(lens, dtype=torch.int32)
+    B = lens.numel()
+    bt, pool = tables(lens, bs)
+    k = torch.randn((pool, Hkv, bs, D), generator=g).to(dt)
+    v = torch.randn((pool, Hkv, bs, D), generator=g).to(dt)
+    bounds = torch.stack((k.amin(2), k.amax(2)), 2).contiguous()
+    q = torch.randn((B, G * Hkv, D), generator=g).to(dt)
+    scale = 1 / math.sqrt(D)
+
+    def lay(x):
+        return (x if layout == "HND" else x.transpose(1, 2)).contiguous().to(cuda_device)
+
+    kd, vd, qd, bd = lay(k), lay(v), q.to(cuda_device), bounds.to(cuda_device)
+    btd, ld = bt.to(cuda_device), lens.to(cuda_device)
+    out = torch.full_like(qd, 9.0)
+    tabs, sl = pa.paged_attention_sparse(out, qd, kd, vd, bd, btd, ld, scale, bs, keep,
+                                         kv_layout=layout)
+    want, wl = expect_select(q, bounds.view(-1, 2, D), bt, lens, bs, keep, 1, 1, Hkv, False)
+    assert torch.equal(tabs.cpu(), want) and torch.equal(sl.cpu(), wl)
+    t2, s2 = pa.select_pages(qd, bd, btd, ld, bs, keep)
+    assert torch.equal(t2, tabs) and torch.equal(s2, sl)
+    # in 64 bits over the selected pages: the probabilities' rounding to T
+    # (half a step of each, against values up to max |v|) and the output's
+    for s in range(B):
+        for h in range(Hkv):
+            L = int(wl[s, h])
+            ids = want[s, h, :(L + bs - 1) // bs].long()
+            kk, vv = (x[ids, h].reshape(-1, D)[:L].double().numpy() for x in (k, v))
+            qq = q[s, h * G:(h + 1) * G].double().numpy()
+            ref = op.attention(qq, kk, vv, scale)
+            have = out[s, h * G:(h + 1) * G].double().cpu().numpy()
+            if L == 0:
+                assert (have == 0).all()
+                continue
+            size = (np.abs(qq) @ np.abs(kk).T).max(1)[:, None] * scale
+            tol = half_step(dt) * (np.abs(ref) + np.abs(vv).max()) + \
+                (2.0 ** -18 + 128 * 2.0 ** -24 * 2 * size) * np.abs(vv).max()
+            assert (np.abs(have - ref) <= tol).all(), (s, h)
+    # keeping every page is the dense call
+    full = torch.empty_like(out)
+    pa.paged_attention(full, qd, kd, vd, btd, ld, scale, bs, kv_layout=layout)
+    n = max(int((lens.max() + bs - 1) // bs), 2)
+    pa.paged_attention_sparse(out, qd, kd, vd, bd, btd, ld, scale, bs, n, kv_layout=layout)
+    tol = 2 * half_step(dt) * (full.float().abs() + v.float().abs().max()) + 1e-3
+    assert ((out.float() - full.float()).abs() <= tol).all()
+
+
+def test_serving_steps_together(cuda_device):
+    """Prompts and steps: bounds, 4-bit append, selection and 4-bit attention
+    over the selection, eager and then replayed from a graph."""
+    dt, D, G, Hkv, bs, B, keep = BF, 128, 4, 2, 16, 3, 6
+    g = torch.Generator().manual_seed(11)
+    prompt = torch.tensor([150, 17, 401], dtype=torch.int32)
+    bt, pool = tables(prompt + 40, bs)
+    btd = bt.to(cuda_device)
+    kc, vc = pa.int4_cache(pool, Hkv, bs, D, device=cuda_device)
+    bounds = torch.zeros((pool, Hkv, 2, D), dtype=dt, device=cuda_device)
+    lens = torch.zeros(B, dtype=torch.int32, device=cuda_device)
+    cu = torch.zeros(B + 1, dtype=torch.int32)
+    cu[1:] = torch.cumsum(prompt, 0)
+    N = int(cu[-1])
+    rows = torch.randn((2, N, Hkv, D), generator=g).to(dt)
+    cud = cu.to(cuda_device)
+    kd, vd = rows.to(cuda_device)
+    pa.update_page_bounds(bounds, kd, lens, btd, bs, cu_new=cud)
+    pa.kv_append_int4(kc, vc, kd, vd, lens, btd, bs, cu_new=cud)
+    keys = [[rows[0, int(cu[s]) + j] for j in range(int(prompt[s]))] for s in range(B)]
+    x = torch.zeros((2, B, Hkv, D), dtype=dt, device=cuda_device)
+    q = torch.zeros((B, G * Hkv, D), dtype=dt, device=cuda_device)
+    out = torch.empty_like(q)
+    res = {}
+
+    def step():
+        pa.update_page_bounds(bounds, x[0], lens, btd, bs)
+        pa.kv_append_int4(kc, vc, x[0], x[1], lens, btd, bs)
+        res["t"], res["l"] = pa.select_pages(q, bounds, btd, lens, bs, keep)
+        pa.paged_attention_int4(out, q, kc, vc, res["t"], res["l"], 0.09, bs)
+
+    def fill():
+        xn = torch.randn((2, B, Hkv, D), generator=g).to(dt)
+        qn = torch.randn((B, G * Hkv, D), generator=g).to(dt)
+        x.copy_(xn)
+        q.copy_(qn)
+        for s in range(B):
+            keys[s].append(xn[0, s])
+        return qn
+
+    def check(qn):
+        torch.cuda.synchronize()
+        n = torch.tensor([len(k) for k in keys], dtype=torch.int32)
+        assert torch.equal(lens.cpu(), n)
+        b = torch.zeros((pool, Hkv, 2, D), dtype=dt)
+        for s in range(B):
+            kk = torch.stack(keys[s])
+            for i in range((len(keys[s]) + bs - 1) // bs):
+                part = kk[i * bs:(i + 1) * bs]
+                b[int(bt[s, i])] = torch.stack((part.amin(0), part.amax(0)), 1)
+        used = torch.cat([bt[s, :(int(n[s]) + bs - 1) // bs] for s in range(B)]).long()
+        assert torch.equal(bounds.cpu()[used], b[used])
+        want, wl = expect_select(qn, b.view(-1, 2, D), bt, n, bs, keep, 1, 1, Hkv, False)
+        assert torch.equal(res["t"].cpu(), want) and torch.equal(res["l"].cpu(), wl)
+        check_attention(out, qn, kc.cpu().numpy().reshape(pool * Hkv, -1),
+                        vc.cpu().numpy().reshape(pool * Hkv, -1), want, wl, 0.09, bs, Hkv, dt)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(18):                        # over a page's end
+            qn = fill()
+            step()
+        check(qn)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        step()
+    for _ in range(4):
+        qn = fill()
+        graph.replay()
+        check(qn)
