@@ -60,7 +60,6 @@
 
 #include <type_traits>
 
-#include "int4.cuh"
 #include "ptx.cuh"
 
 namespace pab {
@@ -133,6 +132,7 @@ struct DecodeParams {
   int64_t num_pages;
   const uint8_t* k_pages;  // 4-bit caches: the pages (no tensor map)
   const uint8_t* v_pages;
+  int32_t unit_pages;   // fewest pages per range where there are enough: fewer ranges otherwise
   int32_t head_in_map;  // NHD layout: kv head is the tensor map's y coordinate
   float scale_log2;     // softmax_scale * log2(e)
   int32_t total_warps;  // W
@@ -401,7 +401,8 @@ __global__ void __launch_bounds__(1024) plan_kernel(const DecodeParams p) {
   // With more warps than pages some warps would own no page and the span
   // count of a head (warp_of_page(last) - warp_of_page(first) + 1) would
   // include them; capping W at the page count gives every warp >= 1 page.
-  const int W = static_cast<int>(total < p.total_warps ? total : p.total_warps);
+  const int64_t units = (total + p.unit_pages - 1) / p.unit_pages;
+  const int W = static_cast<int>(units < p.total_warps ? units : p.total_warps);
   // Dynamic tail chunks of every warp range (tail_chunks).
   int sm_m = 0, sm_k = 0;
   tail_chunks(total, W, p.steal_m_max, p.steal_pps, p.steal_min_stages, &sm_m, &sm_k);
@@ -614,29 +615,24 @@ __device__ __forceinline__ void write_row(const DecodeParams& p, int hd, int g, 
 // group of up to 32 query heads fits at D = 128.  (At D = 64 the pair runs
 // twice the resident warps of the single-warp kernel but is slower: each
 // stage waits on both warps, and the per-stage issue work does not split.)
-// Q4 reads 4-bit pages (int4.cuh): a page is one contiguous untiled bulk copy,
-// the codes are widened to T in registers, and the (scale, minimum) pairs are
-// applied to the scores (keys) and to the probabilities (values), so that the
-// MMAs run on the bare codes, centred on 8.
-template <typename T, int D, int NT, int ST, bool CORE, bool PAIR, bool TC, bool Q4>
-__device__ __forceinline__ void decode_body(const CUtensorMap& kmap, const CUtensorMap& vmap,
-                                            const DecodeParams& p) {
+template <typename T, int D, int NT, int ST, bool CORE, bool PAIR = false, bool TC = false>
+__global__ void __launch_bounds__(kMaxWarpsPerCta * 32, (PAIR && D == 64 && !TC) ? 2 : 1)
+    decode_kernel(const __grid_constant__ CUtensorMap kmap,
+                  const __grid_constant__ CUtensorMap vmap,
+                  const DecodeParams p) {
   constexpr int NH = D / 64;            // 128-byte planes per token row
   constexpr int LOG2_NH = NH == 1 ? 0 : (NH == 2 ? 1 : 2);
   constexpr int MT = ST / 16;           // 16-token MMA tiles per stage
   constexpr int LOG2_ST = ST == 16 ? 4 : (ST == 32 ? 5 : 6);
   constexpr int KS = D / 16;            // k-steps of QK^T == d-tiles of PV
   constexpr int PLANE = ST * 128;       // bytes of one plane of one stage
-  constexpr int NG = D / kInt4Group;    // 4-bit pages: quantisation groups per row
-  // K (or V) bytes per stage
-  constexpr int KV_BYTES = Q4 ? ST * int4_row_bytes(D) : NH * PLANE;
+  constexpr int KV_BYTES = NH * PLANE;  // K (or V) bytes per stage
   constexpr int STAGE_BYTES = 2 * KV_BYTES;
   static_assert(D % 64 == 0 && (ST == 16 || ST == 32 || ST == 64), "shape");
   static_assert(!CORE || (ST == 32 && NT == 1 && D <= 128), "CUDA-core path shape");
   constexpr int DL = D / 32;  // head-dim elements per lane (CUDA-core path)
   static_assert(NH == 1 || NH == 2 || NH == 4, "head size");
   static_assert(!(CORE && PAIR), "the CUDA-core path has no paired variant");
-  static_assert(!(Q4 && (CORE || TC)), "4-bit pages run on mma.sync");
   static_assert(!TC || (PAIR && !CORE && D == 64 && ST == 64 && NT == 2), "tcgen05 path shape");
 
   extern __shared__ uint8_t smem_raw[];
@@ -824,10 +820,8 @@ __device__ __forceinline__ void decode_body(const CUtensorMap& kmap, const CUten
       mbar_init(tcb + 40, 1);
     }
     fence_mbar_init();
-    if constexpr (!Q4) {
-      tma_prefetch_desc(&kmap);
-      tma_prefetch_desc(&vmap);
-    }
+    tma_prefetch_desc(&kmap);
+    tma_prefetch_desc(&vmap);
   }
   if constexpr (PAIR) {
     // The pair's barriers are initialised.  Fixed barrier ids (one per
@@ -1043,47 +1037,6 @@ __device__ __forceinline__ void decode_body(const CUtensorMap& kmap, const CUten
   auto issue = [&](int slot) -> bool {
     if (!nx_valid) return false;
     const uint32_t bar = bars + slot * 8;
-    if constexpr (Q4) {
-      // One bulk copy per page and cache.  A rejected page id has no copy:
-      // its bytes are zeroed here, before the arrival that publishes the
-      // stage (zero codes, scales and minima: rows of zeros).
-      const int pb = int4_row_bytes(D) << log2_bs;
-      const int64_t pid = static_cast<int64_t>(nx_raw) * p.bt_mul + nx_add;
-      const bool mine = lane < nx_np;
-      const bool bad = mine && (pid < 0 || pid >= p.num_pages);
-      const uint32_t bad_mask = __ballot_sync(0xffffffffu, bad);
-      if (bad_mask) {
-        if (prewait)
-          pending_bad = true;
-        else if (lane == 0)
-          atomicOr(p.status, kStatusBadPage);
-        for (int g = 0; g < nx_np; ++g) {
-          if (!(bad_mask >> g & 1u)) continue;
-          for (int c = 0; c < 2; ++c) {
-            uint4* z = reinterpret_cast<uint4*>(smem + (ring - smem_base) + slot * STAGE_BYTES +
-                                                c * KV_BYTES + g * pb);
-            for (int i = lane; i < pb / 16; i += 32) z[i] = make_uint4(0u, 0u, 0u, 0u);
-          }
-        }
-        // before the bulk copies that refill this slot later
-        fence_proxy_async_smem();
-        __syncwarp();
-      }
-      if (lane == 0) {
-        meta[slot * 2] = make_int4(nx_head, nx_lp0, nx_np, nx_len);
-        meta[slot * 2 + 1] = make_int4(nx_slot, 0, nx_vfirst, nx_vlast);
-        mbar_arrive_expect_tx(bar, static_cast<uint32_t>(2 * pb * (nx_np - __popc(bad_mask))));
-      }
-      __syncwarp();
-      // lane -> (page of the stage, K or V): a stage has at most 8 pages
-      const int pg = lane & 7, kv = lane >> 3;
-      const int64_t src = __shfl_sync(0xffffffffu, pid, pg);
-      if (kv < 2 && pg < nx_np && !(bad_mask >> pg & 1u))
-        bulk_load(ring + slot * STAGE_BYTES + kv * KV_BYTES + pg * pb,
-                  (kv ? p.v_pages : p.k_pages) + src * pb, static_cast<uint32_t>(pb), bar, policy);
-      prepare_next();
-      return true;
-    }
     if (lane == 0) {
       meta[slot * 2] = make_int4(nx_head, nx_lp0, nx_np, nx_len);
       meta[slot * 2 + 1] = make_int4(nx_slot, 0, nx_vfirst, nx_vlast);
@@ -1129,14 +1082,6 @@ __device__ __forceinline__ void decode_body(const CUtensorMap& kmap, const CUten
   uint32_t qb[KS][NT][2];
   float acc[KS][NT][4];
   float mrun[NT][2], lrun[NT][2];
-  // 4-bit pages: query sums per group, and this lane's part of the sum of
-  // probability x the value of code 8 (every element of a group shares it).
-  constexpr int NGQ = Q4 ? NG : 1;
-  float qsum[NT][NGQ][2], vmid[NT][NGQ][2];
-  // Head-dim element of accumulator register i of d-tile dt.
-  auto acc_dim = [&](int dt, int i) {
-    return Q4 ? (dt >> 2) * 64 + lr * 8 + (dt & 3) * 2 + (i >> 1) : dt * 16 + lr + (i >> 1) * 8;
-  };
   // CUDA-core path: lane owns head-dim elements [lane*DL, lane*DL + DL) of
   // every query head; cm is the running max (log2 units, warp-uniform), cl
   // this lane's part of the running sum.
@@ -1173,37 +1118,13 @@ __device__ __forceinline__ void decode_body(const CUtensorMap& kmap, const CUten
         for (int ks = 0; ks < KS; ++ks) {
           uint32_t b0 = 0, b1 = 0;
           if (g < G) {
-            // 4-bit keys: this lane's 16 elements of the group, 4 per k-step
-            const T* row = qp + g * p.q_sh +
-                           (Q4 ? (ks >> 2) * 64 + lc * 16 + (ks & 3) * 4 : ks * 16 + lc * 2);
+            const T* row = qp + g * p.q_sh + ks * 16 + lc * 2;
             b0 = *reinterpret_cast<const uint32_t*>(row);
-            b1 = *reinterpret_cast<const uint32_t*>(row + (Q4 ? 2 : 8));
+            b1 = *reinterpret_cast<const uint32_t*>(row + 8);
           }
           qb[ks][nt][0] = b0;
           qb[ks][nt][1] = b1;
         }
-        if constexpr (Q4) {
-          // Sum of the query over each quantisation group (it multiplies the
-          // keys' value of code 8), for the two heads whose scores this lane
-          // holds.
-#pragma unroll
-          for (int gi = 0; gi < NG; ++gi) {
-            float sum = 0.f;
-#pragma unroll
-            for (int ks = 4 * gi; ks < 4 * gi + 4; ++ks) {
-              const float2 u = unpack2<T>(qb[ks][nt][0]), w = unpack2<T>(qb[ks][nt][1]);
-              sum += (u.x + u.y) + (w.x + w.y);
-            }
-            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-            qsum[nt][gi][0] = __shfl_sync(0xffffffffu, sum, lc * 8);
-            qsum[nt][gi][1] = __shfl_sync(0xffffffffu, sum, lc * 8 + 4);
-          }
-        }
-      }
-      if constexpr (Q4) {
-#pragma unroll
-        for (int gi = 0; gi < NG; ++gi) vmid[nt][gi][0] = vmid[nt][gi][1] = 0.f;
       }
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
@@ -1270,25 +1191,6 @@ __device__ __forceinline__ void decode_body(const CUtensorMap& kmap, const CUten
         }
       }
     } else {
-    if constexpr (Q4) {
-      // The share of code 8's values in every output element of their group.
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int gi = 0; gi < NGQ; ++gi)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            float v = vmid[nt][gi][e];
-            v += __shfl_xor_sync(0xffffffffu, v, 4);
-            v += __shfl_xor_sync(0xffffffffu, v, 8);
-            v += __shfl_xor_sync(0xffffffffu, v, 16);
-#pragma unroll
-            for (int m = 0; m < 4; ++m) {
-              acc[gi * 4 + m][nt][e] += v;
-              acc[gi * 4 + m][nt][e + 2] += v;
-            }
-          }
-    }
     float lt[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
@@ -1315,7 +1217,7 @@ __device__ __forceinline__ void decode_body(const CUtensorMap& kmap, const CUten
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int g = g_lo + nt * 8 + lc * 2 + (i & 1);
-            const int d = acc_dim(dt, i);
+            const int d = dt * 16 + lr + (i >> 1) * 8;
             if (g < G) {
               const float v = acc[dt][nt][i] * inv[nt][i & 1];
               const int qh = h * G + g;
@@ -1347,7 +1249,7 @@ __device__ __forceinline__ void decode_body(const CUtensorMap& kmap, const CUten
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int g = g_lo + nt * 8 + lc * 2 + (i & 1);
-          const int d = acc_dim(dt, i);
+          const int d = dt * 16 + lr + (i >> 1) * 8;
           if (g < G) __stcg(ps + g * D + d, acc[dt][nt][i]);
         }
     if (lr == 0) {
@@ -1895,61 +1797,6 @@ __device__ __forceinline__ void decode_body(const CUtensorMap& kmap, const CUten
     // S^T = K Q^T for the valid 16-token tiles; even and odd k-steps go to
     // separate accumulators so the two MMA dependency chains overlap.
     float sc[MT][NT][4];
-    // 4-bit pages: byte offset, within this stage's K (or V), of 8-token
-    // tile t8's page (a page holds whole tiles), its codes and this lane
-    // group's row of (scale, minimum) pairs.
-    const int page_bytes = int4_row_bytes(D) << log2_bs;
-    auto tile_page = [&](int t8) { return ((t8 * 8) >> log2_bs) * page_bytes; };
-    auto tile_codes = [&](int t8) { return tile_page(t8) + ((t8 * 8) & (bs - 1)) * (D / 2); };
-    auto tile_scales = [&](int t8) {
-      return tile_page(t8) + (bs * (D / 2)) + (((t8 * 8) & (bs - 1)) + lr) * (NG * 4);
-    };
-    if constexpr (Q4) {
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) sc[mt][nt][i] = 0.f;
-        if (mt >= mtv) continue;
-        // Rows lr of the two 8-token tiles: this lane's D/8 bytes of codes.
-        uint32_t wa[D / 32], wb[D / 32], ma[NG], mb[NG];
-        ld_shared_words<D / 32>(kbase + tile_codes(2 * mt) + lr * (D / 2) + lc * (D / 8), wa);
-        ld_shared_words<D / 32>(kbase + tile_codes(2 * mt + 1) + lr * (D / 2) + lc * (D / 8), wb);
-        ld_shared_words<NG>(kbase + tile_scales(2 * mt), ma);
-        ld_shared_words<NG>(kbase + tile_scales(2 * mt + 1), mb);
-#pragma unroll
-        for (int gi = 0; gi < NG; ++gi) {
-          float sg[NT][4];
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) sg[nt][i] = 0.f;
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            uint32_t ra[4], rb[4];
-            int4_widen<T>(wa[gi * 2 + j], ra);
-            int4_widen<T>(wb[gi * 2 + j], rb);
-#pragma unroll
-            for (int hf = 0; hf < 2; ++hf) {
-              const uint32_t a[4] = {ra[2 * hf], rb[2 * hf], ra[2 * hf + 1], rb[2 * hf + 1]};
-              const int ks = gi * 4 + j * 2 + hf;
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt)
-                mma_16816<T>(sg[nt], a, qb[ks][nt][0], qb[ks][nt][1]);
-            }
-          }
-          const float2 fa = int4_centre<T>(ma[gi]), fb = int4_centre<T>(mb[gi]);
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              sc[mt][nt][e] += fmaf(fa.x, sg[nt][e], fa.y * qsum[nt][gi][e]);
-              sc[mt][nt][e + 2] += fmaf(fb.x, sg[nt][e + 2], fb.y * qsum[nt][gi][e]);
-            }
-        }
-      }
-    } else {
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
       float s2[NT][4];
@@ -1981,7 +1828,6 @@ __device__ __forceinline__ void decode_body(const CUtensorMap& kmap, const CUten
 #pragma unroll
         for (int i = 0; i < 4; ++i) sc[mt][nt][i] += s2[nt][i];
     }
-    }  // 16-bit / 4-bit scores
     // Scale into log2 units; mask tokens past the valid range (tail only).
     if (ntok == ST) {
 #pragma unroll
@@ -2015,12 +1861,7 @@ __device__ __forceinline__ void decode_body(const CUtensorMap& kmap, const CUten
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
         const float mold = mrun[nt][e];
-        // 4-bit fp16 pages: the reference point is two below the maximum, so
-        // that the products probability x scale rounded to fp16 lie two
-        // binades higher (at most 4 x 65504 x 2 / 15 < 65504); the state
-        // (m, l, acc) is exact for any m.
-        constexpr float kBelow = Q4 && std::is_same<T, __half>::value ? 2.f : 0.f;
-        const float mnew = fmaxf(mold, mx - kBelow);
+        const float mnew = fmaxf(mold, mx);
         grew |= mnew > mold;
         alpha[nt][e] = fast_exp2(mold - mnew);
         mrun[nt][e] = mnew;
@@ -2043,59 +1884,7 @@ __device__ __forceinline__ void decode_body(const CUtensorMap& kmap, const CUten
         for (int dt = 0; dt < KS; ++dt)
 #pragma unroll
           for (int i = 0; i < 4; ++i) acc[dt][nt][i] *= alpha[nt][i & 1];
-      if constexpr (Q4) {
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int gi = 0; gi < NGQ; ++gi)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) vmid[nt][gi][e] *= alpha[nt][e];
-      }
     }
-    if constexpr (Q4) {
-      // O^T += V^T P^T on the codes: the values' scales multiply the
-      // probabilities (one rounding to T, as the plain P has), the values
-      // of code 8 are summed apart in fp32.  Scales of rows past the valid range may
-      // hold anything and are replaced by zeros; their codes are finite.
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
-        if (mt >= mtv) continue;
-        uint32_t wa[D / 32], wb[D / 32], ma[NG], mb[NG];
-        ld_shared_words<D / 32>(vbase + tile_codes(2 * mt) + lane * (D / 8), wa);
-        ld_shared_words<D / 32>(vbase + tile_codes(2 * mt + 1) + lane * (D / 8), wb);
-        ld_shared_words<NG>(vbase + tile_scales(2 * mt), ma);
-        ld_shared_words<NG>(vbase + tile_scales(2 * mt + 1), mb);
-        const bool oka = mt * 16 + lr < ntok, okb = mt * 16 + 8 + lr < ntok;
-#pragma unroll
-        for (int gi = 0; gi < NG; ++gi) {
-          const float2 fa = int4_centre<T>(oka ? ma[gi] : 0u), fb = int4_centre<T>(okb ? mb[gi] : 0u);
-          uint32_t pg[NT][2];
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            pg[nt][0] = movmatrix_trans(pack2<T>(sc[mt][nt][0] * fa.x, sc[mt][nt][1] * fa.x));
-            pg[nt][1] = movmatrix_trans(pack2<T>(sc[mt][nt][2] * fb.x, sc[mt][nt][3] * fb.x));
-#pragma unroll
-            for (int e = 0; e < 2; ++e)
-              vmid[nt][gi][e] = fmaf(sc[mt][nt][e], fa.y,
-                                     fmaf(sc[mt][nt][e + 2], fb.y, vmid[nt][gi][e]));
-          }
-          // Words of one octet of elements for two consecutive tokens ->
-          // pairs (even token, odd token) of one element per register.
-          uint32_t xa[4], ya[4], xb[4], yb[4];
-          int4_widen<T>(__byte_perm(wa[gi], wa[NG + gi], 0x5410), xa);
-          int4_widen<T>(__byte_perm(wa[gi], wa[NG + gi], 0x7632), ya);
-          int4_widen<T>(__byte_perm(wb[gi], wb[NG + gi], 0x5410), xb);
-          int4_widen<T>(__byte_perm(wb[gi], wb[NG + gi], 0x7632), yb);
-#pragma unroll
-          for (int m = 0; m < 4; ++m) {
-            const uint32_t a[4] = {xa[m], ya[m], xb[m], yb[m]};
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-              mma_16816<T>(acc[gi * 4 + m][nt], a, pg[nt][0], pg[nt][1]);
-          }
-        }
-      }
-    } else {
     // P^T fragments (B operand of the PV product) by in-register transpose.
     uint32_t pb[MT][NT][2];
 #pragma unroll
@@ -2136,7 +1925,6 @@ __device__ __forceinline__ void decode_body(const CUtensorMap& kmap, const CUten
           for (int nt = 0; nt < NT; ++nt) mma_16816<T>(acc[dt][nt], a, pb[mt][nt][0], pb[mt][nt][1]);
         }
       }
-    }  // 16-bit / 4-bit values
     }  // MMA path
     __syncwarp();
     if (dirty) {
@@ -2171,21 +1959,6 @@ __device__ __forceinline__ void decode_body(const CUtensorMap& kmap, const CUten
   }  // pipelines
 }
 
-template <typename T, int D, int NT, int ST, bool CORE, bool PAIR = false, bool TC = false>
-__global__ void __launch_bounds__(kMaxWarpsPerCta * 32, (PAIR && D == 64 && !TC) ? 2 : 1)
-    decode_kernel(const __grid_constant__ CUtensorMap kmap,
-                  const __grid_constant__ CUtensorMap vmap,
-                  const __grid_constant__ DecodeParams p) {
-  decode_body<T, D, NT, ST, CORE, PAIR, TC, false>(kmap, vmap, p);
-}
-
-template <typename T, int D, int NT, int ST, bool PAIR>
-__global__ void __launch_bounds__(kMaxWarpsPerCta * 32, 1)
-    decode_int4_kernel(const __grid_constant__ CUtensorMap kmap,
-                       const __grid_constant__ CUtensorMap vmap,
-                       const __grid_constant__ DecodeParams p) {
-  decode_body<T, D, NT, ST, false, PAIR, false, true>(kmap, vmap, p);
-}
 
 // Prologue of every reduce kernel: lets the next call's planner start (it
 // writes nothing, the parity included, before this grid has finished),

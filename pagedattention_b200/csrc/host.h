@@ -64,8 +64,13 @@ KernelOps kernel_ops() {
   return KernelOps{reinterpret_cast<void*>(Kernel), &launch_decode<Kernel>};
 }
 
-// The decode kernel over 4-bit pages for these sizes (int4.cu).
-bool select_int4_kernel(int dtype, int D, int nt, int st, bool pair, KernelOps* o);
+// The decode kernel over 4-bit pages for these sizes (int4_decode.cu).
+struct Int4Kernel {
+  KernelOps ops;
+  int parts;     // token parts of a stage, joined at the end of a head
+  int min_ctas;  // resident CTAs per SM its registers allow
+};
+bool select_int4_kernel(int dtype, int D, int G, Int4Kernel* o);
 
 // A decode over tables that an earlier kernel of the same call wrote: like
 // pab200_decode(), but the planner is launched after everything before it on

@@ -1,5 +1,6 @@
 // 4-bit page cache: append (quantise) and read-back.
 #include "host.h"
+#include "int4.cuh"
 #include "tokens.cuh"
 
 namespace pab {

@@ -12,10 +12,10 @@
 //
 // Codes are stored as 32-bit words of 8 consecutive elements, element i in
 // nibble i / 2 + 4 (i % 2): the low nibbles of the word's two 16-bit halves are
-// elements 0 and 1, so that a mask and an OR give two neighbouring elements in
-// one 16-bit pair.  Where a word goes follows the fragments of the decode's
+// elements 0 and 1, so that a mask gives two neighbouring elements in one pair
+// of 16-bit lanes.  Where a word goes follows the fragments of the decode's
 // matrix instructions, so that every lane reads its codes of 8 tokens with one
-// contiguous, conflict-free load and no transpose:
+// contiguous, conflict-free load:
 //   keys    row-major rows of D/2 bytes; within a row, chunk c of 4 holds the
 //           words of elements 16 c .. 16 c + 15 of every group (D/64 x 2 words)
 //   values  tiles of 8 tokens, 4 D bytes each: [octet o of 8][token pair of 4]
@@ -81,18 +81,29 @@ __device__ __forceinline__ uint32_t and_or(uint32_t x, uint32_t mask, uint32_t b
   return y;
 }
 
-// Nibble m of both 16-bit halves of w, as the pair r[m] of exact values c - 8
-// (-8..7) of type T.  A nibble OR-ed into the low mantissa bits of a power of
-// two P reads as P + c; subtracting P + 8 is exact.  fp16 (10 mantissa bits)
+// Keys: nibble m of both 16-bit halves of w, as they stand: the pair r[m] is two
+// fp16 subnormals c * 2^-24 (m even) or c * 2^-20 (m odd), exact, for the price
+// of a mask.  The queries carry the powers of two.
+__device__ __forceinline__ void int4_key_pairs(uint32_t w, uint32_t (&r)[4]) {
+  const uint32_t v = w >> 8;
+  r[0] = w & 0x000f000fu;
+  r[1] = w & 0x00f000f0u;
+  r[2] = v & 0x000f000fu;
+  r[3] = v & 0x00f000f0u;
+}
+
+// Values: nibble m of both 16-bit halves of w, as the pair r[m] of exact values
+// c - 8 (-8..7) of type T.  A nibble OR-ed into the low mantissa bits of a power
+// of two P reads as P + c; subtracting P + 8 is exact.  fp16 (10 mantissa bits)
 // also takes the nibble at bits 4..7 in place: 1024 + 16 c, times 1/16 minus
-// 72.  Centred codes keep the products small: a value is (lo + 8 s) + s (c - 8),
-// and the rounding of a probability to T is multiplied by |s (c - 8)|, about
-// |x|, instead of by s c, about the group's range.
+// 72.  Centred codes keep the sums small: a value is (lo + 8 s) + s (c - 8), and
+// the rounding of a probability to T is multiplied by |s (c - 8)|, about |x|,
+// instead of by s c, about the group's range.
 template <typename T>
-__device__ __forceinline__ void int4_widen(uint32_t w, uint32_t (&r)[4]);
+__device__ __forceinline__ void int4_value_pairs(uint32_t w, uint32_t (&r)[4]);
 
 template <>
-__device__ __forceinline__ void int4_widen<__half>(uint32_t w, uint32_t (&r)[4]) {
+__device__ __forceinline__ void int4_value_pairs<__half>(uint32_t w, uint32_t (&r)[4]) {
   const uint32_t v = w >> 8;
   const __half2 base = __float2half2_rn(1032.f);
   const __half2 sixteenth = __float2half2_rn(0.0625f), off = __float2half2_rn(-72.f);
@@ -107,7 +118,7 @@ __device__ __forceinline__ void int4_widen<__half>(uint32_t w, uint32_t (&r)[4])
 }
 
 template <>
-__device__ __forceinline__ void int4_widen<__nv_bfloat16>(uint32_t w, uint32_t (&r)[4]) {
+__device__ __forceinline__ void int4_value_pairs<__nv_bfloat16>(uint32_t w, uint32_t (&r)[4]) {
   const __nv_bfloat162 base = __floats2bfloat162_rn(136.f, 136.f);
 #pragma unroll
   for (int m = 0; m < 4; ++m) {

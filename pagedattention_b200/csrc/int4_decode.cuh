@@ -1,0 +1,632 @@
+// Decode attention over 4-bit pages (int4.cuh).
+//
+//   score_t = scale * sum_g [ s_tg (q_g . c_tg) + lo_tg sum(q_g) ]
+//   out_d   = sum_t p_t [ (lo_tg + 8 s_tg) + s_tg (c_td - 8) ] / sum_t p_t
+//
+// A quarter of the bytes of 16-bit pages but the same products, and codes to
+// widen before the matrix instructions can take them: instruction issue bounds
+// the kernel, not HBM, so everything is laid out for few instructions per code.
+//   * One producer warp per CTA walks the CTA's page range (the planner's
+//     equal cut of all pages, as in decode.cuh), reads the block table one
+//     stage ahead and fills a ring of 128-token stages with one untiled bulk
+//     copy per page and cache.  Four consumer warps share every stage, 32
+//     tokens each (groups of more than 16 heads at D 128: two pairs, each pair
+//     16 heads and 64 tokens per warp), and do nothing but arithmetic.
+//   * Keys enter the MMA as fp16 subnormals, the nibbles as they stand (one
+//     mask per pair); the query is brought to fp16 by a power of two per head,
+//     which loses nothing of a bf16 or fp16 query that matters, and the score is
+//     scaled back in fp32.  Values are widened to c - 8 in T.
+//   * Scales and minima never touch the codes: the keys' multiply the partial
+//     scores of their group, the values' scale multiplies the probability
+//     (rounded to T once, as a plain probability is) and the rest of the value,
+//     lo + 8 s, is summed apart in fp32.
+//   * The softmax's reference point moves only when a score exceeds it by
+//     kRaise (log2 units): no shuffles or rescaling in most stages.
+// At the end of a head (or of the CTA's part of it) the consumers' states are
+// joined through shared memory and written: the output, or one partial state
+// for the reduce kernels of decode.cuh.
+#pragma once
+
+#include <type_traits>
+
+#include "decode.cuh"
+#include "int4.cuh"
+
+namespace pab {
+
+constexpr int kQ4Consumers = 4;                       // consumer warps per CTA
+constexpr int kQ4Threads = (kQ4Consumers + 1) * 32;
+constexpr int kQ4Stage = 128;                         // tokens per ring stage
+constexpr int kQ4MaxDepth = 4;
+constexpr int kQ4Early = 1024;                        // heads whose prefix a CTA keeps itself
+
+// Shared memory: ring, then joining buffer, then barriers, records, prefix.
+__host__ __device__ constexpr int q4_stage_bytes(int D) { return 2 * kQ4Stage * int4_row_bytes(D); }
+__host__ __device__ constexpr int q4_join_floats(int D, int G, int parts) {
+  return parts * G * (D + 4) + ((parts * G * 2 + 3) & ~3);
+}
+__host__ __device__ constexpr size_t q4_smem(int D, int G, int parts, int depth) {
+  return 128 + size_t(depth) * q4_stage_bytes(D) + size_t(q4_join_floats(D, G, parts)) * 4 +
+         kQ4MaxDepth * (16 + 16) + 16 + (2 * kQ4Early + 1 + 32) * 4;
+}
+
+template <typename T, int D, int NT, int HS, int MINB>
+__global__ void __launch_bounds__(kQ4Threads, MINB)
+    decode_int4_kernel(const __grid_constant__ CUtensorMap, const __grid_constant__ CUtensorMap,
+                       const __grid_constant__ DecodeParams p) {
+  constexpr int NG = D / kInt4Group;           // quantisation groups per row
+  constexpr int KS = D / 16;                   // k-steps of the scores, d-tiles of the output
+  constexpr int PARTS = kQ4Consumers / HS;     // token parts of a stage
+  constexpr int PT = kQ4Stage / PARTS;         // tokens per part
+  constexpr int MT = PT / 16;                  // 16-token tiles per warp and stage
+  constexpr int STAGE_BYTES = q4_stage_bytes(D), KV_BYTES = STAGE_BYTES / 2;
+  // fp16: probability x scale must stay below 65504 while scales reach
+  // 2 * 65504 / 15: the reference point lies kBelow under the maximum it was
+  // set to, a few binades above fp16's subnormals for small scales, and moves
+  // before 2^kRaise = 7.46 is passed.
+  constexpr bool kHalf = std::is_same<T, __half>::value;
+  constexpr float kBelow = kHalf ? 1.4f : 0.f, kRaise = kHalf ? 2.9f : 8.f;
+
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw_addr = smem_addr(smem_raw);
+  const uint32_t base = (raw_addr + 127u) & ~127u;
+  uint8_t* const smem = smem_raw + (base - raw_addr);
+  const int depth = p.depth, G = p.G, Hkv = p.Hkv, bs = p.bs;
+  float* const join = reinterpret_cast<float*>(smem + depth * STAGE_BYTES);
+  float* const join_ml = join + PARTS * G * (D + 4);
+  uint8_t* const tail = reinterpret_cast<uint8_t*>(join + q4_join_floats(D, G, PARTS));
+  const uint32_t full = smem_addr(tail), empty = full + kQ4MaxDepth * 8;
+  int4* const record = reinterpret_cast<int4*>(tail + kQ4MaxDepth * 16);
+  const uint32_t joined = full + kQ4MaxDepth * 32;  // consumers' own barrier
+  int* const cum_sm = reinterpret_cast<int*>(tail + kQ4MaxDepth * 32 + 16);
+  int* const len_sm = cum_sm + kQ4Early + 1;
+  int* const wsum = len_sm + kQ4Early;
+
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int n_heads = p.B * Hkv, cap = p.maxb * bs;
+  const int log2_bs = __ffs(bs) - 1;
+  auto head_len = [&](int hd) {
+    const int s = hd / Hkv, h = hd - s * Hkv;
+    const int L = p.lens[s * p.l_sb + h * p.l_sh];
+    return L < 0 ? 0 : (L > cap ? cap : L);
+  };
+  grid_launch_dependents();
+  if (tid == 0) {
+    for (int i = 0; i < depth; ++i) {
+      mbar_init(full + i * 8, 1);
+      mbar_init(empty + i * 8, kQ4Consumers);
+    }
+    mbar_init(joined, kQ4Consumers);
+    fence_mbar_init();
+  }
+  // The page-count prefix of all heads, computed by this CTA like the planner
+  // computes it for the reduce kernel (up to kQ4Early heads; more: the
+  // planner's).  The host launches the planner without programmatic
+  // dependence, so the lengths are final here.
+  const bool early = p.early != 0;
+  int total;
+  if (early) {
+    const int per = (n_heads + kQ4Threads - 1) / kQ4Threads;
+    const int h0 = min(tid * per, n_heads), h1 = min(h0 + per, n_heads);
+    int sum = 0;
+    for (int hd = h0; hd < h1; ++hd) {
+      const int L = head_len(hd);
+      len_sm[hd] = L;
+      sum += (L + bs - 1) >> log2_bs;
+    }
+    int x = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    if (lane == 31) wsum[warp] = x;
+    __syncthreads();
+    int run = x - sum;
+    for (int w = 0; w < warp; ++w) run += wsum[w];
+    for (int hd = h0; hd < h1; ++hd) {
+      cum_sm[hd] = run;
+      run += (len_sm[hd] + bs - 1) >> log2_bs;
+    }
+    if (tid == kQ4Threads - 1) cum_sm[n_heads] = run;
+    __syncthreads();
+    total = cum_sm[n_heads];
+  } else {
+    grid_dependency_wait();
+    total = p.cum[n_heads];
+    __syncthreads();
+  }
+  const int64_t units = (static_cast<int64_t>(total) + p.unit_pages - 1) / p.unit_pages;
+  const int W = static_cast<int>(units < p.total_warps ? units : p.total_warps);
+  const int u = blockIdx.x;
+  const int gs = u < W ? static_cast<int>(static_cast<int64_t>(u) * total / W) : 0;
+  const int ge = u < W ? static_cast<int>(static_cast<int64_t>(u + 1) * total / W) : 0;
+
+  if (warp == kQ4Consumers) {
+    // ------------------------------------------------------------ producer
+    const int log2_pps = 7 - log2_bs, pps = 1 << log2_pps;  // pages per stage (2..16)
+    const int pb = int4_row_bytes(D) << log2_bs;
+    const uint64_t policy = l2_policy_evict_first();
+    auto prefix = [&](int hd) { return early ? cum_sm[hd] : p.cum[hd]; };
+    bool bad_seen = false, timeout = false;
+    int issued = 0;
+    if (gs < ge) {
+      int head;
+      {  // largest head whose first page is <= gs
+        int lo = 0, hi = n_heads;
+        while (hi - lo > 1) {
+          const int step = (hi - lo + 31) / 32;
+          const int x = lo + lane * step;
+          const unsigned mask = __ballot_sync(0xffffffffu, x < hi && prefix(x) <= gs);
+          lo += (31 - __clz(mask)) * step;
+          hi = lo + step < hi ? lo + step : hi;
+        }
+        head = lo;
+      }
+      int c_lo = prefix(head), c_hi = prefix(head + 1), gp = gs;
+      int nx_head = 0, nx_lp = 0, nx_np = 0, nx_tok = 0, nx_flags = 0, nx_raw = 0;
+      int64_t nx_add = 0;
+      // The next stage of the range, its block-table entries on their way.
+      auto prepare = [&]() -> bool {
+        if (gp >= ge) return false;
+        while (gp >= c_hi) {
+          ++head;
+          c_lo = c_hi;
+          c_hi = prefix(head + 1);
+        }
+        const int s = head / Hkv, h = head - s * Hkv;
+        int np = pps;
+        if (c_hi - gp < np) np = c_hi - gp;
+        if (ge - gp < np) np = ge - gp;
+        nx_head = head;
+        nx_lp = gp - c_lo;
+        nx_np = np;
+        const int left = (early ? len_sm[head] : head_len(head)) - (nx_lp << log2_bs);
+        nx_tok = left < np << log2_bs ? left : np << log2_bs;
+        // 1: the head's first stage here, 2: its last, 4: the whole head is here
+        nx_flags = (gp == c_lo || gp == gs ? 1 : 0) | (gp + np == c_hi || gp + np == ge ? 2 : 0) |
+                   (c_lo >= gs && c_hi <= ge ? 4 : 0);
+        nx_add = static_cast<int64_t>(h) * p.bt_add;
+        if (lane < np)
+          nx_raw = p.bt[s * p.bt_sb + h * p.bt_sh + static_cast<int64_t>(nx_lp + lane) * p.bt_si];
+        gp += np;
+        return true;
+      };
+      bool more = prepare();
+      while (more) {
+        const int slot = issued % depth;
+        const int np = nx_np;
+        const int4 rec = make_int4(nx_head, nx_tok, nx_flags, 0);
+        const int64_t pid = static_cast<int64_t>(nx_raw) * p.bt_mul + nx_add;
+        const uint32_t bad = __ballot_sync(0xffffffffu, lane < np && (pid < 0 || pid >= p.num_pages));
+        more = prepare();
+        if (issued >= depth &&
+            !__all_sync(0xffffffffu, mbar_wait(empty + slot * 8, ((issued / depth) - 1) & 1, kWaitLimitNs))) {
+          timeout = true;
+          break;
+        }
+        uint8_t* const st = smem + slot * STAGE_BYTES;
+        if (bad) {
+          // A rejected page id has no copy: zeros (codes, scales and minima)
+          // stand in, written before the arrival that publishes the stage.
+          bad_seen = true;
+          for (int g = 0; g < np; ++g) {
+            if (!(bad >> g & 1u)) continue;
+            for (int i = lane; i < pb / 8; i += 32) {
+              const int half = pb / 16;
+              uint4* z = reinterpret_cast<uint4*>(st + (i < half ? 0 : KV_BYTES) + g * pb);
+              z[i < half ? i : i - half] = make_uint4(0u, 0u, 0u, 0u);
+            }
+          }
+          fence_proxy_async_smem();  // before the copies that refill this slot later
+          __syncwarp();
+        }
+        if (lane == 0) {
+          record[slot] = rec;
+          mbar_arrive_expect_tx(full + slot * 8, static_cast<uint32_t>(2 * pb * (np - __popc(bad))));
+        }
+        __syncwarp();
+        const int pg = lane & 15, kv = lane >> 4;
+        const int64_t src = __shfl_sync(0xffffffffu, pid, pg);
+        if (pg < np && !(bad >> pg & 1u))
+          bulk_load(base + slot * STAGE_BYTES + kv * KV_BYTES + pg * pb,
+                    (kv ? p.v_pages : p.k_pages) + src * pb, static_cast<uint32_t>(pb),
+                    full + slot * 8, policy);
+        ++issued;
+      }
+    }
+    // The end record, in a free slot.
+    bool ended = false;
+    if (!timeout) {
+      const int slot = issued % depth;
+      if (issued >= depth &&
+          !__all_sync(0xffffffffu, mbar_wait(empty + slot * 8, ((issued / depth) - 1) & 1, kWaitLimitNs))) {
+        timeout = true;
+      } else {
+        ended = true;
+        if (lane == 0) {
+          record[slot] = make_int4(-1, 0, 0, 0);
+          mbar_arrive(full + slot * 8);
+        }
+      }
+    }
+    // No copy of this CTA is in flight when it ends, whatever the consumers
+    // did (the end record's slot was waited for above).
+    for (int j = max(issued - depth + (ended ? 1 : 0), 0); j < issued; ++j)
+      mbar_wait(full + (j % depth) * 8, (j / depth) & 1, kWaitLimitNs);
+    grid_dependency_wait();  // the planner has reset the status word
+    if (lane == 0 && (bad_seen || timeout))
+      atomicOr(p.status, (bad_seen ? kStatusBadPage : 0u) | (timeout ? kStatusTimeout : 0u));
+    return;
+  }
+
+  // ------------------------------------------------------------- consumers
+  // Heads of length 0 get zeros (an empty state in state mode).
+  for (int hd = u * kQ4Consumers + warp; hd < n_heads; hd += gridDim.x * kQ4Consumers) {
+    if ((early ? len_sm[hd] : head_len(hd)) != 0) continue;
+    const int s = hd / Hkv, h = hd - s * Hkv;
+    for (int g = 0; g < G; ++g) {
+      const int64_t row = static_cast<int64_t>(s) * Hkv * G + h * G + g;
+      for (int c = lane * 4; c < D; c += 128) {
+        if (p.state_o)
+          *reinterpret_cast<float4*>(p.state_o + row * D + c) = make_float4(0.f, 0.f, 0.f, 0.f);
+        else
+          *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + s * p.o_sb + (h * G + g) * p.o_sh + c) =
+              make_uint2(0u, 0u);
+      }
+      if (p.state_o && lane == 0) p.state_lse[row] = -INFINITY;
+    }
+  }
+  const int lr = lane >> 2, lc = lane & 3;
+  const int part = warp / HS, g_lo = (warp % HS) * NT * 8;
+  const int tok0 = part * PT;                  // this warp's first token of a stage
+  const int page_bytes = int4_row_bytes(D) << log2_bs;
+  // Byte offset in a stage's K (or V) of 8-token tile t8: its codes, and this
+  // lane group's row of (scale, minimum) pairs.  A page holds whole tiles.
+  auto tile_codes = [&](int t8) {
+    return ((t8 * 8) >> log2_bs) * page_bytes + ((t8 * 8) & (bs - 1)) * (D / 2);
+  };
+  auto tile_pairs = [&](int t8) {
+    return ((t8 * 8) >> log2_bs) * page_bytes + bs * (D / 2) + (((t8 * 8) & (bs - 1)) + lr) * (NG * 4);
+  };
+
+  uint32_t qb[KS][NT][2];
+  float qsum[NT][NG][2];   // scale_log2 x sum of the query over a group, heads 2 lc + e
+  float qmul[NT][2];       // what a sum of (query x code) products is multiplied by
+  float acc[KS][NT][4], mid[NT][NG][2], m_ref[NT][2], l_sum[NT][2];
+
+  // The query group of head hd, as fp16 scaled by a power of two per head that
+  // brings its largest element to 2^10..2^11 (elements paired with the nibbles
+  // at bits 0..3 are 16 times larger), and a fresh state.
+  auto start_head = [&](int hd) {
+    const int s = hd / Hkv, h = hd - s * Hkv;
+    const T* qp = static_cast<const T*>(p.q) + s * p.q_sb + static_cast<int64_t>(h) * G * p.q_sh;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int g = g_lo + nt * 8 + lr;
+      uint32_t raw[KS][2];
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        raw[ks][0] = raw[ks][1] = 0u;
+        if (g < G) {
+          const T* row = qp + g * p.q_sh + (ks >> 2) * 64 + lc * 16 + (ks & 3) * 4;
+          raw[ks][0] = *reinterpret_cast<const uint32_t*>(row);
+          raw[ks][1] = *reinterpret_cast<const uint32_t*>(row + 2);
+        }
+      }
+      float big = 0.f, sum[NG];
+#pragma unroll
+      for (int gi = 0; gi < NG; ++gi) {
+        sum[gi] = 0.f;
+#pragma unroll
+        for (int ks = 4 * gi; ks < 4 * gi + 4; ++ks) {
+          const float2 a = unpack2<T>(raw[ks][0]), b = unpack2<T>(raw[ks][1]);
+          big = fmaxf(fmaxf(big, fmaxf(fabsf(a.x), fabsf(a.y))), fmaxf(fabsf(b.x), fabsf(b.y)));
+          sum[gi] += (a.x + a.y) + (b.x + b.y);
+        }
+        sum[gi] += __shfl_xor_sync(0xffffffffu, sum[gi], 1);
+        sum[gi] += __shfl_xor_sync(0xffffffffu, sum[gi], 2);
+      }
+      big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
+      big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+      // exponent of the largest element; 0 and non-finite elements: no scaling
+      int ex = static_cast<int>(__float_as_uint(big) >> 23) - 127;
+      if (big == 0.f || ex > 127) ex = 10;
+      if (ex < -110) ex = -110;
+      const float up = __uint_as_float(static_cast<uint32_t>(137 - ex) << 23);      // 2^(10 - ex)
+      // 2^(ex - 10) x 2^20 (the codes' weight), in two factors that stay normal
+      const float down = __uint_as_float(static_cast<uint32_t>(117 + ex > 0 ? 117 + ex : 1) << 23) * 1048576.f;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        const float2 a = unpack2<T>(raw[ks][0]), b = unpack2<T>(raw[ks][1]);
+        qb[ks][nt][0] = pack2<__half>(a.x * up * 16.f, a.y * up * 16.f);
+        qb[ks][nt][1] = pack2<__half>(b.x * up, b.y * up);
+      }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        qmul[nt][e] = __shfl_sync(0xffffffffu, down, lc * 8 + e * 4) * p.scale_log2;
+        m_ref[nt][e] = -INFINITY;
+        l_sum[nt][e] = 0.f;
+#pragma unroll
+        for (int gi = 0; gi < NG; ++gi) {
+          qsum[nt][gi][e] = __shfl_sync(0xffffffffu, sum[gi], lc * 8 + e * 4) * p.scale_log2;
+          mid[nt][gi][e] = 0.f;
+        }
+      }
+#pragma unroll
+      for (int dt = 0; dt < KS; ++dt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[dt][nt][i] = 0.f;
+    }
+  };
+
+  int joins = 0;
+  // Waits for the other consumers (their shared-memory writes are visible);
+  // false after the wait limit.
+  auto consumers_sync = [&]() -> bool {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(joined);
+    const bool ok = mbar_wait(joined, joins & 1, kWaitLimitNs);
+    ++joins;
+    return __all_sync(0xffffffffu, ok);
+  };
+  // Joins the parts' states of head hd and writes the output (whole) or the
+  // partial state of this CTA's range.
+  auto finish_head = [&](int hd, bool whole) -> bool {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float l = l_sum[nt][e];
+        l += __shfl_xor_sync(0xffffffffu, l, 4);
+        l += __shfl_xor_sync(0xffffffffu, l, 8);
+        l += __shfl_xor_sync(0xffffffffu, l, 16);
+        const int g = g_lo + nt * 8 + lc * 2 + e;
+        float* row = join + (part * G + g) * (D + 4) + lr * 8;
+#pragma unroll
+        for (int gi = 0; gi < NG; ++gi) {
+          float v = mid[nt][gi][e];
+          v += __shfl_xor_sync(0xffffffffu, v, 4);
+          v += __shfl_xor_sync(0xffffffffu, v, 8);
+          v += __shfl_xor_sync(0xffffffffu, v, 16);
+          // accumulator (tile 4 gi + m, register e + 2 j): element 64 gi + 8 lr + 2 m + j
+          if (g < G) {
+            *reinterpret_cast<float4*>(row + gi * 64) =
+                make_float4(acc[gi * 4][nt][e] + v, acc[gi * 4][nt][e + 2] + v,
+                            acc[gi * 4 + 1][nt][e] + v, acc[gi * 4 + 1][nt][e + 2] + v);
+            *reinterpret_cast<float4*>(row + gi * 64 + 4) =
+                make_float4(acc[gi * 4 + 2][nt][e] + v, acc[gi * 4 + 2][nt][e + 2] + v,
+                            acc[gi * 4 + 3][nt][e] + v, acc[gi * 4 + 3][nt][e + 2] + v);
+          }
+        }
+        if (lr == 0 && g < G) {
+          join_ml[(part * G + g) * 2] = m_ref[nt][e];
+          join_ml[(part * G + g) * 2 + 1] = l;
+        }
+      }
+    if (!consumers_sync()) return false;
+    const int s = hd / Hkv, h = hd - s * Hkv;
+    for (int idx = tid; idx < G * (D / 4); idx += kQ4Consumers * 32) {
+      const int g = idx / (D / 4), c = (idx - g * (D / 4)) * 4;
+      float M = -INFINITY, L = 0.f, wt[PARTS];
+#pragma unroll
+      for (int w = 0; w < PARTS; ++w) M = fmaxf(M, join_ml[(w * G + g) * 2]);
+      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < PARTS; ++w) {
+        wt[w] = fast_exp2(join_ml[(w * G + g) * 2] - M);
+        L += wt[w] * join_ml[(w * G + g) * 2 + 1];
+        const float4 a = *reinterpret_cast<const float4*>(join + (w * G + g) * (D + 4) + c);
+        o.x = fmaf(wt[w], a.x, o.x);
+        o.y = fmaf(wt[w], a.y, o.y);
+        o.z = fmaf(wt[w], a.z, o.z);
+        o.w = fmaf(wt[w], a.w, o.w);
+      }
+      if (whole) {
+        const float inv = 1.f / L;
+        const int64_t row = static_cast<int64_t>(s) * Hkv * G + h * G + g;
+        if (p.state_o) {
+          *reinterpret_cast<float4*>(p.state_o + row * D + c) =
+              make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+          if (c == 0) p.state_lse[row] = (M + __log2f(L)) * kLn2;
+        } else {
+          *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + s * p.o_sb + (h * G + g) * p.o_sh + c) =
+              make_uint2(pack2<T>(o.x * inv, o.y * inv), pack2<T>(o.z * inv, o.w * inv));
+        }
+      } else {
+        float* ps = p.part + static_cast<int64_t>(hd + u) * p.slot_floats;
+        __stcg(reinterpret_cast<float4*>(ps + g * D + c), o);
+        if (c == 0) {
+          __stcg(ps + G * D + g, M);
+          __stcg(ps + G * D + G + g, L);
+        }
+      }
+    }
+    return consumers_sync();
+  };
+
+  bool timeout = false;
+  for (int it = 0;; ++it) {
+    const int slot = it % depth;
+    if (!__all_sync(0xffffffffu, mbar_wait(full + slot * 8, (it / depth) & 1, kWaitLimitNs))) {
+      timeout = true;
+      break;
+    }
+    const int4 rec = record[slot];
+    if (rec.x < 0) break;
+    if (rec.z & 1) start_head(rec.x);
+    const int ntok = rec.y - tok0;  // this warp's valid tokens (may be <= 0 or > PT)
+    if (ntok > 0) {
+      const uint32_t kbase = base + slot * STAGE_BYTES, vbase = kbase + KV_BYTES;
+      // Scores in log2 units, lanes over (token row lr of an 8-token tile,
+      // heads 2 lc and 2 lc + 1).
+      float sc[MT][NT][4];
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        uint32_t wa[D / 32], wb[D / 32], ma[NG], mb[NG];
+        const int t8 = tok0 / 8 + 2 * mt;
+        ld_shared_words<D / 32>(kbase + tile_codes(t8) + lr * (D / 2) + lc * (D / 8), wa);
+        ld_shared_words<D / 32>(kbase + tile_codes(t8 + 1) + lr * (D / 2) + lc * (D / 8), wb);
+        ld_shared_words<NG>(kbase + tile_pairs(t8), ma);
+        ld_shared_words<NG>(kbase + tile_pairs(t8 + 1), mb);
+        float t[NT][4], z[NT][4];
+#pragma unroll
+        for (int gi = 0; gi < NG; ++gi) {
+          float sg[NT][4];
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sg[nt][i] = 0.f;
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            uint32_t ra[4], rb[4];
+            int4_key_pairs(wa[gi * 2 + j], ra);
+            int4_key_pairs(wb[gi * 2 + j], rb);
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf) {
+              const uint32_t a[4] = {ra[2 * hf], rb[2 * hf], ra[2 * hf + 1], rb[2 * hf + 1]};
+              const int ks = gi * 4 + j * 2 + hf;
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt)
+                mma_16816<__half>(sg[nt], a, qb[ks][nt][0], qb[ks][nt][1]);
+            }
+          }
+          const float2 fa = unpack2<T>(ma[gi]), fb = unpack2<T>(mb[gi]);  // scale, minimum
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float2 f = i < 2 ? fa : fb;
+              if (gi == 0) {
+                t[nt][i] = f.x * sg[nt][i];
+                z[nt][i] = f.y * qsum[nt][gi][i & 1];
+              } else {
+                t[nt][i] = fmaf(f.x, sg[nt][i], t[nt][i]);
+                z[nt][i] = fmaf(f.y, qsum[nt][gi][i & 1], z[nt][i]);
+              }
+            }
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) sc[mt][nt][i] = fmaf(t[nt][i], qmul[nt][i & 1], z[nt][i]);
+      }
+      const bool ragged = ntok < PT;
+      if (ragged) {
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (mt * 16 + lr + (i >> 1) * 8 >= ntok) sc[mt][nt][i] = -INFINITY;
+      }
+      // The reference point of the softmax.
+      float mx[NT][2];
+      bool up = false;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          mx[nt][e] = fmaxf(sc[0][nt][e], sc[0][nt][e + 2]);
+#pragma unroll
+          for (int mt = 1; mt < MT; ++mt)
+            mx[nt][e] = fmaxf(mx[nt][e], fmaxf(sc[mt][nt][e], sc[mt][nt][e + 2]));
+          up |= mx[nt][e] > m_ref[nt][e] + kRaise;
+        }
+      if (__any_sync(0xffffffffu, up)) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float m = mx[nt][e];
+            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
+            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+            m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+            const float mn = fmaxf(m_ref[nt][e], m - kBelow);
+            // no state yet (or no finite score): nothing to rescale
+            const float alpha = m_ref[nt][e] == -INFINITY ? 1.f : fast_exp2(m_ref[nt][e] - mn);
+            m_ref[nt][e] = mn;
+            l_sum[nt][e] *= alpha;
+#pragma unroll
+            for (int gi = 0; gi < NG; ++gi) mid[nt][gi][e] *= alpha;
+#pragma unroll
+            for (int dt = 0; dt < KS; ++dt) {
+              acc[dt][nt][e] *= alpha;
+              acc[dt][nt][e + 2] *= alpha;
+            }
+          }
+      }
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          // scores of -inf only: probabilities 0, not exp(-inf + inf)
+          const float m = m_ref[nt][e] == -INFINITY ? 0.f : m_ref[nt][e];
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int i = e; i < 4; i += 2) {
+              sc[mt][nt][i] = fast_exp2(sc[mt][nt][i] - m);
+              l_sum[nt][e] += sc[mt][nt][i];
+            }
+        }
+      // O^T += V^T P^T on the centred codes.
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        if (ragged && mt * 16 >= ntok) break;
+        uint32_t wa[D / 32], wb[D / 32], ma[NG], mb[NG];
+        const int t8 = tok0 / 8 + 2 * mt;
+        ld_shared_words<D / 32>(vbase + tile_codes(t8) + lane * (D / 8), wa);
+        ld_shared_words<D / 32>(vbase + tile_codes(t8 + 1) + lane * (D / 8), wb);
+        ld_shared_words<NG>(vbase + tile_pairs(t8), ma);
+        ld_shared_words<NG>(vbase + tile_pairs(t8 + 1), mb);
+        if (ragged) {  // rows past the end may hold anything: zero scales
+          const bool oka = mt * 16 + lr < ntok, okb = mt * 16 + 8 + lr < ntok;
+#pragma unroll
+          for (int gi = 0; gi < NG; ++gi) {
+            ma[gi] = oka ? ma[gi] : 0u;
+            mb[gi] = okb ? mb[gi] : 0u;
+          }
+        }
+#pragma unroll
+        for (int gi = 0; gi < NG; ++gi) {
+          const float2 fa = int4_centre<T>(ma[gi]), fb = int4_centre<T>(mb[gi]);
+          uint32_t pg[NT][2];
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            pg[nt][0] = movmatrix_trans(pack2<T>(sc[mt][nt][0] * fa.x, sc[mt][nt][1] * fa.x));
+            pg[nt][1] = movmatrix_trans(pack2<T>(sc[mt][nt][2] * fb.x, sc[mt][nt][3] * fb.x));
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+              mid[nt][gi][e] = fmaf(sc[mt][nt][e], fa.y, fmaf(sc[mt][nt][e + 2], fb.y, mid[nt][gi][e]));
+          }
+          uint32_t xa[4], ya[4], xb[4], yb[4];
+          // The octet's words of two consecutive tokens -> pairs (even token,
+          // odd token) of one element: even elements x, odd elements y.
+          int4_value_pairs<T>(__byte_perm(wa[gi], wa[NG + gi], 0x5410), xa);
+          int4_value_pairs<T>(__byte_perm(wa[gi], wa[NG + gi], 0x7632), ya);
+          int4_value_pairs<T>(__byte_perm(wb[gi], wb[NG + gi], 0x5410), xb);
+          int4_value_pairs<T>(__byte_perm(wb[gi], wb[NG + gi], 0x7632), yb);
+#pragma unroll
+          for (int m = 0; m < 4; ++m) {
+            const uint32_t a[4] = {xa[m], ya[m], xb[m], yb[m]};
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+              mma_16816<T>(acc[gi * 4 + m][nt], a, pg[nt][0], pg[nt][1]);
+          }
+        }
+      }
+    }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(empty + slot * 8);  // the slot may be refilled
+    if ((rec.z & 2) && !finish_head(rec.x, (rec.z & 4) != 0)) {
+      timeout = true;
+      break;
+    }
+  }
+  grid_dependency_wait();  // the reduce kernel follows the planner too
+  if (timeout && lane == 0) atomicOr(p.status, kStatusTimeout);
+}
+
+}  // namespace pab

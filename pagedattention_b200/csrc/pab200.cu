@@ -18,6 +18,7 @@
 #include <mutex>
 
 #include "host.h"
+#include "int4_decode.cuh"
 
 extern char** environ;  // the process environment (POSIX)
 
@@ -180,6 +181,7 @@ struct Plan {
   int n_heads;
   int slot_floats;
   int steal_m_max, steal_min_stages;
+  int unit_pages;  // fewest pages per range where there are enough
   size_t off_cum, off_wstart, off_claims, off_hseg, off_empty, off_part, ws_bytes;
 };
 
@@ -326,13 +328,68 @@ int choose_geometry(const KernelOps& ops, int dev, int depth, size_t stage, bool
   return PAB200_OK;
 }
 
+// CTAs of a 4-bit decode kernel that fit an SM with `smem` bytes each.
+int int4_ctas_per_sm(const KernelOps& ops, int dev, size_t smem, int* out) {
+  struct Entry {
+    int dev;
+    void* fn;
+    size_t smem;
+    int ctas;
+  };
+  static Entry cache[256];
+  static int used = 0;
+  static std::mutex mu;
+  std::lock_guard<std::mutex> lock(mu);
+  for (int i = 0; i < used; ++i)
+    if (cache[i].dev == dev && cache[i].fn == ops.fn && cache[i].smem == smem) {
+      *out = cache[i].ctas;
+      return PAB200_OK;
+    }
+  cudaError_t e = cudaFuncSetAttribute(ops.fn, cudaFuncAttributeMaxDynamicSharedMemorySize, 232448);
+  if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute");
+  int n = 0;
+  e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, ops.fn, pab::kQ4Threads, smem);
+  if (e != cudaSuccess) return cuda_fail(e, "cudaOccupancyMaxActiveBlocksPerMultiprocessor");
+  if (n < 1) return fail(PAB200_ERR_UNSUPPORTED, "decode kernel does not fit on an SM");
+  if (used < 256) cache[used++] = Entry{dev, ops.fn, smem, n};
+  *out = n;
+  return PAB200_OK;
+}
+
+// Workspace: a 256-byte header (status, weff, parity of the current call,
+// empty-head count, dynamic-tail header), then cum, wstart,
+// claim words, per-head segment ranges for two calls, the list of empty
+// heads and the partial slots (n_heads + W * (m_max + 1): one per (head,
+// segment) pair).  Under a scratch cap the tail chunk count per warp is
+// lowered until the workspace fits.
+void lay_out_workspace(Plan* pl, int m_max, size_t scratch_cap) {
+  for (;; --m_max) {
+    size_t off = 256;
+    pl->off_cum = off;
+    off = align256(off + size_t(pl->n_heads + 1) * 4);
+    pl->off_wstart = off;
+    off = align256(off + size_t(pl->W) * 4);
+    pl->off_claims = off;
+    off = align256(off + size_t(pl->W) * 8);
+    pl->off_hseg = off;
+    off = align256(off + size_t(pl->n_heads) * 16);
+    pl->off_empty = off;
+    off = align256(off + size_t(pl->n_heads) * 4);
+    pl->off_part = off;
+    off = align256(off + (size_t(pl->n_heads) + size_t(pl->W) * (m_max + 1)) * pl->slot_floats * 4);
+    pl->ws_bytes = off;
+    if (m_max == 0 || off <= scratch_cap) break;
+  }
+  pl->steal_m_max = m_max;
+}
+
 // Plans one call.  `scratch_cap`: largest workspace the call may use; the
 // tail-chunk count per warp (m_max) is lowered until the workspace fits it
 // (SIZE_MAX for a caller workspace, which is sized to the plan instead).
 int make_plan(const pab200_decode_args* a, Plan* pl, size_t scratch_cap,
-              bool check_pointers = true, bool int4 = false) {
+              bool check_pointers = true) {
   refresh_env();
-  int rc = validate(a, check_pointers, int4);
+  int rc = validate(a, check_pointers, false);
   if (rc) return rc;
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -341,7 +398,8 @@ int make_plan(const pab200_decode_args* a, Plan* pl, size_t scratch_cap,
   if (sms <= 0) return fail(PAB200_ERR_CUDA, "cannot query the SM count of device %d", dev);
 
   const int D = a->head_size, bs = a->block_size;
-  pl->int4 = int4;
+  pl->int4 = false;
+  pl->unit_pages = 1;
   pl->G = a->num_q_heads / a->num_kv_heads;
   pl->nt = pl->G <= 8 ? 1 : (pl->G <= 16 ? 2 : 4);
   // Groups of 17-32 query heads that one warp cannot hold (D = 128): two
@@ -353,8 +411,7 @@ int make_plan(const pab200_decode_args* a, Plan* pl, size_t scratch_cap,
   // tcgen05 path (PAB200_TC=1): groups of 9-32 query heads at D = 64, on
   // the 5th-generation tensor cores with TMEM accumulators; two warps per
   // ring, 64-token stages.
-  pl->tc = !int4 && pl->G > 8 && pl->G <= 32 && D == 64 && bs <= 64 &&
-           env_int("PAB200_TC", 0) != 0;
+  pl->tc = pl->G > 8 && pl->G <= 32 && D == 64 && bs <= 64 && env_int("PAB200_TC", 0) != 0;
   if (pl->tc) pl->pair = true;
   if (pl->pair) pl->nt = 2;
   // Tokens per ring stage: a power of two >= block_size.
@@ -362,23 +419,21 @@ int make_plan(const pab200_decode_args* a, Plan* pl, size_t scratch_cap,
   if ((pl->st != 16 && pl->st != 32 && pl->st != 64) || pl->st < bs)
     return fail(PAB200_ERR_INVALID_ARGUMENT, "PAB200_ST must be 16, 32 or 64 and >= block_size");
   const int nh = D / 64;
-  if (!int4 && 2 * (pl->st / bs) * nh > 32)
+  if (2 * (pl->st / bs) * nh > 32)
     return fail(PAB200_ERR_UNSUPPORTED, "block_size %d with head_size %d needs > 32 copies per stage", bs, D);
   // Arithmetic: tensor-core MMA by default; the CUDA-core variant
   // (PAB200_CORE=1) exists for query groups of at most 4 heads, 32-token
   // stages and D <= 128.
-  pl->core = !int4 && env_int("PAB200_CORE", 0) != 0 && pl->G <= pab::kCoreMaxG && pl->st == 32 && D <= 128;
+  pl->core = env_int("PAB200_CORE", 0) != 0 && pl->G <= pab::kCoreMaxG && pl->st == 32 && D <= 128;
   if (pl->tc) pl->core = false;
-  if (int4 ? !pabh::select_int4_kernel(a->dtype, D, pl->nt, pl->st, pl->pair, &pl->ops)
-           : !select_kernel(a->dtype, D, pl->nt, pl->st, pl->core, pl->pair, pl->tc, &pl->ops))
+  if (!select_kernel(a->dtype, D, pl->nt, pl->st, pl->core, pl->pair, pl->tc, &pl->ops))
     return fail(PAB200_ERR_UNSUPPORTED, "no kernel for head_size %d, group %d", D, pl->G);
 
   // Each warp owns a private ring of `depth` stages.  Throughput grows with
   // resident warps (each warp's stage loop is latency-bound), so the default
   // is a 2-deep ring and as many warps as ~200 KB of shared memory per SM
   // holds (6 warps at 16 KiB stages).
-  const size_t stage =  // K + V bytes of one stage
-      int4 ? size_t(2) * pl->st * pab::int4_row_bytes(D) : size_t(4) * pl->st * D;
+  const size_t stage = size_t(4) * pl->st * D;  // K + V bytes of one stage
   // The tcgen05 path computes the scores of the next stage while the warps
   // work on the current one, so it needs a third stage in flight.
   int depth = env_int("PAB200_DEPTH", pl->tc ? 3 : 2);
@@ -405,33 +460,56 @@ int make_plan(const pab200_decode_args* a, Plan* pl, size_t scratch_cap,
   pl->grid = (W + upc - 1) / upc;
   // Partial-state slot: acc [G][D], m [G], l [G].
   pl->slot_floats = (pl->G * D + 2 * pl->G + 3) & ~3;
-  // Workspace: a 256-byte header (status, weff, parity of the current call,
-  // empty-head count, dynamic-tail header), then cum, wstart,
-  // claim words, per-head segment ranges for two calls, the list of empty
-  // heads and the partial slots (n_heads + W * (m_max + 1): one per (head,
-  // segment) pair).  Under a scratch cap the tail chunk count per warp is
-  // lowered until the workspace fits.
   int m_max = env_int("PAB200_STEAL_M", 4);
   if (m_max < 0) m_max = 0;
-  for (;; --m_max) {
-    size_t off = 256;
-    pl->off_cum = off;
-    off = align256(off + size_t(pl->n_heads + 1) * 4);
-    pl->off_wstart = off;
-    off = align256(off + size_t(W) * 4);
-    pl->off_claims = off;
-    off = align256(off + size_t(W) * 8);
-    pl->off_hseg = off;
-    off = align256(off + size_t(pl->n_heads) * 16);
-    pl->off_empty = off;
-    off = align256(off + size_t(pl->n_heads) * 4);
-    pl->off_part = off;
-    off = align256(off + (size_t(pl->n_heads) + size_t(W) * (m_max + 1)) * pl->slot_floats * 4);
-    pl->ws_bytes = off;
-    if (m_max == 0 || off <= scratch_cap) break;
-  }
-  pl->steal_m_max = m_max;
+  lay_out_workspace(pl, m_max, scratch_cap);
   pl->steal_min_stages = env_int("PAB200_STEAL_MIN_STAGES", 4);
+  return PAB200_OK;
+}
+
+// Plans one call over 4-bit pages: one range of pages per resident CTA, fixed
+// when the call is planned (no tail chunks: the ranges are a few stages to a
+// few hundred long and one CTA's five warps share each).
+int make_plan_int4(const pab200_decode_args* a, Plan* pl) {
+  refresh_env();
+  int rc = validate(a, true, true);
+  if (rc) return rc;
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return cuda_fail(e, "cudaGetDevice");
+  const int sms = device_sm_count(dev);
+  if (sms <= 0) return fail(PAB200_ERR_CUDA, "cannot query the SM count of device %d", dev);
+  const int D = a->head_size;
+  *pl = Plan{};
+  pl->int4 = true;
+  pl->G = a->num_q_heads / a->num_kv_heads;
+  pabh::Int4Kernel k;
+  if (!pabh::select_int4_kernel(a->dtype, D, pl->G, &k))
+    return fail(PAB200_ERR_UNSUPPORTED, "no kernel for head_size %d, group %d", D, pl->G);
+  pl->ops = k.ops;
+  pl->st = pab::kQ4Stage;
+  pl->wpc = pab::kQ4Threads / 32;
+  // The deepest ring (2 to 4 stages) that leaves room for the CTAs per SM the
+  // registers allow.
+  constexpr size_t kSmemPerSm = 228 * 1024, kReserved = 1024;
+  int depth = pab::kQ4MaxDepth;
+  while (depth > 2 &&
+         k.min_ctas * (pab::q4_smem(D, pl->G, k.parts, depth) + kReserved) > kSmemPerSm)
+    --depth;
+  pl->depth = depth;
+  pl->smem = pab::q4_smem(D, pl->G, k.parts, depth);
+  if ((rc = int4_ctas_per_sm(k.ops, dev, pl->smem, &pl->ctas_per_sm))) return rc;
+  pl->n_heads = a->num_seqs * a->num_kv_heads;
+  int W = sms * pl->ctas_per_sm;
+  if (a->num_splits > 1) {
+    const int64_t cap = int64_t(pl->n_heads) * a->num_splits;
+    if (cap < W) W = static_cast<int>(cap);
+  }
+  pl->W = pl->grid = W;
+  pl->unit_pages = pab::kQ4Stage / a->block_size;
+  pl->slot_floats = (pl->G * D + 2 * pl->G + 3) & ~3;
+  lay_out_workspace(pl, 0, SIZE_MAX);
+  pl->steal_min_stages = 1;
   return PAB200_OK;
 }
 
@@ -644,6 +722,7 @@ int decode_impl(const pab200_decode_args* a, const Plan& pl, const pab::AppendPa
   p.empty = reinterpret_cast<int32_t*>(ws + pl.off_empty);
   p.steal_m_max = pl.steal_m_max;
   p.steal_pps = pl.st / a->block_size;
+  p.unit_pages = pl.unit_pages;
   p.steal_min_stages = pl.steal_min_stages;
   p.cum = reinterpret_cast<int32_t*>(ws + pl.off_cum);
   p.wstart = reinterpret_cast<int32_t*>(ws + pl.off_wstart);
@@ -656,6 +735,7 @@ int decode_impl(const pab200_decode_args* a, const Plan& pl, const pab::AppendPa
   // append (the planner writes the lengths and the cache the decode reads)
   // nor with mma.sync warp pairs, and only while the prefix fits shared
   // memory (the tcgen05 path keeps it in its operand tiles).
+  static_assert(pab::kQ4Early == pab::kEarlyMaxHeads, "one bound for both decode kernels");
   p.early = !app && (!pl.pair || pl.tc) && pl.n_heads <= pab::kEarlyMaxHeads &&
             env_int("PAB200_EARLY", 1) != 0;
   if (app) {
@@ -732,14 +812,14 @@ int pabh::decode_after(const pab200_decode_args* a, void* workspace, size_t work
 // ------------------------------------------------------------- 4-bit pages
 PAB200_EXPORT size_t pab200_decode_int4_workspace_size(const pab200_decode_args* args) {
   Plan pl;
-  if (make_plan(args, &pl, SIZE_MAX, true, true) != PAB200_OK) return 0;
+  if (make_plan_int4(args, &pl) != PAB200_OK) return 0;
   return pl.ws_bytes;
 }
 
 PAB200_EXPORT int pab200_decode_int4(const pab200_decode_args* a, void* workspace,
                                      size_t workspace_bytes, void* stream) {
   Plan pl;
-  const int rc = make_plan(a, &pl, SIZE_MAX, true, true);
+  const int rc = make_plan_int4(a, &pl);
   if (rc) return rc;
   return decode_impl(a, pl, nullptr, workspace, workspace_bytes, stream, nullptr, 0, true);
 }
