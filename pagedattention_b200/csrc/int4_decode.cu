@@ -21,7 +21,7 @@ bool select(int D, int G, pabh::Int4Kernel* o) {
   switch (D * 16 + nt) {
     case 64 * 16 + 1: take<T, 64, 1, 1, 4>(o); return true;
     case 64 * 16 + 2: take<T, 64, 2, 1, 3>(o); return true;
-    case 64 * 16 + 4: take<T, 64, 4, 1, 2>(o); return G <= 32;
+    case 64 * 16 + 4: take<T, 64, 2, 2, 3>(o); return G <= 32;   // 16 heads per warp pair
     case 128 * 16 + 1: take<T, 128, 1, 1, 3>(o); return true;
     case 128 * 16 + 2: take<T, 128, 2, 1, 2>(o); return true;
     case 128 * 16 + 4: take<T, 128, 2, 2, 2>(o); return G <= 32;  // 16 heads per warp pair

@@ -57,8 +57,8 @@ __global__ void __launch_bounds__(kQ4Threads, MINB)
   constexpr int NG = D / kInt4Group;           // quantisation groups per row
   constexpr int KS = D / 16;                   // k-steps of the scores, d-tiles of the output
   constexpr int PARTS = kQ4Consumers / HS;     // token parts of a stage
-  constexpr int PT = kQ4Stage / PARTS;         // tokens per part
-  constexpr int MT = PT / 16;                  // 16-token tiles per warp and stage
+  constexpr int PT = kQ4Stage / PARTS;         // tokens per part, in chunks of 32
+  constexpr int MT = 2;                        // 16-token tiles per chunk
   constexpr int STAGE_BYTES = q4_stage_bytes(D), KV_BYTES = STAGE_BYTES / 2;
   // fp16: probability x scale must stay below 65504 while scales reach
   // 2 * 65504 / 15: the reference point lies kBelow under the maximum it was
@@ -149,7 +149,8 @@ __global__ void __launch_bounds__(kQ4Threads, MINB)
     const uint64_t policy = l2_policy_evict_first();
     auto prefix = [&](int hd) { return early ? cum_sm[hd] : p.cum[hd]; };
     bool bad_seen = false, timeout = false;
-    int issued = 0;
+    int issued = 0, slot = 0;
+    uint32_t phase = 1;  // of `empty`: the first round finds every slot free
     if (gs < ge) {
       int head;
       {  // largest head whose first page is <= gs
@@ -194,14 +195,12 @@ __global__ void __launch_bounds__(kQ4Threads, MINB)
       };
       bool more = prepare();
       while (more) {
-        const int slot = issued % depth;
         const int np = nx_np;
         const int4 rec = make_int4(nx_head, nx_tok, nx_flags, 0);
         const int64_t pid = static_cast<int64_t>(nx_raw) * p.bt_mul + nx_add;
         const uint32_t bad = __ballot_sync(0xffffffffu, lane < np && (pid < 0 || pid >= p.num_pages));
         more = prepare();
-        if (issued >= depth &&
-            !__all_sync(0xffffffffu, mbar_wait(empty + slot * 8, ((issued / depth) - 1) & 1, kWaitLimitNs))) {
+        if (!__all_sync(0xffffffffu, mbar_wait(empty + slot * 8, phase, kWaitLimitNs))) {
           timeout = true;
           break;
         }
@@ -233,14 +232,16 @@ __global__ void __launch_bounds__(kQ4Threads, MINB)
                     (kv ? p.v_pages : p.k_pages) + src * pb, static_cast<uint32_t>(pb),
                     full + slot * 8, policy);
         ++issued;
+        if (++slot == depth) {
+          slot = 0;
+          phase ^= 1;
+        }
       }
     }
     // The end record, in a free slot.
     bool ended = false;
     if (!timeout) {
-      const int slot = issued % depth;
-      if (issued >= depth &&
-          !__all_sync(0xffffffffu, mbar_wait(empty + slot * 8, ((issued / depth) - 1) & 1, kWaitLimitNs))) {
+      if (!__all_sync(0xffffffffu, mbar_wait(empty + slot * 8, phase, kWaitLimitNs))) {
         timeout = true;
       } else {
         ended = true;
@@ -280,15 +281,18 @@ __global__ void __launch_bounds__(kQ4Threads, MINB)
   const int lr = lane >> 2, lc = lane & 3;
   const int part = warp / HS, g_lo = (warp % HS) * NT * 8;
   const int tok0 = part * PT;                  // this warp's first token of a stage
-  const int page_bytes = int4_row_bytes(D) << log2_bs;
-  // Byte offset in a stage's K (or V) of 8-token tile t8: its codes, and this
-  // lane group's row of (scale, minimum) pairs.  A page holds whole tiles.
-  auto tile_codes = [&](int t8) {
-    return ((t8 * 8) >> log2_bs) * page_bytes + ((t8 * 8) & (bs - 1)) * (D / 2);
-  };
-  auto tile_pairs = [&](int t8) {
-    return ((t8 * 8) >> log2_bs) * page_bytes + bs * (D / 2) + (((t8 * 8) & (bs - 1)) + lr) * (NG * 4);
-  };
+  // Shared addresses, in slot 0's K, of this lane's codes of the part's 8-token
+  // tiles (a page holds whole tiles; keys and values place lanes alike), and of
+  // row lr of their (scale, minimum) pairs.
+  constexpr int TILES = PT / 8;
+  uint32_t code_at[TILES], pair_at[TILES];
+#pragma unroll
+  for (int i = 0; i < TILES; ++i) {
+    const int t = tok0 + i * 8;
+    const uint32_t page = base + (t >> log2_bs) * (int4_row_bytes(D) << log2_bs);
+    code_at[i] = page + (t & (bs - 1)) * (D / 2) + lane * (D / 8);
+    pair_at[i] = page + bs * (D / 2) + ((t & (bs - 1)) + lr) * (NG * 4);
+  }
 
   uint32_t qb[KS][NT][2];
   float qsum[NT][NG][2];   // scale_log2 x sum of the query over a group, heads 2 lc + e
@@ -446,29 +450,30 @@ __global__ void __launch_bounds__(kQ4Threads, MINB)
   };
 
   bool timeout = false;
-  for (int it = 0;; ++it) {
-    const int slot = it % depth;
-    if (!__all_sync(0xffffffffu, mbar_wait(full + slot * 8, (it / depth) & 1, kWaitLimitNs))) {
+  uint32_t phase = 0, slot_off = 0;
+  for (int slot = 0;;) {
+    if (!__all_sync(0xffffffffu, mbar_wait(full + slot * 8, phase, kWaitLimitNs))) {
       timeout = true;
       break;
     }
     const int4 rec = record[slot];
     if (rec.x < 0) break;
     if (rec.z & 1) start_head(rec.x);
-    const int ntok = rec.y - tok0;  // this warp's valid tokens (may be <= 0 or > PT)
-    if (ntok > 0) {
-      const uint32_t kbase = base + slot * STAGE_BYTES, vbase = kbase + KV_BYTES;
+#pragma unroll
+    for (int ch = 0; ch < PT / 32; ++ch) {
+      const int ntok = rec.y - tok0 - ch * 32;  // valid tokens from here (may be <= 0 or > 32)
+      if (ntok <= 0) break;
       // Scores in log2 units, lanes over (token row lr of an 8-token tile,
       // heads 2 lc and 2 lc + 1).
       float sc[MT][NT][4];
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
         uint32_t wa[D / 32], wb[D / 32], ma[NG], mb[NG];
-        const int t8 = tok0 / 8 + 2 * mt;
-        ld_shared_words<D / 32>(kbase + tile_codes(t8) + lr * (D / 2) + lc * (D / 8), wa);
-        ld_shared_words<D / 32>(kbase + tile_codes(t8 + 1) + lr * (D / 2) + lc * (D / 8), wb);
-        ld_shared_words<NG>(kbase + tile_pairs(t8), ma);
-        ld_shared_words<NG>(kbase + tile_pairs(t8 + 1), mb);
+        const int t8 = ch * 4 + 2 * mt;
+        ld_shared_words<D / 32>(code_at[t8] + slot_off, wa);
+        ld_shared_words<D / 32>(code_at[t8 + 1] + slot_off, wb);
+        ld_shared_words<NG>(pair_at[t8] + slot_off, ma);
+        ld_shared_words<NG>(pair_at[t8 + 1] + slot_off, mb);
         float t[NT][4], z[NT][4];
 #pragma unroll
         for (int gi = 0; gi < NG; ++gi) {
@@ -511,7 +516,7 @@ __global__ void __launch_bounds__(kQ4Threads, MINB)
 #pragma unroll
           for (int i = 0; i < 4; ++i) sc[mt][nt][i] = fmaf(t[nt][i], qmul[nt][i & 1], z[nt][i]);
       }
-      const bool ragged = ntok < PT;
+      const bool ragged = ntok < 32;
       if (ragged) {
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
@@ -576,11 +581,11 @@ __global__ void __launch_bounds__(kQ4Threads, MINB)
       for (int mt = 0; mt < MT; ++mt) {
         if (ragged && mt * 16 >= ntok) break;
         uint32_t wa[D / 32], wb[D / 32], ma[NG], mb[NG];
-        const int t8 = tok0 / 8 + 2 * mt;
-        ld_shared_words<D / 32>(vbase + tile_codes(t8) + lane * (D / 8), wa);
-        ld_shared_words<D / 32>(vbase + tile_codes(t8 + 1) + lane * (D / 8), wb);
-        ld_shared_words<NG>(vbase + tile_pairs(t8), ma);
-        ld_shared_words<NG>(vbase + tile_pairs(t8 + 1), mb);
+        const int t8 = ch * 4 + 2 * mt;
+        ld_shared_words<D / 32>(code_at[t8] + slot_off + KV_BYTES, wa);
+        ld_shared_words<D / 32>(code_at[t8 + 1] + slot_off + KV_BYTES, wb);
+        ld_shared_words<NG>(pair_at[t8] + slot_off + KV_BYTES, ma);
+        ld_shared_words<NG>(pair_at[t8 + 1] + slot_off + KV_BYTES, mb);
         if (ragged) {  // rows past the end may hold anything: zero scales
           const bool oka = mt * 16 + lr < ntok, okb = mt * 16 + 8 + lr < ntok;
 #pragma unroll
@@ -620,6 +625,12 @@ __global__ void __launch_bounds__(kQ4Threads, MINB)
     }
     __syncwarp();
     if (lane == 0) mbar_arrive(empty + slot * 8);  // the slot may be refilled
+    slot_off += STAGE_BYTES;
+    if (++slot == depth) {
+      slot = 0;
+      slot_off = 0;
+      phase ^= 1;
+    }
     if ((rec.z & 2) && !finish_head(rec.x, (rec.z & 4) != 0)) {
       timeout = true;
       break;
