@@ -66,6 +66,9 @@ __global__ void __launch_bounds__(kQ4Threads, MINB)
   // before 2^kRaise = 7.46 is passed.
   constexpr bool kHalf = std::is_same<T, __half>::value;
   constexpr float kBelow = kHalf ? 1.4f : 0.f, kRaise = kHalf ? 2.9f : 8.f;
+  // Reference point of an empty state: below every score, and finite, so that
+  // a score of -inf has probability 0.
+  constexpr float kNoScore = -3e38f;
 
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_addr = smem_addr(smem_raw);
@@ -167,29 +170,39 @@ __global__ void __launch_bounds__(kQ4Threads, MINB)
       int c_lo = prefix(head), c_hi = prefix(head + 1), gp = gs;
       int nx_head = 0, nx_lp = 0, nx_np = 0, nx_tok = 0, nx_flags = 0, nx_raw = 0;
       int64_t nx_add = 0;
+      const int32_t* c_bt = p.bt;
+      int c_h = 0, c_len = 0;
+      auto enter_head = [&]() {
+        const int s = head / Hkv;
+        c_h = head - s * Hkv;
+        c_bt = p.bt + s * p.bt_sb + c_h * p.bt_sh;
+        c_len = early ? len_sm[head] : head_len(head);
+      };
+      enter_head();
       // The next stage of the range, its block-table entries on their way.
       auto prepare = [&]() -> bool {
         if (gp >= ge) return false;
-        while (gp >= c_hi) {
-          ++head;
-          c_lo = c_hi;
-          c_hi = prefix(head + 1);
+        if (gp >= c_hi) {
+          do {
+            ++head;
+            c_lo = c_hi;
+            c_hi = prefix(head + 1);
+          } while (gp >= c_hi);
+          enter_head();
         }
-        const int s = head / Hkv, h = head - s * Hkv;
         int np = pps;
         if (c_hi - gp < np) np = c_hi - gp;
         if (ge - gp < np) np = ge - gp;
         nx_head = head;
         nx_lp = gp - c_lo;
         nx_np = np;
-        const int left = (early ? len_sm[head] : head_len(head)) - (nx_lp << log2_bs);
+        const int left = c_len - (nx_lp << log2_bs);
         nx_tok = left < np << log2_bs ? left : np << log2_bs;
         // 1: the head's first stage here, 2: its last, 4: the whole head is here
         nx_flags = (gp == c_lo || gp == gs ? 1 : 0) | (gp + np == c_hi || gp + np == ge ? 2 : 0) |
                    (c_lo >= gs && c_hi <= ge ? 4 : 0);
-        nx_add = static_cast<int64_t>(h) * p.bt_add;
-        if (lane < np)
-          nx_raw = p.bt[s * p.bt_sb + h * p.bt_sh + static_cast<int64_t>(nx_lp + lane) * p.bt_si];
+        nx_add = static_cast<int64_t>(c_h) * p.bt_add;
+        if (lane < np) nx_raw = c_bt[static_cast<int64_t>(nx_lp + lane) * p.bt_si];
         gp += np;
         return true;
       };
@@ -281,18 +294,19 @@ __global__ void __launch_bounds__(kQ4Threads, MINB)
   const int lr = lane >> 2, lc = lane & 3;
   const int part = warp / HS, g_lo = (warp % HS) * NT * 8;
   const int tok0 = part * PT;                  // this warp's first token of a stage
-  // Shared addresses, in slot 0's K, of this lane's codes of the part's 8-token
-  // tiles (a page holds whole tiles; keys and values place lanes alike), and of
-  // row lr of their (scale, minimum) pairs.
-  constexpr int TILES = PT / 8;
-  uint32_t code_at[TILES], pair_at[TILES];
-#pragma unroll
-  for (int i = 0; i < TILES; ++i) {
-    const int t = tok0 + i * 8;
-    const uint32_t page = base + (t >> log2_bs) * (int4_row_bytes(D) << log2_bs);
-    code_at[i] = page + (t & (bs - 1)) * (D / 2) + lane * (D / 8);
-    pair_at[i] = page + bs * (D / 2) + ((t & (bs - 1)) + lr) * (NG * 4);
-  }
+  // Byte offsets of an 8-token tile's codes and (scale, minimum) pairs from the
+  // part's first: a page holds whole tiles, and a part begins with a page or
+  // with half of one.  Keys and values place lanes alike.
+  const int page_bytes = int4_row_bytes(D) << log2_bs;
+  auto code_off = [&](int t8) {
+    return ((t8 * 8) >> log2_bs) * page_bytes + ((t8 * 8) & (bs - 1)) * (D / 2);
+  };
+  auto pair_off = [&](int t8) {
+    return ((t8 * 8) >> log2_bs) * page_bytes + ((t8 * 8) & (bs - 1)) * (NG * 4);
+  };
+  const uint32_t part_base = base + (tok0 >> log2_bs) * page_bytes;
+  uint32_t code_at = part_base + (tok0 & (bs - 1)) * (D / 2) + lane * (D / 8);
+  uint32_t pair_at = part_base + bs * (D / 2) + ((tok0 & (bs - 1)) + lr) * (NG * 4);
 
   uint32_t qb[KS][NT][2];
   float qsum[NT][NG][2];   // scale_log2 x sum of the query over a group, heads 2 lc + e
@@ -349,7 +363,7 @@ __global__ void __launch_bounds__(kQ4Threads, MINB)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         qmul[nt][e] = __shfl_sync(0xffffffffu, down, lc * 8 + e * 4) * p.scale_log2;
-        m_ref[nt][e] = -INFINITY;
+        m_ref[nt][e] = kNoScore;
         l_sum[nt][e] = 0.f;
 #pragma unroll
         for (int gi = 0; gi < NG; ++gi) {
@@ -450,7 +464,7 @@ __global__ void __launch_bounds__(kQ4Threads, MINB)
   };
 
   bool timeout = false;
-  uint32_t phase = 0, slot_off = 0;
+  uint32_t phase = 0;
   for (int slot = 0;;) {
     if (!__all_sync(0xffffffffu, mbar_wait(full + slot * 8, phase, kWaitLimitNs))) {
       timeout = true;
@@ -470,10 +484,10 @@ __global__ void __launch_bounds__(kQ4Threads, MINB)
       for (int mt = 0; mt < MT; ++mt) {
         uint32_t wa[D / 32], wb[D / 32], ma[NG], mb[NG];
         const int t8 = ch * 4 + 2 * mt;
-        ld_shared_words<D / 32>(code_at[t8] + slot_off, wa);
-        ld_shared_words<D / 32>(code_at[t8 + 1] + slot_off, wb);
-        ld_shared_words<NG>(pair_at[t8] + slot_off, ma);
-        ld_shared_words<NG>(pair_at[t8 + 1] + slot_off, mb);
+        ld_shared_words<D / 32>(code_at + code_off(t8), wa);
+        ld_shared_words<D / 32>(code_at + code_off(t8 + 1), wb);
+        ld_shared_words<NG>(pair_at + pair_off(t8), ma);
+        ld_shared_words<NG>(pair_at + pair_off(t8 + 1), mb);
         float t[NT][4], z[NT][4];
 #pragma unroll
         for (int gi = 0; gi < NG; ++gi) {
@@ -549,8 +563,7 @@ __global__ void __launch_bounds__(kQ4Threads, MINB)
             m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
             m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
             const float mn = fmaxf(m_ref[nt][e], m - kBelow);
-            // no state yet (or no finite score): nothing to rescale
-            const float alpha = m_ref[nt][e] == -INFINITY ? 1.f : fast_exp2(m_ref[nt][e] - mn);
+            const float alpha = fast_exp2(m_ref[nt][e] - mn);
             m_ref[nt][e] = mn;
             l_sum[nt][e] *= alpha;
 #pragma unroll
@@ -566,13 +579,11 @@ __global__ void __launch_bounds__(kQ4Threads, MINB)
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          // scores of -inf only: probabilities 0, not exp(-inf + inf)
-          const float m = m_ref[nt][e] == -INFINITY ? 0.f : m_ref[nt][e];
 #pragma unroll
           for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
             for (int i = e; i < 4; i += 2) {
-              sc[mt][nt][i] = fast_exp2(sc[mt][nt][i] - m);
+              sc[mt][nt][i] = fast_exp2(sc[mt][nt][i] - m_ref[nt][e]);
               l_sum[nt][e] += sc[mt][nt][i];
             }
         }
@@ -582,10 +593,10 @@ __global__ void __launch_bounds__(kQ4Threads, MINB)
         if (ragged && mt * 16 >= ntok) break;
         uint32_t wa[D / 32], wb[D / 32], ma[NG], mb[NG];
         const int t8 = ch * 4 + 2 * mt;
-        ld_shared_words<D / 32>(code_at[t8] + slot_off + KV_BYTES, wa);
-        ld_shared_words<D / 32>(code_at[t8 + 1] + slot_off + KV_BYTES, wb);
-        ld_shared_words<NG>(pair_at[t8] + slot_off + KV_BYTES, ma);
-        ld_shared_words<NG>(pair_at[t8 + 1] + slot_off + KV_BYTES, mb);
+        ld_shared_words<D / 32>(code_at + KV_BYTES + code_off(t8), wa);
+        ld_shared_words<D / 32>(code_at + KV_BYTES + code_off(t8 + 1), wb);
+        ld_shared_words<NG>(pair_at + KV_BYTES + pair_off(t8), ma);
+        ld_shared_words<NG>(pair_at + KV_BYTES + pair_off(t8 + 1), mb);
         if (ragged) {  // rows past the end may hold anything: zero scales
           const bool oka = mt * 16 + lr < ntok, okb = mt * 16 + 8 + lr < ntok;
 #pragma unroll
@@ -625,11 +636,13 @@ __global__ void __launch_bounds__(kQ4Threads, MINB)
     }
     __syncwarp();
     if (lane == 0) mbar_arrive(empty + slot * 8);  // the slot may be refilled
-    slot_off += STAGE_BYTES;
+    code_at += STAGE_BYTES;
+    pair_at += STAGE_BYTES;
     if (++slot == depth) {
       slot = 0;
-      slot_off = 0;
       phase ^= 1;
+      code_at -= depth * STAGE_BYTES;
+      pair_at -= depth * STAGE_BYTES;
     }
     if ((rec.z & 2) && !finish_head(rec.x, (rec.z & 4) != 0)) {
       timeout = true;
