@@ -413,10 +413,11 @@ int pab200_kv_append_int4(const pab200_int4_rows_args* args, int32_t increment, 
 /* Read rows back: k_rows / v_rows token j of sequence s becomes lo + s * c,
  * rounded to dtype (saturating), of position starts[s * starts_stride] + j (starts null: j);
  * zeros at positions outside [0, seqlens(s, h)) and on pages out of range.
- * Rows outside every [cu[s], cu[s+1]) are left as they are.  k_rows and v_rows
- * 16-byte aligned, strides multiples of 8. */
+ * Rows before cu[0] and from cu[num_seqs] on become zeros with `zero_rest` and
+ * are left as they are without.  k_rows and v_rows 16-byte aligned, strides
+ * multiples of 8. */
 int pab200_kv_read_int4(const pab200_int4_rows_args* args, const int32_t* starts,
-                        int64_t starts_stride, void* stream);
+                        int64_t starts_stride, int32_t zero_rest, void* stream);
 
 /* Decode over 4-bit caches: pab200_decode() with k_cache / v_cache holding
  * 4-bit pages whose scales have q's type, layout PAGES.  The attention is that

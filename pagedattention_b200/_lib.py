@@ -257,7 +257,7 @@ def load() -> ctypes.CDLL:
     for name, res, args in (
             ("pab200_int4_page_bytes", Z, [I32, I32]),
             ("pab200_kv_append_int4", ctypes.c_int, [R, I32, V]),
-            ("pab200_kv_read_int4", ctypes.c_int, [R, V, I64, V]),
+            ("pab200_kv_read_int4", ctypes.c_int, [R, V, I64, I32, V]),
             ("pab200_decode_int4_workspace_size", Z, [P]),
             ("pab200_decode_int4", ctypes.c_int, [P, V, Z, V]),
             ("pab200_update_page_bounds", ctypes.c_int, [ctypes.POINTER(PageBoundsArgs), V]),

@@ -13,113 +13,269 @@ struct Int4AppendParams {
   uint32_t* status;
   int64_t r_st, r_sh;      // strides of the new rows (elements)
   int32_t vec;             // rows may be read in 16-byte units
+  int32_t increment;
 };
 
-// Quantises 8 of the 64 elements of a group held by 8 consecutive lanes:
-// returns their code word, and the group's (scale, minimum) pair.  The code is
-// the quotient (x - lo) / s rounded to the nearest integer, ties to even: the
-// product with the reciprocal is within one of it, and the remainder
-// x - lo - c s, exact in fp32, settles the rest.
+// Codes of a group whose scale is below T's normal numbers (rounded coarsely,
+// so that quotients pass 15), as in int4_quantise; lo and s of the group.
 template <typename T>
-__device__ __forceinline__ uint32_t int4_quantise(const float (&f)[8], uint32_t* pair) {
-  float lo = f[0], hi = f[0];
-#pragma unroll
-  for (int i = 1; i < 8; ++i) {
-    lo = min_nan(lo, f[i]);
-    hi = max_nan(hi, f[i]);
-  }
-#pragma unroll
-  for (int o = 1; o < 8; o <<= 1) {
-    lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-    hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-  }
-  const float range = hi - lo;
-  const bool finite = fabsf(range) <= 3.4028235e38f;  // false for NaN and infinities
-  *pair = pack2<T>(finite ? __fdiv_rn(range, 15.f) : __int_as_float(0x7fffffff),
-                   finite ? lo : __int_as_float(0x7fffffff));
-  const float s = unpack2<T>(*pair).x;
+__device__ __noinline__ uint32_t int4_quantise_tiny(uint4 x, float lo, float s) {
+  const uint32_t v[4] = {x.x, x.y, x.z, x.w};
   uint32_t word = 0;
-  if (finite && s > 0.f) {
-    const float inv = __frcp_rn(s);
-    const bool tiny = s < 1e-37f;  // the reciprocal overflows
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float a = f[i] - lo;
-      float c = rintf(tiny ? __fdiv_rn(a, s) : a * inv);
-      c = fminf(c, 15.f);
-      const float r = 2.f * fmaf(-c, s, a);
-      const int ci = static_cast<int>(c);
-      int d = 0;
-      if (r > s || (r == s && (ci & 1))) d = 1;
-      if (r < -s || (r == -s && (ci & 1))) d = -1;
-      const int q = min(max(ci + d, 0), 15);
-      word |= static_cast<uint32_t>(q) << (4 * (i / 2 + 4 * (i % 2)));
-    }
+  for (int i = 0; i < 8 && s > 0.f; ++i) {
+    const float2 f = unpack2<T>(v[i / 2]);
+    const float q = rintf(__fdiv_rn((i & 1 ? f.y : f.x) - lo, s));
+    word |= static_cast<uint32_t>(fminf(q, 15.f)) << (4 * (i / 2 + 4 * (i % 2)));
   }
   return word;
 }
 
-// One lane per 8 elements: D/8 lanes hold a row; blockIdx.y 0 keys, 1 values.
-template <typename T, int D>
-__global__ void __launch_bounds__(256) int4_append_kernel(const Int4AppendParams p) {
-  constexpr int LR = D / 8;
-  const TokenMap& m = p.map;
-  const int kv = blockIdx.y;
-  const int64_t row = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) / LR;
-  const int e = threadIdx.x % LR, g = e / 8, o = e % 8;
-  const int64_t i = row / m.Hkv;
-  const int h = static_cast<int>(row - i * m.Hkv);
-  uint32_t flags = 0;
-  int64_t pid = -1;
-  int r = 0;
-  float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  int s, j;
-  if (i < m.num_tokens && find_token(m, i, &s, &j)) {
-    const int L = p.lens[s * m.l_sb + h * m.l_sh];
-    if (L < 0) {
-      flags |= kStatusNegative;
-    } else {
-      const int64_t pos = static_cast<int64_t>(L) + j;
-      pid = find_page(m, s, h, pos, &flags);
-      r = static_cast<int>(pos % m.bs);
-    }
-    load8<T>(static_cast<const T*>(p.rows[kv]) + i * p.r_st + h * p.r_sh + e * 8, p.vec != 0, f);
-  }
-  uint32_t pair;
-  const uint32_t word = int4_quantise<T>(f, &pair);
-  if (flags && p.status) atomicOr(p.status, flags);
-  if (pid < 0) return;
-  uint8_t* page = p.cache[kv] + pid * (static_cast<int64_t>(m.bs) * int4_row_bytes(D));
-  *reinterpret_cast<uint32_t*>(page + (kv ? int4_value_word(D, r, g, o) : int4_key_word(D, r, g, o))) = word;
-  if (o == 0) *reinterpret_cast<uint32_t*>(page + int4_pair(D, m.bs, r, g)) = pair;
+// (minimum, -maximum) of the 64 elements of a group, 8 in each of 8 consecutive
+// lanes, in every lane: one comparison per step (a 16-bit float changes sign by
+// its top bit).
+template <typename T>
+__device__ __forceinline__ uint32_t group_range(const uint4& x) {
+  const uint32_t lo = min2_nan<T>(min2_nan<T>(x.x, x.y), min2_nan<T>(x.z, x.w));
+  const uint32_t hi = max2_nan<T>(max2_nan<T>(x.x, x.y), max2_nan<T>(x.z, x.w)) ^ 0x80008000u;
+  uint32_t both = min2_nan<T>(__byte_perm(lo, hi, 0x5410), __byte_perm(lo, hi, 0x7632));
+#pragma unroll
+  for (int o = 1; o < 8; o <<= 1) both = min2_nan<T>(both, __shfl_xor_sync(0xffffffffu, both, o));
+  return both;
 }
 
-// The lengths of one sequence, after its rows are written: each grows by the
-// number of new tokens before the first that had no place.  A length shared by
-// the sequence's heads grows by the least of theirs.  One warp per sequence.
+// Smallest scale whose quotients stay at 15 (1 + 2^-8) at most: the normal
+// numbers of fp16; of bf16, those whose reciprocal is finite.
+template <typename T>
+__device__ constexpr float int4_least_scale() {
+  return std::is_same<T, __half>::value ? 6.103515625e-5f : 1e-36f;
+}
+
+// A group's (scale, minimum) pair and 1 / scale from its (minimum, -maximum).
+template <typename T>
+__device__ __forceinline__ uint32_t int4_scale(uint32_t both, float* inv) {
+  const float2 lh = unpack2<T>(both);
+  const float range = -lh.y - lh.x;
+  const bool finite = fabsf(range) <= 3.4028235e38f;  // false for NaN and infinities
+  const float nan = __int_as_float(0x7fffffff);
+  const uint32_t pair = pack2<T>(finite ? __fdiv_rn(range, 15.f) : nan, finite ? lh.x : nan);
+  const float s = unpack2<T>(pair).x;
+  *inv = s >= int4_least_scale<T>() ? __frcp_rn(s) : 0.f;
+  return pair;
+}
+
+// Code word of 8 elements (element i in nibble i / 2 + 4 (i % 2)).
+//
+// A code is the quotient a / s, a = x - lo, rounded to the nearest integer, ties
+// to even.  The quotient is formed as q0 = a (1/s) corrected once by its
+// remainder, q0 + (a - q0 s)(1/s), which is the correctly rounded a / s (P.
+// Markstein, IBM J. Res. Dev. 34, 1990), so that exact ties, common among 16-bit
+// inputs, stay ties; adding 1.5 * 2^23 rounds it.
+template <typename T>
+__device__ __forceinline__ uint32_t int4_codes_of(const uint4& x, uint32_t pair, float inv) {
+  const float2 sl = unpack2<T>(pair);
+  if (inv == 0.f) return int4_quantise_tiny<T>(x, sl.y, sl.x);  // no code if s is 0 or NaN
+  constexpr float kMagic = 12582912.f;  // 1.5 * 2^23
+  const uint32_t v[4] = {x.x, x.y, x.z, x.w};
+  float c[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = unpack2<T>(v[i]);
+    const float a0 = f.x - sl.y, a1 = f.y - sl.y;
+    const float q0 = a0 * inv, q1 = a1 * inv;
+    c[2 * i] = (fmaf(fmaf(-q0, sl.x, a0), inv, q0) + kMagic) - kMagic;
+    c[2 * i + 1] = (fmaf(fmaf(-q1, sl.x, a1), inv, q1) + kMagic) - kMagic;
+  }
+  // four codes are one exact integer below 2^16 in fp32
+  const float even = fmaf(fmaf(fmaf(c[6], 16.f, c[4]), 16.f, c[2]), 16.f, c[0]);
+  const float odd = fmaf(fmaf(fmaf(c[7], 16.f, c[5]), 16.f, c[3]), 16.f, c[1]);
+  return __byte_perm(__float_as_uint(even + kMagic), __float_as_uint(odd + kMagic), 0x5410);
+}
+
+// 4 x 4 transpose of the words of 4 lanes that differ in lane bits A and B:
+// lane (a, b) with w[j] ends with w[i] = the word j = 2 a + b of lane i.
+template <int A, int B>
+__device__ __forceinline__ void transpose4(uint32_t (&w)[4], bool a, bool b) {
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {  // exchange w[j] / w[j + 2] with the lane across A
+    const uint32_t got = __shfl_xor_sync(0xffffffffu, a ? w[j] : w[j + 2], A);
+    if (a)
+      w[j] = got;
+    else
+      w[j + 2] = got;
+  }
+#pragma unroll
+  for (int j = 0; j < 4; j += 2) {
+    const uint32_t got = __shfl_xor_sync(0xffffffffu, b ? w[j] : w[j + 1], B);
+    if (b)
+      w[j] = got;
+    else
+      w[j + 1] = got;
+  }
+}
+
+// Quantises the tokens [r0, r1) (rows of an 8-token tile; FULL: all 8, in 16-byte
+// reads) of one (sequence, kv head) into its page (`off` bytes into both caches),
+// the tile starting at row `tile`.  `src0`: offset of row 0's elements.
+//
+// A warp holds the tile as D/8 lanes per row: 256/D rows at a time, in D/32
+// rounds.  The divisions for a round's scales are made by one lane of each
+// group's 8 and handed round.  Keys: a row's words fill D/2 contiguous bytes.
+// Values: a tile's words are [octet][pair][parity][group]; with D = 128 the lanes
+// of one octet (2 groups x 2 row parities) hold 4 rounds = 4 pairs of words,
+// which a 4 x 4 transpose turns into 16 contiguous bytes per lane, 512 per warp.
+template <typename T, int D, bool FULL>
+__device__ __forceinline__ void append_tile(const Int4AppendParams& p, int64_t off, int tile, int r0,
+                                            int r1, int64_t src0) {
+  constexpr int LR = D / 8, RP = 32 / LR, ROUNDS = 8 / RP;
+  const int lane = threadIdx.x & 31, e = lane % LR, rr = lane / LR, g = e / 8, o = e % 8;
+  const int bs = p.map.bs;
+  uint4 x[2][ROUNDS];
+#pragma unroll
+  for (int kv = 0; kv < 2; ++kv) {
+    const T* row = static_cast<const T*>(p.rows[kv]) + src0 + rr * p.r_st + e * 8;
+#pragma unroll
+    for (int i = 0; i < ROUNDS; ++i, row += RP * p.r_st) {
+      const int r = i * RP + rr;
+      x[kv][i] = make_uint4(0u, 0u, 0u, 0u);
+      if (FULL)
+        x[kv][i] = load_row8<T>(row, true);
+      else if (r >= r0 && r < r1)
+        x[kv][i] = load_row8<T>(row, p.vec != 0);
+    }
+  }
+#pragma unroll
+  for (int kv = 0; kv < 2; ++kv) {
+    uint8_t* page = p.cache[kv] + off;
+    uint32_t mine = 0u;
+#pragma unroll
+    for (int i = 0; i < ROUNDS; ++i) {
+      const uint32_t both = group_range<T>(x[kv][i]);
+      if (o % ROUNDS == i) mine = both;
+    }
+    float inv;
+    const uint32_t pair = int4_scale<T>(mine, &inv);
+    const int mr = o % ROUNDS * RP + rr;  // the row this lane has scaled
+    if (o < ROUNDS && (FULL || (mr >= r0 && mr < r1)))
+      *reinterpret_cast<uint32_t*>(page + int4_pair(D, bs, tile + mr, g)) = pair;
+    uint32_t w[ROUNDS];
+#pragma unroll
+    for (int i = 0; i < ROUNDS; ++i) {
+      const int from = (lane & 24) + i;
+      const uint32_t pi = __shfl_sync(0xffffffffu, pair, from);
+      const float vi = __shfl_sync(0xffffffffu, inv, from);
+      w[i] = int4_codes_of<T>(x[kv][i], pi, vi);
+    }
+    if constexpr (FULL && D == 128) {
+      if (kv == 1) {
+        // lanes of octet o: parity rr (bit 16), group g (bit 8); round i = pair i
+        transpose4<16, 8>(w, rr != 0, g != 0);
+        uint8_t* at = page + (tile >> 3) * (4 * D) + (o * 4 + rr * 2 + g) * 16;
+        *reinterpret_cast<uint4*>(at) = make_uint4(w[0], w[1], w[2], w[3]);
+        continue;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < ROUNDS; ++i) {
+      const int r = i * RP + rr;
+      if (FULL || (r >= r0 && r < r1))
+        *reinterpret_cast<uint32_t*>(page + (kv ? int4_value_word(D, tile + r, g, o)
+                                                : int4_key_word(D, tile + r, g, o))) = w[i];
+    }
+  }
+}
+
+// Ragged runs of tokens: one warp per (8-token tile, kv head).
+template <typename T, int D>
+__global__ void __launch_bounds__(256, 4) int4_append_kernel(const Int4AppendParams p, int warps) {
+  const TokenMap& m = p.map;
+  const int wid = blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (wid >= warps) return;
+  const int slot = wid / m.Hkv, h = wid - slot * m.Hkv;
+  const TokenRun t = find_run(m, slot, 3);
+  if (t.n == 0) return;
+  const int L = p.lens[t.s * m.l_sb + h * m.l_sh];
+  uint32_t flags = 0;
+  if (L < 0) {
+    flags = kStatusNegative;
+  } else {
+    const int64_t pos0 = ((static_cast<int64_t>(L) >> 3) + t.run) << 3;  // the tile's position
+    const int64_t a = L > pos0 ? L - pos0 : 0;
+    const int64_t end = static_cast<int64_t>(L) + t.n - pos0;
+    if (end <= 0) return;
+    const int64_t pid = find_page(m, t.s, h, pos0 >> m.log2_bs, &flags);
+    if (pid >= 0) {
+      const int64_t src0 = (t.t0 + pos0 - L) * p.r_st + h * p.r_sh;
+      const int64_t off = pid * (static_cast<int64_t>(m.bs) * int4_row_bytes(D));
+      const int tile = static_cast<int>(pos0) & (m.bs - 1);
+      if (a == 0 && end >= 8 && p.vec)
+        append_tile<T, D, true>(p, off, tile, 0, 8, src0);
+      else
+        append_tile<T, D, false>(p, off, tile, static_cast<int>(a),
+                                 end < 8 ? static_cast<int>(end) : 8, src0);
+    }
+  }
+  if (flags && p.status && (threadIdx.x & 31) == 0) atomicOr(p.status, flags);
+}
+
+// One token per sequence: one CTA per sequence, a warp per kv head, and the
+// length, which every warp has read by then, in the same launch.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) int4_append_step_kernel(const Int4AppendParams p) {
+  const TokenMap& m = p.map;
+  const int s = blockIdx.x, lane = threadIdx.x & 31;
+  uint32_t flags = 0;
+  bool all = true;
+  for (int h = threadIdx.x >> 5; h < m.Hkv; h += blockDim.x >> 5) {
+    int32_t* lp = p.lens + s * m.l_sb + h * m.l_sh;
+    const int L = *lp;
+    uint32_t f = L < 0 ? kStatusNegative : 0u;
+    const int64_t pid = L < 0 ? -1 : find_page(m, s, h, L >> m.log2_bs, &f);
+    if (pid >= 0) {
+      const int row = L & (m.bs - 1);
+      append_tile<T, D, false>(p, pid * (static_cast<int64_t>(m.bs) * int4_row_bytes(D)), row & ~7,
+                               row & 7, (row & 7) + 1,
+                               (static_cast<int64_t>(s) - (row & 7)) * p.r_st + h * p.r_sh);
+    }
+    if (pid >= 0 && m.l_sh != 0 && p.increment && lane == 0) *lp = L + 1;
+    all = all && pid >= 0;
+    flags |= f;
+  }
+  if (flags && p.status && lane == 0) atomicOr(p.status, flags);
+  if (m.l_sh == 0) {
+    const bool ok = __syncthreads_and(all) != 0;  // every warp has read the length
+    if (ok && p.increment && threadIdx.x == 0) p.lens[s * m.l_sb] += 1;
+  }
+}
+
+// The lengths of ragged runs, after the rows: each grows by the number of new
+// tokens before the first that had no place.  A length shared by the
+// sequence's heads grows by the least of theirs.  One warp per sequence.
 __global__ void __launch_bounds__(128) int4_lengths_kernel(const Int4AppendParams p) {
   const TokenMap& m = p.map;
   const int lane = threadIdx.x & 31;
   const int s = blockIdx.x * 4 + (threadIdx.x >> 5);
   if (s >= m.B) return;
-  int64_t n = 1;
-  if (m.cu) {
-    n = static_cast<int64_t>(m.cu[s + 1]) - m.cu[s];
-    if (m.cu[s] < 0 || m.cu[s + 1] > m.num_tokens) n = 0;
-  }
-  if (n <= 0) return;
+  const int t0 = m.cu[s], t1 = m.cu[s + 1];
+  if (t0 < 0 || t1 > m.num_tokens || t1 <= t0) return;
+  const int64_t n = t1 - t0;
+  grid_dependency_wait();  // the rows' kernel has read every length
   int64_t least = n;
-  for (int h = 0; h < m.Hkv; ++h) {
+  // Heads whose ids come from one table entry of a pool are in range together.
+  const bool alike = m.l_sh == 0 && m.bt_sh == 0 && m.bt_add == 1 && m.bt_mul == m.Hkv &&
+                     m.num_pages % m.Hkv == 0;
+  const int heads = alike ? 1 : m.Hkv;
+  for (int h = 0; h < heads; ++h) {
     int32_t* lp = p.lens + s * m.l_sb + h * m.l_sh;
     const int64_t L = *lp;
     int64_t got = L < 0 ? 0 : n;
     uint32_t flags = 0;
-    for (int64_t pg = L / m.bs + lane; got > 0 && pg * m.bs < L + n; pg += 32)
-      if (find_page(m, s, h, pg * m.bs, &flags) < 0) {
-        const int64_t before = pg * m.bs - L;
-        got = before < 0 ? 0 : before;
-        break;
-      }
+    if (L >= 0)
+      for (int64_t pg = (L >> m.log2_bs) + lane; (pg << m.log2_bs) < L + n; pg += 32)
+        if (find_page(m, s, h, pg, &flags) < 0) {
+          const int64_t before = (pg << m.log2_bs) - L;
+          got = before < 0 ? 0 : before;
+          break;
+        }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
       const int64_t x = __shfl_xor_sync(0xffffffffu, got, o);
@@ -142,52 +298,87 @@ struct Int4ReadParams {
   const int32_t* starts;   // [B] first position read, or null: 0
   uint32_t* status;
   int64_t o_st, o_sh, start_sb;
+  int32_t zero_rest;       // rows of no sequence become zeros
 };
 
-// lo + s c of 8 elements, rounded to T.  The rounding of s may put code 15 of a
-// range as wide as T's past T's largest value: such a value saturates.
+// lo + s c of 8 elements: c, s and lo are exact in T, so one packed fma rounds
+// once.  The rounding of s may put code 15 of a range as wide as T's past T's
+// largest value: such a value saturates.
 template <typename T>
-__device__ __forceinline__ uint4 int4_values(uint32_t word, float2 sl) {
-  constexpr float kMax = std::is_same<T, __half>::value ? 65504.f : 3.38953139e38f;
-  float v[8];
+__device__ __forceinline__ uint4 int4_values(uint32_t word, uint32_t pair) {
+  uint32_t r[4];
+  int4_codes<T>(word, r);
+  const uint32_t s = __byte_perm(pair, pair, 0x1010), lo = __byte_perm(pair, pair, 0x3232);
+  constexpr uint32_t kMax = std::is_same<T, __half>::value ? 0x7bff7bffu : 0x7f7f7f7fu;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    v[i] = fmaf(sl.x, static_cast<float>((word >> (4 * (i / 2 + 4 * (i % 2)))) & 15u), sl.y);
-    if (v[i] > kMax) v[i] = kMax;  // a NaN stays
-  }
-  return make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]),
-                    pack2<T>(v[6], v[7]));
+  for (int m = 0; m < 4; ++m) r[m] = min2_nan<T>(fma2<T>(s, r[m], lo), kMax);
+  return make_uint4(r[0], r[1], r[2], r[3]);
 }
 
+// One warp per (8-token tile, kv head), lanes as in append_tile.
 template <typename T, int D>
-__global__ void __launch_bounds__(256) int4_read_kernel(const Int4ReadParams p) {
-  constexpr int LR = D / 8;
+__global__ void __launch_bounds__(256) int4_read_kernel(const Int4ReadParams p, int warps) {
+  constexpr int LR = D / 8, RP = 32 / LR, ROUNDS = 8 / RP;
   const TokenMap& m = p.map;
-  const int kv = blockIdx.y;
-  const int64_t row = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) / LR;
-  const int e = threadIdx.x % LR, g = e / 8, o = e % 8;
-  const int64_t i = row / m.Hkv;
-  const int h = static_cast<int>(row - i * m.Hkv);
-  int s, j;
-  if (i >= m.num_tokens || !find_token(m, i, &s, &j)) return;
-  const int L = p.lens[s * m.l_sb + h * m.l_sh];
-  const int64_t pos = static_cast<int64_t>(p.starts ? p.starts[s * p.start_sb] : 0) + j;
-  uint4 v = make_uint4(0u, 0u, 0u, 0u);
-  if (pos >= 0 && pos < L) {
-    uint32_t flags = 0;
-    const int64_t pid = find_page(m, s, h, pos, &flags);
-    if (flags && p.status)
+  const int wid = blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (wid >= warps) return;
+  const int slot = wid / m.Hkv, h = wid - slot * m.Hkv;
+  const int lane = threadIdx.x & 31, e = lane % LR, rr = lane / LR, g = e / 8, o = e % 8;
+  auto put = [&](int64_t row, int kv, const uint4& v) {
+    *reinterpret_cast<uint4*>(static_cast<T*>(p.out[kv]) + row * p.o_st + h * p.o_sh + e * 8) = v;
+  };
+  if (p.zero_rest && m.cu) {
+    // Slots past the last sequence's: rows from cu[B]; the slots before the
+    // first sequence's: rows up to cu[0].
+    const int first = m.cu[0], last = max(m.cu[m.B], 0);
+    const int past = slot - ((last >> 3) + 2 * m.B);
+    const int64_t z0 = past >= 0 ? last + 8 * static_cast<int64_t>(past) : 8 * static_cast<int64_t>(slot);
+    const int64_t z1 = past >= 0 ? m.num_tokens : min(first, m.num_tokens);
+    if (past >= 0 || z0 < z1)
+      for (int64_t r = z0 + rr; r < z1 && r < z0 + 8; r += RP) {
+        put(r, 0, make_uint4(0u, 0u, 0u, 0u));
+        put(r, 1, make_uint4(0u, 0u, 0u, 0u));
+      }
+    if (past >= 0) return;
+  }
+  const TokenRun t = find_run(m, slot, 3);
+  if (t.n == 0) return;
+  const int L = p.lens[t.s * m.l_sb + h * m.l_sh];
+  const int64_t start = p.starts ? p.starts[t.s * p.start_sb] : 0;
+  const int64_t pos0 = ((start >> 3) + t.run) << 3;  // the tile's position (start may be < 0)
+  const int64_t a = start > pos0 ? start - pos0 : 0, end = start + t.n - pos0;
+  if (end <= 0) return;
+  const int r0 = static_cast<int>(a), r1 = end < 8 ? static_cast<int>(end) : 8;
+  uint32_t flags = 0;
+  int64_t pid = -1;
+  if (pos0 >= 0 && pos0 + r0 < L) {
+    pid = find_page(m, t.s, h, pos0 >> m.log2_bs, &flags);
+    if (flags && p.status && lane == 0)
       atomicOr(p.status, flags & kStatusAppendFull ? kStatusClamp : flags);
-    if (pid >= 0) {
-      const int r = static_cast<int>(pos % m.bs);
-      const uint8_t* page = p.cache[kv] + pid * (static_cast<int64_t>(m.bs) * int4_row_bytes(D));
-      const uint32_t word = *reinterpret_cast<const uint32_t*>(
-          page + (kv ? int4_value_word(D, r, g, o) : int4_key_word(D, r, g, o)));
-      const uint32_t pair = *reinterpret_cast<const uint32_t*>(page + int4_pair(D, m.bs, r, g));
-      v = int4_values<T>(word, unpack2<T>(pair));
+  }
+  const int64_t left = L - pos0;  // rows of the tile that hold a token
+  const int tile = static_cast<int>(pos0) & (m.bs - 1);
+  const int64_t off = pid * (static_cast<int64_t>(m.bs) * int4_row_bytes(D));
+#pragma unroll
+  for (int kv = 0; kv < 2; ++kv) {
+    uint32_t w[ROUNDS], pr[ROUNDS];
+#pragma unroll
+    for (int i = 0; i < ROUNDS; ++i) {
+      const int r = i * RP + rr;
+      w[i] = pr[i] = 0u;
+      if (pid >= 0 && r >= r0 && r < r1 && r < left) {
+        const uint8_t* page = p.cache[kv] + off;
+        w[i] = __ldg(reinterpret_cast<const uint32_t*>(
+            page + (kv ? int4_value_word(D, tile + r, g, o) : int4_key_word(D, tile + r, g, o))));
+        pr[i] = __ldg(reinterpret_cast<const uint32_t*>(page + int4_pair(D, m.bs, tile + r, g)));
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < ROUNDS; ++i) {
+      const int r = i * RP + rr;
+      if (r >= r0 && r < r1) put(t.t0 + pos0 + r - start, kv, int4_values<T>(w[i], pr[i]));
     }
   }
-  *reinterpret_cast<uint4*>(static_cast<T*>(p.out[kv]) + i * p.o_st + h * p.o_sh + e * 8) = v;
 }
 
 }  // namespace pab
@@ -215,9 +406,11 @@ int check_int4(const pab200_int4_rows_args* a, pab::TokenMap* m) {
     return fail(PAB200_ERR_INVALID_ARGUMENT,
                 "without cu_tokens there is one token per sequence: num_tokens %lld, num_seqs %d",
                 static_cast<long long>(a->num_tokens), a->num_seqs);
-  if (int64_t(a->max_blocks) * bs >= (int64_t(1) << 31) || a->num_tokens >= (int64_t(1) << 31) ||
-      a->num_tokens * a->num_kv_heads * (D / 8) / 256 >= (int64_t(1) << 31) - 1)
-    return fail(PAB200_ERR_UNSUPPORTED, "max_blocks*block_size or num_tokens too large (>= 2^31)");
+  if (int64_t(a->max_blocks) * bs >= (int64_t(1) << 31) || a->num_tokens >= (int64_t(1) << 30) ||
+      (pab::num_slots(a->num_tokens, a->num_seqs, a->cu_tokens != nullptr, 3) + 8) * a->num_kv_heads >=
+          (int64_t(1) << 31))
+    return fail(PAB200_ERR_UNSUPPORTED,
+                "max_blocks*block_size, or num_tokens*num_kv_heads/8, too large (>= 2^31)");
   if (a->num_seqs == 0 || a->num_tokens == 0) return PAB200_OK;
   if (!a->k_rows || !a->v_rows || !a->seqlens)
     return fail(PAB200_ERR_INVALID_ARGUMENT, "k_rows, v_rows or seqlens is null");
@@ -236,12 +429,13 @@ int check_int4(const pab200_int4_rows_args* a, pab::TokenMap* m) {
   m->l_sb = a->seqlens_stride_b;
   m->l_sh = a->seqlens_stride_h;
   m->num_pages = a->num_pages;
-  m->num_tokens = a->num_tokens;
+  m->num_tokens = static_cast<int32_t>(a->num_tokens);
   m->bt_mul = a->bt_page_mul;
   m->bt_add = a->bt_page_add;
   m->B = a->num_seqs;
   m->Hkv = a->num_kv_heads;
   m->bs = bs;
+  m->log2_bs = bs == 8 ? 3 : (bs == 16 ? 4 : (bs == 32 ? 5 : 6));
   m->maxb = a->num_pages > 0 ? a->max_blocks : 0;
   return PAB200_OK;
 }
@@ -251,26 +445,41 @@ bool rows_vec(const pab200_int4_rows_args* a) {
          a->row_stride_h % 8 == 0;
 }
 
-dim3 rows_grid(const pab200_int4_rows_args* a) {
-  const int64_t threads = a->num_tokens * a->num_kv_heads * (a->head_size / 8);
-  return dim3(static_cast<unsigned>((threads + 255) / 256), 2);
+// Warps of a kernel over (8-token tile, kv head) pairs.
+int tile_warps(const pab200_int4_rows_args* a) {
+  // two slots more: the read-back's rows behind the last sequence
+  const int more = a->cu_tokens ? 2 : 0;
+  return static_cast<int>(
+      (pab::num_slots(a->num_tokens, a->num_seqs, a->cu_tokens != nullptr, 3) + more) *
+      a->num_kv_heads);
 }
 
-template <typename T>
-void launch_append(const pab::Int4AppendParams& p, int D, dim3 grid, cudaStream_t s) {
-  switch (D) {
-    case 64: pab::int4_append_kernel<T, 64><<<grid, 256, 0, s>>>(p); break;
-    case 128: pab::int4_append_kernel<T, 128><<<grid, 256, 0, s>>>(p); break;
-    default: pab::int4_append_kernel<T, 256><<<grid, 256, 0, s>>>(p); break;
+template <typename T, int D>
+void launch_append(const pab::Int4AppendParams& p, int warps, cudaStream_t s) {
+  if (p.map.cu) {
+    pab::int4_append_kernel<T, D><<<(warps + 7) / 8, 256, 0, s>>>(p, warps);
+  } else {
+    const int per_cta = p.map.Hkv < 8 ? p.map.Hkv : 8;
+    pab::int4_append_step_kernel<T, D><<<p.map.B, per_cta * 32, 0, s>>>(p);
   }
 }
 
 template <typename T>
-void launch_read(const pab::Int4ReadParams& p, int D, dim3 grid, cudaStream_t s) {
+void launch_append_d(const pab::Int4AppendParams& p, int D, int warps, cudaStream_t s) {
   switch (D) {
-    case 64: pab::int4_read_kernel<T, 64><<<grid, 256, 0, s>>>(p); break;
-    case 128: pab::int4_read_kernel<T, 128><<<grid, 256, 0, s>>>(p); break;
-    default: pab::int4_read_kernel<T, 256><<<grid, 256, 0, s>>>(p); break;
+    case 64: launch_append<T, 64>(p, warps, s); break;
+    case 128: launch_append<T, 128>(p, warps, s); break;
+    default: launch_append<T, 256>(p, warps, s); break;
+  }
+}
+
+template <typename T>
+void launch_read(const pab::Int4ReadParams& p, int D, int warps, cudaStream_t s) {
+  const int grid = (warps + 7) / 8;
+  switch (D) {
+    case 64: pab::int4_read_kernel<T, 64><<<grid, 256, 0, s>>>(p, warps); break;
+    case 128: pab::int4_read_kernel<T, 128><<<grid, 256, 0, s>>>(p, warps); break;
+    default: pab::int4_read_kernel<T, 256><<<grid, 256, 0, s>>>(p, warps); break;
   }
 }
 
@@ -297,21 +506,23 @@ PAB200_EXPORT int pab200_kv_append_int4(const pab200_int4_rows_args* a, int32_t 
   p.r_st = a->row_stride_t;
   p.r_sh = a->row_stride_h;
   p.vec = rows_vec(a);
+  p.increment = increment ? 1 : 0;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (a->dtype == PAB200_DTYPE_BF16)
-    launch_append<__nv_bfloat16>(p, a->head_size, rows_grid(a), s);
+    launch_append_d<__nv_bfloat16>(p, a->head_size, tile_warps(a), s);
   else
-    launch_append<__half>(p, a->head_size, rows_grid(a), s);
+    launch_append_d<__half>(p, a->head_size, tile_warps(a), s);
   cudaError_t e = cudaGetLastError();
-  if (e == cudaSuccess && increment) {
-    pab::int4_lengths_kernel<<<(a->num_seqs + 3) / 4, 128, 0, s>>>(p);
-    e = cudaGetLastError();
+  if (e == cudaSuccess && increment && a->cu_tokens) {
+    // scheduled while the rows' kernel drains; waits for it before any length
+    pabh::LaunchCfg lc(dim3((a->num_seqs + 3) / 4), dim3(128), 0, s, true);
+    e = cudaLaunchKernelEx(&lc.cfg, pab::int4_lengths_kernel, p);
   }
   return e == cudaSuccess ? PAB200_OK : pabh::cuda_fail(e, "4-bit append launch");
 }
 
 PAB200_EXPORT int pab200_kv_read_int4(const pab200_int4_rows_args* a, const int32_t* starts,
-                                      int64_t starts_stride, void* stream) {
+                                      int64_t starts_stride, int32_t zero_rest, void* stream) {
   pab::Int4ReadParams p{};
   const int rc = check_int4(a, &p.map);
   if (rc || a->num_seqs == 0 || a->num_tokens == 0) return rc;
@@ -324,14 +535,15 @@ PAB200_EXPORT int pab200_kv_read_int4(const pab200_int4_rows_args* a, const int3
   p.lens = a->seqlens;
   p.starts = starts;
   p.start_sb = starts_stride;
+  p.zero_rest = zero_rest ? 1 : 0;
   p.status = a->status;
   p.o_st = a->row_stride_t;
   p.o_sh = a->row_stride_h;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (a->dtype == PAB200_DTYPE_BF16)
-    launch_read<__nv_bfloat16>(p, a->head_size, rows_grid(a), s);
+    launch_read<__nv_bfloat16>(p, a->head_size, tile_warps(a), s);
   else
-    launch_read<__half>(p, a->head_size, rows_grid(a), s);
+    launch_read<__half>(p, a->head_size, tile_warps(a), s);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? PAB200_OK : pabh::cuda_fail(e, "4-bit read launch");
 }

@@ -128,6 +128,45 @@ __device__ __forceinline__ void int4_value_pairs<__nv_bfloat16>(uint32_t w, uint
   }
 }
 
+// Nibble m of both halves of w as the pair r[m] of exact values c (0..15) of T.
+template <typename T>
+__device__ __forceinline__ void int4_codes(uint32_t w, uint32_t (&r)[4]);
+template <>
+__device__ __forceinline__ void int4_codes<__half>(uint32_t w, uint32_t (&r)[4]) {
+#pragma unroll
+  for (int m = 0; m < 4; ++m) {
+    const uint32_t t = and_or(w >> (4 * m), 0x000f000fu, 0x64006400u);
+    const __half2 y = __hsub2(*reinterpret_cast<const __half2*>(&t), __float2half2_rn(1024.f));
+    r[m] = *reinterpret_cast<const uint32_t*>(&y);
+  }
+}
+template <>
+__device__ __forceinline__ void int4_codes<__nv_bfloat16>(uint32_t w, uint32_t (&r)[4]) {
+#pragma unroll
+  for (int m = 0; m < 4; ++m) {
+    const uint32_t t = and_or(w >> (4 * m), 0x000f000fu, 0x43004300u);
+    const __nv_bfloat162 y =
+        __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&t), __floats2bfloat162_rn(128.f, 128.f));
+    r[m] = *reinterpret_cast<const uint32_t*>(&y);
+  }
+}
+
+// a * b + c of two pairs of T, one rounding.
+template <typename T>
+__device__ __forceinline__ uint32_t fma2(uint32_t a, uint32_t b, uint32_t c);
+template <>
+__device__ __forceinline__ uint32_t fma2<__half>(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t r;
+  asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+  return r;
+}
+template <>
+__device__ __forceinline__ uint32_t fma2<__nv_bfloat16>(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t r;
+  asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+  return r;
+}
+
 // (scale, value of code 8) of a (scale, minimum) pair.
 template <typename T>
 __device__ __forceinline__ float2 int4_centre(uint32_t pair) {

@@ -15,87 +15,74 @@ struct BoundsParams {
   int32_t vec;
 };
 
-// Page slots of a call: sequence s owns slots [cu[s]/bs + 2s, cu[s+1]/bs +
-// 2(s+1)), at least as many as the pages its new tokens touch.
-__device__ __forceinline__ int64_t first_slot(const TokenMap& m, int s) {
-  return (m.cu ? static_cast<int64_t>(m.cu[s]) / m.bs : 0) + (m.cu ? 2 : 1) * static_cast<int64_t>(s);
-}
-
-// One warp per (slot, kv head): the minimum and maximum of the page's new
-// rows, D/8 lanes per row, joined with the page's bounds when it began before.
+// One warp per (page, kv head): the minimum and maximum of the page's new rows,
+// D/8 lanes per row and 256/D rows at a time, joined with the page's bounds when
+// it began before.  Comparisons work on the 16-bit pairs as they are.
 template <typename T, int D>
-__global__ void __launch_bounds__(256) page_bounds_kernel(const BoundsParams p, int64_t slots) {
+__global__ void __launch_bounds__(256) page_bounds_kernel(const BoundsParams p, int warps) {
   constexpr int LR = D / 8, RP = 32 / LR;
   const TokenMap& m = p.map;
   const int lane = threadIdx.x & 31;
-  const int64_t w = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
-  const int64_t slot = w / m.Hkv;
-  const int h = static_cast<int>(w - slot * m.Hkv);
-  if (slot >= slots) return;
-  int lo = 0, hi = m.B - 1;  // last s with first_slot(s) <= slot
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (first_slot(m, mid) <= slot)
-      lo = mid;
-    else
-      hi = mid - 1;
-  }
-  const int s = lo;
-  const int64_t t0 = m.cu ? m.cu[s] : s;
-  const int64_t n = m.cu ? m.cu[s + 1] - t0 : 1;
-  if (t0 < 0 || n <= 0 || t0 + n > m.num_tokens) return;
-  const int64_t L = p.lens[s * m.l_sb + h * m.l_sh];
-  uint32_t flags = L < 0 ? kStatusNegative : 0u;
-  const int64_t pg = L / m.bs + (slot - first_slot(m, s));
-  if (L < 0 || pg * m.bs >= L + n) {
-    if (flags && p.status && lane == 0) atomicOr(p.status, flags);
-    return;
-  }
-  const int64_t pid = find_page(m, s, h, pg * m.bs, &flags);
+  const int wid = blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (wid >= warps) return;
+  const int slot = wid / m.Hkv, h = wid - slot * m.Hkv;
+  const TokenRun t = find_run(m, slot, m.log2_bs);
+  if (t.n == 0) return;
+  const int L = p.lens[t.s * m.l_sb + h * m.l_sh];
+  uint32_t flags = 0;
+  const int64_t pg = (static_cast<int64_t>(L) >> m.log2_bs) + t.run;
+  const int64_t pos0 = pg << m.log2_bs;                 // the page's position
+  const int64_t end = static_cast<int64_t>(L) + t.n - pos0;
+  if (L >= 0 && end <= 0) return;
+  const int64_t pid = L < 0 ? -1 : find_page(m, t.s, h, pg, &flags);
   if (pid < 0) {
-    if (p.status && lane == 0) atomicOr(p.status, flags);
+    if (p.status && lane == 0) atomicOr(p.status, L < 0 ? kStatusNegative : flags);
     return;
   }
-  const int64_t a = pg * m.bs < L ? L : pg * m.bs;                       // first new position
-  const int64_t b = (pg + 1) * m.bs < L + n ? (pg + 1) * m.bs : L + n;   // end
+  const int r0 = L > pos0 ? static_cast<int>(L - pos0) : 0;  // first new row, and the end
+  const int r1 = end < m.bs ? static_cast<int>(end) : m.bs;
   const int e = lane % LR, rr = lane / LR;
-  float mn[8], mx[8];
+  const T* rows = static_cast<const T*>(p.rows) + (t.t0 + pos0 - L) * p.r_st + h * p.r_sh + e * 8;
+  constexpr uint32_t kInf = std::is_same<T, __half>::value ? 0x7c007c00u : 0x7f807f80u;
+  uint32_t mn[4], mx[4];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    mn[i] = INFINITY;
-    mx[i] = -INFINITY;
+  for (int i = 0; i < 4; ++i) {
+    mn[i] = kInf;
+    mx[i] = kInf | 0x80008000u;
   }
-  const T* rows = static_cast<const T*>(p.rows) + h * p.r_sh + e * 8;
-  for (int64_t pos = a + rr; pos < b; pos += RP) {
-    float f[8];
-    load8<T>(rows + (t0 + pos - L) * p.r_st, p.vec != 0, f);
+  auto take = [&](const uint4& lo, const uint4& hi) {
+    mn[0] = min2_nan<T>(mn[0], lo.x);
+    mn[1] = min2_nan<T>(mn[1], lo.y);
+    mn[2] = min2_nan<T>(mn[2], lo.z);
+    mn[3] = min2_nan<T>(mn[3], lo.w);
+    mx[0] = max2_nan<T>(mx[0], hi.x);
+    mx[1] = max2_nan<T>(mx[1], hi.y);
+    mx[2] = max2_nan<T>(mx[2], hi.z);
+    mx[3] = max2_nan<T>(mx[3], hi.w);
+  };
+  T* out = static_cast<T*>(p.bounds) + pid * (2 * D) + e * 8;
+  if (r0 > 0) take(*reinterpret_cast<const uint4*>(out), *reinterpret_cast<const uint4*>(out + D));
+  constexpr int U = 8;  // rows in flight per lane
+  for (int r = r0 + rr; r < r1; r += RP * U) {
+    uint4 x[U];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      mn[i] = min_nan(mn[i], f[i]);
-      mx[i] = max_nan(mx[i], f[i]);
+    for (int u = 0; u < U; ++u) {
+      const int ru = r + u * RP < r1 ? r + u * RP : r;  // past the end: row r again
+      x[u] = load_row8<T>(rows + ru * p.r_st, p.vec != 0);
     }
+#pragma unroll
+    for (int u = 0; u < U; ++u) take(x[u], x[u]);
   }
 #pragma unroll
   for (int o = LR; o < 32; o <<= 1)
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      mn[i] = min_nan(mn[i], __shfl_xor_sync(0xffffffffu, mn[i], o));
-      mx[i] = max_nan(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], o));
+    for (int i = 0; i < 4; ++i) {
+      mn[i] = min2_nan<T>(mn[i], __shfl_xor_sync(0xffffffffu, mn[i], o));
+      mx[i] = max2_nan<T>(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], o));
     }
   if (rr != 0) return;
-  T* out = static_cast<T*>(p.bounds) + pid * (2 * D) + e * 8;
-  if (a > pg * m.bs) {
-    float f[8], u[8];
-    load8<T>(out, true, f);
-    load8<T>(out + D, true, u);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      mn[i] = min_nan(mn[i], f[i]);
-      mx[i] = max_nan(mx[i], u[i]);
-    }
-  }
-  store8<T>(out, mn);
-  store8<T>(out + D, mx);
+  *reinterpret_cast<uint4*>(out) = make_uint4(mn[0], mn[1], mn[2], mn[3]);
+  *reinterpret_cast<uint4*>(out + D) = make_uint4(mx[0], mx[1], mx[2], mx[3]);
 }
 
 struct SelectParams {
@@ -163,8 +150,8 @@ __global__ void __launch_bounds__(256) page_scores_kernel(const SelectParams p) 
       if (!bad) {
         const T* b = static_cast<const T*>(p.bounds) + pid * (2 * D) + e * 8;
         float mn[8], mx[8];
-        load8<T>(b, true, mn);
-        load8<T>(b + D, true, mx);
+        unpack8<T>(__ldg(reinterpret_cast<const uint4*>(b)), mn);
+        unpack8<T>(__ldg(reinterpret_cast<const uint4*>(b + D)), mx);
 #pragma unroll
         for (int i = 0; i < 8; ++i)
           sum = fma(static_cast<double>(mx[i]), up[i], fma(static_cast<double>(mn[i]), dn[i], sum));
@@ -465,12 +452,12 @@ PAB200_EXPORT int pab200_decode_sparse(const pab200_decode_args* a, const pab200
 namespace {
 
 template <typename T>
-void launch_bounds(const pab::BoundsParams& p, int D, int64_t slots, cudaStream_t s) {
-  const unsigned grid = static_cast<unsigned>((slots * p.map.Hkv + 7) / 8);
+void launch_bounds(const pab::BoundsParams& p, int D, int warps, cudaStream_t s) {
+  const int grid = (warps + 7) / 8;
   switch (D) {
-    case 64: pab::page_bounds_kernel<T, 64><<<grid, 256, 0, s>>>(p, slots); break;
-    case 128: pab::page_bounds_kernel<T, 128><<<grid, 256, 0, s>>>(p, slots); break;
-    default: pab::page_bounds_kernel<T, 256><<<grid, 256, 0, s>>>(p, slots); break;
+    case 64: pab::page_bounds_kernel<T, 64><<<grid, 256, 0, s>>>(p, warps); break;
+    case 128: pab::page_bounds_kernel<T, 128><<<grid, 256, 0, s>>>(p, warps); break;
+    default: pab::page_bounds_kernel<T, 256><<<grid, 256, 0, s>>>(p, warps); break;
   }
 }
 
@@ -488,10 +475,11 @@ PAB200_EXPORT int pab200_update_page_bounds(const pab200_page_bounds_args* a, vo
     return fail(PAB200_ERR_INVALID_ARGUMENT,
                 "without cu_tokens there is one token per sequence: num_tokens %lld, num_seqs %d",
                 static_cast<long long>(a->num_tokens), a->num_seqs);
-  const int64_t slots = a->cu_tokens ? a->num_tokens / a->block_size + 2 * int64_t(a->num_seqs)
-                                     : a->num_seqs;
-  if (int64_t(a->max_blocks) * a->block_size >= (int64_t(1) << 31) ||
-      a->num_tokens >= (int64_t(1) << 31) || slots * a->num_kv_heads / 8 >= (int64_t(1) << 31) - 1)
+  const int bs = a->block_size, log2_bs = bs == 8 ? 3 : (bs == 16 ? 4 : (bs == 32 ? 5 : 6));
+  const int64_t warps =
+      pab::num_slots(a->num_tokens, a->num_seqs, a->cu_tokens != nullptr, log2_bs) * a->num_kv_heads;
+  if (int64_t(a->max_blocks) * bs >= (int64_t(1) << 31) || a->num_tokens >= (int64_t(1) << 30) ||
+      warps >= (int64_t(1) << 31) - 8)
     return fail(PAB200_ERR_UNSUPPORTED, "max_blocks*block_size or num_tokens too large (>= 2^31)");
   if (a->num_seqs == 0 || a->num_tokens == 0) return PAB200_OK;
   if (!a->k_rows || !a->seqlens) return fail(PAB200_ERR_INVALID_ARGUMENT, "k_rows or seqlens is null");
@@ -508,12 +496,13 @@ PAB200_EXPORT int pab200_update_page_bounds(const pab200_page_bounds_args* a, vo
   p.map.l_sb = a->seqlens_stride_b;
   p.map.l_sh = a->seqlens_stride_h;
   p.map.num_pages = a->num_pages;
-  p.map.num_tokens = a->num_tokens;
+  p.map.num_tokens = static_cast<int32_t>(a->num_tokens);
   p.map.bt_mul = a->bounds_page_mul;
   p.map.bt_add = a->bounds_page_add;
   p.map.B = a->num_seqs;
   p.map.Hkv = a->num_kv_heads;
-  p.map.bs = a->block_size;
+  p.map.bs = bs;
+  p.map.log2_bs = log2_bs;
   p.map.maxb = a->num_pages > 0 ? a->max_blocks : 0;
   p.bounds = a->page_bounds;
   p.rows = a->k_rows;
@@ -524,9 +513,9 @@ PAB200_EXPORT int pab200_update_page_bounds(const pab200_page_bounds_args* a, vo
   p.vec = aligned(a->k_rows, 16) && a->row_stride_t % 8 == 0 && a->row_stride_h % 8 == 0;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (a->dtype == PAB200_DTYPE_BF16)
-    launch_bounds<__nv_bfloat16>(p, a->head_size, slots, s);
+    launch_bounds<__nv_bfloat16>(p, a->head_size, static_cast<int>(warps), s);
   else
-    launch_bounds<__half>(p, a->head_size, slots, s);
+    launch_bounds<__half>(p, a->head_size, static_cast<int>(warps), s);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? PAB200_OK : pabh::cuda_fail(e, "page bounds launch");
 }

@@ -166,21 +166,21 @@ def kv_read_int4(key_cache, value_cache, block_table, cache_seqlens, block_size,
     positions starts[s], starts[s] + 1, ... of sequence s (``starts`` None: from
     0); ``cu_out`` int32 (num_seqs + 1,) with ``num_tokens`` rows in all, or
     None: one row per sequence.  Positions at or past cache_seqlens and pages
-    with an invalid id read as zeros.  ``out``: a (k, v) pair to fill; rows
-    behind cu_out's last are left as they were.
+    with an invalid id read as zeros, and so do rows of no sequence.  ``out``: a
+    (k, v) pair to fill; its rows of no sequence are left as they were.
     """
     if dtype not in _DTYPES:
         raise TypeError(f"dtype must be bfloat16 or float16, got {dtype}")
     lens = _as_int32(cache_seqlens, "cache_seqlens")
     B = lens.shape[0]
     cu = _check_offsets(cu_out, B, "cu_out")
-    if out is None:
+    fresh = out is None
+    if fresh:
         if cu is not None and num_tokens is None:
             raise ValueError("cu_out needs num_tokens (or out)")
         n = B if cu is None else int(num_tokens)
         heads = key_cache.shape[1] if key_cache.dim() == 3 else block_table.shape[1]
-        make = torch.empty if cu is None else torch.zeros   # rows in no sequence are not written
-        out = tuple(make((n, heads, head_size), dtype=dtype, device=key_cache.device)
+        out = tuple(torch.empty((n, heads, head_size), dtype=dtype, device=key_cache.device)
                     for _ in range(2))
     k, v = out
     if k.dtype != dtype or k.dim() != 3 or k.shape[2] != head_size:
@@ -195,7 +195,7 @@ def kv_read_int4(key_cache, value_cache, block_table, cache_seqlens, block_size,
     lib = _lib.load()
     with torch.cuda.device(device):
         rc = lib.pab200_kv_read_int4(ctypes.byref(a), None if starts is None else starts.data_ptr(),
-                                     0 if starts is None else starts.stride(0),
+                                     0 if starts is None else starts.stride(0), int(fresh),
                                      _current_stream_handle(device))
     _raise_for(lib, rc, "pab200_kv_read_int4")
     del keep

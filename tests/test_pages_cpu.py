@@ -98,7 +98,7 @@ def test_rows_refusals(field, value, code):
     a = _rows()
     setattr(a, field, value)
     assert lib.pab200_kv_append_int4(ctypes.byref(a), 1, None) == code
-    assert lib.pab200_kv_read_int4(ctypes.byref(a), None, 0, None) == code
+    assert lib.pab200_kv_read_int4(ctypes.byref(a), None, 0, 0, None) == code
     assert lib.pab200_last_error() != b""
 
 
@@ -108,10 +108,10 @@ def test_rows_edge_calls():
     a = _rows()
     a.num_seqs = a.num_tokens = 0
     assert lib.pab200_kv_append_int4(ctypes.byref(a), 1, None) == _lib.OK     # nothing to do
-    assert lib.pab200_kv_read_int4(ctypes.byref(a), None, 0, None) == _lib.OK
+    assert lib.pab200_kv_read_int4(ctypes.byref(a), None, 0, 0, None) == _lib.OK
     a = _rows()
     a.row_stride_t = 260                                                     # reads back in 16 bytes
-    assert lib.pab200_kv_read_int4(ctypes.byref(a), None, 0, None) == _lib.ERR_ALIGNMENT
+    assert lib.pab200_kv_read_int4(ctypes.byref(a), None, 0, 0, None) == _lib.ERR_ALIGNMENT
 
 
 def _decode():
