@@ -5,7 +5,7 @@ Drop-in for the decode path of lashhw/pagedattention: the same
 hand-written CUDA kernels in ``libpab200.so`` (C ABI: include/pab200.h).
 """
 from .common import _validate_decode_inputs
-from .int4_cache import (
+from .int4 import (
     int4_cache,
     int4_page_bytes,
     kv_append_int4,

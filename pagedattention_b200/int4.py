@@ -15,16 +15,18 @@ page takes 9/32 of the bytes of its 16-bit rows.
 """
 from __future__ import annotations
 
-import ctypes
-
 import torch
 
 from . import _lib
 from .kernel_b200 import (_DTYPES, _append_status_word, _as_int32, _check_device,
-                          _current_stream_handle, _fill_common, _keep_workspace, _raise_for)
+                          _keep_workspace, _on_device, _raise_for)
 
 _HEAD_SIZES = (64, 128, 256)
 _BLOCK_SIZES = (8, 16, 32, 64)
+
+
+def _append_status_ptr(device) -> int:
+    return _append_status_word(device).data_ptr()
 
 
 def int4_page_bytes(head_size: int, block_size: int) -> int:
@@ -42,46 +44,53 @@ def int4_cache(num_blocks, num_kv_heads, block_size, head_size, device="cuda"):
     return tuple(torch.zeros(shape, dtype=torch.uint8, device=device) for _ in range(2))
 
 
+def _check_table(block_table, num_seqs, num_kv_heads):
+    """The block table as int32, its max_blocks and strides (b, h, i)."""
+    bt = _as_int32(block_table, "block_table")
+    shape, st = bt.shape, bt.stride()
+    if len(shape) == 2 and shape[0] == num_seqs:
+        return bt, shape[1], (st[0], 0, st[1])
+    if len(shape) == 3 and shape[0] == num_seqs and shape[1] == num_kv_heads:
+        return bt, shape[2], st
+    raise ValueError("block table must be (num_seqs, max_blocks) or "
+                     "(num_seqs, num_kv_heads, max_blocks)")
+
+
 def _check_caches(key_cache, value_cache, block_table, head_size, block_size, num_seqs,
                   num_kv_heads):
     """Checks of the caches and their table; returns (table, page count, kv
     heads, bt_page_mul, bt_page_add, max_blocks, table strides)."""
     if key_cache.dtype != torch.uint8 or value_cache.dtype != torch.uint8:
         raise TypeError("4-bit caches must be uint8 tensors")
-    if tuple(key_cache.shape) != tuple(value_cache.shape):
+    shape = key_cache.shape
+    if shape != value_cache.shape:
         raise ValueError("key_cache and value_cache shapes differ")
     if not (key_cache.is_contiguous() and value_cache.is_contiguous()):
         raise ValueError("key_cache and value_cache must be contiguous")
-    if key_cache.shape[-1] != int4_page_bytes(head_size, block_size):
-        raise ValueError(f"pages of {key_cache.shape[-1]} bytes, head_size {head_size} and "
+    if shape[-1] != int4_page_bytes(head_size, block_size):
+        raise ValueError(f"pages of {shape[-1]} bytes, head_size {head_size} and "
                          f"block_size {block_size} need {int4_page_bytes(head_size, block_size)}")
-    bt = _as_int32(block_table, "block_table")
-    if key_cache.dim() == 3:
-        nb, heads, _ = key_cache.shape
-        num_pages, mul, add = nb * heads, heads, 1
-    elif key_cache.dim() == 2:
-        if bt.dim() != 3:
+    if len(shape) == 3:
+        heads = shape[1]
+        num_pages, mul, add = shape[0] * heads, heads, 1
+    elif len(shape) == 2:
+        if block_table.dim() != 3:
             raise ValueError("a 2-D (per-head page) cache needs a block table "
                              "(num_seqs, num_kv_heads, max_blocks)")
-        num_pages, heads, mul, add = key_cache.shape[0], bt.shape[1], 1, 0
+        num_pages, heads, mul, add = shape[0], block_table.shape[1], 1, 0
     else:
-        raise ValueError(f"unsupported 4-bit cache rank {key_cache.dim()}")
+        raise ValueError(f"unsupported 4-bit cache rank {len(shape)}")
     if num_kv_heads is not None and heads != num_kv_heads:
         raise ValueError(f"cache has {heads} kv heads, the rows {num_kv_heads}")
-    if bt.dim() == 3 and tuple(bt.shape[:2]) == (num_seqs, heads):
-        strides, maxb = bt.stride(), bt.shape[2]
-    elif bt.dim() == 2 and bt.shape[0] == num_seqs:
-        strides, maxb = (bt.stride(0), 0, bt.stride(1)), bt.shape[1]
-    else:
-        raise ValueError("block table must be (num_seqs, max_blocks) or "
-                         "(num_seqs, num_kv_heads, max_blocks)")
+    bt, maxb, strides = _check_table(block_table, num_seqs, heads)
     return bt, num_pages, heads, mul, add, maxb, strides
 
 
 def _length_strides(lens, num_seqs, heads, name):
-    if lens.dim() == 1 and lens.shape[0] == num_seqs:
+    shape = lens.shape
+    if len(shape) == 1 and shape[0] == num_seqs:
         return lens.stride(0), 0
-    if lens.dim() == 2 and tuple(lens.shape) == (num_seqs, heads):
+    if len(shape) == 2 and shape[0] == num_seqs and shape[1] == heads:
         return lens.stride()
     raise ValueError(f"{name} must be (num_seqs,) or (num_seqs, num_kv_heads)")
 
@@ -99,35 +108,30 @@ def _check_offsets(cu, num_seqs, name):
 
 def _rows_args(key_cache, value_cache, k, v, lens, block_table, cu, block_size, what):
     """The arguments append and read-back share."""
-    if k.dim() != 3 or tuple(k.shape) != tuple(v.shape):
+    shape, st = k.shape, k.stride()
+    if len(shape) != 3 or shape != v.shape:
         raise ValueError(f"{what} must be (num_tokens, num_kv_heads, head_size)")
-    if k.dtype not in _DTYPES or v.dtype != k.dtype:
+    code = _DTYPES.get(k.dtype)
+    if code is None or v.dtype != k.dtype:
         raise TypeError(f"{what} must share one dtype, bfloat16 or float16")
-    if k.stride(2) != 1 or v.stride(2) != 1 or k.stride() != v.stride():
+    if st[2] != 1 or v.stride() != st:
         raise ValueError(f"{what} must share strides, contiguous in head_size")
-    N, Hkv, D = k.shape
+    N, Hkv, D = shape
     B = lens.shape[0]
     bt, num_pages, _, mul, add, maxb, bts = _check_caches(key_cache, value_cache, block_table, D,
                                                           block_size, B, Hkv)
     lsb, lsh = _length_strides(lens, B, Hkv, "cache_seqlens")
-    if cu is None and N != B:
-        raise ValueError(f"{N} tokens for {B} sequences need token offsets")
-    tensors = [key_cache, value_cache, k, v, lens, bt] + ([] if cu is None else [cu])
-    device = _check_device(*tensors)
-    a = _lib.Int4RowsArgs()
-    a.k_cache, a.v_cache = key_cache.data_ptr(), value_cache.data_ptr()
-    a.k_rows, a.v_rows = k.data_ptr(), v.data_ptr()
-    a.seqlens, a.block_table = lens.data_ptr(), bt.data_ptr()
-    a.cu_tokens = None if cu is None else cu.data_ptr()
-    a.status = _append_status_word(device).data_ptr()
-    a.dtype, a.num_seqs, a.num_kv_heads = _DTYPES[k.dtype], B, Hkv
-    a.head_size, a.block_size, a.max_blocks = D, block_size, maxb
-    a.num_pages, a.num_tokens = num_pages, N
-    a.row_stride_t, a.row_stride_h = k.stride(0), k.stride(1)
-    a.seqlens_stride_b, a.seqlens_stride_h = lsb, lsh
-    a.bt_stride_b, a.bt_stride_h, a.bt_stride_i = bts
-    a.bt_page_mul, a.bt_page_add = mul, add
-    return a, device, bt
+    if cu is None:
+        if N != B:
+            raise ValueError(f"{N} tokens for {B} sequences need token offsets")
+        device = _check_device(key_cache, value_cache, k, v, lens, bt)
+    else:
+        device = _check_device(key_cache, value_cache, k, v, lens, bt, cu)
+    args = _lib.Int4RowsArgs(
+        key_cache.data_ptr(), value_cache.data_ptr(), k.data_ptr(), v.data_ptr(), lens.data_ptr(),
+        bt.data_ptr(), None if cu is None else cu.data_ptr(), _append_status_ptr(device), code, B, Hkv,
+        D, block_size, maxb, num_pages, N, st[0], st[1], lsb, lsh, *bts, mul, add)
+    return args, device, bt
 
 
 def kv_append_int4(key_cache, value_cache, k_new, v_new, cache_seqlens, block_table, block_size,
@@ -150,10 +154,9 @@ def kv_append_int4(key_cache, value_cache, k_new, v_new, cache_seqlens, block_ta
     a, device, keep = _rows_args(key_cache, value_cache, k_new, v_new, cache_seqlens, block_table,
                                  cu, block_size, "k_new and v_new")
     lib = _lib.load()
-    with torch.cuda.device(device):
-        rc = lib.pab200_kv_append_int4(ctypes.byref(a), 1 if increment else 0,
-                                       _current_stream_handle(device))
-    _raise_for(lib, rc, "pab200_kv_append_int4")
+    rc = _on_device(device, lib.pab200_kv_append_int4, a, 1 if increment else 0)
+    if rc:
+        _raise_for(lib, rc, "pab200_kv_append_int4")
     del keep
 
 
@@ -180,9 +183,10 @@ def kv_read_int4(key_cache, value_cache, block_table, cache_seqlens, block_size,
             raise ValueError("cu_out needs num_tokens (or out)")
         n = B if cu is None else int(num_tokens)
         heads = key_cache.shape[1] if key_cache.dim() == 3 else block_table.shape[1]
-        out = tuple(torch.empty((n, heads, head_size), dtype=dtype, device=key_cache.device)
-                    for _ in range(2))
-    k, v = out
+        k, v = torch.empty((2, n, heads, head_size), dtype=dtype,
+                           device=key_cache.device).unbind(0)
+    else:
+        k, v = out
     if k.dtype != dtype or k.dim() != 3 or k.shape[2] != head_size:
         raise ValueError("out must be a pair of (num_tokens, num_kv_heads, head_size) of dtype")
     if starts is not None:
@@ -190,14 +194,15 @@ def kv_read_int4(key_cache, value_cache, block_table, cache_seqlens, block_size,
         if starts.dim() != 1 or starts.shape[0] != B:
             raise ValueError("starts must be (num_seqs,)")
         _check_device(key_cache, starts)
+        first, step = starts.data_ptr(), starts.stride(0)
+    else:
+        first, step = None, 0
     a, device, keep = _rows_args(key_cache, value_cache, k, v, lens, block_table, cu, block_size,
                                  "out")
     lib = _lib.load()
-    with torch.cuda.device(device):
-        rc = lib.pab200_kv_read_int4(ctypes.byref(a), None if starts is None else starts.data_ptr(),
-                                     0 if starts is None else starts.stride(0), int(fresh),
-                                     _current_stream_handle(device))
-    _raise_for(lib, rc, "pab200_kv_read_int4")
+    rc = _on_device(device, lib.pab200_kv_read_int4, a, first, step, 1 if fresh else 0)
+    if rc:
+        _raise_for(lib, rc, "pab200_kv_read_int4")
     del keep
     return k, v
 
@@ -212,19 +217,21 @@ def paged_attention_int4(out, query, key_cache, value_cache, block_tables, conte
     context_lens (num_seqs,) or (num_seqs, num_kv_heads).  Query groups as for
     ``paged_attention``.
     """
-    if query.dim() != 3:
+    shape, qst, ost = query.shape, query.stride(), out.stride()
+    if len(shape) != 3:
         raise ValueError("query must be (num_seqs, num_q_heads, head_size)")
-    if query.dtype not in _DTYPES:
+    code = _DTYPES.get(query.dtype)
+    if code is None:
         raise TypeError(f"query must be bfloat16 or float16, got {query.dtype}")
-    if query.stride(2) != 1:
+    if qst[2] != 1:
         raise ValueError("query must be contiguous in head_size")
-    if out.shape != query.shape or out.dtype != query.dtype:
+    if out.shape != shape or out.dtype != query.dtype:
         raise ValueError("out must match query in shape and dtype")
-    if out.stride(2) != 1:
+    if ost[2] != 1:
         raise ValueError("out must be contiguous in head_size")
     if num_splits < 0:
         raise ValueError("num_splits must be >= 0")
-    B, Hq, D = query.shape
+    B, Hq, D = shape
     bt, num_pages, Hkv, mul, add, maxb, bts = _check_caches(key_cache, value_cache, block_tables, D,
                                                             block_size, B, None)
     if Hq % Hkv != 0:
@@ -234,23 +241,21 @@ def paged_attention_int4(out, query, key_cache, value_cache, block_tables, conte
     device = _check_device(query, out, key_cache, value_cache, bt, lens)
     if B == 0:
         return
-    args = _lib.DecodeArgs()
-    _fill_common(args, q=query, k_cache=key_cache, v_cache=value_cache, lens=lens, bt=bt,
-                 dtype=query.dtype, B=B, Hq=Hq, Hkv=Hkv, D=D, bs=block_size, num_pages=num_pages,
-                 scale=scale, num_splits=num_splits)
-    args.layout, args.max_blocks, args.out = _lib.LAYOUT_PAGES, maxb, out.data_ptr()
-    args.q_stride_b, args.q_stride_h = query.stride(0), query.stride(1)
-    args.out_stride_b, args.out_stride_h = out.stride(0), out.stride(1)
-    args.seqlens_stride_b, args.seqlens_stride_h = lsb, lsh
-    args.bt_stride_b, args.bt_stride_h, args.bt_stride_i = bts
-    args.bt_page_mul, args.bt_page_add = mul, add
+    args = _lib.DecodeArgs(
+        out.data_ptr(), query.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(),
+        lens.data_ptr(), bt.data_ptr(), code, _lib.LAYOUT_PAGES, B, Hq, Hkv, D, block_size, maxb,
+        num_pages, qst[0], qst[1], ost[0], ost[1], lsb, lsh, *bts, mul, add, float(scale),
+        int(num_splits))
+    _on_device(device, _run_int4, args, device)
+
+
+def _run_int4(args, device, stream):
     lib = _lib.load()
-    with torch.cuda.device(device):
-        need = lib.pab200_decode_int4_workspace_size(ctypes.byref(args))
-        if need == 0:
-            raise ValueError(f"pab200_decode_int4: {lib.pab200_last_error().decode()}")
-        ws = torch.empty(need, dtype=torch.uint8, device=device)
-        stream = _current_stream_handle(device)
-        rc = lib.pab200_decode_int4(ctypes.byref(args), ws.data_ptr(), need, stream)
-    _raise_for(lib, rc, "pab200_decode_int4")
+    need = lib.pab200_decode_int4_workspace_size(args)
+    if need == 0:
+        raise ValueError(f"pab200_decode_int4: {lib.pab200_last_error().decode()}")
+    ws = torch.empty(need, dtype=torch.uint8, device=device)
+    rc = lib.pab200_decode_int4(args, ws.data_ptr(), need, stream)
+    if rc:
+        _raise_for(lib, rc, "pab200_decode_int4")
     _keep_workspace(device, ws, stream)

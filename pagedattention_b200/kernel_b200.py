@@ -185,6 +185,14 @@ def _raise_for(lib, rc, what) -> None:
     _lib.check(lib, rc, what)
 
 
+def _on_device(device, fn, *args):
+    """``fn(*args, stream)`` with ``device`` current and its current stream."""
+    if torch.cuda.current_device() == device.index:
+        return fn(*args, _current_stream_handle(device))
+    with torch.cuda.device(device):
+        return fn(*args, _current_stream_handle(device))
+
+
 def _keep_workspace(device, ws, stream_handle) -> None:
     """The workspace whose status word ``read_status`` reports next."""
     _last_ws[device.index] = (ws, stream_handle)

@@ -10,14 +10,12 @@ entry point takes; ``paged_attention_sparse`` selects and attends in one call.
 """
 from __future__ import annotations
 
-import ctypes
-
 import torch
 
 from . import _lib
-from .int4_cache import _check_offsets, _length_strides
-from .kernel_b200 import (_DTYPES, _append_status_word, _as_int32, _check_device,
-                          _current_stream_handle, _keep_workspace, _paged_args, _raise_for)
+from .int4 import _append_status_ptr, _check_offsets, _check_table, _length_strides
+from .kernel_b200 import (_DTYPES, _as_int32, _check_device, _keep_workspace, _on_device,
+                          _paged_args, _raise_for)
 
 
 def _check_bounds(page_bounds, block_table, num_seqs, num_kv_heads, head_size, dtype):
@@ -27,28 +25,22 @@ def _check_bounds(page_bounds, block_table, num_seqs, num_kv_heads, head_size, d
         raise TypeError(f"page_bounds must have the keys' dtype {dtype}, got {page_bounds.dtype}")
     if not page_bounds.is_contiguous():
         raise ValueError("page_bounds must be contiguous")
-    if tuple(page_bounds.shape[-2:]) != (2, head_size):
+    shape = page_bounds.shape
+    if len(shape) < 2 or shape[-2] != 2 or shape[-1] != head_size:
         raise ValueError("page_bounds must end in (2, head_size)")
-    bt = _as_int32(block_table, "block_table")
-    if page_bounds.dim() == 4:
-        if page_bounds.shape[1] != num_kv_heads:
-            raise ValueError(f"page_bounds has {page_bounds.shape[1]} kv heads, not {num_kv_heads}")
-        num_pages, mul, add = page_bounds.shape[0] * num_kv_heads, num_kv_heads, 1
-    elif page_bounds.dim() == 3:
-        if bt.dim() != 3:
+    if len(shape) == 4:
+        if shape[1] != num_kv_heads:
+            raise ValueError(f"page_bounds has {shape[1]} kv heads, not {num_kv_heads}")
+        num_pages, mul, add = shape[0] * num_kv_heads, num_kv_heads, 1
+    elif len(shape) == 3:
+        if block_table.dim() != 3:
             raise ValueError("3-D (per-head page) bounds need a block table "
                              "(num_seqs, num_kv_heads, max_blocks)")
-        num_pages, mul, add = page_bounds.shape[0], 1, 0
+        num_pages, mul, add = shape[0], 1, 0
     else:
         raise ValueError("page_bounds must be (num_blocks, num_kv_heads, 2, head_size) or "
                          "(num_pages, 2, head_size)")
-    if bt.dim() == 3 and tuple(bt.shape[:2]) == (num_seqs, num_kv_heads):
-        strides, maxb = bt.stride(), bt.shape[2]
-    elif bt.dim() == 2 and bt.shape[0] == num_seqs:
-        strides, maxb = (bt.stride(0), 0, bt.stride(1)), bt.shape[1]
-    else:
-        raise ValueError("block table must be (num_seqs, max_blocks) or "
-                         "(num_seqs, num_kv_heads, max_blocks)")
+    bt, maxb, strides = _check_table(block_table, num_seqs, num_kv_heads)
     return bt, num_pages, mul, add, maxb, strides
 
 
@@ -63,52 +55,51 @@ def update_page_bounds(page_bounds, k_new, cache_seqlens, block_table, block_siz
     afresh, any other is widened.  Tokens without a place are left out and set a
     bit read by ``kv_append_status``.
     """
-    if k_new.dim() != 3:
+    shape, st = k_new.shape, k_new.stride()
+    if len(shape) != 3:
         raise ValueError("k_new must be (num_tokens, num_kv_heads, head_size)")
-    if k_new.dtype not in _DTYPES:
+    code = _DTYPES.get(k_new.dtype)
+    if code is None:
         raise TypeError(f"k_new must be bfloat16 or float16, got {k_new.dtype}")
-    if k_new.stride(2) != 1:
+    if st[2] != 1:
         raise ValueError("k_new must be contiguous in head_size")
-    N, Hkv, D = k_new.shape
+    N, Hkv, D = shape
     lens = _as_int32(cache_seqlens, "cache_seqlens")
     B = lens.shape[0]
     cu = _check_offsets(cu_new, B, "cu_new")
-    if cu is None and N != B:
-        raise ValueError(f"{N} tokens for {B} sequences need cu_new")
     bt, num_pages, mul, add, maxb, bts = _check_bounds(page_bounds, block_table, B, Hkv, D,
                                                        k_new.dtype)
     lsb, lsh = _length_strides(lens, B, Hkv, "cache_seqlens")
-    device = _check_device(*([page_bounds, k_new, lens, bt] + ([] if cu is None else [cu])))
-    a = _lib.PageBoundsArgs()
-    a.page_bounds, a.k_rows = page_bounds.data_ptr(), k_new.data_ptr()
-    a.seqlens, a.block_table = lens.data_ptr(), bt.data_ptr()
-    a.cu_tokens = None if cu is None else cu.data_ptr()
-    a.status = _append_status_word(device).data_ptr()
-    a.dtype, a.num_seqs, a.num_kv_heads = _DTYPES[k_new.dtype], B, Hkv
-    a.head_size, a.block_size, a.max_blocks = D, block_size, maxb
-    a.num_pages, a.num_tokens = num_pages, N
-    a.row_stride_t, a.row_stride_h = k_new.stride(0), k_new.stride(1)
-    a.seqlens_stride_b, a.seqlens_stride_h = lsb, lsh
-    a.bt_stride_b, a.bt_stride_h, a.bt_stride_i = bts
-    a.bounds_page_mul, a.bounds_page_add = mul, add
+    if cu is None:
+        if N != B:
+            raise ValueError(f"{N} tokens for {B} sequences need cu_new")
+        device = _check_device(page_bounds, k_new, lens, bt)
+    else:
+        device = _check_device(page_bounds, k_new, lens, bt, cu)
+    a = _lib.PageBoundsArgs(
+        page_bounds.data_ptr(), k_new.data_ptr(), lens.data_ptr(), bt.data_ptr(),
+        None if cu is None else cu.data_ptr(), _append_status_ptr(device), code, B, Hkv, D,
+        block_size, maxb, num_pages, N, st[0], st[1], lsb, lsh, *bts, mul, add)
     lib = _lib.load()
-    with torch.cuda.device(device):
-        rc = lib.pab200_update_page_bounds(ctypes.byref(a), _current_stream_handle(device))
-    _raise_for(lib, rc, "pab200_update_page_bounds")
+    rc = _on_device(device, lib.pab200_update_page_bounds, a)
+    if rc:
+        _raise_for(lib, rc, "pab200_update_page_bounds")
 
 
 def _select_args(query, page_bounds, block_tables, context_lens, block_size, num_selected, num_sink,
                  num_recent, num_kv_heads):
-    if query.dim() != 3:
+    shape, qst = query.shape, query.stride()
+    if len(shape) != 3:
         raise ValueError("query must be (num_seqs, num_q_heads, head_size)")
-    if query.dtype not in _DTYPES:
+    code = _DTYPES.get(query.dtype)
+    if code is None:
         raise TypeError(f"query must be bfloat16 or float16, got {query.dtype}")
-    if query.stride(2) != 1:
+    if qst[2] != 1:
         raise ValueError("query must be contiguous in head_size")
     if num_sink < 0 or num_recent < 1 or num_sink + num_recent > num_selected:
         raise ValueError("need num_sink >= 0, num_recent >= 1 and "
                          "num_sink + num_recent <= num_selected")
-    B, Hq, D = query.shape
+    B, Hq, D = shape
     if B < 1 or Hq % num_kv_heads != 0:
         raise ValueError(f"num_q_heads {Hq} is not a multiple of num_kv_heads {num_kv_heads}, "
                          "or there is no sequence")
@@ -119,19 +110,10 @@ def _select_args(query, page_bounds, block_tables, context_lens, block_size, num
     device = _check_device(query, page_bounds, bt, lens)
     tables = torch.empty((B, num_kv_heads, num_selected), dtype=torch.int32, device=device)
     out_lens = torch.empty((B, num_kv_heads), dtype=torch.int32, device=device)
-    a = _lib.SelectArgs()
-    a.q, a.page_bounds = query.data_ptr(), page_bounds.data_ptr()
-    a.seqlens, a.block_table = lens.data_ptr(), bt.data_ptr()
-    a.tables, a.selected_lens = tables.data_ptr(), out_lens.data_ptr()
-    a.status = _append_status_word(device).data_ptr()
-    a.dtype, a.num_seqs, a.num_q_heads, a.num_kv_heads = _DTYPES[query.dtype], B, Hq, num_kv_heads
-    a.head_size, a.block_size, a.max_blocks = D, block_size, maxb
-    a.num_selected, a.num_sink, a.num_recent = num_selected, num_sink, num_recent
-    a.num_pages = num_pages
-    a.q_stride_b, a.q_stride_h = query.stride(0), query.stride(1)
-    a.seqlens_stride_b, a.seqlens_stride_h = lsb, lsh
-    a.bt_stride_b, a.bt_stride_h, a.bt_stride_i = bts
-    a.bounds_page_mul, a.bounds_page_add = mul, add
+    a = _lib.SelectArgs(
+        query.data_ptr(), page_bounds.data_ptr(), lens.data_ptr(), bt.data_ptr(), tables.data_ptr(),
+        out_lens.data_ptr(), _append_status_ptr(device), code, B, Hq, num_kv_heads, D, block_size,
+        maxb, num_selected, num_sink, num_recent, num_pages, qst[0], qst[1], lsb, lsh, *bts, mul, add)
     return a, device, tables, out_lens, (bt, lens)
 
 
@@ -158,17 +140,20 @@ def select_pages(query, page_bounds, block_tables, context_lens, block_size, num
     a, device, tables, lens, keep = _select_args(query, page_bounds, block_tables, context_lens,
                                                  block_size, num_selected, num_sink, num_recent,
                                                  heads)
-    lib = _lib.load()
-    with torch.cuda.device(device):
-        need = lib.pab200_select_pages_workspace_size(ctypes.byref(a))
-        if need == 0:
-            raise ValueError(f"pab200_select_pages: {lib.pab200_last_error().decode()}")
-        ws = torch.empty(need, dtype=torch.uint8, device=device)
-        rc = lib.pab200_select_pages(ctypes.byref(a), ws.data_ptr(), need,
-                                     _current_stream_handle(device))
-    _raise_for(lib, rc, "pab200_select_pages")
+    _on_device(device, _run_select, a, device)
     del keep
     return tables, lens
+
+
+def _run_select(a, device, stream):
+    lib = _lib.load()
+    need = lib.pab200_select_pages_workspace_size(a)
+    if need == 0:
+        raise ValueError(f"pab200_select_pages: {lib.pab200_last_error().decode()}")
+    ws = torch.empty(need, dtype=torch.uint8, device=device)
+    rc = lib.pab200_select_pages(a, ws.data_ptr(), need, stream)
+    if rc:
+        _raise_for(lib, rc, "pab200_select_pages")
 
 
 def paged_attention_sparse(out, query, key_cache, value_cache, page_bounds, block_tables,
@@ -195,16 +180,18 @@ def paged_attention_sparse(out, query, key_cache, value_cache, page_bounds, bloc
                                                 args.num_kv_heads)
     if dev != device:
         raise ValueError(f"page_bounds must be on {device}")
-    lib = _lib.load()
-    with torch.cuda.device(device):
-        need = lib.pab200_decode_sparse_workspace_size(ctypes.byref(args), ctypes.byref(sel))
-        if need == 0:
-            raise ValueError(f"pab200_decode_sparse: {lib.pab200_last_error().decode()}")
-        ws = torch.empty(need, dtype=torch.uint8, device=device)
-        stream = _current_stream_handle(device)
-        rc = lib.pab200_decode_sparse(ctypes.byref(args), ctypes.byref(sel), ws.data_ptr(), need,
-                                      stream)
-    _raise_for(lib, rc, "pab200_decode_sparse")
-    _keep_workspace(device, ws, stream)
+    _on_device(device, _run_sparse, args, sel, device)
     del keep, kept
     return tables, lens
+
+
+def _run_sparse(args, sel, device, stream):
+    lib = _lib.load()
+    need = lib.pab200_decode_sparse_workspace_size(args, sel)
+    if need == 0:
+        raise ValueError(f"pab200_decode_sparse: {lib.pab200_last_error().decode()}")
+    ws = torch.empty(need, dtype=torch.uint8, device=device)
+    rc = lib.pab200_decode_sparse(args, sel, ws.data_ptr(), need, stream)
+    if rc:
+        _raise_for(lib, rc, "pab200_decode_sparse")
+    _keep_workspace(device, ws, stream)
