@@ -95,7 +95,7 @@ struct SelectParams {
   float* scores;       // [B * Hkv][maxb]
   uint32_t* status;
   int64_t q_sb, q_sh, l_sb, l_sh, bt_sb, bt_sh, bt_si, num_pages;
-  int32_t bt_mul, bt_add, B, Hkv, G, bs, maxb, keep, sink, recent;
+  int32_t bt_mul, bt_add, B, Hkv, G, bs, maxb, keep, sink, recent, chunk;
 };
 
 __device__ __forceinline__ int clamped_length(const SelectParams& p, int s, int h) {
@@ -108,61 +108,87 @@ __device__ __forceinline__ int clamped_length(const SelectParams& p, int s, int 
 // elements of max * (sum of the group's positive query parts) + min * (sum of
 // the negative ones), the upper bound of the group's summed scores.  Summed in
 // 64 bits and rounded once, so that the order of the sum cannot change which
-// pages rank next to the border.
+// pages rank next to the border.  Bound: the bounds' bytes, nearly level with
+// the conversions to 64 bits (16 a clock and SM, one per bound).
+//
+// blockIdx.x: chunk of p.chunk pages, 8 warps of p.chunk / 8 (at most 32); D/8
+// lanes per page, kUnroll steps of 256/D pages in flight.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) page_scores_kernel(const SelectParams p) {
-  constexpr int LP = D / 8, PW = 32 / LP;  // lanes per page, pages per warp step
+  constexpr int LP = D / 8, PW = 32 / LP, kUnroll = 4;
   __shared__ double qs[2][D];
+  grid_launch_dependents();
   const int u = blockIdx.y, s = u / p.Hkv, h = u - s * p.Hkv;
-  const int L = clamped_length(p, s, h);
-  const int n = (L + p.bs - 1) / p.bs;
-  if (n <= p.keep) return;
+  const int n = (clamped_length(p, s, h) + p.bs - 1) / p.bs;
+  const int c0 = p.sink + blockIdx.x * p.chunk, c1 = min(c0 + p.chunk, n - p.recent);
+  if (n <= p.keep || c0 >= c1) return;
+  const int lane = threadIdx.x & 31, e = lane % LP, per = p.chunk / 8;
+  const int w0 = c0 + (threadIdx.x >> 5) * per;
+  // This warp's pages, one id per lane; -1: out of range.
+  int id = -1;
+  if (lane < per && w0 + lane < c1) {
+    const int64_t pid =
+        static_cast<int64_t>(p.bt[s * p.bt_sb + h * p.bt_sh + (w0 + lane) * p.bt_si]) * p.bt_mul +
+        static_cast<int64_t>(h) * p.bt_add;
+    if (pid >= 0 && pid < p.num_pages)
+      id = static_cast<int>(pid);
+    else if (p.status)
+      atomicOr(p.status, kStatusBadPage);
+  }
   const T* q = static_cast<const T*>(p.q) + s * p.q_sb + static_cast<int64_t>(h) * p.G * p.q_sh;
   for (int d = threadIdx.x; d < D; d += 256) {
     double up = 0.0, dn = 0.0;
     for (int g = 0; g < p.G; ++g) {
-      const double x = static_cast<double>(static_cast<float>(q[g * p.q_sh + d]));
-      up += x > 0.0 ? x : 0.0;
-      dn += x < 0.0 ? x : (x > 0.0 ? 0.0 : x);
+      const float x = static_cast<float>(q[g * p.q_sh + d]);
+      up += x > 0.f ? x : 0.f;
+      dn += x > 0.f ? 0.f : x;  // a NaN makes this one NaN
     }
     qs[0][d] = up;
     qs[1][d] = dn;
   }
   __syncthreads();
-  const int lane = threadIdx.x & 31, e = lane % LP;
   double up[8], dn[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     up[i] = qs[0][e * 8 + i];
     dn[i] = qs[1][e * 8 + i];
   }
-  const int warps = gridDim.x * 8;
-  uint32_t flags = 0;
-  const int c1 = n - p.recent;
-  for (int c0 = p.sink + (blockIdx.x * 8 + (threadIdx.x >> 5)) * PW; c0 < c1; c0 += warps * PW) {
-    const int c = c0 + lane / LP;
-    double sum = 0.0;
-    bool bad = false;
-    if (c < c1) {
-      const int64_t pid = static_cast<int64_t>(p.bt[s * p.bt_sb + h * p.bt_sh + c * p.bt_si]) * p.bt_mul +
-                          static_cast<int64_t>(h) * p.bt_add;
-      bad = pid < 0 || pid >= p.num_pages;
-      if (!bad) {
-        const T* b = static_cast<const T*>(p.bounds) + pid * (2 * D) + e * 8;
-        float mn[8], mx[8];
-        unpack8<T>(__ldg(reinterpret_cast<const uint4*>(b)), mn);
-        unpack8<T>(__ldg(reinterpret_cast<const uint4*>(b + D)), mx);
+  float* out = p.scores + static_cast<int64_t>(u) * p.maxb + w0;
+  const int count = min(per, c1 - w0);
+  for (int t = 0; t < count; t += PW * kUnroll) {
+    uint4 mn[kUnroll], mx[kUnroll];
+    int pid[kUnroll];
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          sum = fma(static_cast<double>(mx[i]), up[i], fma(static_cast<double>(mn[i]), dn[i], sum));
+    for (int v = 0; v < kUnroll; ++v) {
+      const int at = t + v * PW + lane / LP;
+      pid[v] = __shfl_sync(0xffffffffu, id, at & 31);
+      if (at >= count) pid[v] = -1;
+      mn[v] = mx[v] = make_uint4(0u, 0u, 0u, 0u);
+      if (pid[v] >= 0) {
+        const T* b = static_cast<const T*>(p.bounds) + static_cast<int64_t>(pid[v]) * (2 * D) + e * 8;
+        mn[v] = __ldg(reinterpret_cast<const uint4*>(b));
+        mx[v] = __ldg(reinterpret_cast<const uint4*>(b + D));
       }
     }
 #pragma unroll
-    for (int o = 1; o < LP; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (bad) flags |= kStatusBadPage;
-    if (e == 0 && c < c1) p.scores[static_cast<int64_t>(u) * p.maxb + c] = bad ? -INFINITY : static_cast<float>(sum);
+    for (int v = 0; v < kUnroll; ++v) {
+      if (t + v * PW >= count) break;
+      float lo[8], hi[8];
+      unpack8<T>(mn[v], lo);
+      unpack8<T>(mx[v], hi);
+      double a = 0.0, b = 0.0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        a = fma(static_cast<double>(hi[i]), up[i], a);
+        b = fma(static_cast<double>(lo[i]), dn[i], b);
+      }
+      a += b;
+#pragma unroll
+      for (int o = 1; o < LP; o <<= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
+      const int at = t + v * PW + lane / LP;
+      if (e == 0 && at < count) out[at] = pid[v] < 0 ? -INFINITY : static_cast<float>(a);
+    }
   }
-  if (flags && p.status) atomicOr(p.status, flags);
 }
 
 // Order-preserving key of a score: larger scores have larger keys, -0 and +0
@@ -173,7 +199,8 @@ __device__ __forceinline__ uint32_t score_key(float f) {
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
-// Sum of x over the block's threads before this one, and the total.
+// Sum of x over the block's threads before this one, and the total (1024
+// threads; `warp_sum` 32 words, free to reuse after the next barrier).
 __device__ __forceinline__ int block_scan(int x, int* warp_sum, int* total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int v = x;
@@ -182,99 +209,124 @@ __device__ __forceinline__ int block_scan(int x, int* warp_sum, int* total) {
     const int y = __shfl_up_sync(0xffffffffu, v, o);
     if (lane >= o) v += y;
   }
-  __syncthreads();
   if (lane == 31) warp_sum[warp] = v;
   __syncthreads();
-  int before = 0, all = 0;
-  for (int w = 0; w < static_cast<int>(blockDim.x >> 5); ++w) {
-    if (w < warp) before += warp_sum[w];
-    all += warp_sum[w];
+  int w = warp_sum[lane];
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, w, o);
+    if (lane >= o) w += y;
   }
-  *total = all;
-  return before + v - x;
+  *total = __shfl_sync(0xffffffffu, w, 31);
+  const int before = __shfl_sync(0xffffffffu, w, warp ? warp - 1 : 0);
+  return (warp ? before : 0) + v - x;
 }
 
-// One CTA per (sequence, kv head): the pages to attend to, ascending.  Radix
-// selection of the k-th largest key, 8 bits a pass; the pages above it, and
-// the first of those equal to it, are kept.
+// One CTA per (sequence, kv head): the pages to attend to, ascending.  The k-th
+// largest key is found by counting: the range between the smallest and the
+// largest key is cut into 1024 bins, the bin that holds the k-th becomes the
+// range, until a bin is one key wide (at most four passes, mostly two: the
+// scores fill their own range, so that no bin is crowded and the shared-memory
+// counters do not serialise).  Keys above it are kept, of the equal ones the
+// first.  A thread owns consecutive pages, so that one scan places them in
+// order; up to kPer of its keys stay in registers.
 __global__ void __launch_bounds__(1024) select_pages_kernel(const SelectParams p) {
-  __shared__ int hist[256];
-  __shared__ int warp_sum[32];
-  __shared__ uint32_t sh_prefix;
+  constexpr int kBins = 1024, kPer = 8;
+  __shared__ int hist[kBins];
+  __shared__ int sum_a[32], sum_b[32];
+  __shared__ uint32_t sh_lo[32], sh_hi[32];
+  __shared__ uint32_t sh_bin;
   __shared__ int sh_rank;
+  grid_launch_dependents();
   const int u = blockIdx.x, s = u / p.Hkv, h = u - s * p.Hkv;
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int L = clamped_length(p, s, h);
   const int raw = p.lens[s * p.l_sb + h * p.l_sh];
-  if (tid == 0 && raw != L && p.status) atomicOr(p.status, raw < 0 ? kStatusNegative : kStatusClamp);
   const int n = (L + p.bs - 1) / p.bs;
   const int32_t* bt = p.bt + s * p.bt_sb + h * p.bt_sh;
   int32_t* out = p.tables + static_cast<int64_t>(u) * p.keep;
+  grid_dependency_wait();  // the scores; nothing of this call is written before
+  if (tid == 0 && raw != L && p.status) atomicOr(p.status, raw < 0 ? kStatusNegative : kStatusClamp);
   if (n <= p.keep) {
     for (int i = tid; i < p.keep; i += 1024) out[i] = i < n ? bt[i * p.bt_si] : -1;
     if (tid == 0) p.out_lens[u] = L;
     return;
   }
-  const float* sc = p.scores + static_cast<int64_t>(u) * p.maxb;
-  const int c0 = p.sink, c1 = n - p.recent;
-  const int k = p.keep - p.sink - p.recent;  // candidates kept
-  uint32_t prefix = 0;
-  int rank = k;  // the rank-th largest key is looked for among keys that begin with prefix
-  if (k > 0) {
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      if (tid < 256) hist[tid] = 0;
-      __syncthreads();
-      for (int c = c0 + tid; c < c1; c += 1024) {
-        const uint32_t key = score_key(sc[c]);
-        if (shift == 24 || (key >> (shift + 8)) == (prefix >> (shift + 8)))
-          atomicAdd(&hist[(key >> shift) & 255u], 1);
-      }
-      __syncthreads();
-      if (tid < 32) {  // bins from the top: lane l holds bins 255 - 8 l .. 248 - 8 l
-        int sum = 0;
-        for (int i = 0; i < 8; ++i) sum += hist[255 - (tid * 8 + i)];
-        int v = sum;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const int y = __shfl_up_sync(0xffffffffu, v, o);
-          if (tid >= o) v += y;
-        }
-        int before = v - sum;
-        if (before < rank && rank <= v) {
-          for (int i = 0; i < 8; ++i) {
-            const int bin = 255 - (tid * 8 + i);
-            if (rank <= before + hist[bin]) {
-              sh_prefix = prefix | static_cast<uint32_t>(bin) << shift;
-              sh_rank = rank - before;
-              break;
-            }
-            before += hist[bin];
-          }
-        }
-      }
-      __syncthreads();
-      prefix = sh_prefix;
-      rank = sh_rank;
-      __syncthreads();
-    }
-  }
-  // Keys above `prefix` are kept, of the equal ones the first `rank`.
-  int kept = 0, equal = 0;
-  for (int b0 = c0; b0 < c1 && k > 0; b0 += 1024) {
-    const int c = b0 + tid;
-    const uint32_t key = c < c1 ? score_key(sc[c]) : 0u;
-    const bool eq = c < c1 && key == prefix;
-    int total;
-    const int eq_before = equal + block_scan(eq, warp_sum, &total);
-    equal += total;
-    const bool take = c < c1 && (key > prefix || (eq && eq_before < rank));
-    const int at = kept + block_scan(take, warp_sum, &total);
-    kept += total;
-    if (take) out[p.sink + at] = bt[c * p.bt_si];
-  }
+  const int c0 = p.sink, m = n - p.sink - p.recent;  // candidates, of which k are kept
+  const int k = p.keep - p.sink - p.recent;
   for (int i = tid; i < p.sink; i += 1024) out[i] = bt[i * p.bt_si];
-  for (int i = tid; i < p.recent; i += 1024) out[p.keep - p.recent + i] = bt[(c1 + i) * p.bt_si];
+  for (int i = tid; i < p.recent; i += 1024)
+    out[p.keep - p.recent + i] = bt[(n - p.recent + i) * p.bt_si];
   if (tid == 0) p.out_lens[u] = (p.keep - 1) * p.bs + L - (n - 1) * p.bs;
+  if (k == 0) return;
+  const float* sc = p.scores + static_cast<int64_t>(u) * p.maxb + c0;
+  const int per = (m + 1023) >> 10;
+  const int i0 = min(tid * per, m), i1 = min(i0 + per, m);
+  uint32_t key[kPer];
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) key[j] = i0 + j < i1 ? score_key(__ldcg(sc + i0 + j)) : 0u;
+  auto each = [&](auto&& fn) {  // this thread's keys, in page order
+#pragma unroll
+    for (int j = 0; j < kPer; ++j)
+      if (i0 + j < i1) fn(i0 + j, key[j]);
+    for (int i = i0 + kPer; i < i1; ++i) fn(i, score_key(__ldcg(sc + i)));
+  };
+  uint32_t lo = 0xffffffffu, hi = 0u;
+  each([&](int, uint32_t x) {
+    lo = min(lo, x);
+    hi = max(hi, x);
+  });
+  lo = __reduce_min_sync(0xffffffffu, lo);
+  hi = __reduce_max_sync(0xffffffffu, hi);
+  if (lane == 0) {
+    sh_lo[warp] = lo;
+    sh_hi[warp] = hi;
+  }
+  hist[tid] = 0;
+  __syncthreads();
+  lo = __reduce_min_sync(0xffffffffu, sh_lo[lane]);
+  hi = __reduce_max_sync(0xffffffffu, sh_hi[lane]);
+  int rank = k;  // the rank-th largest key of [lo, hi] is looked for
+  while (lo < hi) {
+    const int bits = 32 - __clz(hi - lo);
+    const int shift = bits > 10 ? bits - 10 : 0;
+    each([&](int, uint32_t x) {
+      if (x >= lo && x <= hi) atomicAdd(&hist[(x - lo) >> shift], 1);
+    });
+    __syncthreads();
+    // thread t looks at bin 1023 - t: how many keys lie in the bins above it
+    const int mine = hist[kBins - 1 - tid];
+    int total;
+    const int above = block_scan(mine, sum_a, &total);
+    if (above < rank && rank <= above + mine) {
+      sh_bin = kBins - 1 - tid;
+      sh_rank = rank - above;
+    }
+    hist[kBins - 1 - tid] = 0;
+    __syncthreads();
+    const uint32_t bin = sh_bin;
+    rank = sh_rank;
+    const uint32_t first = lo + (bin << shift);
+    const uint32_t last = first + ((1u << shift) - 1u);
+    lo = first;
+    hi = last < hi ? last : hi;
+    if (shift == 0) hi = lo;
+  }
+  // Keys above lo are kept, of the equal ones the first `rank`.
+  int gt = 0, eq = 0;
+  each([&](int, uint32_t x) {
+    gt += x > lo;
+    eq += x == lo;
+  });
+  int total;
+  __syncthreads();
+  const int gt_before = block_scan(gt, sum_a, &total);
+  int eq_before = block_scan(eq, sum_b, &total);
+  int at = gt_before + min(eq_before, rank);
+  each([&](int i, uint32_t x) {
+    if (x > lo || (x == lo && eq_before < rank)) out[p.sink + at++] = bt[(c0 + i) * p.bt_si];
+    eq_before += x == lo;
+  });
 }
 
 }  // namespace pab
@@ -365,17 +417,23 @@ int launch_select(const pab200_select_args* a, void* scores, cudaStream_t s) {
   p.sink = a->num_sink;
   p.recent = a->num_recent;
   const unsigned units = static_cast<unsigned>(p.B * p.Hkv);
-  if (p.maxb > p.keep) {
-    const int per_cta = 8 * 32 / (a->head_size / 8) * 4;
-    unsigned chunks = static_cast<unsigned>((p.maxb + per_cta - 1) / per_cta);
-    const unsigned most = (8u * pabh::device_sm_count_current() + units - 1) / units;
-    if (chunks > most) chunks = most;
+  const bool scored = p.maxb > p.keep;
+  if (scored) {
+    // Pages per CTA: 256 (32 per warp), fewer while that leaves SMs idle.
+    const int64_t pages = int64_t(units) * p.maxb;
+    int chunk = 256;
+    while (chunk > 32 && pages / chunk < 4 * pabh::device_sm_count_current()) chunk /= 2;
+    p.chunk = chunk;
+    const dim3 grid((p.maxb + chunk - 1) / chunk, units);
     if (a->dtype == PAB200_DTYPE_BF16)
-      launch_scores<__nv_bfloat16>(p, a->head_size, dim3(chunks, units), s);
+      launch_scores<__nv_bfloat16>(p, a->head_size, grid, s);
     else
-      launch_scores<__half>(p, a->head_size, dim3(chunks, units), s);
+      launch_scores<__half>(p, a->head_size, grid, s);
   }
-  pab::select_pages_kernel<<<units, 1024, 0, s>>>(p);
+  // Scheduled while the scores drain; waits for them before it reads any.
+  pabh::LaunchCfg lc(dim3(units), dim3(1024), 0, s, scored);
+  cudaError_t err = cudaLaunchKernelEx(&lc.cfg, pab::select_pages_kernel, p);
+  if (err != cudaSuccess) return pabh::cuda_fail(err, "page selection launch");
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? PAB200_OK : pabh::cuda_fail(e, "page selection launch");
 }
