@@ -1,6 +1,7 @@
 // Page-sparse decode: key bounds of pages, selection of pages by a query, and
 // the decode over the selected pages.
 #include "host.h"
+#include "int4.cuh"
 #include "tokens.cuh"
 
 namespace pab {
@@ -85,6 +86,24 @@ __global__ void __launch_bounds__(256) page_bounds_kernel(const BoundsParams p, 
   *reinterpret_cast<uint4*>(out + D) = make_uint4(mx[0], mx[1], mx[2], mx[3]);
 }
 
+// N consecutive 32-bit words (aligned to min(N, 4) words), read once.
+template <int N>
+__device__ __forceinline__ void ld_global_words(const void* p, uint32_t (&w)[N]) {
+  if constexpr (N == 1) {
+    w[0] = __ldg(static_cast<const uint32_t*>(p));
+  } else if constexpr (N == 2) {
+    const uint2 v = __ldg(static_cast<const uint2*>(p));
+    w[0] = v.x;
+    w[1] = v.y;
+  } else {
+    const uint4 v = __ldg(static_cast<const uint4*>(p));
+    w[0] = v.x;
+    w[1] = v.y;
+    w[2] = v.z;
+    w[3] = v.w;
+  }
+}
+
 struct SelectParams {
   const void* q;
   const void* bounds;
@@ -111,33 +130,26 @@ __device__ __forceinline__ int clamped_length(const SelectParams& p, int s, int 
 // pages rank next to the border.  Bound: the bounds' bytes, nearly level with
 // the conversions to 64 bits (16 a clock and SM, one per bound).
 //
-// blockIdx.x: chunk of p.chunk pages, 8 warps of p.chunk / 8 (at most 32); D/8
-// lanes per page, kUnroll steps of 256/D pages in flight.
+// blockIdx.x: chunk of p.chunk pages, 8 warps of p.chunk / 8 (at most 16), a
+// whole warp per page with kUnroll pages in flight.  The query, the length and
+// the table entries are loaded together, before it is known whether the chunk
+// holds a page.
 template <typename T, int D>
-__global__ void __launch_bounds__(256) page_scores_kernel(const SelectParams p) {
-  constexpr int LP = D / 8, PW = 32 / LP, kUnroll = 4;
+__global__ void __launch_bounds__(256, 4) page_scores_kernel(const SelectParams p) {
+  constexpr int V = D / 32;                         // elements per lane
+  constexpr int W = V / 2;                          // 32-bit words of them
+  constexpr int kUnroll = D == 256 ? 4 : 8;
   __shared__ double qs[2][D];
   grid_launch_dependents();
   const int u = blockIdx.y, s = u / p.Hkv, h = u - s * p.Hkv;
-  const int n = (clamped_length(p, s, h) + p.bs - 1) / p.bs;
-  const int c0 = p.sink + blockIdx.x * p.chunk, c1 = min(c0 + p.chunk, n - p.recent);
-  if (n <= p.keep || c0 >= c1) return;
-  const int lane = threadIdx.x & 31, e = lane % LP, per = p.chunk / 8;
-  const int w0 = c0 + (threadIdx.x >> 5) * per;
-  // This warp's pages, one id per lane; -1: out of range.
-  int id = -1;
-  if (lane < per && w0 + lane < c1) {
-    const int64_t pid =
-        static_cast<int64_t>(p.bt[s * p.bt_sb + h * p.bt_sh + (w0 + lane) * p.bt_si]) * p.bt_mul +
-        static_cast<int64_t>(h) * p.bt_add;
-    if (pid >= 0 && pid < p.num_pages)
-      id = static_cast<int>(pid);
-    else if (p.status)
-      atomicOr(p.status, kStatusBadPage);
-  }
+  const int lane = threadIdx.x & 31, per = p.chunk / 8;
+  const int c0 = p.sink + blockIdx.x * p.chunk, w0 = c0 + (threadIdx.x >> 5) * per;
+  const bool mine = lane < per && w0 + lane < p.maxb;
+  const int entry = mine ? p.bt[s * p.bt_sb + h * p.bt_sh + (w0 + lane) * p.bt_si] : 0;
   const T* q = static_cast<const T*>(p.q) + s * p.q_sb + static_cast<int64_t>(h) * p.G * p.q_sh;
   for (int d = threadIdx.x; d < D; d += 256) {
     double up = 0.0, dn = 0.0;
+#pragma unroll 8
     for (int g = 0; g < p.G; ++g) {
       const float x = static_cast<float>(q[g * p.q_sh + d]);
       up += x > 0.f ? x : 0.f;
@@ -146,48 +158,56 @@ __global__ void __launch_bounds__(256) page_scores_kernel(const SelectParams p) 
     qs[0][d] = up;
     qs[1][d] = dn;
   }
+  const int n = (clamped_length(p, s, h) + p.bs - 1) / p.bs;
+  const int c1 = min(c0 + p.chunk, n - p.recent);
+  if (n <= p.keep || c0 >= c1) return;
+  // This warp's pages, one id per lane; -1: out of range.
+  int id = -1;
+  if (mine && w0 + lane < c1) {
+    const int64_t pid = static_cast<int64_t>(entry) * p.bt_mul + static_cast<int64_t>(h) * p.bt_add;
+    if (pid >= 0 && pid < p.num_pages)
+      id = static_cast<int>(pid);
+    else if (p.status)
+      atomicOr(p.status, kStatusBadPage);
+  }
   __syncthreads();
-  double up[8], dn[8];
+  double up[V], dn[V];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    up[i] = qs[0][e * 8 + i];
-    dn[i] = qs[1][e * 8 + i];
+  for (int i = 0; i < V; ++i) {
+    up[i] = qs[0][lane * V + i];
+    dn[i] = qs[1][lane * V + i];
   }
   float* out = p.scores + static_cast<int64_t>(u) * p.maxb + w0;
   const int count = min(per, c1 - w0);
-  for (int t = 0; t < count; t += PW * kUnroll) {
-    uint4 mn[kUnroll], mx[kUnroll];
+  for (int t = 0; t < count; t += kUnroll) {
+    uint32_t mn[kUnroll][W], mx[kUnroll][W];
     int pid[kUnroll];
 #pragma unroll
     for (int v = 0; v < kUnroll; ++v) {
-      const int at = t + v * PW + lane / LP;
-      pid[v] = __shfl_sync(0xffffffffu, id, at & 31);
-      if (at >= count) pid[v] = -1;
-      mn[v] = mx[v] = make_uint4(0u, 0u, 0u, 0u);
-      if (pid[v] >= 0) {
-        const T* b = static_cast<const T*>(p.bounds) + static_cast<int64_t>(pid[v]) * (2 * D) + e * 8;
-        mn[v] = __ldg(reinterpret_cast<const uint4*>(b));
-        mx[v] = __ldg(reinterpret_cast<const uint4*>(b + D));
-      }
+      pid[v] = __shfl_sync(0xffffffffu, id, t + v);
+      const T* b = static_cast<const T*>(p.bounds) +
+                   static_cast<int64_t>(pid[v] < 0 || t + v >= count ? 0 : pid[v]) * (2 * D) + lane * V;
+      ld_global_words<W>(b, mn[v]);
+      ld_global_words<W>(b + D, mx[v]);
     }
+    float res = 0.f;
 #pragma unroll
     for (int v = 0; v < kUnroll; ++v) {
-      if (t + v * PW >= count) break;
-      float lo[8], hi[8];
-      unpack8<T>(mn[v], lo);
-      unpack8<T>(mx[v], hi);
       double a = 0.0, b = 0.0;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        a = fma(static_cast<double>(hi[i]), up[i], a);
-        b = fma(static_cast<double>(lo[i]), dn[i], b);
+      for (int i = 0; i < W; ++i) {
+        const float2 lo = unpack2<T>(mn[v][i]), hi = unpack2<T>(mx[v][i]);
+        a = fma(static_cast<double>(hi.x), up[2 * i], a);
+        b = fma(static_cast<double>(lo.x), dn[2 * i], b);
+        a = fma(static_cast<double>(hi.y), up[2 * i + 1], a);
+        b = fma(static_cast<double>(lo.y), dn[2 * i + 1], b);
       }
       a += b;
 #pragma unroll
-      for (int o = 1; o < LP; o <<= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
-      const int at = t + v * PW + lane / LP;
-      if (e == 0 && at < count) out[at] = pid[v] < 0 ? -INFINITY : static_cast<float>(a);
+      for (int o = 1; o < 32; o <<= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
+      if (lane == v) res = pid[v] < 0 ? -INFINITY : static_cast<float>(a);
     }
+    if (lane < kUnroll && t + lane < count) out[t + lane] = res;
   }
 }
 
@@ -199,44 +219,47 @@ __device__ __forceinline__ uint32_t score_key(float f) {
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
-// Sum of x over the block's threads before this one, and the total (1024
-// threads; `warp_sum` 32 words, free to reuse after the next barrier).
-__device__ __forceinline__ int block_scan(int x, int* warp_sum, int* total) {
+// Sums of x.x and of x.y over the block's threads before this one, and the
+// totals (1024 threads; `warp_sum` is free again after the next barrier).
+__device__ __forceinline__ int2 block_scan(int2 x, int2* warp_sum, int2* total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int v = x;
+  auto scan = [&](int2 v) {
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int y = __shfl_up_sync(0xffffffffu, v, o);
-    if (lane >= o) v += y;
-  }
+    for (int o = 1; o < 32; o <<= 1) {
+      const int a = __shfl_up_sync(0xffffffffu, v.x, o), b = __shfl_up_sync(0xffffffffu, v.y, o);
+      if (lane >= o) {
+        v.x += a;
+        v.y += b;
+      }
+    }
+    return v;
+  };
+  const int2 v = scan(x);
   if (lane == 31) warp_sum[warp] = v;
   __syncthreads();
-  int w = warp_sum[lane];
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int y = __shfl_up_sync(0xffffffffu, w, o);
-    if (lane >= o) w += y;
-  }
-  *total = __shfl_sync(0xffffffffu, w, 31);
-  const int before = __shfl_sync(0xffffffffu, w, warp ? warp - 1 : 0);
-  return (warp ? before : 0) + v - x;
+  const int2 w = scan(warp_sum[lane]);
+  *total = make_int2(__shfl_sync(0xffffffffu, w.x, 31), __shfl_sync(0xffffffffu, w.y, 31));
+  const int before_x = __shfl_sync(0xffffffffu, w.x, warp ? warp - 1 : 0);
+  const int before_y = __shfl_sync(0xffffffffu, w.y, warp ? warp - 1 : 0);
+  return make_int2((warp ? before_x : 0) + v.x - x.x, (warp ? before_y : 0) + v.y - x.y);
 }
 
 // One CTA per (sequence, kv head): the pages to attend to, ascending.  The k-th
 // largest key is found by counting: the range between the smallest and the
-// largest key is cut into 1024 bins, the bin that holds the k-th becomes the
-// range, until a bin is one key wide (at most four passes, mostly two: the
-// scores fill their own range, so that no bin is crowded and the shared-memory
-// counters do not serialise).  Keys above it are kept, of the equal ones the
-// first.  A thread owns consecutive pages, so that one scan places them in
+// largest key is cut into 1024 bins (the scores fill their own range, so that no
+// bin is crowded and the shared-memory counters do not serialise); when the bin
+// that holds the k-th has at most 1024 keys, they are compared with one another,
+// else it becomes the range.  Keys above the k-th are kept, of the equal ones
+// the first.  A thread owns consecutive pages, so that one scan places them in
 // order; up to kPer of its keys stay in registers.
 __global__ void __launch_bounds__(1024) select_pages_kernel(const SelectParams p) {
   constexpr int kBins = 1024, kPer = 8;
   __shared__ int hist[kBins];
-  __shared__ int sum_a[32], sum_b[32];
+  __shared__ uint32_t list[kBins];
+  __shared__ int2 sums[2][32];
   __shared__ uint32_t sh_lo[32], sh_hi[32];
-  __shared__ uint32_t sh_bin;
-  __shared__ int sh_rank;
+  __shared__ uint32_t sh_key;
+  __shared__ int sh_bin, sh_rank, sh_count, sh_listed;
   grid_launch_dependents();
   const int u = blockIdx.x, s = u / p.Hkv, h = u - s * p.Hkv;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -245,6 +268,8 @@ __global__ void __launch_bounds__(1024) select_pages_kernel(const SelectParams p
   const int n = (L + p.bs - 1) / p.bs;
   const int32_t* bt = p.bt + s * p.bt_sb + h * p.bt_sh;
   int32_t* out = p.tables + static_cast<int64_t>(u) * p.keep;
+  hist[tid] = 0;
+  if (tid == 0) sh_listed = 0;
   grid_dependency_wait();  // the scores; nothing of this call is written before
   if (tid == 0 && raw != L && p.status) atomicOr(p.status, raw < 0 ? kStatusNegative : kStatusClamp);
   if (n <= p.keep) {
@@ -282,7 +307,6 @@ __global__ void __launch_bounds__(1024) select_pages_kernel(const SelectParams p
     sh_lo[warp] = lo;
     sh_hi[warp] = hi;
   }
-  hist[tid] = 0;
   __syncthreads();
   lo = __reduce_min_sync(0xffffffffu, sh_lo[lane]);
   hi = __reduce_max_sync(0xffffffffu, sh_hi[lane]);
@@ -296,36 +320,54 @@ __global__ void __launch_bounds__(1024) select_pages_kernel(const SelectParams p
     __syncthreads();
     // thread t looks at bin 1023 - t: how many keys lie in the bins above it
     const int mine = hist[kBins - 1 - tid];
-    int total;
-    const int above = block_scan(mine, sum_a, &total);
+    int2 total;
+    const int above = block_scan(make_int2(mine, 0), sums[0], &total).x;
     if (above < rank && rank <= above + mine) {
       sh_bin = kBins - 1 - tid;
       sh_rank = rank - above;
+      sh_count = mine;
     }
     hist[kBins - 1 - tid] = 0;
     __syncthreads();
-    const uint32_t bin = sh_bin;
     rank = sh_rank;
-    const uint32_t first = lo + (bin << shift);
-    const uint32_t last = first + ((1u << shift) - 1u);
-    lo = first;
+    lo += static_cast<uint32_t>(sh_bin) << shift;
+    const uint32_t last = lo + ((1u << shift) - 1u);
     hi = last < hi ? last : hi;
-    if (shift == 0) hi = lo;
+    const int count = sh_count;
+    if (lo < hi && count <= kBins) {
+      each([&](int, uint32_t x) {
+        if (x >= lo && x <= hi) list[atomicAdd(&sh_listed, 1)] = x;
+      });
+      __syncthreads();
+      if (tid < count) {
+        const uint32_t x = list[tid];
+        int above_x = 0, equal_x = 0;
+        for (int i = 0; i < count; ++i) {
+          above_x += list[i] > x;
+          equal_x += list[i] == x;
+        }
+        // equal keys all write the same two words
+        if (above_x < rank && rank <= above_x + equal_x) {
+          sh_key = x;
+          sh_bin = rank - above_x;
+        }
+      }
+      __syncthreads();
+      lo = hi = sh_key;
+      rank = sh_bin;
+    }
   }
   // Keys above lo are kept, of the equal ones the first `rank`.
-  int gt = 0, eq = 0;
+  int2 cnt = make_int2(0, 0), total;
   each([&](int, uint32_t x) {
-    gt += x > lo;
-    eq += x == lo;
+    cnt.x += x > lo;
+    cnt.y += x == lo;
   });
-  int total;
-  __syncthreads();
-  const int gt_before = block_scan(gt, sum_a, &total);
-  int eq_before = block_scan(eq, sum_b, &total);
-  int at = gt_before + min(eq_before, rank);
+  const int2 before = block_scan(cnt, sums[1], &total);
+  int eq = before.y, at = before.x + min(before.y, rank);
   each([&](int i, uint32_t x) {
-    if (x > lo || (x == lo && eq_before < rank)) out[p.sink + at++] = bt[(c0 + i) * p.bt_si];
-    eq_before += x == lo;
+    if (x > lo || (x == lo && eq < rank)) out[p.sink + at++] = bt[(c0 + i) * p.bt_si];
+    eq += x == lo;
   });
 }
 
@@ -419,9 +461,9 @@ int launch_select(const pab200_select_args* a, void* scores, cudaStream_t s) {
   const unsigned units = static_cast<unsigned>(p.B * p.Hkv);
   const bool scored = p.maxb > p.keep;
   if (scored) {
-    // Pages per CTA: 256 (32 per warp), fewer while that leaves SMs idle.
+    // Pages per CTA: 128 (16 per warp), fewer while that leaves SMs idle.
     const int64_t pages = int64_t(units) * p.maxb;
-    int chunk = 256;
+    int chunk = 128;
     while (chunk > 32 && pages / chunk < 4 * pabh::device_sm_count_current()) chunk /= 2;
     p.chunk = chunk;
     const dim3 grid((p.maxb + chunk - 1) / chunk, units);
