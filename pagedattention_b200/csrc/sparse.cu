@@ -130,22 +130,28 @@ __device__ __forceinline__ int clamped_length(const SelectParams& p, int s, int 
 // pages rank next to the border.  Bound: the bounds' bytes, nearly level with
 // the conversions to 64 bits (16 a clock and SM, one per bound).
 //
-// blockIdx.x: chunk of p.chunk pages, 8 warps of p.chunk / 8 (at most 16), a
-// whole warp per page with kUnroll pages in flight.  The query, the length and
-// the table entries are loaded together, before it is known whether the chunk
-// holds a page.
+// blockIdx.x: chunk of p.chunk pages, 8 warps of p.chunk / 8 (at most 64), a
+// whole warp per page.  A warp lives for dozens of pages with the next four on
+// their way while it sums four: with 16 pages per warp and no overlap the same
+// pass took 40 us for the 24,400 pages x 8 kv heads of 4 x 32k-128k tokens.
 template <typename T, int D>
 __global__ void __launch_bounds__(256, 4) page_scores_kernel(const SelectParams p) {
   constexpr int V = D / 32;                         // elements per lane
   constexpr int W = V / 2;                          // 32-bit words of them
-  constexpr int kUnroll = D == 256 ? 4 : 8;
+  constexpr int U = 4;                              // pages at a time
   __shared__ double qs[2][D];
   grid_launch_dependents();
   const int u = blockIdx.y, s = u / p.Hkv, h = u - s * p.Hkv;
   const int lane = threadIdx.x & 31, per = p.chunk / 8;
   const int c0 = p.sink + blockIdx.x * p.chunk, w0 = c0 + (threadIdx.x >> 5) * per;
-  const bool mine = lane < per && w0 + lane < p.maxb;
-  const int entry = mine ? p.bt[s * p.bt_sb + h * p.bt_sh + (w0 + lane) * p.bt_si] : 0;
+  // The table entries, the query and the length are loaded together, before it
+  // is known whether the chunk holds a page.
+  int id[2];
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int i = 32 * j + lane;
+    id[j] = i < per && w0 + i < p.maxb ? p.bt[s * p.bt_sb + h * p.bt_sh + (w0 + i) * p.bt_si] : 0;
+  }
   const T* q = static_cast<const T*>(p.q) + s * p.q_sb + static_cast<int64_t>(h) * p.G * p.q_sh;
   for (int d = threadIdx.x; d < D; d += 256) {
     double up = 0.0, dn = 0.0;
@@ -161,14 +167,14 @@ __global__ void __launch_bounds__(256, 4) page_scores_kernel(const SelectParams 
   const int n = (clamped_length(p, s, h) + p.bs - 1) / p.bs;
   const int c1 = min(c0 + p.chunk, n - p.recent);
   if (n <= p.keep || c0 >= c1) return;
-  // This warp's pages, one id per lane; -1: out of range.
-  int id = -1;
-  if (mine && w0 + lane < c1) {
-    const int64_t pid = static_cast<int64_t>(entry) * p.bt_mul + static_cast<int64_t>(h) * p.bt_add;
-    if (pid >= 0 && pid < p.num_pages)
-      id = static_cast<int>(pid);
-    else if (p.status)
-      atomicOr(p.status, kStatusBadPage);
+  const int count = min(per, c1 - w0);
+  // This warp's pages: ids, -1 for one out of range.
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int64_t pid = static_cast<int64_t>(id[j]) * p.bt_mul + static_cast<int64_t>(h) * p.bt_add;
+    const bool ok = pid >= 0 && pid < p.num_pages;
+    if (!ok && 32 * j + lane < count && p.status) atomicOr(p.status, kStatusBadPage);
+    id[j] = ok ? static_cast<int>(pid) : -1;
   }
   __syncthreads();
   double up[V], dn[V];
@@ -177,37 +183,63 @@ __global__ void __launch_bounds__(256, 4) page_scores_kernel(const SelectParams 
     up[i] = qs[0][lane * V + i];
     dn[i] = qs[1][lane * V + i];
   }
-  float* out = p.scores + static_cast<int64_t>(u) * p.maxb + w0;
-  const int count = min(per, c1 - w0);
-  for (int t = 0; t < count; t += kUnroll) {
-    uint32_t mn[kUnroll][W], mx[kUnroll][W];
-    int pid[kUnroll];
+  struct Pages {
+    uint32_t mn[U][W], mx[U][W];
+    int bad;  // bit v: page v has no bounds
+  };
+  auto load = [&](int t, Pages& x) {
+    x.bad = 0;
 #pragma unroll
-    for (int v = 0; v < kUnroll; ++v) {
-      pid[v] = __shfl_sync(0xffffffffu, id, t + v);
+    for (int v = 0; v < U; ++v) {
+      const int pid = __shfl_sync(0xffffffffu, t + v < 32 ? id[0] : id[1], (t + v) & 31);
+      if (pid < 0) x.bad |= 1 << v;
+      // past the end: any page will do
       const T* b = static_cast<const T*>(p.bounds) +
-                   static_cast<int64_t>(pid[v] < 0 || t + v >= count ? 0 : pid[v]) * (2 * D) + lane * V;
-      ld_global_words<W>(b, mn[v]);
-      ld_global_words<W>(b + D, mx[v]);
+                   static_cast<int64_t>(t + v < count && pid >= 0 ? pid : 0) * (2 * D) + lane * V;
+      ld_global_words<W>(b, x.mn[v]);
+      ld_global_words<W>(b + D, x.mx[v]);
     }
-    float res = 0.f;
+  };
+  float* out = p.scores + static_cast<int64_t>(u) * p.maxb + w0;
+  auto score = [&](int t, const Pages& x) {
+    double a[U];
 #pragma unroll
-    for (int v = 0; v < kUnroll; ++v) {
-      double a = 0.0, b = 0.0;
+    for (int v = 0; v < U; ++v) {
+      double b = 0.0;
+      a[v] = 0.0;
 #pragma unroll
       for (int i = 0; i < W; ++i) {
-        const float2 lo = unpack2<T>(mn[v][i]), hi = unpack2<T>(mx[v][i]);
-        a = fma(static_cast<double>(hi.x), up[2 * i], a);
+        const float2 lo = unpack2<T>(x.mn[v][i]), hi = unpack2<T>(x.mx[v][i]);
+        a[v] = fma(static_cast<double>(hi.x), up[2 * i], a[v]);
         b = fma(static_cast<double>(lo.x), dn[2 * i], b);
-        a = fma(static_cast<double>(hi.y), up[2 * i + 1], a);
+        a[v] = fma(static_cast<double>(hi.y), up[2 * i + 1], a[v]);
         b = fma(static_cast<double>(lo.y), dn[2 * i + 1], b);
       }
-      a += b;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
-      if (lane == v) res = pid[v] < 0 ? -INFINITY : static_cast<float>(a);
+      a[v] += b;
     }
-    if (lane < kUnroll && t + lane < count) out[t + lane] = res;
+    // Four sums over the warp at once: lanes of the upper half go on with pages
+    // 2 and 3, of every half's upper half with the odd one.
+    const bool h16 = lane & 16, h8 = lane & 8;
+    const double g0 = __shfl_xor_sync(0xffffffffu, h16 ? a[0] : a[2], 16);
+    const double g1 = __shfl_xor_sync(0xffffffffu, h16 ? a[1] : a[3], 16);
+    const double b0 = (h16 ? a[2] : a[0]) + g0, b1 = (h16 ? a[3] : a[1]) + g1;
+    double r = (h8 ? b1 : b0) + __shfl_xor_sync(0xffffffffu, h8 ? b0 : b1, 8);
+    r += __shfl_xor_sync(0xffffffffu, r, 4);
+    r += __shfl_xor_sync(0xffffffffu, r, 2);
+    r += __shfl_xor_sync(0xffffffffu, r, 1);
+    const int v = (h16 ? 2 : 0) + (h8 ? 1 : 0);
+    if ((lane & 7) == 0 && t + v < count)
+      out[t + v] = x.bad >> v & 1 ? -INFINITY : static_cast<float>(r);
+  };
+  if (count <= 0) return;
+  Pages x, y;
+  load(0, x);
+  for (int t = 0; t < count; t += 2 * U) {
+    if (t + U < count) load(t + U, y);
+    score(t, x);
+    if (t + U >= count) break;
+    if (t + 2 * U < count) load(t + 2 * U, x);
+    score(t + U, y);
   }
 }
 
@@ -220,7 +252,8 @@ __device__ __forceinline__ uint32_t score_key(float f) {
 }
 
 // Sums of x.x and of x.y over the block's threads before this one, and the
-// totals (1024 threads; `warp_sum` is free again after the next barrier).
+// totals (`warp_sum` is free again after the next barrier).
+template <int NTH>
 __device__ __forceinline__ int2 block_scan(int2 x, int2* warp_sum, int2* total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   auto scan = [&](int2 v) {
@@ -237,7 +270,7 @@ __device__ __forceinline__ int2 block_scan(int2 x, int2* warp_sum, int2* total) 
   const int2 v = scan(x);
   if (lane == 31) warp_sum[warp] = v;
   __syncthreads();
-  const int2 w = scan(warp_sum[lane]);
+  const int2 w = scan(lane < NTH / 32 ? warp_sum[lane] : make_int2(0, 0));
   *total = make_int2(__shfl_sync(0xffffffffu, w.x, 31), __shfl_sync(0xffffffffu, w.y, 31));
   const int before_x = __shfl_sync(0xffffffffu, w.x, warp ? warp - 1 : 0);
   const int before_y = __shfl_sync(0xffffffffu, w.y, warp ? warp - 1 : 0);
@@ -246,14 +279,15 @@ __device__ __forceinline__ int2 block_scan(int2 x, int2* warp_sum, int2* total) 
 
 // One CTA per (sequence, kv head): the pages to attend to, ascending.  The k-th
 // largest key is found by counting: the range between the smallest and the
-// largest key is cut into 1024 bins (the scores fill their own range, so that no
+// largest key is cut into NTH bins (the scores fill their own range, so that no
 // bin is crowded and the shared-memory counters do not serialise); when the bin
-// that holds the k-th has at most 1024 keys, they are compared with one another,
+// that holds the k-th has at most NTH keys, they are compared with one another,
 // else it becomes the range.  Keys above the k-th are kept, of the equal ones
 // the first.  A thread owns consecutive pages, so that one scan places them in
 // order; up to kPer of its keys stay in registers.
-__global__ void __launch_bounds__(1024) select_pages_kernel(const SelectParams p) {
-  constexpr int kBins = 1024, kPer = 8;
+template <int NTH>
+__global__ void __launch_bounds__(NTH) select_pages_kernel(const SelectParams p) {
+  constexpr int kBins = NTH, kLog2Bins = NTH == 1024 ? 10 : 8, kPer = 8;
   __shared__ int hist[kBins];
   __shared__ uint32_t list[kBins];
   __shared__ int2 sums[2][32];
@@ -273,19 +307,19 @@ __global__ void __launch_bounds__(1024) select_pages_kernel(const SelectParams p
   grid_dependency_wait();  // the scores; nothing of this call is written before
   if (tid == 0 && raw != L && p.status) atomicOr(p.status, raw < 0 ? kStatusNegative : kStatusClamp);
   if (n <= p.keep) {
-    for (int i = tid; i < p.keep; i += 1024) out[i] = i < n ? bt[i * p.bt_si] : -1;
+    for (int i = tid; i < p.keep; i += NTH) out[i] = i < n ? bt[i * p.bt_si] : -1;
     if (tid == 0) p.out_lens[u] = L;
     return;
   }
   const int c0 = p.sink, m = n - p.sink - p.recent;  // candidates, of which k are kept
   const int k = p.keep - p.sink - p.recent;
-  for (int i = tid; i < p.sink; i += 1024) out[i] = bt[i * p.bt_si];
-  for (int i = tid; i < p.recent; i += 1024)
+  for (int i = tid; i < p.sink; i += NTH) out[i] = bt[i * p.bt_si];
+  for (int i = tid; i < p.recent; i += NTH)
     out[p.keep - p.recent + i] = bt[(n - p.recent + i) * p.bt_si];
   if (tid == 0) p.out_lens[u] = (p.keep - 1) * p.bs + L - (n - 1) * p.bs;
   if (k == 0) return;
   const float* sc = p.scores + static_cast<int64_t>(u) * p.maxb + c0;
-  const int per = (m + 1023) >> 10;
+  const int per = (m + NTH - 1) / NTH;
   const int i0 = min(tid * per, m), i1 = min(i0 + per, m);
   uint32_t key[kPer];
 #pragma unroll
@@ -308,20 +342,20 @@ __global__ void __launch_bounds__(1024) select_pages_kernel(const SelectParams p
     sh_hi[warp] = hi;
   }
   __syncthreads();
-  lo = __reduce_min_sync(0xffffffffu, sh_lo[lane]);
-  hi = __reduce_max_sync(0xffffffffu, sh_hi[lane]);
+  lo = __reduce_min_sync(0xffffffffu, sh_lo[lane % (NTH / 32)]);
+  hi = __reduce_max_sync(0xffffffffu, sh_hi[lane % (NTH / 32)]);
   int rank = k;  // the rank-th largest key of [lo, hi] is looked for
   while (lo < hi) {
     const int bits = 32 - __clz(hi - lo);
-    const int shift = bits > 10 ? bits - 10 : 0;
+    const int shift = bits > kLog2Bins ? bits - kLog2Bins : 0;
     each([&](int, uint32_t x) {
       if (x >= lo && x <= hi) atomicAdd(&hist[(x - lo) >> shift], 1);
     });
     __syncthreads();
-    // thread t looks at bin 1023 - t: how many keys lie in the bins above it
+    // thread t looks at bin NTH - 1 - t: how many keys lie in the bins above it
     const int mine = hist[kBins - 1 - tid];
     int2 total;
-    const int above = block_scan(make_int2(mine, 0), sums[0], &total).x;
+    const int above = block_scan<NTH>(make_int2(mine, 0), sums[0], &total).x;
     if (above < rank && rank <= above + mine) {
       sh_bin = kBins - 1 - tid;
       sh_rank = rank - above;
@@ -363,7 +397,7 @@ __global__ void __launch_bounds__(1024) select_pages_kernel(const SelectParams p
     cnt.x += x > lo;
     cnt.y += x == lo;
   });
-  const int2 before = block_scan(cnt, sums[1], &total);
+  const int2 before = block_scan<NTH>(cnt, sums[1], &total);
   int eq = before.y, at = before.x + min(before.y, rank);
   each([&](int i, uint32_t x) {
     if (x > lo || (x == lo && eq < rank)) out[p.sink + at++] = bt[(c0 + i) * p.bt_si];
@@ -461,10 +495,12 @@ int launch_select(const pab200_select_args* a, void* scores, cudaStream_t s) {
   const unsigned units = static_cast<unsigned>(p.B * p.Hkv);
   const bool scored = p.maxb > p.keep;
   if (scored) {
-    // Pages per CTA: 128 (16 per warp), fewer while that leaves SMs idle.
+    // Pages per CTA: what gives every SM about three CTAs, in whole steps of the
+    // 8 warps, at most 64 pages per warp.
     const int64_t pages = int64_t(units) * p.maxb;
-    int chunk = 128;
-    while (chunk > 32 && pages / chunk < 4 * pabh::device_sm_count_current()) chunk /= 2;
+    int64_t each = pages / (3 * pabh::device_sm_count_current());
+    each = (each + 63) / 64 * 64;
+    const int chunk = each < 64 ? 64 : (each > 512 ? 512 : static_cast<int>(each));
     p.chunk = chunk;
     const dim3 grid((p.maxb + chunk - 1) / chunk, units);
     if (a->dtype == PAB200_DTYPE_BF16)
@@ -473,8 +509,12 @@ int launch_select(const pab200_select_args* a, void* scores, cudaStream_t s) {
       launch_scores<__half>(p, a->head_size, grid, s);
   }
   // Scheduled while the scores drain; waits for them before it reads any.
-  pabh::LaunchCfg lc(dim3(units), dim3(1024), 0, s, scored);
-  cudaError_t err = cudaLaunchKernelEx(&lc.cfg, pab::select_pages_kernel, p);
+  // 256 threads while 8 registers hold a thread's keys, so that several units
+  // share an SM.
+  const bool small = p.maxb <= 2048;
+  pabh::LaunchCfg lc(dim3(units), dim3(small ? 256 : 1024), 0, s, scored);
+  cudaError_t err = small ? cudaLaunchKernelEx(&lc.cfg, pab::select_pages_kernel<256>, p)
+                          : cudaLaunchKernelEx(&lc.cfg, pab::select_pages_kernel<1024>, p);
   if (err != cudaSuccess) return pabh::cuda_fail(err, "page selection launch");
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? PAB200_OK : pabh::cuda_fail(e, "page selection launch");
