@@ -111,7 +111,7 @@ struct SelectParams {
   const int32_t* bt;
   int32_t* tables;     // [B][Hkv][keep]
   int32_t* out_lens;   // [B][Hkv]
-  float* scores;       // [B * Hkv][maxb]
+  float2* scores;      // [B * Hkv][maxb]: score, sum of its terms' sizes
   uint32_t* status;
   int64_t q_sb, q_sh, l_sb, l_sh, bt_sb, bt_sh, bt_si, num_pages;
   int32_t bt_mul, bt_add, B, Hkv, G, bs, maxb, keep, sink, recent, chunk;
@@ -123,23 +123,41 @@ __device__ __forceinline__ int clamped_length(const SelectParams& p, int s, int 
   return L < 0 ? 0 : (L > cap ? static_cast<int>(cap) : L);
 }
 
-// Score of every candidate page of a (sequence, kv head): sum over the head
-// elements of max * (sum of the group's positive query parts) + min * (sum of
-// the negative ones), the upper bound of the group's summed scores.  Summed in
-// 64 bits and rounded once, so that the order of the sum cannot change which
-// pages rank next to the border.  Bound: the bounds' bytes, nearly level with
-// the conversions to 64 bits (16 a clock and SM, one per bound).
-//
+// A page's score is the sum over the head elements of max * (sum of the group's
+// positive query parts) + min * (sum of the negative ones), the upper bound of
+// the group's summed scores; by definition in 64 bits, rounded to fp32.  Which
+// pages rank next to the border must not hang on the order of an fp32 sum, but
+// 64-bit conversions and sums cost twice the time the bounds take to read (36
+// against 18 us for the 24,400 pages x 8 kv heads of 4 x 32k-128k tokens).  So
+// this kernel sums in fp32, with the sum A of the terms' sizes beside it: an fp32
+// score is within kScoreError * A of the rounded 64-bit one (at most 17 rounded
+// products and sums per lane, 5 sums over the warp, the rounding of the query
+// sums, of the 64-bit score and of A: 25 * 2^-24).  The selection settles the few
+// pages that this leaves open in 64 bits.
+constexpr float kScoreError = 32.f / 16777216.f;
+
+// Positive and negative parts of the query, summed over the group in 64 bits.
+template <typename T>
+__device__ __forceinline__ double2 query_parts(const SelectParams& p, const T* q, int d) {
+  double up = 0.0, dn = 0.0;
+#pragma unroll 8
+  for (int g = 0; g < p.G; ++g) {
+    const float x = static_cast<float>(q[g * p.q_sh + d]);
+    up += x > 0.f ? x : 0.f;
+    dn += x > 0.f ? 0.f : x;  // a NaN makes this one NaN
+  }
+  return make_double2(up, dn);
+}
+
 // blockIdx.x: chunk of p.chunk pages, 8 warps of p.chunk / 8 (at most 64), a
 // whole warp per page.  A warp lives for dozens of pages with the next four on
-// their way while it sums four: with 16 pages per warp and no overlap the same
-// pass took 40 us for the 24,400 pages x 8 kv heads of 4 x 32k-128k tokens.
+// their way while it sums four.
 template <typename T, int D>
 __global__ void __launch_bounds__(256, 4) page_scores_kernel(const SelectParams p) {
   constexpr int V = D / 32;                         // elements per lane
   constexpr int W = V / 2;                          // 32-bit words of them
   constexpr int U = 4;                              // pages at a time
-  __shared__ double qs[2][D];
+  __shared__ float qs[2][D];
   grid_launch_dependents();
   const int u = blockIdx.y, s = u / p.Hkv, h = u - s * p.Hkv;
   const int lane = threadIdx.x & 31, per = p.chunk / 8;
@@ -154,15 +172,9 @@ __global__ void __launch_bounds__(256, 4) page_scores_kernel(const SelectParams 
   }
   const T* q = static_cast<const T*>(p.q) + s * p.q_sb + static_cast<int64_t>(h) * p.G * p.q_sh;
   for (int d = threadIdx.x; d < D; d += 256) {
-    double up = 0.0, dn = 0.0;
-#pragma unroll 8
-    for (int g = 0; g < p.G; ++g) {
-      const float x = static_cast<float>(q[g * p.q_sh + d]);
-      up += x > 0.f ? x : 0.f;
-      dn += x > 0.f ? 0.f : x;  // a NaN makes this one NaN
-    }
-    qs[0][d] = up;
-    qs[1][d] = dn;
+    const double2 x = query_parts<T>(p, q, d);
+    qs[0][d] = static_cast<float>(x.x);
+    qs[1][d] = static_cast<float>(x.y);
   }
   const int n = (clamped_length(p, s, h) + p.bs - 1) / p.bs;
   const int c1 = min(c0 + p.chunk, n - p.recent);
@@ -177,7 +189,7 @@ __global__ void __launch_bounds__(256, 4) page_scores_kernel(const SelectParams 
     id[j] = ok ? static_cast<int>(pid) : -1;
   }
   __syncthreads();
-  double up[V], dn[V];
+  float up[V], dn[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     up[i] = qs[0][lane * V + i];
@@ -200,36 +212,41 @@ __global__ void __launch_bounds__(256, 4) page_scores_kernel(const SelectParams 
       ld_global_words<W>(b + D, x.mx[v]);
     }
   };
-  float* out = p.scores + static_cast<int64_t>(u) * p.maxb + w0;
+  // Four sums over the warp at once: lanes of the upper half go on with pages 2
+  // and 3, of every half's upper half with the odd one.
+  const bool h16 = lane & 16, h8 = lane & 8;
+  auto warp_sums = [&](const float (&a)[U]) {
+    const float g0 = __shfl_xor_sync(0xffffffffu, h16 ? a[0] : a[2], 16);
+    const float g1 = __shfl_xor_sync(0xffffffffu, h16 ? a[1] : a[3], 16);
+    const float b0 = (h16 ? a[2] : a[0]) + g0, b1 = (h16 ? a[3] : a[1]) + g1;
+    float r = (h8 ? b1 : b0) + __shfl_xor_sync(0xffffffffu, h8 ? b0 : b1, 8);
+    r += __shfl_xor_sync(0xffffffffu, r, 4);
+    r += __shfl_xor_sync(0xffffffffu, r, 2);
+    return r + __shfl_xor_sync(0xffffffffu, r, 1);
+  };
+  float2* out = p.scores + static_cast<int64_t>(u) * p.maxb + w0;
   auto score = [&](int t, const Pages& x) {
-    double a[U];
+    float a[U], size[U];
 #pragma unroll
     for (int v = 0; v < U; ++v) {
-      double b = 0.0;
-      a[v] = 0.0;
+      a[v] = size[v] = 0.f;
 #pragma unroll
       for (int i = 0; i < W; ++i) {
         const float2 lo = unpack2<T>(x.mn[v][i]), hi = unpack2<T>(x.mx[v][i]);
-        a[v] = fma(static_cast<double>(hi.x), up[2 * i], a[v]);
-        b = fma(static_cast<double>(lo.x), dn[2 * i], b);
-        a[v] = fma(static_cast<double>(hi.y), up[2 * i + 1], a[v]);
-        b = fma(static_cast<double>(lo.y), dn[2 * i + 1], b);
+        a[v] = fmaf(hi.x, up[2 * i], a[v]);
+        a[v] = fmaf(lo.x, dn[2 * i], a[v]);
+        a[v] = fmaf(hi.y, up[2 * i + 1], a[v]);
+        a[v] = fmaf(lo.y, dn[2 * i + 1], a[v]);
+        size[v] = fmaf(fabsf(hi.x), up[2 * i], size[v]);
+        size[v] = fmaf(fabsf(lo.x), -dn[2 * i], size[v]);
+        size[v] = fmaf(fabsf(hi.y), up[2 * i + 1], size[v]);
+        size[v] = fmaf(fabsf(lo.y), -dn[2 * i + 1], size[v]);
       }
-      a[v] += b;
     }
-    // Four sums over the warp at once: lanes of the upper half go on with pages
-    // 2 and 3, of every half's upper half with the odd one.
-    const bool h16 = lane & 16, h8 = lane & 8;
-    const double g0 = __shfl_xor_sync(0xffffffffu, h16 ? a[0] : a[2], 16);
-    const double g1 = __shfl_xor_sync(0xffffffffu, h16 ? a[1] : a[3], 16);
-    const double b0 = (h16 ? a[2] : a[0]) + g0, b1 = (h16 ? a[3] : a[1]) + g1;
-    double r = (h8 ? b1 : b0) + __shfl_xor_sync(0xffffffffu, h8 ? b0 : b1, 8);
-    r += __shfl_xor_sync(0xffffffffu, r, 4);
-    r += __shfl_xor_sync(0xffffffffu, r, 2);
-    r += __shfl_xor_sync(0xffffffffu, r, 1);
+    const float r = warp_sums(a), z = warp_sums(size);
     const int v = (h16 ? 2 : 0) + (h8 ? 1 : 0);
     if ((lane & 7) == 0 && t + v < count)
-      out[t + v] = x.bad >> v & 1 ? -INFINITY : static_cast<float>(r);
+      out[t + v] = x.bad >> v & 1 ? make_float2(-INFINITY, 0.f) : make_float2(r, z);
   };
   if (count <= 0) return;
   Pages x, y;
@@ -243,12 +260,31 @@ __global__ void __launch_bounds__(256, 4) page_scores_kernel(const SelectParams 
   }
 }
 
+// The score of page `pid` by its definition, in every lane of a warp; `qs`: the
+// query's parts in 64 bits.
+template <typename T, int D>
+__device__ __forceinline__ float exact_score(const SelectParams& p, int64_t pid, const double* qs) {
+  if (pid < 0 || pid >= p.num_pages) return -INFINITY;
+  const T* b = static_cast<const T*>(p.bounds) + pid * (2 * D);
+  double a = 0.0;
+  for (int d = threadIdx.x & 31; d < D; d += 32) {
+    a = fma(static_cast<double>(static_cast<float>(b[D + d])), qs[d], a);
+    a = fma(static_cast<double>(static_cast<float>(b[d])), qs[D + d], a);
+  }
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
+  return static_cast<float>(a);
+}
+
 // Order-preserving key of a score: larger scores have larger keys, -0 and +0
-// the same, NaN the largest.
+// the same, NaN the largest; and the score of a key.
 __device__ __forceinline__ uint32_t score_key(float f) {
   if (f != f) return 0xffffffffu;
   const uint32_t b = __float_as_uint(f + 0.f);
   return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float key_score(uint32_t k) {
+  return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
 }
 
 // Sums of x.x and of x.y over the block's threads before this one, and the
@@ -277,21 +313,28 @@ __device__ __forceinline__ int2 block_scan(int2 x, int2* warp_sum, int2* total) 
   return make_int2((warp ? before_x : 0) + v.x - x.x, (warp ? before_y : 0) + v.y - x.y);
 }
 
-// One CTA per (sequence, kv head): the pages to attend to, ascending.  The k-th
-// largest key is found by counting: the range between the smallest and the
-// largest key is cut into NTH bins (the scores fill their own range, so that no
-// bin is crowded and the shared-memory counters do not serialise); when the bin
-// that holds the k-th has at most NTH keys, they are compared with one another,
-// else it becomes the range.  Keys above the k-th are kept, of the equal ones
-// the first.  A thread owns consecutive pages, so that one scan places them in
-// order; up to kPer of its keys stay in registers.
-template <int NTH>
+// One CTA per (sequence, kv head): the pages to attend to, ascending.
+//
+// The k-th largest fp32 score T is found by counting: the range between the
+// smallest and the largest key is cut into NTH bins (the scores fill their own
+// range, so that no bin is crowded and the shared-memory counters do not
+// serialise); when the bin that holds the k-th has at most NTH keys, they are
+// compared with one another, else it becomes the range.  With e the bound of the
+// scores' errors, the true k-th lies within e of T: pages above T + 2 e are kept,
+// pages below T - 2 e are not, and unless exactly as many as are still wanted lie
+// between, those are scored in 64 bits and ranked by the same counting, equal
+// ones by page.  (A score or a size that is not finite leaves every page open.)
+// A thread owns consecutive pages, so that one scan places them in order; up to
+// kPer of its keys stay in registers.
+template <typename T, int D, int NTH>
 __global__ void __launch_bounds__(NTH) select_pages_kernel(const SelectParams p) {
   constexpr int kBins = NTH, kLog2Bins = NTH == 1024 ? 10 : 8, kPer = 8;
   __shared__ int hist[kBins];
   __shared__ uint32_t list[kBins];
-  __shared__ int2 sums[2][32];
+  __shared__ double qs[2 * D];
+  __shared__ int2 sums[3][32];
   __shared__ uint32_t sh_lo[32], sh_hi[32];
+  __shared__ float sh_size[32];
   __shared__ uint32_t sh_key;
   __shared__ int sh_bin, sh_rank, sh_count, sh_listed;
   grid_launch_dependents();
@@ -318,90 +361,182 @@ __global__ void __launch_bounds__(NTH) select_pages_kernel(const SelectParams p)
     out[p.keep - p.recent + i] = bt[(n - p.recent + i) * p.bt_si];
   if (tid == 0) p.out_lens[u] = (p.keep - 1) * p.bs + L - (n - 1) * p.bs;
   if (k == 0) return;
-  const float* sc = p.scores + static_cast<int64_t>(u) * p.maxb + c0;
+  float2* sc = p.scores + static_cast<int64_t>(u) * p.maxb + c0;
   const int per = (m + NTH - 1) / NTH;
   const int i0 = min(tid * per, m), i1 = min(i0 + per, m);
   uint32_t key[kPer];
+  float size = 0.f;
 #pragma unroll
-  for (int j = 0; j < kPer; ++j) key[j] = i0 + j < i1 ? score_key(__ldcg(sc + i0 + j)) : 0u;
-  auto each = [&](auto&& fn) {  // this thread's keys, in page order
+  for (int j = 0; j < kPer; ++j) {
+    key[j] = 0u;
+    if (i0 + j < i1) {
+      const float2 x = __ldcg(sc + i0 + j);
+      key[j] = score_key(x.x);
+      size = x.y <= size ? size : x.y;  // a NaN is kept
+    }
+  }
+  for (int i = i0 + kPer; i < i1; ++i) {
+    const float z = __ldcg(&sc[i].y);
+    size = z <= size ? size : z;
+  }
+  // This thread's pages and keys, in order.
+  auto each = [&](auto&& fn) {
 #pragma unroll
     for (int j = 0; j < kPer; ++j)
       if (i0 + j < i1) fn(i0 + j, key[j]);
-    for (int i = i0 + kPer; i < i1; ++i) fn(i, score_key(__ldcg(sc + i)));
+    for (int i = i0 + kPer; i < i1; ++i) fn(i, score_key(__ldcg(&sc[i].x)));
   };
-  uint32_t lo = 0xffffffffu, hi = 0u;
-  each([&](int, uint32_t x) {
-    lo = min(lo, x);
-    hi = max(hi, x);
-  });
-  lo = __reduce_min_sync(0xffffffffu, lo);
-  hi = __reduce_max_sync(0xffffffffu, hi);
-  if (lane == 0) {
-    sh_lo[warp] = lo;
-    sh_hi[warp] = hi;
-  }
-  __syncthreads();
-  lo = __reduce_min_sync(0xffffffffu, sh_lo[lane % (NTH / 32)]);
-  hi = __reduce_max_sync(0xffffffffu, sh_hi[lane % (NTH / 32)]);
-  int rank = k;  // the rank-th largest key of [lo, hi] is looked for
-  while (lo < hi) {
-    const int bits = 32 - __clz(hi - lo);
-    const int shift = bits > kLog2Bins ? bits - kLog2Bins : 0;
-    each([&](int, uint32_t x) {
-      if (x >= lo && x <= hi) atomicAdd(&hist[(x - lo) >> shift], 1);
+  // The rank-th largest of the keys that `walk` visits, and its rank among the
+  // equal ones.  All threads call it together; `hist` is zero before and after.
+  auto kth = [&](auto&& walk, int rank) -> int2 {
+    uint32_t lo = 0xffffffffu, hi = 0u;
+    walk([&](int, uint32_t x) {
+      lo = min(lo, x);
+      hi = max(hi, x);
     });
+    lo = __reduce_min_sync(0xffffffffu, lo);
+    hi = __reduce_max_sync(0xffffffffu, hi);
     __syncthreads();
-    // thread t looks at bin NTH - 1 - t: how many keys lie in the bins above it
-    const int mine = hist[kBins - 1 - tid];
-    int2 total;
-    const int above = block_scan<NTH>(make_int2(mine, 0), sums[0], &total).x;
-    if (above < rank && rank <= above + mine) {
-      sh_bin = kBins - 1 - tid;
-      sh_rank = rank - above;
-      sh_count = mine;
+    if (lane == 0) {
+      sh_lo[warp] = lo;
+      sh_hi[warp] = hi;
     }
-    hist[kBins - 1 - tid] = 0;
     __syncthreads();
-    rank = sh_rank;
-    lo += static_cast<uint32_t>(sh_bin) << shift;
-    const uint32_t last = lo + ((1u << shift) - 1u);
-    hi = last < hi ? last : hi;
-    const int count = sh_count;
-    if (lo < hi && count <= kBins) {
-      each([&](int, uint32_t x) {
-        if (x >= lo && x <= hi) list[atomicAdd(&sh_listed, 1)] = x;
+    lo = __reduce_min_sync(0xffffffffu, sh_lo[lane % (NTH / 32)]);
+    hi = __reduce_max_sync(0xffffffffu, sh_hi[lane % (NTH / 32)]);
+    while (lo < hi) {
+      const int bits = 32 - __clz(hi - lo);
+      const int shift = bits > kLog2Bins ? bits - kLog2Bins : 0;
+      walk([&](int, uint32_t x) {
+        if (x >= lo && x <= hi) atomicAdd(&hist[(x - lo) >> shift], 1);
       });
+      if (tid == 0) sh_listed = 0;
       __syncthreads();
-      if (tid < count) {
-        const uint32_t x = list[tid];
-        int above_x = 0, equal_x = 0;
-        for (int i = 0; i < count; ++i) {
-          above_x += list[i] > x;
-          equal_x += list[i] == x;
-        }
-        // equal keys all write the same two words
-        if (above_x < rank && rank <= above_x + equal_x) {
-          sh_key = x;
-          sh_bin = rank - above_x;
-        }
+      // thread t looks at bin NTH - 1 - t: how many keys lie in the bins above it
+      const int mine = hist[kBins - 1 - tid];
+      int2 total;
+      const int above = block_scan<NTH>(make_int2(mine, 0), sums[0], &total).x;
+      if (above < rank && rank <= above + mine) {
+        sh_bin = kBins - 1 - tid;
+        sh_rank = rank - above;
+        sh_count = mine;
       }
+      hist[kBins - 1 - tid] = 0;
       __syncthreads();
-      lo = hi = sh_key;
-      rank = sh_bin;
+      rank = sh_rank;
+      lo += static_cast<uint32_t>(sh_bin) << shift;
+      const uint32_t last = lo + ((1u << shift) - 1u);
+      hi = last < hi ? last : hi;
+      const int count = sh_count;
+      if (lo < hi && count <= kBins) {
+        walk([&](int, uint32_t x) {
+          if (x >= lo && x <= hi) list[atomicAdd(&sh_listed, 1)] = x;
+        });
+        __syncthreads();
+        if (tid < count) {
+          const uint32_t x = list[tid];
+          int above_x = 0, equal_x = 0;
+          for (int i = 0; i < count; ++i) {
+            above_x += list[i] > x;
+            equal_x += list[i] == x;
+          }
+          // equal keys all write the same two words
+          if (above_x < rank && rank <= above_x + equal_x) {
+            sh_key = x;
+            sh_rank = rank - above_x;
+          }
+        }
+        __syncthreads();
+        lo = hi = sh_key;
+        rank = sh_rank;
+      }
     }
+    return make_int2(static_cast<int>(lo), rank);
+  };
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const float z = __shfl_xor_sync(0xffffffffu, size, o);
+    size = z <= size ? size : z;
   }
-  // Keys above lo are kept, of the equal ones the first `rank`.
+  if (lane == 0) sh_size[warp] = size;
+  const uint32_t tkey = static_cast<uint32_t>(kth(each, k).x);  // its barriers publish sh_size
+  for (int w = 0; w < NTH / 32; ++w) size = sh_size[w] <= size ? size : sh_size[w];
+  // Keys above khi are kept, below klo not.
+  const float t = key_score(tkey), e2 = 2.f * (size * kScoreError + 1e-37f);
+  const bool sure = e2 <= 3e38f && t == t;
+  const uint32_t khi = sure ? score_key(t + e2) : 0xffffffffu, klo = sure ? score_key(t - e2) : 0u;
+  auto open = [&](uint32_t x) { return !sure || (x <= khi && x >= klo); };
   int2 cnt = make_int2(0, 0), total;
   each([&](int, uint32_t x) {
-    cnt.x += x > lo;
-    cnt.y += x == lo;
+    cnt.x += sure && x > khi;
+    cnt.y += open(x);
   });
-  const int2 before = block_scan<NTH>(cnt, sums[1], &total);
-  int eq = before.y, at = before.x + min(before.y, rank);
+  int2 before = block_scan<NTH>(cnt, sums[1], &total);
+  const int want = k - total.x;  // of the total.y open pages
+  uint32_t last_key = 0u;        // open pages above it are kept, and `ties` equal to it
+  int ties = 0;
+  const bool rescore = want < total.y;
+  if (rescore) {
+    const T* q = static_cast<const T*>(p.q) + s * p.q_sb + static_cast<int64_t>(h) * p.G * p.q_sh;
+    for (int d = tid; d < D; d += NTH) {
+      const double2 x = query_parts<T>(p, q, d);
+      qs[d] = x.x;
+      qs[D + d] = x.y;
+    }
+    auto settle = [&](int i) {  // a warp's work
+      const int64_t pid = static_cast<int64_t>(bt[(c0 + i) * p.bt_si]) * p.bt_mul +
+                          static_cast<int64_t>(h) * p.bt_add;
+      const float x = exact_score<T, D>(p, pid, qs);
+      if (lane == 0) __stcg(&sc[i].y, x);  // the sizes have been read
+    };
+    if (total.y <= kBins) {
+      int at = before.y;
+      each([&](int i, uint32_t x) {
+        if (open(x)) list[at++] = static_cast<uint32_t>(i);
+      });
+      __syncthreads();
+      for (int j = warp; j < total.y; j += NTH / 32) settle(static_cast<int>(list[j]));
+    } else {
+      __syncthreads();
+      for (int i = warp; i < m; i += NTH / 32)
+        if (open(score_key(__ldcg(&sc[i].x)))) settle(i);
+    }
+    __syncthreads();
+    const int2 found = kth(
+        [&](auto&& fn) {
+          each([&](int i, uint32_t x) {
+            if (open(x)) fn(i, score_key(__ldcg(&sc[i].y)));
+          });
+        },
+        want);
+    last_key = static_cast<uint32_t>(found.x);
+    ties = found.y;
+    // ties before this thread's pages, then kept pages before them
+    int2 eq = make_int2(0, 0);
+    cnt.y = 0;
+    each([&](int i, uint32_t x) {
+      if (!open(x)) return;
+      const uint32_t y = score_key(__ldcg(&sc[i].y));
+      cnt.y += y > last_key;
+      eq.x += y == last_key;
+    });
+    __syncthreads();
+    const int2 eq_before = block_scan<NTH>(eq, sums[0], &total);
+    before = block_scan<NTH>(cnt, sums[2], &total);
+    ties -= eq_before.x;  // left for this thread's pages
+    before.y += min(eq_before.x, found.y);
+  }
+  int at = before.x + before.y;
   each([&](int i, uint32_t x) {
-    if (x > lo || (x == lo && eq < rank)) out[p.sink + at++] = bt[(c0 + i) * p.bt_si];
-    eq += x == lo;
+    bool take = sure && x > khi;
+    if (open(x)) {
+      take = !rescore;
+      if (rescore) {
+        const uint32_t y = score_key(__ldcg(&sc[i].y));
+        take = y > last_key || (y == last_key && ties-- > 0);
+      }
+    }
+    if (take) out[p.sink + at++] = bt[(c0 + i) * p.bt_si];
   });
 }
 
@@ -452,7 +587,7 @@ int check_select(const pab200_select_args* a) {
 }
 
 size_t scores_bytes(const pab200_select_args* a) {
-  return pabh::align256(size_t(a->num_seqs) * a->num_kv_heads * (a->max_blocks > 0 ? a->max_blocks : 1) * 4);
+  return pabh::align256(size_t(a->num_seqs) * a->num_kv_heads * (a->max_blocks > 0 ? a->max_blocks : 1) * 8);
 }
 
 template <typename T>
@@ -464,6 +599,22 @@ void launch_scores(const pab::SelectParams& p, int D, dim3 grid, cudaStream_t s)
   }
 }
 
+template <typename T, int D>
+cudaError_t launch_selection_d(const pab::SelectParams& p, bool small, const cudaLaunchConfig_t* cfg) {
+  return small ? cudaLaunchKernelEx(cfg, pab::select_pages_kernel<T, D, 256>, p)
+               : cudaLaunchKernelEx(cfg, pab::select_pages_kernel<T, D, 1024>, p);
+}
+
+template <typename T>
+cudaError_t launch_selection(const pab::SelectParams& p, int D, bool small,
+                             const cudaLaunchConfig_t* cfg) {
+  switch (D) {
+    case 64: return launch_selection_d<T, 64>(p, small, cfg);
+    case 128: return launch_selection_d<T, 128>(p, small, cfg);
+    default: return launch_selection_d<T, 256>(p, small, cfg);
+  }
+}
+
 int launch_select(const pab200_select_args* a, void* scores, cudaStream_t s) {
   pab::SelectParams p{};
   p.q = a->q;
@@ -472,7 +623,7 @@ int launch_select(const pab200_select_args* a, void* scores, cudaStream_t s) {
   p.bt = a->block_table;
   p.tables = a->tables;
   p.out_lens = a->selected_lens;
-  p.scores = static_cast<float*>(scores);
+  p.scores = static_cast<float2*>(scores);
   p.status = a->status;
   p.q_sb = a->q_stride_b;
   p.q_sh = a->q_stride_h;
@@ -513,8 +664,9 @@ int launch_select(const pab200_select_args* a, void* scores, cudaStream_t s) {
   // share an SM.
   const bool small = p.maxb <= 2048;
   pabh::LaunchCfg lc(dim3(units), dim3(small ? 256 : 1024), 0, s, scored);
-  cudaError_t err = small ? cudaLaunchKernelEx(&lc.cfg, pab::select_pages_kernel<256>, p)
-                          : cudaLaunchKernelEx(&lc.cfg, pab::select_pages_kernel<1024>, p);
+  const cudaError_t err = a->dtype == PAB200_DTYPE_BF16
+                              ? launch_selection<__nv_bfloat16>(p, a->head_size, small, &lc.cfg)
+                              : launch_selection<__half>(p, a->head_size, small, &lc.cfg);
   if (err != cudaSuccess) return pabh::cuda_fail(err, "page selection launch");
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? PAB200_OK : pabh::cuda_fail(e, "page selection launch");

@@ -178,6 +178,50 @@ def test_select_ties_nan_and_bad_pages(cuda_device):
         assert torch.equal(out.cpu(), wl) and torch.equal(tabs.cpu(), want)
 
 
+@pytest.mark.parametrize("dt,n,keep,spread", [
+    (BF, 3000, 700, 0.0),      # all alike but one page in seven: only the order decides
+    (HF, 5000, 1200, 2.0 ** -22), (BF, 9000, 40, 2.0 ** -20), (HF, 600, 300, 2.0 ** -24)])
+def test_select_scores_next_to_the_border(cuda_device, dt, n, keep, spread):
+    """Scores that an fp32 sum cannot tell apart: a common large part, and
+    differences of a few fp32 units, across hundreds of pages."""
+    D, G, bs = 128, 4, 8
+    g = torch.Generator().manual_seed(n)
+    q = torch.randn((1, G, D), generator=g).to(dt)
+    q[:, :, 1] = spread
+    base = torch.randn((1, 2, D), generator=g).abs() + 0.5
+    bounds = base.expand(n, 2, D).clone()
+    bounds[:, 0] = -bounds[:, 0]
+    bounds = bounds.to(dt)
+    # element 1 moves the score by spread * its value
+    bounds[:, :, 1] = torch.randint(0, 40, (n, 1), generator=g).to(dt)
+    if spread == 0.0:
+        bounds[::7, 1, 2] += 1.0
+    bt = torch.randperm(n, generator=g).to(torch.int32)[None]
+    lens = torch.tensor([n * bs], dtype=torch.int32)
+    tabs, out = pa.select_pages(q.to(cuda_device), bounds.to(cuda_device).view(n, 1, 2, D),
+                                bt.to(cuda_device), lens.to(cuda_device), bs, keep)
+    want, wl = expect_select(q, bounds, bt, lens, bs, keep, 1, 1, 1, False)
+    assert torch.equal(out.cpu(), wl) and torch.equal(tabs.cpu(), want)
+
+
+def test_select_infinite_bounds(cuda_device):
+    """A page with infinite bounds leaves its unit to the 64-bit scores."""
+    dt, D, bs, n = HF, 64, 8, 2500
+    g = torch.Generator().manual_seed(4)
+    x = torch.randn((n, 2, D), generator=g).to(dt)
+    bounds = torch.stack((x.amin(1), x.amax(1)), 1)
+    bounds[77, 1, 5] = float("inf")
+    bounds[1234, 0, 5] = -float("inf")
+    q = torch.randn((1, 3, D), generator=g).to(dt)
+    q[0, :, 5] = torch.tensor([1.0, -1.0, 2.0])    # no 0 * inf in either form of the sum
+    bt = torch.randperm(n, generator=g).to(torch.int32)[None]
+    lens = torch.tensor([n * bs - 1], dtype=torch.int32)
+    tabs, out = pa.select_pages(q.to(cuda_device), bounds.to(cuda_device).view(n, 1, 2, D),
+                                bt.to(cuda_device), lens.to(cuda_device), bs, 200)
+    want, wl = expect_select(q, bounds, bt, lens, bs, 200, 1, 1, 1, False)
+    assert torch.equal(out.cpu(), wl) and torch.equal(tabs.cpu(), want)
+
+
 def test_select_lengths_out_of_range(cuda_device):
     dt, D, bs = HF, 64, 8
     g = torch.Generator().manual_seed(0)
