@@ -322,15 +322,19 @@ __device__ __forceinline__ int2 block_scan(int2 x, int2* warp_sum, int2* total) 
 // compared with one another, else it becomes the range.  With e the bound of the
 // scores' errors, the true k-th lies within e of T: pages above T + 2 e are kept,
 // pages below T - 2 e are not, and unless exactly as many as are still wanted lie
-// between, those are scored in 64 bits and ranked by the same counting, equal
-// ones by page.  (A score or a size that is not finite leaves every page open.)
-// A thread owns consecutive pages, so that one scan places them in order; up to
-// kPer of its keys stay in registers.
+// between, those are scored in 64 bits and ranked, equal ones by page.  (A score
+// or a size that is not finite leaves every page open.)  A thread owns
+// consecutive pages, so that one scan places them in order.  The kernel is a
+// chain of short steps run once by few CTAs: loops are kept rolled, since cold
+// instructions cost as much as the steps.
 template <typename T, int D, int NTH>
 __global__ void __launch_bounds__(NTH) select_pages_kernel(const SelectParams p) {
-  constexpr int kBins = NTH, kLog2Bins = NTH == 1024 ? 10 : 8, kPer = 8;
-  __shared__ int hist[kBins];
-  __shared__ uint32_t list[kBins];
+  constexpr int kLog2Bins = NTH == 1024 ? 10 : 8;
+  constexpr int kHeld = NTH * 8;  // keys kept in shared memory (padded: no bank conflicts)
+  constexpr int kFew = 64;        // open pages compared directly
+  __shared__ uint32_t keys[kHeld + kHeld / 32];
+  __shared__ int hist[NTH];
+  __shared__ uint32_t list[NTH];
   __shared__ double qs[2 * D];
   __shared__ int2 sums[3][32];
   __shared__ uint32_t sh_lo[32], sh_hi[32];
@@ -346,57 +350,76 @@ __global__ void __launch_bounds__(NTH) select_pages_kernel(const SelectParams p)
   const int32_t* bt = p.bt + s * p.bt_sb + h * p.bt_sh;
   int32_t* out = p.tables + static_cast<int64_t>(u) * p.keep;
   hist[tid] = 0;
-  if (tid == 0) sh_listed = 0;
+  if (n > p.keep) {  // the query's parts, while the scores are still summed
+    const T* q = static_cast<const T*>(p.q) + s * p.q_sb + static_cast<int64_t>(h) * p.G * p.q_sh;
+    for (int d = tid; d < D; d += NTH) {
+      const double2 x = query_parts<T>(p, q, d);
+      qs[d] = x.x;
+      qs[D + d] = x.y;
+    }
+  }
   grid_dependency_wait();  // the scores; nothing of this call is written before
-  if (tid == 0 && raw != L && p.status) atomicOr(p.status, raw < 0 ? kStatusNegative : kStatusClamp);
+  if (tid == 0) {
+    if (raw != L && p.status) atomicOr(p.status, raw < 0 ? kStatusNegative : kStatusClamp);
+    p.out_lens[u] = n <= p.keep ? L : (p.keep - 1) * p.bs + L - (n - 1) * p.bs;
+  }
   if (n <= p.keep) {
     for (int i = tid; i < p.keep; i += NTH) out[i] = i < n ? bt[i * p.bt_si] : -1;
-    if (tid == 0) p.out_lens[u] = L;
     return;
   }
   const int c0 = p.sink, m = n - p.sink - p.recent;  // candidates, of which k are kept
   const int k = p.keep - p.sink - p.recent;
-  for (int i = tid; i < p.sink; i += NTH) out[i] = bt[i * p.bt_si];
-  for (int i = tid; i < p.recent; i += NTH)
-    out[p.keep - p.recent + i] = bt[(n - p.recent + i) * p.bt_si];
-  if (tid == 0) p.out_lens[u] = (p.keep - 1) * p.bs + L - (n - 1) * p.bs;
+  for (int i = tid; i < p.sink + p.recent; i += NTH) {
+    const bool first = i < p.sink;
+    out[first ? i : p.keep - p.recent + i - p.sink] =
+        bt[(first ? i : n - p.recent + i - p.sink) * p.bt_si];
+  }
   if (k == 0) return;
   float2* sc = p.scores + static_cast<int64_t>(u) * p.maxb + c0;
-  const int per = (m + NTH - 1) / NTH;
-  const int i0 = min(tid * per, m), i1 = min(i0 + per, m);
-  uint32_t key[kPer];
+  uint32_t lo = 0xffffffffu, hi = 0u;
   float size = 0.f;
-#pragma unroll
-  for (int j = 0; j < kPer; ++j) {
-    key[j] = 0u;
-    if (i0 + j < i1) {
-      const float2 x = __ldcg(sc + i0 + j);
-      key[j] = score_key(x.x);
-      size = x.y <= size ? size : x.y;  // a NaN is kept
-    }
+#pragma unroll 4
+  for (int i = tid; i < m; i += NTH) {
+    const float2 x = __ldcg(sc + i);
+    const uint32_t key = score_key(x.x);
+    if (i < kHeld) keys[i + (i >> 5)] = key;
+    lo = min(lo, key);
+    hi = max(hi, key);
+    size = x.y <= size ? size : x.y;  // a NaN is kept
   }
-  for (int i = i0 + kPer; i < i1; ++i) {
-    const float z = __ldcg(&sc[i].y);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const float z = __shfl_xor_sync(0xffffffffu, size, o);
     size = z <= size ? size : z;
   }
-  // This thread's pages and keys, in order.
-  auto each = [&](auto&& fn) {
-#pragma unroll
-    for (int j = 0; j < kPer; ++j)
-      if (i0 + j < i1) fn(i0 + j, key[j]);
-    for (int i = i0 + kPer; i < i1; ++i) fn(i, score_key(__ldcg(&sc[i].x)));
+  if (lane == 0) sh_size[warp] = size;
+  // This thread's pages, in order, with their keys.
+  const int per = (m + NTH - 1) / NTH;
+  const int i0 = min(tid * per, m), i1 = min(i0 + per, m);
+  auto key_of = [&](int i) { return i < kHeld ? keys[i + (i >> 5)] : score_key(__ldcg(&sc[i].x)); };
+  uint32_t khi = 0xffffffffu, klo = 0u;  // keys above khi are kept, below klo not
+  bool sure = true, exact = false;       // exact: the search is among the open pages
+  auto open = [&](uint32_t x) { return !sure || (x <= khi && x >= klo); };
+  // The keys the search is among: all, or the 64-bit ones (in place of the
+  // sizes, read by then) of the open pages.
+  auto walk = [&](auto&& fn) {
+#pragma unroll 1
+    for (int i = i0; i < i1; ++i) {
+      const uint32_t x = key_of(i);
+      if (!exact)
+        fn(x);
+      else if (open(x))
+        fn(score_key(__ldcg(&sc[i].y)));
+    }
   };
-  // The rank-th largest of the keys that `walk` visits, and its rank among the
-  // equal ones.  All threads call it together; `hist` is zero before and after.
-  auto kth = [&](auto&& walk, int rank) -> int2 {
-    uint32_t lo = 0xffffffffu, hi = 0u;
-    walk([&](int, uint32_t x) {
-      lo = min(lo, x);
-      hi = max(hi, x);
-    });
+  int rank = k, want = 0, opened = 0;
+  int2 before = make_int2(0, 0), total;
+  bool few = false;
+#pragma unroll 1
+  for (;;) {
+    // The rank-th largest key, left in lo, with its rank among the equal ones.
     lo = __reduce_min_sync(0xffffffffu, lo);
     hi = __reduce_max_sync(0xffffffffu, hi);
-    __syncthreads();
     if (lane == 0) {
       sh_lo[warp] = lo;
       sh_hi[warp] = hi;
@@ -404,32 +427,32 @@ __global__ void __launch_bounds__(NTH) select_pages_kernel(const SelectParams p)
     __syncthreads();
     lo = __reduce_min_sync(0xffffffffu, sh_lo[lane % (NTH / 32)]);
     hi = __reduce_max_sync(0xffffffffu, sh_hi[lane % (NTH / 32)]);
+#pragma unroll 1
     while (lo < hi) {
       const int bits = 32 - __clz(hi - lo);
       const int shift = bits > kLog2Bins ? bits - kLog2Bins : 0;
-      walk([&](int, uint32_t x) {
+      walk([&](uint32_t x) {
         if (x >= lo && x <= hi) atomicAdd(&hist[(x - lo) >> shift], 1);
       });
       if (tid == 0) sh_listed = 0;
       __syncthreads();
       // thread t looks at bin NTH - 1 - t: how many keys lie in the bins above it
-      const int mine = hist[kBins - 1 - tid];
-      int2 total;
+      const int mine = hist[NTH - 1 - tid];
       const int above = block_scan<NTH>(make_int2(mine, 0), sums[0], &total).x;
       if (above < rank && rank <= above + mine) {
-        sh_bin = kBins - 1 - tid;
+        sh_bin = NTH - 1 - tid;
         sh_rank = rank - above;
         sh_count = mine;
       }
-      hist[kBins - 1 - tid] = 0;
+      hist[NTH - 1 - tid] = 0;
       __syncthreads();
       rank = sh_rank;
       lo += static_cast<uint32_t>(sh_bin) << shift;
       const uint32_t last = lo + ((1u << shift) - 1u);
       hi = last < hi ? last : hi;
       const int count = sh_count;
-      if (lo < hi && count <= kBins) {
-        walk([&](int, uint32_t x) {
+      if (lo < hi && count <= NTH) {
+        walk([&](uint32_t x) {
           if (x >= lo && x <= hi) list[atomicAdd(&sh_listed, 1)] = x;
         });
         __syncthreads();
@@ -451,93 +474,100 @@ __global__ void __launch_bounds__(NTH) select_pages_kernel(const SelectParams p)
         rank = sh_rank;
       }
     }
-    return make_int2(static_cast<int>(lo), rank);
-  };
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const float z = __shfl_xor_sync(0xffffffffu, size, o);
-    size = z <= size ? size : z;
-  }
-  if (lane == 0) sh_size[warp] = size;
-  const uint32_t tkey = static_cast<uint32_t>(kth(each, k).x);  // its barriers publish sh_size
-  for (int w = 0; w < NTH / 32; ++w) size = sh_size[w] <= size ? size : sh_size[w];
-  // Keys above khi are kept, below klo not.
-  const float t = key_score(tkey), e2 = 2.f * (size * kScoreError + 1e-37f);
-  const bool sure = e2 <= 3e38f && t == t;
-  const uint32_t khi = sure ? score_key(t + e2) : 0xffffffffu, klo = sure ? score_key(t - e2) : 0u;
-  auto open = [&](uint32_t x) { return !sure || (x <= khi && x >= klo); };
-  int2 cnt = make_int2(0, 0), total;
-  each([&](int, uint32_t x) {
-    cnt.x += sure && x > khi;
-    cnt.y += open(x);
-  });
-  int2 before = block_scan<NTH>(cnt, sums[1], &total);
-  const int want = k - total.x;  // of the total.y open pages
-  uint32_t last_key = 0u;        // open pages above it are kept, and `ties` equal to it
-  int ties = 0;
-  const bool rescore = want < total.y;
-  if (rescore) {
-    const T* q = static_cast<const T*>(p.q) + s * p.q_sb + static_cast<int64_t>(h) * p.G * p.q_sh;
-    for (int d = tid; d < D; d += NTH) {
-      const double2 x = query_parts<T>(p, q, d);
-      qs[d] = x.x;
-      qs[D + d] = x.y;
+    if (exact) break;
+    for (int w = 0; w < NTH / 32; ++w) size = sh_size[w] <= size ? size : sh_size[w];
+    const float t = key_score(lo), e2 = 2.f * (size * kScoreError + 1e-37f);
+    sure = e2 <= 3e38f && t == t;
+    if (sure) {
+      khi = score_key(t + e2);
+      klo = score_key(t - e2);
     }
-    auto settle = [&](int i) {  // a warp's work
+    int2 cnt = make_int2(0, 0);
+#pragma unroll 1
+    for (int i = i0; i < i1; ++i) {
+      const uint32_t x = key_of(i);
+      cnt.x += sure && x > khi;
+      cnt.y += open(x);
+    }
+    before = block_scan<NTH>(cnt, sums[1], &total);
+    want = k - total.x;  // of the open pages
+    opened = total.y;
+    if (want == opened) break;
+    few = opened <= kFew;
+    // The open pages' 64-bit scores, a warp each.
+    if (opened <= NTH) {
+      int at = before.y;
+#pragma unroll 1
+      for (int i = i0; i < i1; ++i)
+        if (open(key_of(i))) list[at++] = static_cast<uint32_t>(i);
+    }
+    __syncthreads();
+    const int todo = opened <= NTH ? opened : m;
+#pragma unroll 1
+    for (int j = warp; j < todo; j += NTH / 32) {
+      const int i = opened <= NTH ? static_cast<int>(list[j]) : j;
+      if (opened > NTH && !open(key_of(i))) continue;
       const int64_t pid = static_cast<int64_t>(bt[(c0 + i) * p.bt_si]) * p.bt_mul +
                           static_cast<int64_t>(h) * p.bt_add;
       const float x = exact_score<T, D>(p, pid, qs);
-      if (lane == 0) __stcg(&sc[i].y, x);  // the sizes have been read
-    };
-    if (total.y <= kBins) {
-      int at = before.y;
-      each([&](int i, uint32_t x) {
-        if (open(x)) list[at++] = static_cast<uint32_t>(i);
-      });
-      __syncthreads();
-      for (int j = warp; j < total.y; j += NTH / 32) settle(static_cast<int>(list[j]));
-    } else {
-      __syncthreads();
-      for (int i = warp; i < m; i += NTH / 32)
-        if (open(score_key(__ldcg(&sc[i].x)))) settle(i);
+      if (lane == 0) {
+        if (few)
+          list[kFew + j] = score_key(x);
+        else
+          __stcg(&sc[i].y, x);
+      }
     }
     __syncthreads();
-    const int2 found = kth(
-        [&](auto&& fn) {
-          each([&](int i, uint32_t x) {
-            if (open(x)) fn(i, score_key(__ldcg(&sc[i].y)));
-          });
-        },
-        want);
-    last_key = static_cast<uint32_t>(found.x);
-    ties = found.y;
-    // ties before this thread's pages, then kept pages before them
-    int2 eq = make_int2(0, 0);
-    cnt.y = 0;
-    each([&](int i, uint32_t x) {
-      if (!open(x)) return;
-      const uint32_t y = score_key(__ldcg(&sc[i].y));
-      cnt.y += y > last_key;
-      eq.x += y == last_key;
+    if (few) break;
+    exact = true;
+    rank = want;
+    lo = 0xffffffffu;
+    hi = 0u;
+    walk([&](uint32_t x) {
+      lo = min(lo, x);
+      hi = max(hi, x);
     });
-    __syncthreads();
-    const int2 eq_before = block_scan<NTH>(eq, sums[0], &total);
-    before = block_scan<NTH>(cnt, sums[2], &total);
-    ties -= eq_before.x;  // left for this thread's pages
-    before.y += min(eq_before.x, found.y);
   }
-  int at = before.x + before.y;
-  each([&](int i, uint32_t x) {
+  // Pages above khi and, of the open ones: all; of a few, those with fewer than
+  // `want` before them; of many, those above lo and the first `rank` equal to it.
+  int at = before.x + before.y, ties = 0;
+  if (few) {
+    if (tid < opened) {
+      const uint32_t x = list[kFew + tid];
+      int ahead = 0;
+      for (int i = 0; i < opened; ++i)
+        ahead += list[kFew + i] > x || (list[kFew + i] == x && i < tid);
+      hist[tid] = ahead < want;
+    }
+    __syncthreads();
+    at = before.x;
+    for (int i = 0; i < before.y; ++i) at += hist[i];
+  } else if (exact) {
+    int2 cnt = make_int2(0, 0);
+    walk([&](uint32_t y) {
+      cnt.x += y > lo;
+      cnt.y += y == lo;
+    });
+    const int2 b = block_scan<NTH>(cnt, sums[2], &total);
+    ties = rank - b.y;  // left for this thread's pages
+    at = before.x + b.x + min(b.y, rank);
+  }
+  int j = before.y;
+#pragma unroll 1
+  for (int i = i0; i < i1; ++i) {
+    const uint32_t x = key_of(i);
     bool take = sure && x > khi;
     if (open(x)) {
-      take = !rescore;
-      if (rescore) {
+      take = true;
+      if (few) {
+        take = hist[j++] != 0;
+      } else if (exact) {
         const uint32_t y = score_key(__ldcg(&sc[i].y));
-        take = y > last_key || (y == last_key && ties-- > 0);
+        take = y > lo || (y == lo && ties-- > 0);
       }
     }
     if (take) out[p.sink + at++] = bt[(c0 + i) * p.bt_si];
-  });
+  }
 }
 
 }  // namespace pab
