@@ -169,6 +169,12 @@ struct DecodeParams {
   // cross-device state output (optional)
   float* state_o;
   float* state_lse;
+  // Lengths and most pages per head the planner plans with: the lengths the
+  // decode reads, or, of a page-sparse call, whose tables and lengths are still
+  // being selected, the whole contexts' and the pages each keeps at most.
+  const int32_t* plan_lens;
+  int64_t plan_sb, plan_sh;
+  int32_t plan_maxb, plan_most;
   // optional: append each (sequence, kv head)'s new token before planning
   int32_t append;
   AppendParams app;
@@ -325,7 +331,7 @@ __global__ void __launch_bounds__(1024) plan_kernel(const DecodeParams p) {
   __shared__ uint32_t par_sm;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int n_heads = p.B * p.Hkv;
-  const int cap = p.maxb * p.bs;
+  const int cap = p.plan_maxb * p.bs;
   // This kernel may start while the previous call's kernels on the stream
   // still run (programmatic dependent launch: the previous reduce kernel
   // lets it start at once), and it lets the decode grid start at once.  Nothing is written before the wait for the
@@ -343,7 +349,7 @@ __global__ void __launch_bounds__(1024) plan_kernel(const DecodeParams p) {
   uint32_t flags = 0;
   auto head_pages = [&](int hd) {
     const int s = hd / p.Hkv, h = hd - s * p.Hkv;
-    int L = p.lens[s * p.l_sb + h * p.l_sh];
+    int L = p.plan_lens[s * p.plan_sb + h * p.plan_sh];
     if (L < 0) {
       flags |= kStatusNegative;
       L = 0;
@@ -351,7 +357,7 @@ __global__ void __launch_bounds__(1024) plan_kernel(const DecodeParams p) {
       flags |= kStatusClamp;
       L = cap;
     }
-    return (L + p.bs - 1) / p.bs;
+    return min((L + p.bs - 1) / p.bs, p.plan_most);
   };
   if constexpr (APPEND) {
     // The step's new tokens go into the cache first, once the previous

@@ -72,10 +72,19 @@ struct Int4Kernel {
 };
 bool select_int4_kernel(int dtype, int D, int G, Int4Kernel* o);
 
-// A decode over tables that an earlier kernel of the same call wrote: like
-// pab200_decode(), but the planner is launched after everything before it on
-// the stream has finished (pab200.cu).
-int decode_after(const pab200_decode_args* a, void* workspace, size_t workspace_bytes,
-                 void* stream);
+// A selection of pages inside a decode call: the whole contexts' lengths and
+// table width, and the launch of the kernels that write the call's tables and
+// lengths (programmatically dependent on the planner before them, which touches
+// nothing of theirs; the last of them starts the decode grid's dependency).
+struct Selection {
+  const int32_t* lens;
+  int64_t l_sb, l_sh;
+  int32_t max_blocks;
+  int (*launch)(const void* what, cudaStream_t s);
+  const void* what;
+};
+// pab200_decode() over the tables that `sel` writes.
+int decode_selected(const pab200_decode_args* a, const Selection& sel, void* workspace,
+                    size_t workspace_bytes, void* stream);
 
 }  // namespace pabh

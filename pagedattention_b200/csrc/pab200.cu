@@ -670,13 +670,14 @@ cudaError_t launch_exchange(const pab::ExchangeParams& p, int out_dtype, int fus
 // step's tokens; with `exchange`, the call ends in the fused exchange + merge
 // of a context split across GPUs instead of the reduce kernel.
 // `after_inputs`: the planner is launched without programmatic dependence, so
-// that everything before it on the stream, the writer of this call's tables
-// and lengths among it, has finished before the planner or the decode grid
-// reads anything.
+// that everything before it on the stream has finished before it or the decode
+// grid reads anything.  `sel`: a page-sparse call (after_inputs too): the planner
+// plans from the whole contexts' lengths, then the selection is launched, which
+// writes the tables and lengths of `a`, then the decode grid, which waits for it.
 int decode_impl(const pab200_decode_args* a, const Plan& pl, const pab::AppendParams* app,
                 void* workspace, size_t workspace_bytes, void* stream,
                 pab::ExchangeParams* exchange = nullptr, int exchange_dtype = 0,
-                bool after_inputs = false) {
+                bool after_inputs = false, const pabh::Selection* sel = nullptr) {
   int rc = PAB200_OK;
   if (!workspace || workspace_bytes < pl.ws_bytes)
     return fail(PAB200_ERR_WORKSPACE, "workspace of %zu bytes needed, %zu given", pl.ws_bytes,
@@ -707,6 +708,11 @@ int decode_impl(const pab200_decode_args* a, const Plan& pl, const pab::AppendPa
   p.D = a->head_size;
   p.bs = a->block_size;
   p.maxb = a->max_blocks;
+  p.plan_lens = sel ? sel->lens : p.lens;
+  p.plan_sb = sel ? sel->l_sb : p.l_sb;
+  p.plan_sh = sel ? sel->l_sh : p.l_sh;
+  p.plan_maxb = sel ? sel->max_blocks : p.maxb;
+  p.plan_most = p.maxb;
   p.num_pages = a->num_pages;
   p.head_in_map = a->layout == PAB200_LAYOUT_NHD ? 1 : 0;
   p.scale_log2 = a->softmax_scale * pab::kLog2e;
@@ -736,7 +742,7 @@ int decode_impl(const pab200_decode_args* a, const Plan& pl, const pab::AppendPa
   // nor with mma.sync warp pairs, and only while the prefix fits shared
   // memory (the tcgen05 path keeps it in its operand tiles).
   static_assert(pab::kQ4Early == pab::kEarlyMaxHeads, "one bound for both decode kernels");
-  p.early = !app && (!pl.pair || pl.tc) && pl.n_heads <= pab::kEarlyMaxHeads &&
+  p.early = !app && !sel && (!pl.pair || pl.tc) && pl.n_heads <= pab::kEarlyMaxHeads &&
             env_int("PAB200_EARLY", 1) != 0;
   if (app) {
     p.app = *app;
@@ -761,6 +767,7 @@ int decode_impl(const pab200_decode_args* a, const Plan& pl, const pab::AppendPa
   cudaError_t e = a->dtype == PAB200_DTYPE_BF16 ? launch_plan<__nv_bfloat16>(p, s, pdl_plan)
                                                  : launch_plan<__half>(p, s, pdl_plan);
   if (e != cudaSuccess) return cuda_fail(e, "plan kernel launch");
+  if (sel && (rc = sel->launch(sel->what, s))) return rc;
   if (a->event_before) {
     e = cudaEventRecord(static_cast<cudaEvent_t>(a->event_before), s);
     if (e != cudaSuccess) return cuda_fail(e, "cudaEventRecord");
@@ -801,12 +808,16 @@ PAB200_EXPORT int pab200_decode(const pab200_decode_args* a, void* workspace,
   return decode_impl(a, pl, nullptr, workspace, workspace_bytes, stream);
 }
 
-int pabh::decode_after(const pab200_decode_args* a, void* workspace, size_t workspace_bytes,
-                       void* stream) {
+int pabh::decode_selected(const pab200_decode_args* a, const Selection& sel, void* workspace,
+                          size_t workspace_bytes, void* stream) {
   Plan pl;
   const int rc = make_plan(a, &pl, SIZE_MAX);
   if (rc) return rc;
-  return decode_impl(a, pl, nullptr, workspace, workspace_bytes, stream, nullptr, 0, true);
+  // Equal pages per head and a few stages per warp: claiming tail chunks costs
+  // more than the balance it buys (48 sequences x 8 kv heads x 64 pages of 32
+  // tokens: 113 us per call without, 120 us with).
+  lay_out_workspace(&pl, 0, SIZE_MAX);
+  return decode_impl(a, pl, nullptr, workspace, workspace_bytes, stream, nullptr, 0, true, &sel);
 }
 
 // ------------------------------------------------------------- 4-bit pages

@@ -178,7 +178,10 @@ __global__ void __launch_bounds__(256, 4) page_scores_kernel(const SelectParams 
   }
   const int n = (clamped_length(p, s, h) + p.bs - 1) / p.bs;
   const int c1 = min(c0 + p.chunk, n - p.recent);
-  if (n <= p.keep || c0 >= c1) return;
+  if (n <= p.keep || c0 >= c1) {
+    grid_dependency_wait();
+    return;
+  }
   const int count = min(per, c1 - w0);
   // This warp's pages: ids, -1 for one out of range.
 #pragma unroll
@@ -248,9 +251,8 @@ __global__ void __launch_bounds__(256, 4) page_scores_kernel(const SelectParams 
     if ((lane & 7) == 0 && t + v < count)
       out[t + v] = x.bad >> v & 1 ? make_float2(-INFINITY, 0.f) : make_float2(r, z);
   };
-  if (count <= 0) return;
   Pages x, y;
-  load(0, x);
+  if (count > 0) load(0, x);
   for (int t = 0; t < count; t += 2 * U) {
     if (t + U < count) load(t + U, y);
     score(t, x);
@@ -258,6 +260,9 @@ __global__ void __launch_bounds__(256, 4) page_scores_kernel(const SelectParams 
     if (t + 2 * U < count) load(t + 2 * U, x);
     score(t + U, y);
   }
+  // In a decode call the planner runs beside this kernel: what waits for this
+  // grid must be able to count on the planner's end too.
+  grid_dependency_wait();
 }
 
 // The score of page `pid` by its definition, in every lane of a warp; `qs`: the
@@ -621,11 +626,11 @@ size_t scores_bytes(const pab200_select_args* a) {
 }
 
 template <typename T>
-void launch_scores(const pab::SelectParams& p, int D, dim3 grid, cudaStream_t s) {
+cudaError_t launch_scores(const pab::SelectParams& p, int D, const cudaLaunchConfig_t* cfg) {
   switch (D) {
-    case 64: pab::page_scores_kernel<T, 64><<<grid, 256, 0, s>>>(p); break;
-    case 128: pab::page_scores_kernel<T, 128><<<grid, 256, 0, s>>>(p); break;
-    default: pab::page_scores_kernel<T, 256><<<grid, 256, 0, s>>>(p); break;
+    case 64: return cudaLaunchKernelEx(cfg, pab::page_scores_kernel<T, 64>, p);
+    case 128: return cudaLaunchKernelEx(cfg, pab::page_scores_kernel<T, 128>, p);
+    default: return cudaLaunchKernelEx(cfg, pab::page_scores_kernel<T, 256>, p);
   }
 }
 
@@ -645,7 +650,8 @@ cudaError_t launch_selection(const pab::SelectParams& p, int D, bool small,
   }
 }
 
-int launch_select(const pab200_select_args* a, void* scores, cudaStream_t s) {
+// `pdl`: programmatically dependent on the kernel before it (the planner).
+int launch_select(const pab200_select_args* a, void* scores, bool pdl, cudaStream_t s) {
   pab::SelectParams p{};
   p.q = a->q;
   p.bounds = a->page_bounds;
@@ -684,16 +690,17 @@ int launch_select(const pab200_select_args* a, void* scores, cudaStream_t s) {
     const int chunk = each < 64 ? 64 : (each > 512 ? 512 : static_cast<int>(each));
     p.chunk = chunk;
     const dim3 grid((p.maxb + chunk - 1) / chunk, units);
-    if (a->dtype == PAB200_DTYPE_BF16)
-      launch_scores<__nv_bfloat16>(p, a->head_size, grid, s);
-    else
-      launch_scores<__half>(p, a->head_size, grid, s);
+    pabh::LaunchCfg sc(grid, dim3(256), 0, s, pdl);
+    const cudaError_t e = a->dtype == PAB200_DTYPE_BF16
+                              ? launch_scores<__nv_bfloat16>(p, a->head_size, &sc.cfg)
+                              : launch_scores<__half>(p, a->head_size, &sc.cfg);
+    if (e != cudaSuccess) return pabh::cuda_fail(e, "page scores launch");
   }
   // Scheduled while the scores drain; waits for them before it reads any.
   // 256 threads while 8 registers hold a thread's keys, so that several units
   // share an SM.
   const bool small = p.maxb <= 2048;
-  pabh::LaunchCfg lc(dim3(units), dim3(small ? 256 : 1024), 0, s, scored);
+  pabh::LaunchCfg lc(dim3(units), dim3(small ? 256 : 1024), 0, s, scored || pdl);
   const cudaError_t err = a->dtype == PAB200_DTYPE_BF16
                               ? launch_selection<__nv_bfloat16>(p, a->head_size, small, &lc.cfg)
                               : launch_selection<__half>(p, a->head_size, small, &lc.cfg);
@@ -743,7 +750,7 @@ PAB200_EXPORT int pab200_select_pages(const pab200_select_args* a, void* workspa
     return fail(PAB200_ERR_WORKSPACE, "workspace of %zu bytes needed, %zu given", scores_bytes(a),
                 workspace ? workspace_bytes : size_t(0));
   if (!aligned(workspace, 256)) return fail(PAB200_ERR_ALIGNMENT, "workspace must be 256-byte aligned");
-  return launch_select(a, workspace, static_cast<cudaStream_t>(stream));
+  return launch_select(a, workspace, false, static_cast<cudaStream_t>(stream));
 }
 
 PAB200_EXPORT size_t pab200_decode_sparse_workspace_size(const pab200_decode_args* a,
@@ -766,9 +773,22 @@ PAB200_EXPORT int pab200_decode_sparse(const pab200_decode_args* a, const pab200
     return fail(PAB200_ERR_WORKSPACE, "workspace of %zu bytes needed, %zu given", all,
                 workspace ? workspace_bytes : size_t(0));
   if (!aligned(workspace, 256)) return fail(PAB200_ERR_ALIGNMENT, "workspace must be 256-byte aligned");
-  rc = launch_select(sel, static_cast<uint8_t*>(workspace) + at, static_cast<cudaStream_t>(stream));
-  if (rc) return rc;
-  return pabh::decode_after(&d, workspace, need, stream);
+  struct What {
+    const pab200_select_args* sel;
+    void* scores;
+  };
+  const What what{sel, static_cast<uint8_t*>(workspace) + at};
+  pabh::Selection in{};
+  in.lens = sel->seqlens;
+  in.l_sb = sel->seqlens_stride_b;
+  in.l_sh = sel->seqlens_stride_h;
+  in.max_blocks = sel->num_pages > 0 ? sel->max_blocks : 0;
+  in.launch = [](const void* w, cudaStream_t s) {
+    const What* x = static_cast<const What*>(w);
+    return launch_select(x->sel, x->scores, true, s);
+  };
+  in.what = &what;
+  return pabh::decode_selected(&d, in, workspace, need, stream);
 }
 
 namespace {

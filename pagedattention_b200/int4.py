@@ -18,8 +18,8 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from .kernel_b200 import (_DTYPES, _append_status_word, _as_int32, _check_device,
-                          _keep_workspace, _on_device, _raise_for)
+from .kernel_b200 import (_DTYPES, _append_status_word, _as_int32, _call_with_workspace,
+                          _check_device, _keep_workspace, _on_device, _raise_for)
 
 _HEAD_SIZES = (64, 128, 256)
 _BLOCK_SIZES = (8, 16, 32, 64)
@@ -250,12 +250,8 @@ def paged_attention_int4(out, query, key_cache, value_cache, block_tables, conte
 
 
 def _run_int4(args, device, stream):
-    lib = _lib.load()
-    need = lib.pab200_decode_int4_workspace_size(args)
-    if need == 0:
-        raise ValueError(f"pab200_decode_int4: {lib.pab200_last_error().decode()}")
-    ws = torch.empty(need, dtype=torch.uint8, device=device)
-    rc = lib.pab200_decode_int4(args, ws.data_ptr(), need, stream)
-    if rc:
-        _raise_for(lib, rc, "pab200_decode_int4")
+    ws = _call_with_workspace(
+        _lib.load(), "pab200_decode_int4", device,
+        (args.dtype, args.num_seqs, args.num_q_heads, args.num_kv_heads, args.head_size,
+         args.block_size, args.max_blocks, args.num_splits), (args,), stream)
     _keep_workspace(device, ws, stream)

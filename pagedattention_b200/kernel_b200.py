@@ -193,6 +193,32 @@ def _on_device(device, fn, *args):
         return fn(*args, _current_stream_handle(device))
 
 
+_call_ws_sizes: dict[tuple, int] = {}
+
+
+def _call_with_workspace(lib, call, device, sizes, args, stream) -> torch.Tensor:
+    """``call(*args, workspace, bytes, stream)`` with a workspace of its own: the
+    caching allocator orders it with the stream, and a captured graph keeps it.
+    Its size depends on the call's sizes and the device alone and is asked for
+    once (again when a tuning variable has changed it).  Returns the workspace."""
+    key = (call, device.index) + sizes
+    for _ in range(2):
+        need = _call_ws_sizes.get(key)
+        if need is None:
+            need = getattr(lib, call + "_workspace_size")(*args)
+            if need == 0:
+                raise ValueError(f"{call}: {lib.pab200_last_error().decode()}")
+            _call_ws_sizes[key] = need
+        ws = torch.empty(need, dtype=torch.uint8, device=device)
+        rc = getattr(lib, call)(*args, ws.data_ptr(), need, stream)
+        if rc != _lib.ERR_WORKSPACE:
+            break
+        _call_ws_sizes.clear()
+    if rc:
+        _raise_for(lib, rc, call)
+    return ws
+
+
 def _keep_workspace(device, ws, stream_handle) -> None:
     """The workspace whose status word ``read_status`` reports next."""
     _last_ws[device.index] = (ws, stream_handle)

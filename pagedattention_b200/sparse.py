@@ -14,8 +14,8 @@ import torch
 
 from . import _lib
 from .int4 import _append_status_ptr, _check_offsets, _check_table, _length_strides
-from .kernel_b200 import (_DTYPES, _as_int32, _check_device, _keep_workspace, _on_device,
-                          _paged_args, _raise_for)
+from .kernel_b200 import (_DTYPES, _as_int32, _call_with_workspace, _check_device,
+                          _keep_workspace, _on_device, _paged_args, _raise_for)
 
 
 def _check_bounds(page_bounds, block_table, num_seqs, num_kv_heads, head_size, dtype):
@@ -146,14 +146,8 @@ def select_pages(query, page_bounds, block_tables, context_lens, block_size, num
 
 
 def _run_select(a, device, stream):
-    lib = _lib.load()
-    need = lib.pab200_select_pages_workspace_size(a)
-    if need == 0:
-        raise ValueError(f"pab200_select_pages: {lib.pab200_last_error().decode()}")
-    ws = torch.empty(need, dtype=torch.uint8, device=device)
-    rc = lib.pab200_select_pages(a, ws.data_ptr(), need, stream)
-    if rc:
-        _raise_for(lib, rc, "pab200_select_pages")
+    _call_with_workspace(_lib.load(), "pab200_select_pages", device,
+                         (a.num_seqs, a.num_kv_heads, a.max_blocks), (a,), stream)
 
 
 def paged_attention_sparse(out, query, key_cache, value_cache, page_bounds, block_tables,
@@ -186,12 +180,8 @@ def paged_attention_sparse(out, query, key_cache, value_cache, page_bounds, bloc
 
 
 def _run_sparse(args, sel, device, stream):
-    lib = _lib.load()
-    need = lib.pab200_decode_sparse_workspace_size(args, sel)
-    if need == 0:
-        raise ValueError(f"pab200_decode_sparse: {lib.pab200_last_error().decode()}")
-    ws = torch.empty(need, dtype=torch.uint8, device=device)
-    rc = lib.pab200_decode_sparse(args, sel, ws.data_ptr(), need, stream)
-    if rc:
-        _raise_for(lib, rc, "pab200_decode_sparse")
+    ws = _call_with_workspace(
+        _lib.load(), "pab200_decode_sparse", device,
+        (args.dtype, args.num_seqs, args.num_q_heads, args.num_kv_heads, args.head_size,
+         args.block_size, args.num_splits, sel.max_blocks, sel.num_selected), (args, sel), stream)
     _keep_workspace(device, ws, stream)
