@@ -132,6 +132,7 @@ struct DecodeParams {
   int64_t num_pages;
   const uint8_t* k_pages;  // 4-bit caches: the pages (no tensor map)
   const uint8_t* v_pages;
+  int32_t gather;       // four pages per copy, through the tensor maps
   int32_t unit_pages;   // fewest pages per range where there are enough: fewer ranges otherwise
   int32_t head_in_map;  // NHD layout: kv head is the tensor map's y coordinate
   float scale_log2;     // softmax_scale * log2(e)

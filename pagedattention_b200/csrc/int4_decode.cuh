@@ -7,9 +7,10 @@
 // widen before the matrix instructions can take them: instruction issue bounds
 // the kernel, not HBM, so everything is laid out for few instructions per code.
 //   * One producer warp per CTA walks the CTA's page range (the planner's
-//     equal cut of all pages, as in decode.cuh), reads the block table one
-//     stage ahead and fills a ring of 128-token stages with one untiled bulk
-//     copy per page and cache.  Four consumer warps share every stage, 32
+//     equal cut of all pages with its tail chunks, as in decode.cuh), reads the
+//     block table one stage ahead and fills a ring of 128-token stages: four
+//     pages of a cache per copy (rows gathered through a tensor map, pages up to
+//     2 KB), or one untiled bulk copy per page.  Four consumer warps share every stage, 32
 //     tokens each (groups of more than 16 heads at D 128: two pairs, each pair
 //     16 heads and 64 tokens per warp), and do nothing but arithmetic.
 //   * Keys enter the MMA as fp16 subnormals, the nibbles as they stand (one
@@ -38,6 +39,7 @@ constexpr int kQ4Consumers = 4;                       // consumer warps per CTA
 constexpr int kQ4Threads = (kQ4Consumers + 1) * 32;
 constexpr int kQ4Stage = 128;                         // tokens per ring stage
 constexpr int kQ4MaxDepth = 4;
+constexpr int kQ4NoHead = 1 << 27;                    // in a stage record: no next head
 constexpr int kQ4Early = 1024;                        // heads whose prefix a CTA keeps itself
 
 // Shared memory: ring, then joining buffer, then barriers, records, prefix.
@@ -52,7 +54,8 @@ __host__ __device__ constexpr size_t q4_smem(int D, int G, int parts, int depth)
 
 template <typename T, int D, int NT, int HS, int MINB>
 __global__ void __launch_bounds__(kQ4Threads, MINB)
-    decode_int4_kernel(const __grid_constant__ CUtensorMap, const __grid_constant__ CUtensorMap,
+    decode_int4_kernel(const __grid_constant__ CUtensorMap kmap,
+                       const __grid_constant__ CUtensorMap vmap,
                        const __grid_constant__ DecodeParams p) {
   constexpr int NG = D / kInt4Group;           // quantisation groups per row
   constexpr int KS = D / 16;                   // k-steps of the scores, d-tiles of the output
@@ -80,7 +83,8 @@ __global__ void __launch_bounds__(kQ4Threads, MINB)
   uint8_t* const tail = reinterpret_cast<uint8_t*>(join + q4_join_floats(D, G, PARTS));
   const uint32_t full = smem_addr(tail), empty = full + kQ4MaxDepth * 8;
   int4* const record = reinterpret_cast<int4*>(tail + kQ4MaxDepth * 16);
-  const uint32_t joined = full + kQ4MaxDepth * 32;  // consumers' own barrier
+  // consumers' own barriers: states deposited, states read
+  const uint32_t joined = full + kQ4MaxDepth * 32, drained = joined + 8;
   int* const cum_sm = reinterpret_cast<int*>(tail + kQ4MaxDepth * 32 + 16);
   int* const len_sm = cum_sm + kQ4Early + 1;
   int* const wsum = len_sm + kQ4Early;
@@ -100,7 +104,12 @@ __global__ void __launch_bounds__(kQ4Threads, MINB)
       mbar_init(empty + i * 8, kQ4Consumers);
     }
     mbar_init(joined, kQ4Consumers);
+    mbar_init(drained, kQ4Consumers);
     fence_mbar_init();
+    if (p.gather) {
+      tma_prefetch_desc(&kmap);
+      tma_prefetch_desc(&vmap);
+    }
   }
   // The page-count prefix of all heads, computed by this CTA like the planner
   // computes it for the reduce kernel (up to kQ4Early heads; more: the
@@ -111,11 +120,17 @@ __global__ void __launch_bounds__(kQ4Threads, MINB)
   if (early) {
     const int per = (n_heads + kQ4Threads - 1) / kQ4Threads;
     const int h0 = min(tid * per, n_heads), h1 = min(h0 + per, n_heads);
-    int sum = 0;
+    int sum = 0, s = h0 / Hkv, h = h0 - s * Hkv;
+#pragma unroll 1
     for (int hd = h0; hd < h1; ++hd) {
-      const int L = head_len(hd);
+      int L = p.lens[s * p.l_sb + h * p.l_sh];
+      L = L < 0 ? 0 : (L > cap ? cap : L);
       len_sm[hd] = L;
       sum += (L + bs - 1) >> log2_bs;
+      if (++h == Hkv) {
+        h = 0;
+        ++s;
+      }
     }
     int x = sum;
 #pragma unroll
@@ -127,6 +142,7 @@ __global__ void __launch_bounds__(kQ4Threads, MINB)
     __syncthreads();
     int run = x - sum;
     for (int w = 0; w < warp; ++w) run += wsum[w];
+#pragma unroll 1
     for (int hd = h0; hd < h1; ++hd) {
       cum_sm[hd] = run;
       run += (len_sm[hd] + bs - 1) >> log2_bs;
@@ -141,6 +157,8 @@ __global__ void __launch_bounds__(kQ4Threads, MINB)
   }
   const int64_t units = (static_cast<int64_t>(total) + p.unit_pages - 1) / p.unit_pages;
   const int W = static_cast<int>(units < p.total_warps ? units : p.total_warps);
+  int sm_m = 0, sm_k = 0;  // tail chunks of every range, pages per chunk
+  tail_chunks(total, W, p.steal_m_max, p.steal_pps, p.steal_min_stages, &sm_m, &sm_k);
   const int u = blockIdx.x;
   const int gs = u < W ? static_cast<int>(static_cast<int64_t>(u) * total / W) : 0;
   const int ge = u < W ? static_cast<int>(static_cast<int64_t>(u + 1) * total / W) : 0;
@@ -151,24 +169,34 @@ __global__ void __launch_bounds__(kQ4Threads, MINB)
     const int pb = int4_row_bytes(D) << log2_bs;
     const uint64_t policy = l2_policy_evict_first();
     auto prefix = [&](int hd) { return early ? cum_sm[hd] : p.cum[hd]; };
-    bool bad_seen = false, timeout = false;
+    bool bad_seen = false, timeout = false, waited = false;
     int issued = 0, slot = 0;
     uint32_t phase = 1;  // of `empty`: the first round finds every slot free
-    if (gs < ge) {
-      int head;
-      {  // largest head whose first page is <= gs
-        int lo = 0, hi = n_heads;
-        while (hi - lo > 1) {
-          const int step = (hi - lo + 31) / 32;
-          const int x = lo + lane * step;
-          const unsigned mask = __ballot_sync(0xffffffffu, x < hi && prefix(x) <= gs);
-          lo += (31 - __clz(mask)) * step;
-          hi = lo + step < hi ? lo + step : hi;
-        }
-        head = lo;
+    // Largest head whose first page is <= P.
+    auto find_head = [&](int P) -> int {
+      int lo = 0, hi = n_heads;
+      while (hi - lo > 1) {
+        const int step = (hi - lo + 31) / 32;
+        const int x = lo + lane * step;
+        const unsigned mask = __ballot_sync(0xffffffffu, x < hi && prefix(x) <= P);
+        lo += (31 - __clz(mask)) * step;
+        hi = lo + step < hi ? lo + step : hi;
       }
+      return lo;
+    };
+    // The planner's claim words are in place (and its status word).
+    auto wait_plan = [&]() {
+      if (!waited) grid_dependency_wait();
+      waited = true;
+    };
+    if (gs < ge) {
+      // Current segment [gp, seg_end) from seg_start: the range's static part,
+      // then tail chunks claimed from the front of this CTA's tail, then chunks
+      // taken from the back of other CTAs' (as in decode_body).
+      int seg_start = gs, seg_end = ge - sm_m * sm_k, mode = 0;
+      int head = find_head(gs);
       int c_lo = prefix(head), c_hi = prefix(head + 1), gp = gs;
-      int nx_head = 0, nx_lp = 0, nx_np = 0, nx_tok = 0, nx_flags = 0, nx_raw = 0;
+      int nx_head = 0, nx_np = 0, nx_tok = 0, nx_flags = 0, nx_slot = 0, nx_raw = 0;
       int64_t nx_add = 0;
       const int32_t* c_bt = p.bt;
       int c_h = 0, c_len = 0;
@@ -179,10 +207,67 @@ __global__ void __launch_bounds__(kQ4Threads, MINB)
         c_len = early ? len_sm[head] : head_len(head);
       };
       enter_head();
-      // The next stage of the range, its block-table entries on their way.
+      auto next_segment = [&]() -> bool {
+        if (sm_m == 0) return false;
+        wait_plan();
+        if (mode == 0) {
+          unsigned long long old = 0ull;
+          if (lane == 0) old = atomicAdd(p.claims + u, 1ull);
+          old = __shfl_sync(0xffffffffu, old, 0);
+          if (static_cast<uint32_t>(old) + static_cast<uint32_t>(old >> 32) < static_cast<uint32_t>(sm_m)) {
+            if (lane == 0) atomicSub(p.steal + 2, 1);
+            seg_start = gp = seg_end;
+            seg_end += sm_k;
+            return true;
+          }
+          mode = 1;
+        }
+        // Rounds of 32 claim words picked by a shared cursor; the CTA with the
+        // most chunks left is tried.
+        const int rounds = 2 * ((W + 31) / 32) + 2;
+        for (int r = 0; r < rounds; ++r) {
+          int left = 0;
+          uint32_t at = 0;
+          if (lane == 0) {
+            left = *reinterpret_cast<volatile int32_t*>(p.steal + 2);
+            at = atomicAdd(reinterpret_cast<unsigned int*>(p.steal + 3), 32u);
+          }
+          left = __shfl_sync(0xffffffffu, left, 0);
+          if (left <= 0) return false;
+          at = __shfl_sync(0xffffffffu, at, 0);
+          const int v = static_cast<int>((at + lane) % static_cast<uint32_t>(W));
+          const unsigned long long wd = *reinterpret_cast<volatile unsigned long long*>(p.claims + v);
+          const int used = static_cast<int>(static_cast<uint32_t>(wd)) +
+                           static_cast<int>(static_cast<uint32_t>(wd >> 32));
+          const int rem = used < sm_m ? sm_m - used : 0;
+          const int best = __reduce_max_sync(0xffffffffu, (rem << 5) | (31 - lane));
+          if ((best >> 5) == 0) continue;
+          const int vb = __shfl_sync(0xffffffffu, v, 31 - (best & 31));
+          unsigned long long old = 0ull;
+          if (lane == 0) old = atomicAdd(p.claims + vb, 1ull << 32);
+          old = __shfl_sync(0xffffffffu, old, 0);
+          const uint32_t f = static_cast<uint32_t>(old), bk = static_cast<uint32_t>(old >> 32);
+          if (f + bk < static_cast<uint32_t>(sm_m)) {
+            if (lane == 0) atomicSub(p.steal + 2, 1);
+            const int end = static_cast<int>(static_cast<int64_t>(vb + 1) * total / W);
+            seg_start = gp = end - static_cast<int>(bk + 1) * sm_k;
+            seg_end = seg_start + sm_k;
+            return true;
+          }
+        }
+        return false;
+      };
+      // The next stage, its block-table entries on their way.
       auto prepare = [&]() -> bool {
-        if (gp >= ge) return false;
-        if (gp >= c_hi) {
+        if (gp >= seg_end) {
+          if (!next_segment()) return false;
+          if (gp < c_lo || gp >= c_hi) {
+            head = find_head(gp);
+            c_lo = prefix(head);
+            c_hi = prefix(head + 1);
+            enter_head();
+          }
+        } else if (gp >= c_hi) {
           do {
             ++head;
             c_lo = c_hi;
@@ -190,60 +275,84 @@ __global__ void __launch_bounds__(kQ4Threads, MINB)
           } while (gp >= c_hi);
           enter_head();
         }
+        const int lp = gp - c_lo;
         int np = pps;
         if (c_hi - gp < np) np = c_hi - gp;
-        if (ge - gp < np) np = ge - gp;
+        if (seg_end - gp < np) np = seg_end - gp;
         nx_head = head;
-        nx_lp = gp - c_lo;
         nx_np = np;
-        const int left = c_len - (nx_lp << log2_bs);
+        const int left = c_len - (lp << log2_bs);
         nx_tok = left < np << log2_bs ? left : np << log2_bs;
-        // 1: the head's first stage here, 2: its last, 4: the whole head is here
-        nx_flags = (gp == c_lo || gp == gs ? 1 : 0) | (gp + np == c_hi || gp + np == ge ? 2 : 0) |
-                   (c_lo >= gs && c_hi <= ge ? 4 : 0);
+        // 1: the head's first stage in the segment, 2: its last, 4: the whole
+        // head is in the segment
+        nx_flags = (gp == c_lo || gp == seg_start ? 1 : 0) |
+                   (gp + np == c_hi || gp + np == seg_end ? 2 : 0) |
+                   (c_lo >= seg_start && c_hi <= seg_end ? 4 : 0);
+        if (nx_flags & 2) nx_slot = head + segment_of_page(gp, total, W, sm_m, sm_k);
         nx_add = static_cast<int64_t>(c_h) * p.bt_add;
-        if (lane < np) nx_raw = c_bt[static_cast<int64_t>(nx_lp + lane) * p.bt_si];
+        if (lane < np) nx_raw = c_bt[static_cast<int64_t>(lp + lane) * p.bt_si];
         gp += np;
         return true;
       };
+      // Rows per gathering copy: four pages of one cache.
+      const int quads = pps >> 2;
       bool more = prepare();
       while (more) {
         const int np = nx_np;
-        const int4 rec = make_int4(nx_head, nx_tok, nx_flags, 0);
+        int4 rec = make_int4(nx_head, nx_tok, nx_flags, nx_slot);
         const int64_t pid = static_cast<int64_t>(nx_raw) * p.bt_mul + nx_add;
-        const uint32_t bad = __ballot_sync(0xffffffffu, lane < np && (pid < 0 || pid >= p.num_pages));
+        const bool ok = lane < np && pid >= 0 && pid < p.num_pages;
+        const uint32_t bad = __ballot_sync(0xffffffffu, lane < np && !ok);
+        bad_seen |= bad != 0;
         more = prepare();
+        // the next stage's head, while it fits beside the flags
+        rec.z |= (more && nx_head < kQ4NoHead ? nx_head : kQ4NoHead) << 3;
         if (!__all_sync(0xffffffffu, mbar_wait(empty + slot * 8, phase, kWaitLimitNs))) {
           timeout = true;
           break;
         }
-        uint8_t* const st = smem + slot * STAGE_BYTES;
-        if (bad) {
-          // A rejected page id has no copy: zeros (codes, scales and minima)
-          // stand in, written before the arrival that publishes the stage.
-          bad_seen = true;
-          for (int g = 0; g < np; ++g) {
-            if (!(bad >> g & 1u)) continue;
-            for (int i = lane; i < pb / 8; i += 32) {
-              const int half = pb / 16;
-              uint4* z = reinterpret_cast<uint4*>(st + (i < half ? 0 : KV_BYTES) + g * pb);
-              z[i < half ? i : i - half] = make_uint4(0u, 0u, 0u, 0u);
-            }
+        const uint32_t st = base + slot * STAGE_BYTES, bar = full + slot * 8;
+        if (p.gather) {
+          // Pages that are not there (past np, or rejected) read as zeros.
+          const int row = ok ? static_cast<int>(pid) : static_cast<int>(p.num_pages);
+          const int quad = lane & 3, kv = lane >> 2;
+          int32_t r[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) r[i] = __shfl_sync(0xffffffffu, row, quad * 4 + i);
+          if (lane == 0) {
+            record[slot] = rec;
+            mbar_arrive_expect_tx(bar, static_cast<uint32_t>(2 * pb * ((np + 3) & ~3)));
           }
-          fence_proxy_async_smem();  // before the copies that refill this slot later
           __syncwarp();
+          if (kv < 2 && quad < quads && quad * 4 < np)
+            tma_gather4(st + kv * KV_BYTES + quad * 4 * pb, kv ? &vmap : &kmap, 0, r, bar, policy);
+        } else {
+          if (bad) {
+            // A rejected page id has no copy: zeros (codes, scales and minima)
+            // stand in, written before the arrival that publishes the stage.
+            uint8_t* const sp = smem + slot * STAGE_BYTES;
+            for (int g = 0; g < np; ++g) {
+              if (!(bad >> g & 1u)) continue;
+              for (int i = lane; i < pb / 8; i += 32) {
+                const int half = pb / 16;
+                uint4* z = reinterpret_cast<uint4*>(sp + (i < half ? 0 : KV_BYTES) + g * pb);
+                z[i < half ? i : i - half] = make_uint4(0u, 0u, 0u, 0u);
+              }
+            }
+            fence_proxy_async_smem();  // before the copies that refill this slot later
+            __syncwarp();
+          }
+          if (lane == 0) {
+            record[slot] = rec;
+            mbar_arrive_expect_tx(bar, static_cast<uint32_t>(2 * pb * (np - __popc(bad))));
+          }
+          __syncwarp();
+          const int pg = lane & 15, kv = lane >> 4;
+          const int64_t src = __shfl_sync(0xffffffffu, pid, pg);
+          if (pg < np && !(bad >> pg & 1u))
+            bulk_load(st + kv * KV_BYTES + pg * pb, (kv ? p.v_pages : p.k_pages) + src * pb,
+                      static_cast<uint32_t>(pb), bar, policy);
         }
-        if (lane == 0) {
-          record[slot] = rec;
-          mbar_arrive_expect_tx(full + slot * 8, static_cast<uint32_t>(2 * pb * (np - __popc(bad))));
-        }
-        __syncwarp();
-        const int pg = lane & 15, kv = lane >> 4;
-        const int64_t src = __shfl_sync(0xffffffffu, pid, pg);
-        if (pg < np && !(bad >> pg & 1u))
-          bulk_load(base + slot * STAGE_BYTES + kv * KV_BYTES + pg * pb,
-                    (kv ? p.v_pages : p.k_pages) + src * pb, static_cast<uint32_t>(pb),
-                    full + slot * 8, policy);
         ++issued;
         if (++slot == depth) {
           slot = 0;
@@ -268,7 +377,7 @@ __global__ void __launch_bounds__(kQ4Threads, MINB)
     // did (the end record's slot was waited for above).
     for (int j = max(issued - depth + (ended ? 1 : 0), 0); j < issued; ++j)
       mbar_wait(full + (j % depth) * 8, (j / depth) & 1, kWaitLimitNs);
-    grid_dependency_wait();  // the planner has reset the status word
+    wait_plan();  // the planner has reset the status word
     if (lane == 0 && (bad_seen || timeout))
       atomicOr(p.status, (bad_seen ? kStatusBadPage : 0u) | (timeout ? kStatusTimeout : 0u));
     return;
@@ -378,19 +487,27 @@ __global__ void __launch_bounds__(kQ4Threads, MINB)
     }
   };
 
-  int joins = 0;
-  // Waits for the other consumers (their shared-memory writes are visible);
-  // false after the wait limit.
-  auto consumers_sync = [&]() -> bool {
-    __syncwarp();
-    if (lane == 0) mbar_arrive(joined);
-    const bool ok = mbar_wait(joined, joins & 1, kWaitLimitNs);
-    ++joins;
-    return __all_sync(0xffffffffu, ok);
+  // The queries of the head after this one on their way to L1 while the last
+  // stage of this one is computed: lane l touches every 32nd sector.
+  auto fetch_queries = [&](int hd) {
+    if (hd >= kQ4NoHead) return;
+    const int s = hd / Hkv, h = hd - s * Hkv;
+    const T* qp = static_cast<const T*>(p.q) + s * p.q_sb + static_cast<int64_t>(h) * G * p.q_sh;
+    constexpr int kPerRow = D * 2 / 32;  // sectors
+    for (int i = lane; i < G * kPerRow; i += 32) {
+      uint32_t x;
+      asm volatile("ld.global.ca.u32 %0, [%1];"
+                   : "=r"(x)
+                   : "l"(qp + (i / kPerRow) * p.q_sh + (i % kPerRow) * 16));
+    }
   };
+  uint32_t joins = 0;  // heads finished so far
   // Joins the parts' states of head hd and writes the output (whole) or the
   // partial state of this CTA's range.
-  auto finish_head = [&](int hd, bool whole) -> bool {
+  auto finish_head = [&](int hd, bool whole, int slot) -> bool {
+    // The joining buffer is free once every consumer has read the last head's
+    // states (a fresh barrier's previous phase counts as complete).
+    if (!__all_sync(0xffffffffu, mbar_wait(drained, (joins & 1) ^ 1, kWaitLimitNs))) return false;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -422,7 +539,10 @@ __global__ void __launch_bounds__(kQ4Threads, MINB)
           join_ml[(part * G + g) * 2 + 1] = l;
         }
       }
-    if (!consumers_sync()) return false;
+    __syncwarp();
+    if (lane == 0) mbar_arrive(joined);
+    if (!__all_sync(0xffffffffu, mbar_wait(joined, joins & 1, kWaitLimitNs))) return false;
+    ++joins;
     const int s = hd / Hkv, h = hd - s * Hkv;
     for (int idx = tid; idx < G * (D / 4); idx += kQ4Consumers * 32) {
       const int g = idx / (D / 4), c = (idx - g * (D / 4)) * 4;
@@ -452,7 +572,7 @@ __global__ void __launch_bounds__(kQ4Threads, MINB)
               make_uint2(pack2<T>(o.x * inv, o.y * inv), pack2<T>(o.z * inv, o.w * inv));
         }
       } else {
-        float* ps = p.part + static_cast<int64_t>(hd + u) * p.slot_floats;
+        float* ps = p.part + static_cast<int64_t>(slot) * p.slot_floats;
         __stcg(reinterpret_cast<float4*>(ps + g * D + c), o);
         if (c == 0) {
           __stcg(ps + G * D + g, M);
@@ -460,7 +580,9 @@ __global__ void __launch_bounds__(kQ4Threads, MINB)
         }
       }
     }
-    return consumers_sync();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(drained);
+    return true;
   };
 
   bool timeout = false;
@@ -473,6 +595,7 @@ __global__ void __launch_bounds__(kQ4Threads, MINB)
     const int4 rec = record[slot];
     if (rec.x < 0) break;
     if (rec.z & 1) start_head(rec.x);
+    if (rec.z & 2) fetch_queries(rec.z >> 3);
 #pragma unroll
     for (int ch = 0; ch < PT / 32; ++ch) {
       const int ntok = rec.y - tok0 - ch * 32;  // valid tokens from here (may be <= 0 or > 32)
@@ -644,7 +767,7 @@ __global__ void __launch_bounds__(kQ4Threads, MINB)
       code_at -= depth * STAGE_BYTES;
       pair_at -= depth * STAGE_BYTES;
     }
-    if ((rec.z & 2) && !finish_head(rec.x, (rec.z & 4) != 0)) {
+    if ((rec.z & 2) && !finish_head(rec.x, (rec.z & 4) != 0, rec.w)) {
       timeout = true;
       break;
     }

@@ -467,9 +467,8 @@ int make_plan(const pab200_decode_args* a, Plan* pl, size_t scratch_cap,
   return PAB200_OK;
 }
 
-// Plans one call over 4-bit pages: one range of pages per resident CTA, fixed
-// when the call is planned (no tail chunks: the ranges are a few stages to a
-// few hundred long and one CTA's five warps share each).
+// Plans one call over 4-bit pages: one range of pages per resident CTA, whose
+// five warps share it.
 int make_plan_int4(const pab200_decode_args* a, Plan* pl) {
   refresh_env();
   int rc = validate(a, true, true);
@@ -508,8 +507,11 @@ int make_plan_int4(const pab200_decode_args* a, Plan* pl) {
   pl->W = pl->grid = W;
   pl->unit_pages = pab::kQ4Stage / a->block_size;
   pl->slot_floats = (pl->G * D + 2 * pl->G + 3) & ~3;
-  lay_out_workspace(pl, 0, SIZE_MAX);
-  pl->steal_min_stages = 1;
+  // The CTAs of an SM do not get equal shares of its issue slots (64 x 4096
+  // tokens: they end between 65 and 88 us without tail chunks).
+  int m_max = env_int("PAB200_STEAL_M", 0);
+  lay_out_workspace(pl, m_max < 0 ? 0 : m_max, SIZE_MAX);
+  pl->steal_min_stages = env_int("PAB200_STEAL_MIN_STAGES", 2);
   return PAB200_OK;
 }
 
@@ -546,6 +548,27 @@ int encode_cache_map(const pab200_decode_args* a, const void* base, CUtensorMap*
   cache[next] = Entry{base, a->num_pages, a->dtype, a->layout, a->head_size, a->block_size, hkv, *map};
   next = (next + 1) % kEntries;
   if (used < kEntries) ++used;
+  return PAB200_OK;
+}
+
+// 4-bit pages as rows of a 2-D map of 8-byte elements, one row per box, for
+// copies that gather four of them; rows have at most 256 elements.
+bool int4_gathers(const pab200_decode_args* a) {
+  return a->block_size * pab::int4_row_bytes(a->head_size) <= 256 * 8;
+}
+
+int encode_page_map(const pab200_decode_args* a, const void* base, CUtensorMap* map) {
+  PFN_cuTensorMapEncodeTiled_v12000 enc = tensor_map_encoder();
+  if (!enc) return fail(PAB200_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
+  const cuuint64_t bytes = cuuint64_t(a->block_size) * pab::int4_row_bytes(a->head_size);
+  const cuuint64_t dims[2] = {bytes / 8, cuuint64_t(a->num_pages)};
+  const cuuint64_t strides[1] = {bytes};
+  const cuuint32_t box[2] = {cuuint32_t(bytes / 8), 1}, estr[2] = {1, 1};
+  const CUresult r =
+      enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT64, 2, const_cast<void*>(base), dims, strides, box, estr,
+          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
+          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(PAB200_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", int(r));
   return PAB200_OK;
 }
 
@@ -752,7 +775,11 @@ int decode_impl(const pab200_decode_args* a, const Plan& pl, const pab::AppendPa
   p.k_pages = static_cast<const uint8_t*>(a->k_cache);
   p.v_pages = static_cast<const uint8_t*>(a->v_cache);
   CUtensorMap kmap, vmap;
-  if (a->num_pages > 0 && !pl.int4) {
+  p.gather = pl.int4 && a->num_pages > 0 && int4_gathers(a);
+  if (p.gather) {
+    if ((rc = encode_page_map(a, a->k_cache, &kmap))) return rc;
+    if ((rc = encode_page_map(a, a->v_cache, &vmap))) return rc;
+  } else if (a->num_pages > 0 && !pl.int4) {
     if ((rc = encode_cache_map(a, a->k_cache, &kmap))) return rc;
     if ((rc = encode_cache_map(a, a->v_cache, &vmap))) return rc;
   } else {

@@ -161,6 +161,19 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
       : "memory");
 }
 
+// Four rows r[0..3] of a 2-D tensor map (box one row high) global -> shared, one
+// after the other from `dst`; a row out of range reads as zeros.  Completion
+// counted in bytes on the mbarrier.  No multicast.
+__device__ __forceinline__ void tma_gather4(uint32_t dst, const CUtensorMap* map, int32_t x,
+                                            const int32_t (&r)[4], uint32_t bar, uint64_t policy) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes"
+      ".L2::cache_hint [%0], [%1, {%2, %3, %4, %5, %6}], [%7], %8;" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]),
+      "r"(bar), "l"(policy)
+      : "memory");
+}
+
 // ---------------------------------------------------------------- MMA
 // D(16x8,f32) += A(16x16) * B(16x8), A row-major, B column-major.
 template <typename T>
