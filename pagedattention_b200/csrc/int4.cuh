@@ -81,10 +81,10 @@ __device__ __forceinline__ uint32_t and_or(uint32_t x, uint32_t mask, uint32_t b
   return y;
 }
 
-// Keys: nibble m of both 16-bit halves of w, as they stand: the pair r[m] is two
-// fp16 subnormals c * 2^-24 (m even) or c * 2^-20 (m odd), exact, for the price
-// of a mask.  The queries carry the powers of two.
-__device__ __forceinline__ void int4_key_pairs(uint32_t w, uint32_t (&r)[4]) {
+// Nibble m of both 16-bit halves of w as it stands: the pair r[m] is two fp16
+// subnormals c * 2^-24 (m even) or c * 2^-20 (m odd), exact, for the price of a
+// mask.  What they are multiplied with carries the powers of two.
+__device__ __forceinline__ void int4_raw_pairs(uint32_t w, uint32_t (&r)[4]) {
   const uint32_t v = w >> 8;
   r[0] = w & 0x000f000fu;
   r[1] = w & 0x00f000f0u;
@@ -92,18 +92,16 @@ __device__ __forceinline__ void int4_key_pairs(uint32_t w, uint32_t (&r)[4]) {
   r[3] = v & 0x00f000f0u;
 }
 
-// Values: nibble m of both 16-bit halves of w, as the pair r[m] of exact values
-// c - 8 (-8..7) of type T.  A nibble OR-ed into the low mantissa bits of a power
-// of two P reads as P + c; subtracting P + 8 is exact.  fp16 (10 mantissa bits)
-// also takes the nibble at bits 4..7 in place: 1024 + 16 c, times 1/16 minus
-// 72.  Centred codes keep the sums small: a value is (lo + 8 s) + s (c - 8), and
-// the rounding of a probability to T is multiplied by |s (c - 8)|, about |x|,
-// instead of by s c, about the group's range.
-template <typename T>
-__device__ __forceinline__ void int4_value_pairs(uint32_t w, uint32_t (&r)[4]);
-
-template <>
-__device__ __forceinline__ void int4_value_pairs<__half>(uint32_t w, uint32_t (&r)[4]) {
+// Nibble m of both 16-bit halves of w as the fp16 pair r[m] of c - 8 (CENTRED;
+// -8..7, exact) or as it stands.  A nibble OR-ed into the low mantissa bits of
+// 1024 reads as 1024 + c, at bits 4..7 as 1024 + 16 c: subtracting 1032 from the
+// one, and 1/16 of the other minus 72, are exact.
+template <bool CENTRED>
+__device__ __forceinline__ void int4_value_pairs(uint32_t w, uint32_t (&r)[4]) {
+  if constexpr (!CENTRED) {
+    int4_raw_pairs(w, r);
+    return;
+  }
   const uint32_t v = w >> 8;
   const __half2 base = __float2half2_rn(1032.f);
   const __half2 sixteenth = __float2half2_rn(0.0625f), off = __float2half2_rn(-72.f);
@@ -117,15 +115,20 @@ __device__ __forceinline__ void int4_value_pairs<__half>(uint32_t w, uint32_t (&
   }
 }
 
+// Maximum of two pairs of T.
+template <typename T>
+__device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b);
 template <>
-__device__ __forceinline__ void int4_value_pairs<__nv_bfloat16>(uint32_t w, uint32_t (&r)[4]) {
-  const __nv_bfloat162 base = __floats2bfloat162_rn(136.f, 136.f);
-#pragma unroll
-  for (int m = 0; m < 4; ++m) {
-    const uint32_t t = and_or(w >> (4 * m), 0x000f000fu, 0x43004300u);
-    const __nv_bfloat162 y = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&t), base);
-    r[m] = *reinterpret_cast<const uint32_t*>(&y);
-  }
+__device__ __forceinline__ uint32_t max2<__nv_bfloat16>(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+template <>
+__device__ __forceinline__ uint32_t max2<__half>(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
 }
 
 // Nibble m of both halves of w as the pair r[m] of exact values c (0..15) of T.

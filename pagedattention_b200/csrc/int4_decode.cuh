@@ -18,9 +18,17 @@
 //     which loses nothing of a bf16 or fp16 query that matters, and the score is
 //     scaled back in fp32.  Values are widened to c - 8 in T.
 //   * Scales and minima never touch the codes: the keys' multiply the partial
-//     scores of their group, the values' scale multiplies the probability
-//     (rounded to T once, as a plain probability is) and the rest of the value,
-//     lo + 8 s, is summed apart in fp32.
+//     scores of their group, the values' scale multiplies the probability, which
+//     is rounded to fp16 once, and the rest of the value is summed apart in fp32.
+//     How the values' codes enter depends on T.
+//     fp16: as c - 8, so that the rounding of p s is multiplied by s (c - 8), about
+//     |x|, not by s c, about the group's range: the output keeps fp16's 11 bits.
+//     bf16: as they stand, like the keys', which spares seven instructions per
+//     eight codes (64 x 4096 tokens: 82 -> 72 us): an fp16 p s is eight times
+//     finer than the bf16 output needs.  Its scales reach past fp16, so they carry
+//     a power of two that follows the largest scale seen; and since sums of
+//     codes >= 0 only grow, and the tensor cores cut their fp32 sums short, the
+//     accumulators are emptied into shared memory every kFlush chunks of 32 tokens.
 //   * The softmax's reference point moves only when a score exceeds it by
 //     kRaise (log2 units): no shuffles or rescaling in most stages.
 // At the end of a head (or of the CTA's part of it) the consumers' states are
@@ -63,12 +71,13 @@ __global__ void __launch_bounds__(kQ4Threads, MINB)
   constexpr int PT = kQ4Stage / PARTS;         // tokens per part, in chunks of 32
   constexpr int MT = 2;                        // 16-token tiles per chunk
   constexpr int STAGE_BYTES = q4_stage_bytes(D), KV_BYTES = STAGE_BYTES / 2;
-  // fp16: probability x scale must stay below 65504 while scales reach
-  // 2 * 65504 / 15: the reference point lies kBelow under the maximum it was
-  // set to, a few binades above fp16's subnormals for small scales, and moves
-  // before 2^kRaise = 7.46 is passed.
+  // Probability x scale must stay below 65504, a probability stays below
+  // 2^kRaise = 7.46.  fp16: scales reach 2 * 65504 / 15, and the reference point
+  // lies kBelow under the maximum it was set to, a few binades further above
+  // fp16's subnormals for small scales.  bf16: scales are brought to 2^13 at most.
   constexpr bool kHalf = std::is_same<T, __half>::value;
-  constexpr float kBelow = kHalf ? 1.4f : 0.f, kRaise = kHalf ? 2.9f : 8.f;
+  constexpr float kBelow = kHalf ? 1.4f : 0.f, kRaise = 2.9f;
+  constexpr int kFlush = 32;  // bf16: chunks between two emptyings of the accumulators
   // Reference point of an empty state: below every score, and finite, so that
   // a score of -inf has probability 0.
   constexpr float kNoScore = -3e38f;
@@ -421,6 +430,12 @@ __global__ void __launch_bounds__(kQ4Threads, MINB)
   float qsum[NT][NG][2];   // scale_log2 x sum of the query over a group, heads 2 lc + e
   float qmul[NT][2];       // what a sum of (query x code) products is multiplied by
   float acc[KS][NT][4], mid[NT][NG][2], m_ref[NT][2], l_sum[NT][2];
+  // bf16: the scales' power of two, the largest scale it allows; chunks since the
+  // accumulators were emptied, and the reference points then (`emptied`: there
+  // is something in shared memory).
+  float nu = 1.f, s_lim = -1.f, m_then[NT][2];
+  int chunks = 0;
+  bool emptied = false;
 
   // The query group of head hd, as fp16 scaled by a power of two per head that
   // brings its largest element to 2^10..2^11 (elements paired with the nibbles
@@ -485,6 +500,9 @@ __global__ void __launch_bounds__(kQ4Threads, MINB)
 #pragma unroll
         for (int i = 0; i < 4; ++i) acc[dt][nt][i] = 0.f;
     }
+    s_lim = -1.f;
+    chunks = 0;
+    emptied = false;
   };
 
   // The queries of the head after this one on their way to L1 while the last
@@ -502,12 +520,61 @@ __global__ void __launch_bounds__(kQ4Threads, MINB)
     }
   };
   uint32_t joins = 0;  // heads finished so far
+  // Adds the accumulators, in units of the output, to this lane's elements of the
+  // joining buffer (or puts them there), with `mid` (the sums of the values'
+  // other part) at a head's end.  False if the buffer did not become free: every
+  // consumer has read the last head's states by then (a fresh barrier's previous
+  // phase counts as complete).
+  auto deposit = [&](bool last) -> bool {
+    if (!emptied && !__all_sync(0xffffffffu, mbar_wait(drained, (joins & 1) ^ 1, kWaitLimitNs)))
+      return false;
+    // codes entered as c 2^-24 (even registers of a word) or c 2^-20 (odd ones)
+    const float down = kHalf ? 1.f : __uint_as_float((254u << 23) - __float_as_uint(nu)) * 1048576.f;
+    const float w0 = kHalf ? 1.f : down * 16.f, w1 = down;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int g = g_lo + nt * 8 + lc * 2 + e;
+        float* row = join + (part * G + g) * (D + 4) + lr * 8;
+        const float keep = emptied ? fast_exp2(m_then[nt][e] - m_ref[nt][e]) : 0.f;
+        m_then[nt][e] = m_ref[nt][e];
+#pragma unroll
+        for (int gi = 0; gi < NG; ++gi) {
+          float v = 0.f;
+          if (last) {
+            v = mid[nt][gi][e];
+            v += __shfl_xor_sync(0xffffffffu, v, 4);
+            v += __shfl_xor_sync(0xffffffffu, v, 8);
+            v += __shfl_xor_sync(0xffffffffu, v, 16);
+          }
+          // accumulator (tile 4 gi + m, register e + 2 j): element 64 gi + 8 lr + 2 m + j
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            float4 x = make_float4(fmaf(acc[gi * 4 + 2 * half][nt][e], w0, v),
+                                   fmaf(acc[gi * 4 + 2 * half][nt][e + 2], w0, v),
+                                   fmaf(acc[gi * 4 + 2 * half + 1][nt][e], w1, v),
+                                   fmaf(acc[gi * 4 + 2 * half + 1][nt][e + 2], w1, v));
+            float4* at = reinterpret_cast<float4*>(row + gi * 64 + half * 4);
+            if (g < G) {
+              if (emptied) {
+                const float4 old = *at;
+                x = make_float4(fmaf(old.x, keep, x.x), fmaf(old.y, keep, x.y),
+                                fmaf(old.z, keep, x.z), fmaf(old.w, keep, x.w));
+              }
+              *at = x;
+            }
+            acc[gi * 4 + 2 * half][nt][e] = acc[gi * 4 + 2 * half][nt][e + 2] = 0.f;
+            acc[gi * 4 + 2 * half + 1][nt][e] = acc[gi * 4 + 2 * half + 1][nt][e + 2] = 0.f;
+          }
+        }
+      }
+    return true;
+  };
   // Joins the parts' states of head hd and writes the output (whole) or the
-  // partial state of this CTA's range.
+  // partial state of this CTA's segment.
   auto finish_head = [&](int hd, bool whole, int slot) -> bool {
-    // The joining buffer is free once every consumer has read the last head's
-    // states (a fresh barrier's previous phase counts as complete).
-    if (!__all_sync(0xffffffffu, mbar_wait(drained, (joins & 1) ^ 1, kWaitLimitNs))) return false;
+    if (!deposit(true)) return false;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -517,23 +584,6 @@ __global__ void __launch_bounds__(kQ4Threads, MINB)
         l += __shfl_xor_sync(0xffffffffu, l, 8);
         l += __shfl_xor_sync(0xffffffffu, l, 16);
         const int g = g_lo + nt * 8 + lc * 2 + e;
-        float* row = join + (part * G + g) * (D + 4) + lr * 8;
-#pragma unroll
-        for (int gi = 0; gi < NG; ++gi) {
-          float v = mid[nt][gi][e];
-          v += __shfl_xor_sync(0xffffffffu, v, 4);
-          v += __shfl_xor_sync(0xffffffffu, v, 8);
-          v += __shfl_xor_sync(0xffffffffu, v, 16);
-          // accumulator (tile 4 gi + m, register e + 2 j): element 64 gi + 8 lr + 2 m + j
-          if (g < G) {
-            *reinterpret_cast<float4*>(row + gi * 64) =
-                make_float4(acc[gi * 4][nt][e] + v, acc[gi * 4][nt][e + 2] + v,
-                            acc[gi * 4 + 1][nt][e] + v, acc[gi * 4 + 1][nt][e + 2] + v);
-            *reinterpret_cast<float4*>(row + gi * 64 + 4) =
-                make_float4(acc[gi * 4 + 2][nt][e] + v, acc[gi * 4 + 2][nt][e + 2] + v,
-                            acc[gi * 4 + 3][nt][e] + v, acc[gi * 4 + 3][nt][e + 2] + v);
-          }
-        }
         if (lr == 0 && g < G) {
           join_ml[(part * G + g) * 2] = m_ref[nt][e];
           join_ml[(part * G + g) * 2 + 1] = l;
@@ -622,8 +672,8 @@ __global__ void __launch_bounds__(kQ4Threads, MINB)
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
             uint32_t ra[4], rb[4];
-            int4_key_pairs(wa[gi * 2 + j], ra);
-            int4_key_pairs(wb[gi * 2 + j], rb);
+            int4_raw_pairs(wa[gi * 2 + j], ra);
+            int4_raw_pairs(wb[gi * 2 + j], rb);
 #pragma unroll
             for (int hf = 0; hf < 2; ++hf) {
               const uint32_t a[4] = {ra[2 * hf], rb[2 * hf], ra[2 * hf + 1], rb[2 * hf + 1]};
@@ -710,32 +760,71 @@ __global__ void __launch_bounds__(kQ4Threads, MINB)
               l_sum[nt][e] += sc[mt][nt][i];
             }
         }
-      // O^T += V^T P^T on the centred codes.
+      // The values' scales and minima; rows past the end may hold anything: zeros.
+      uint32_t ma[MT][NG], mb[MT][NG];
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
-        if (ragged && mt * 16 >= ntok) break;
-        uint32_t wa[D / 32], wb[D / 32], ma[NG], mb[NG];
         const int t8 = ch * 4 + 2 * mt;
-        ld_shared_words<D / 32>(code_at + KV_BYTES + code_off(t8), wa);
-        ld_shared_words<D / 32>(code_at + KV_BYTES + code_off(t8 + 1), wb);
-        ld_shared_words<NG>(pair_at + KV_BYTES + pair_off(t8), ma);
-        ld_shared_words<NG>(pair_at + KV_BYTES + pair_off(t8 + 1), mb);
-        if (ragged) {  // rows past the end may hold anything: zero scales
+        ld_shared_words<NG>(pair_at + KV_BYTES + pair_off(t8), ma[mt]);
+        ld_shared_words<NG>(pair_at + KV_BYTES + pair_off(t8 + 1), mb[mt]);
+        if (ragged) {
           const bool oka = mt * 16 + lr < ntok, okb = mt * 16 + 8 + lr < ntok;
 #pragma unroll
           for (int gi = 0; gi < NG; ++gi) {
-            ma[gi] = oka ? ma[gi] : 0u;
-            mb[gi] = okb ? mb[gi] : 0u;
+            ma[mt][gi] = oka ? ma[mt][gi] : 0u;
+            mb[mt][gi] = okb ? mb[mt][gi] : 0u;
           }
         }
+      }
+      if constexpr (!kHalf) {
+        uint32_t big = ma[0][0];  // pairs (scale, minimum): the low half counts
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int gi = 0; gi < NG; ++gi) {
+            if (mt + gi) big = max2<T>(big, ma[mt][gi]);
+            big = max2<T>(big, mb[mt][gi]);
+          }
+        const float s_max = unpack2<T>(big).x;
+        if (__any_sync(0xffffffffu, s_max > s_lim)) {
+          // Scales are >= 0 (or NaN, which stays out): their bits order them.
+          const uint32_t bits = __reduce_max_sync(0xffffffffu, s_max > 0.f ? __float_as_uint(s_max) : 0u);
+          // four times the power of two above the largest becomes 2^13
+          uint32_t ex = min(max((bits >> 23) + 3u, 16u), 255u);
+          const float nu_new = __uint_as_float((267u - ex) << 23);
+          const float f = s_lim < 0.f ? 0.f : nu_new * __uint_as_float((254u << 23) - __float_as_uint(nu));
+          nu = nu_new;
+          s_lim = __uint_as_float(ex << 23);
+#pragma unroll
+          for (int dt = 0; dt < KS; ++dt)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) acc[dt][nt][i] *= f;
+        }
+      }
+      // O^T += V^T P^T on the codes.
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        if (ragged && mt * 16 >= ntok) break;
+        uint32_t wa[D / 32], wb[D / 32];
+        const int t8 = ch * 4 + 2 * mt;
+        ld_shared_words<D / 32>(code_at + KV_BYTES + code_off(t8), wa);
+        ld_shared_words<D / 32>(code_at + KV_BYTES + code_off(t8 + 1), wb);
 #pragma unroll
         for (int gi = 0; gi < NG; ++gi) {
-          const float2 fa = int4_centre<T>(ma[gi]), fb = int4_centre<T>(mb[gi]);
+          // (scale, value of the code that enters as 0)
+          float2 fa = kHalf ? int4_centre<T>(ma[mt][gi]) : unpack2<T>(ma[mt][gi]);
+          float2 fb = kHalf ? int4_centre<T>(mb[mt][gi]) : unpack2<T>(mb[mt][gi]);
+          if (!kHalf) {
+            fa.x *= nu;
+            fb.x *= nu;
+          }
           uint32_t pg[NT][2];
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            pg[nt][0] = movmatrix_trans(pack2<T>(sc[mt][nt][0] * fa.x, sc[mt][nt][1] * fa.x));
-            pg[nt][1] = movmatrix_trans(pack2<T>(sc[mt][nt][2] * fb.x, sc[mt][nt][3] * fb.x));
+            pg[nt][0] = movmatrix_trans(pack2<__half>(sc[mt][nt][0] * fa.x, sc[mt][nt][1] * fa.x));
+            pg[nt][1] = movmatrix_trans(pack2<__half>(sc[mt][nt][2] * fb.x, sc[mt][nt][3] * fb.x));
 #pragma unroll
             for (int e = 0; e < 2; ++e)
               mid[nt][gi][e] = fmaf(sc[mt][nt][e], fa.y, fmaf(sc[mt][nt][e + 2], fb.y, mid[nt][gi][e]));
@@ -743,20 +832,31 @@ __global__ void __launch_bounds__(kQ4Threads, MINB)
           uint32_t xa[4], ya[4], xb[4], yb[4];
           // The octet's words of two consecutive tokens -> pairs (even token,
           // odd token) of one element: even elements x, odd elements y.
-          int4_value_pairs<T>(__byte_perm(wa[gi], wa[NG + gi], 0x5410), xa);
-          int4_value_pairs<T>(__byte_perm(wa[gi], wa[NG + gi], 0x7632), ya);
-          int4_value_pairs<T>(__byte_perm(wb[gi], wb[NG + gi], 0x5410), xb);
-          int4_value_pairs<T>(__byte_perm(wb[gi], wb[NG + gi], 0x7632), yb);
+          int4_value_pairs<kHalf>(__byte_perm(wa[gi], wa[NG + gi], 0x5410), xa);
+          int4_value_pairs<kHalf>(__byte_perm(wa[gi], wa[NG + gi], 0x7632), ya);
+          int4_value_pairs<kHalf>(__byte_perm(wb[gi], wb[NG + gi], 0x5410), xb);
+          int4_value_pairs<kHalf>(__byte_perm(wb[gi], wb[NG + gi], 0x7632), yb);
 #pragma unroll
           for (int m = 0; m < 4; ++m) {
             const uint32_t a[4] = {xa[m], ya[m], xb[m], yb[m]};
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
-              mma_16816<T>(acc[gi * 4 + m][nt], a, pg[nt][0], pg[nt][1]);
+              mma_16816<__half>(acc[gi * 4 + m][nt], a, pg[nt][0], pg[nt][1]);
           }
         }
       }
+      if constexpr (!kHalf) {
+        if (++chunks == kFlush) {
+          chunks = 0;
+          if (!deposit(false)) {
+            timeout = true;
+            break;
+          }
+          emptied = true;
+        }
+      }
     }
+    if (timeout) break;
     __syncwarp();
     if (lane == 0) mbar_arrive(empty + slot * 8);  // the slot may be refilled
     code_at += STAGE_BYTES;
