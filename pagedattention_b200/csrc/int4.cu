@@ -76,19 +76,19 @@ __device__ __forceinline__ uint32_t int4_codes_of(const uint4& x, uint32_t pair,
   if (inv == 0.f) return int4_quantise_tiny<T>(x, sl.y, sl.x);  // no code if s is 0 or NaN
   constexpr float kMagic = 12582912.f;  // 1.5 * 2^23
   const uint32_t v[4] = {x.x, x.y, x.z, x.w};
-  float c[8];
+  uint32_t c[8];  // 0x4b400000 + code
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const float2 f = unpack2<T>(v[i]);
     const float a0 = f.x - sl.y, a1 = f.y - sl.y;
     const float q0 = a0 * inv, q1 = a1 * inv;
-    c[2 * i] = (fmaf(fmaf(-q0, sl.x, a0), inv, q0) + kMagic) - kMagic;
-    c[2 * i + 1] = (fmaf(fmaf(-q1, sl.x, a1), inv, q1) + kMagic) - kMagic;
+    c[2 * i] = __float_as_uint(fmaf(fmaf(-q0, sl.x, a0), inv, q0) + kMagic);
+    c[2 * i + 1] = __float_as_uint(fmaf(fmaf(-q1, sl.x, a1), inv, q1) + kMagic);
   }
-  // four codes are one exact integer below 2^16 in fp32
-  const float even = fmaf(fmaf(fmaf(c[6], 16.f, c[4]), 16.f, c[2]), 16.f, c[0]);
-  const float odd = fmaf(fmaf(fmaf(c[7], 16.f, c[5]), 16.f, c[3]), 16.f, c[1]);
-  return __byte_perm(__float_as_uint(even + kMagic), __float_as_uint(odd + kMagic), 0x5410);
+  // c0 + 16 c2 + 256 c4 + 4096 c6: the constant leaves the low 16 bits alone
+  const uint32_t even = ((c[6] * 16u + c[4]) * 16u + c[2]) * 16u + c[0];
+  const uint32_t odd = ((c[7] * 16u + c[5]) * 16u + c[3]) * 16u + c[1];
+  return __byte_perm(even, odd, 0x5410);
 }
 
 // 4 x 4 transpose of the words of 4 lanes that differ in lane bits A and B:

@@ -682,10 +682,10 @@ int launch_select(const pab200_select_args* a, void* scores, bool pdl, cudaStrea
   const unsigned units = static_cast<unsigned>(p.B * p.Hkv);
   const bool scored = p.maxb > p.keep;
   if (scored) {
-    // Pages per CTA: what gives every SM about three CTAs, in whole steps of the
+    // Pages per CTA: what gives every SM about four CTAs, in whole steps of the
     // 8 warps, at most 64 pages per warp.
     const int64_t pages = int64_t(units) * p.maxb;
-    int64_t each = pages / (3 * pabh::device_sm_count_current());
+    int64_t each = pages / (4 * pabh::device_sm_count_current());
     each = (each + 63) / 64 * 64;
     const int chunk = each < 64 ? 64 : (each > 512 ? 512 : static_cast<int>(each));
     p.chunk = chunk;
