@@ -254,11 +254,13 @@ __global__ void __launch_bounds__(128) int4_lengths_kernel(const Int4AppendParam
   const TokenMap& m = p.map;
   const int lane = threadIdx.x & 31;
   const int s = blockIdx.x * 4 + (threadIdx.x >> 5);
+  // The rows' kernel has read every length; and whatever waits for this grid can
+  // count on the rows.
+  grid_dependency_wait();
   if (s >= m.B) return;
   const int t0 = m.cu[s], t1 = m.cu[s + 1];
   if (t0 < 0 || t1 > m.num_tokens || t1 <= t0) return;
   const int64_t n = t1 - t0;
-  grid_dependency_wait();  // the rows' kernel has read every length
   int64_t least = n;
   // Heads whose ids come from one table entry of a pool are in range together.
   const bool alike = m.l_sh == 0 && m.bt_sh == 0 && m.bt_add == 1 && m.bt_mul == m.Hkv &&
