@@ -480,11 +480,12 @@ typedef struct pab200_select_args {
  * the highest score
  *   u(page) = sum_g sum_d max(q[g, d] * min[d], q[g, d] * max[d]),
  * g over the kv head's query group: no token of the page has a larger sum of
- * raw scores.  Scores are summed in 64 bits and rounded to fp32; equal scores
+ * raw scores.  Scores are those of a sum in 64 bits, rounded to fp32; equal scores
  * go to the lower page, a score that is NaN ranks first, a page id out of range
  * last.  tables[s, h] receives the block-table entries of the kept pages in
  * ascending page order (-1 behind them) and selected_lens[s, h] the number of
- * their tokens: a block table and lengths for any decode entry point. */
+ * their tokens: a block table and lengths for any decode entry point.
+ * At most 65,535 (sequence, kv head) pairs. */
 size_t pab200_select_pages_workspace_size(const pab200_select_args* args);
 int pab200_select_pages(const pab200_select_args* args, void* workspace, size_t workspace_bytes,
                         void* stream);

@@ -215,7 +215,8 @@ def paged_attention_int4(out, query, key_cache, value_cache, block_tables, conte
     out, query: (num_seqs, num_q_heads, head_size); block_tables (num_seqs,
     max_blocks) or, per kv head, (num_seqs, num_kv_heads, max_blocks);
     context_lens (num_seqs,) or (num_seqs, num_kv_heads).  Query groups as for
-    ``paged_attention``.
+    ``paged_attention``.  ``out`` must not overlap ``query``.  An invalid page id
+    reads as rows of zeros and sets a bit read by ``read_status``.
     """
     shape, qst, ost = query.shape, query.stride(), out.stride()
     if len(shape) != 3:
@@ -229,6 +230,8 @@ def paged_attention_int4(out, query, key_cache, value_cache, block_tables, conte
         raise ValueError("out must match query in shape and dtype")
     if ost[2] != 1:
         raise ValueError("out must be contiguous in head_size")
+    if out.data_ptr() == query.data_ptr() and query.numel():
+        raise ValueError("out must not be query: queries are read until the call ends")
     if num_splits < 0:
         raise ValueError("num_splits must be >= 0")
     B, Hq, D = shape

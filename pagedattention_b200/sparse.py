@@ -131,8 +131,10 @@ def select_pages(query, page_bounds, block_tables, context_lens, block_size, num
     first ``num_sink`` and last ``num_recent`` (>= 1) pages are kept, and of the
     others those with the highest score: the sum over the kv head's query group
     and the head elements of max(q * min, q * max), which no token of the page
-    exceeds.  Scores are summed in 64 bits and rounded to fp32; ties go to the
-    earlier page, a NaN score ranks first.  query: (num_seqs, num_q_heads,
+    exceeds.  Scores are those of a sum in 64 bits, rounded to fp32; ties go to the
+    earlier page, a NaN score ranks first, an invalid page id last (it, and a
+    length out of range, set bits read by ``kv_append_status``).  At most 65,535
+    (sequence, kv head) pairs.  query: (num_seqs, num_q_heads,
     head_size); page_bounds as kept by ``update_page_bounds``; block_tables,
     context_lens as for ``paged_attention``.
     """
@@ -157,7 +159,7 @@ def paged_attention_sparse(out, query, key_cache, value_cache, page_bounds, bloc
     ``out`` and returns the (tables, lens) it attended to.
 
     Arguments as for ``paged_attention`` (16-bit caches of either layout) and
-    ``select_pages``.
+    ``select_pages``; ``out`` must not overlap ``query``.
     """
     args, device, keep = _paged_args(query, key_cache, value_cache, block_tables, context_lens,
                                      scale, block_size, kv_layout, num_splits)
@@ -165,6 +167,8 @@ def paged_attention_sparse(out, query, key_cache, value_cache, page_bounds, bloc
         raise ValueError("out must match query in shape, dtype and device")
     if out.stride(2) != 1:
         raise ValueError("out must be contiguous in head_size")
+    if out.data_ptr() == query.data_ptr() and query.numel():
+        raise ValueError("out must not be query: queries are read until the call ends")
     if num_splits < 0:
         raise ValueError("num_splits must be >= 0")
     args.out = out.data_ptr()

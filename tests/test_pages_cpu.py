@@ -247,14 +247,16 @@ def test_read_refusals():
 def test_attention_int4_refusals():
     k, v, x, lens, bt = _tensors()
     q = torch.zeros((2, 8, 128), dtype=torch.bfloat16)
+    o = q.clone()
     for bad, err in [
             (dict(q=q.float(), out=q.float()), TypeError), (dict(q=q[0]), ValueError),
+            (dict(out=q), ValueError),                 # in place
             (dict(out=q.half()), ValueError), (dict(out=q[:1]), ValueError),
             (dict(q=q[:, :7], out=q[:, :7]), ValueError), (dict(lens=lens[:1]), ValueError),
             (dict(bt=bt[0]), ValueError), (dict(bs=32), ValueError), (dict(n=-1), ValueError),
             (dict(k=k.view(torch.int8)), TypeError), (dict(k=k.view(32, -1)), ValueError),
             (dict(q=q[:, :, ::2], out=q[:, :, ::2]), ValueError), (dict(), ValueError)]:
-        a = dict(out=q, q=q, k=k, v=v, bt=bt, lens=lens, bs=16, n=0) | bad
+        a = dict(out=o, q=q, k=k, v=v, bt=bt, lens=lens, bs=16, n=0) | bad
         with pytest.raises(err):
             pa.paged_attention_int4(a["out"], a["q"], a["k"], a["v"], a["bt"], a["lens"], 0.1,
                                     a["bs"], num_splits=a["n"])

@@ -295,6 +295,82 @@ def test_sparse_attention(cuda_device, dt, D, G, Hkv, bs, lens, keep, layout):
     assert ((out.float() - full.float()).abs() <= tol).all()
 
 
+def test_captured_ragged_and_sparse_calls(cuda_device):
+    """A chunk of a prompt (bounds, append, read-back) and a page-sparse decode in
+    two graphs, replayed in turn on two streams while their inputs change."""
+    dt, D, G, Hkv, bs, B, keep = HF, 64, 8, 2, 8, 3, 5
+    g = torch.Generator().manual_seed(12)
+    lens = torch.tensor([3, 0, 40], dtype=torch.int32)
+    new = torch.tensor([20, 1, 9], dtype=torch.int32)
+    cu = torch.zeros(B + 1, dtype=torch.int32)
+    cu[1:] = torch.cumsum(new, 0)
+    bt, pool = tables(lens + new, bs)
+    N = int(new.sum())
+    kc, vc = pa.int4_cache(pool, Hkv, bs, D, device=cuda_device)
+    bounds = torch.zeros((pool, Hkv, 2, D), dtype=dt, device=cuda_device)
+    kp = torch.randn((pool, Hkv, bs, D), generator=g).to(dt).to(cuda_device)
+    vp = torch.randn((pool, Hkv, bs, D), generator=g).to(dt).to(cuda_device)
+    kb = torch.stack((kp.amin(2), kp.amax(2)), 2).contiguous()
+    x = torch.zeros((2, N, Hkv, D), dtype=dt, device=cuda_device)
+    q = torch.zeros((B, G * Hkv, D), dtype=dt, device=cuda_device)
+    out = torch.empty_like(q)
+    l0, l1 = lens.to(cuda_device), lens.to(cuda_device)
+    tot = (lens + new).to(cuda_device)
+    btd, cud = bt.to(cuda_device), cu.to(cuda_device)
+    res = {}
+
+    def chunk():
+        l1.copy_(l0)
+        pa.update_page_bounds(bounds, x[0], l1, btd, bs, cu_new=cud)
+        pa.kv_append_int4(kc, vc, x[0], x[1], l1, btd, bs, cu_new=cud)
+        res["k"], res["v"] = pa.kv_read_int4(kc, vc, btd, l1, bs, D, dt, starts=l0, cu_out=cud,
+                                             num_tokens=N)
+
+    def attend():
+        res["t"], res["l"] = pa.paged_attention_sparse(out, q, kp, vp, kb, btd, tot, 0.1, bs, keep)
+
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    graphs = []
+    torch.cuda.synchronize()
+    for fn, st in zip((chunk, attend), streams):
+        with torch.cuda.stream(st):
+            fn()
+        torch.cuda.synchronize()
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr, stream=st):
+            fn()
+        graphs.append(gr)
+    for _ in range(3):
+        xn = torch.randn((2, N, Hkv, D), generator=g).to(dt)
+        qn = torch.randn((B, G * Hkv, D), generator=g).to(dt)
+        x.copy_(xn)
+        q.copy_(qn)
+        torch.cuda.synchronize()
+        for gr, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                gr.replay()
+                gr.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(l1.cpu(), lens + new)
+        for i, name in enumerate(("k", "v")):
+            c, s, lo = op.quantise(xn[i])
+            want = lo.double()[..., None] + s.double()[..., None] * c.unflatten(-1, (-1, 64)).double()
+            err = (res[name].cpu().double() - want.flatten(-2)).abs()
+            assert (err <= half_step(dt) * want.flatten(-2).abs() + 2.0 ** -25).all()
+        b = torch.zeros((pool * Hkv, 2, D), dtype=dt)
+        expect_bounds(b, xn[0], lens, bt, bs, cu, False)
+        fresh = [int(bt[s, i]) for s in range(B)
+                 for i in range((int(lens[s]) + bs - 1) // bs, (int(lens[s] + new[s]) + bs - 1) // bs)]
+        assert torch.equal(bounds.cpu()[fresh], b.view(pool, Hkv, 2, D)[fresh])
+        want, wl = expect_select(qn, kb.cpu().view(-1, 2, D), bt, lens + new, bs, keep, 1, 1, Hkv, False)
+        assert torch.equal(res["t"].cpu(), want) and torch.equal(res["l"].cpu(), wl)
+        full = torch.empty_like(out)
+        pa.paged_attention(full, q, kp, vp, res["t"], res["l"], 0.1, bs)
+        # the same tables through the dense call: other splits of the same sums
+        tol = 2 * half_step(dt) * (full.float().abs() + vp.float().abs().max()) + 1e-3
+        assert ((out.float() - full.float()).abs() <= tol).all()
+
+
 def test_serving_steps_together(cuda_device):
     """Prompts and steps: bounds, 4-bit append, selection and 4-bit attention
     over the selection, eager and then replayed from a graph."""
