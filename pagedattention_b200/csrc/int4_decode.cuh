@@ -6,13 +6,13 @@
 // A quarter of the bytes of 16-bit pages but the same products, and codes to
 // widen before the matrix instructions can take them: instruction issue bounds
 // the kernel, not HBM, so everything is laid out for few instructions per code.
-//   * One producer warp per CTA walks the CTA's page range (the planner's
-//     equal cut of all pages with its tail chunks, as in decode.cuh), reads the
-//     block table one stage ahead and fills a ring of 128-token stages: four
-//     pages of a cache per copy (rows gathered through a tensor map, pages up to
-//     2 KB), or one untiled bulk copy per page.  Four consumer warps share every stage, 32
-//     tokens each (groups of more than 16 heads at D 128: two pairs, each pair
-//     16 heads and 64 tokens per warp), and do nothing but arithmetic.
+//   * One producer warp per CTA walks the CTA's page range (the planner's equal
+//     cut of all pages), reads the block table one stage ahead and fills a ring of
+//     128-token stages: four pages of a cache per copy (rows gathered through a
+//     tensor map, pages up to 2 KB), or one untiled bulk copy per page.  Four
+//     consumer warps share every stage, 32 tokens each (groups of more than 16
+//     heads: two pairs, each warp 16 heads and 64 tokens), and do nothing but
+//     arithmetic.
 //   * Keys enter the MMA as fp16 subnormals, the nibbles as they stand (one
 //     mask per pair); the query is brought to fp16 by a power of two per head,
 //     which loses nothing of a bf16 or fp16 query that matters, and the score is
@@ -23,17 +23,28 @@
 //     How the values' codes enter depends on T.
 //     fp16: as c - 8, so that the rounding of p s is multiplied by s (c - 8), about
 //     |x|, not by s c, about the group's range: the output keeps fp16's 11 bits.
-//     bf16: as they stand, like the keys', which spares seven instructions per
-//     eight codes (64 x 4096 tokens: 82 -> 72 us): an fp16 p s is eight times
-//     finer than the bf16 output needs.  Its scales reach past fp16, so they carry
-//     a power of two that follows the largest scale seen; and since sums of
-//     codes >= 0 only grow, and the tensor cores cut their fp32 sums short, the
-//     accumulators are emptied into shared memory every kFlush chunks of 32 tokens.
+//     bf16: as they stand, like the keys': an fp16 p s is eight times finer than
+//     the bf16 output needs, and than a bf16 p s (error against 64 bits 0.0017,
+//     0.0023 with bf16 c - 8; 4 contexts of 32768 to 131072 tokens 111 -> 108 us).
+//     Its scales reach past fp16, so they carry a power of two that follows the
+//     largest scale seen (values whose scale lies more than 2^27 below that lose
+//     bits); and since sums of codes >= 0 only grow, and the tensor cores cut
+//     their fp32 sums short, the accumulators are emptied into shared memory every
+//     kFlush chunks of 32 tokens.
 //   * The softmax's reference point moves only when a score exceeds it by
 //     kRaise (log2 units): no shuffles or rescaling in most stages.
 // At the end of a head (or of the CTA's part of it) the consumers' states are
 // joined through shared memory and written: the output, or one partial state
 // for the reduce kernels of decode.cuh.
+//
+// Measured (bf16, 8 kv heads of 4 query heads, D 128, pages of 16): 64 sequences
+// of 4096 tokens 82 us, 3.7 TB/s of the 6.55 a copy reaches.  About 618 warp
+// instructions per 32 tokens and head keep the issue slots 52 % and the ALU pipe
+// 55 % busy; the copies alone take 59 us, the arithmetic alone 77.  Without a
+// producing warp (the last warp of a stage refills its slot) 97, with 4 CTAs per
+// SM at 96 registers (which spill) 94.  Handing CTAs that end early the last
+// chunks of others, as decode.cuh does, costs one more join per chunk: 82.3 to
+// 90 us with 1 to 4 chunks, so the ranges are fixed.
 #pragma once
 
 #include <type_traits>
@@ -166,8 +177,6 @@ __global__ void __launch_bounds__(kQ4Threads, MINB)
   }
   const int64_t units = (static_cast<int64_t>(total) + p.unit_pages - 1) / p.unit_pages;
   const int W = static_cast<int>(units < p.total_warps ? units : p.total_warps);
-  int sm_m = 0, sm_k = 0;  // tail chunks of every range, pages per chunk
-  tail_chunks(total, W, p.steal_m_max, p.steal_pps, p.steal_min_stages, &sm_m, &sm_k);
   const int u = blockIdx.x;
   const int gs = u < W ? static_cast<int>(static_cast<int64_t>(u) * total / W) : 0;
   const int ge = u < W ? static_cast<int>(static_cast<int64_t>(u + 1) * total / W) : 0;
@@ -178,7 +187,7 @@ __global__ void __launch_bounds__(kQ4Threads, MINB)
     const int pb = int4_row_bytes(D) << log2_bs;
     const uint64_t policy = l2_policy_evict_first();
     auto prefix = [&](int hd) { return early ? cum_sm[hd] : p.cum[hd]; };
-    bool bad_seen = false, timeout = false, waited = false;
+    bool bad_seen = false, timeout = false;
     int issued = 0, slot = 0;
     uint32_t phase = 1;  // of `empty`: the first round finds every slot free
     // Largest head whose first page is <= P.
@@ -193,19 +202,10 @@ __global__ void __launch_bounds__(kQ4Threads, MINB)
       }
       return lo;
     };
-    // The planner's claim words are in place (and its status word).
-    auto wait_plan = [&]() {
-      if (!waited) grid_dependency_wait();
-      waited = true;
-    };
     if (gs < ge) {
-      // Current segment [gp, seg_end) from seg_start: the range's static part,
-      // then tail chunks claimed from the front of this CTA's tail, then chunks
-      // taken from the back of other CTAs' (as in decode_body).
-      int seg_start = gs, seg_end = ge - sm_m * sm_k, mode = 0;
       int head = find_head(gs);
       int c_lo = prefix(head), c_hi = prefix(head + 1), gp = gs;
-      int nx_head = 0, nx_np = 0, nx_tok = 0, nx_flags = 0, nx_slot = 0, nx_raw = 0;
+      int nx_head = 0, nx_np = 0, nx_tok = 0, nx_flags = 0, nx_raw = 0;
       int64_t nx_add = 0;
       const int32_t* c_bt = p.bt;
       int c_h = 0, c_len = 0;
@@ -216,67 +216,10 @@ __global__ void __launch_bounds__(kQ4Threads, MINB)
         c_len = early ? len_sm[head] : head_len(head);
       };
       enter_head();
-      auto next_segment = [&]() -> bool {
-        if (sm_m == 0) return false;
-        wait_plan();
-        if (mode == 0) {
-          unsigned long long old = 0ull;
-          if (lane == 0) old = atomicAdd(p.claims + u, 1ull);
-          old = __shfl_sync(0xffffffffu, old, 0);
-          if (static_cast<uint32_t>(old) + static_cast<uint32_t>(old >> 32) < static_cast<uint32_t>(sm_m)) {
-            if (lane == 0) atomicSub(p.steal + 2, 1);
-            seg_start = gp = seg_end;
-            seg_end += sm_k;
-            return true;
-          }
-          mode = 1;
-        }
-        // Rounds of 32 claim words picked by a shared cursor; the CTA with the
-        // most chunks left is tried.
-        const int rounds = 2 * ((W + 31) / 32) + 2;
-        for (int r = 0; r < rounds; ++r) {
-          int left = 0;
-          uint32_t at = 0;
-          if (lane == 0) {
-            left = *reinterpret_cast<volatile int32_t*>(p.steal + 2);
-            at = atomicAdd(reinterpret_cast<unsigned int*>(p.steal + 3), 32u);
-          }
-          left = __shfl_sync(0xffffffffu, left, 0);
-          if (left <= 0) return false;
-          at = __shfl_sync(0xffffffffu, at, 0);
-          const int v = static_cast<int>((at + lane) % static_cast<uint32_t>(W));
-          const unsigned long long wd = *reinterpret_cast<volatile unsigned long long*>(p.claims + v);
-          const int used = static_cast<int>(static_cast<uint32_t>(wd)) +
-                           static_cast<int>(static_cast<uint32_t>(wd >> 32));
-          const int rem = used < sm_m ? sm_m - used : 0;
-          const int best = __reduce_max_sync(0xffffffffu, (rem << 5) | (31 - lane));
-          if ((best >> 5) == 0) continue;
-          const int vb = __shfl_sync(0xffffffffu, v, 31 - (best & 31));
-          unsigned long long old = 0ull;
-          if (lane == 0) old = atomicAdd(p.claims + vb, 1ull << 32);
-          old = __shfl_sync(0xffffffffu, old, 0);
-          const uint32_t f = static_cast<uint32_t>(old), bk = static_cast<uint32_t>(old >> 32);
-          if (f + bk < static_cast<uint32_t>(sm_m)) {
-            if (lane == 0) atomicSub(p.steal + 2, 1);
-            const int end = static_cast<int>(static_cast<int64_t>(vb + 1) * total / W);
-            seg_start = gp = end - static_cast<int>(bk + 1) * sm_k;
-            seg_end = seg_start + sm_k;
-            return true;
-          }
-        }
-        return false;
-      };
       // The next stage, its block-table entries on their way.
       auto prepare = [&]() -> bool {
-        if (gp >= seg_end) {
-          if (!next_segment()) return false;
-          if (gp < c_lo || gp >= c_hi) {
-            head = find_head(gp);
-            c_lo = prefix(head);
-            c_hi = prefix(head + 1);
-            enter_head();
-          }
-        } else if (gp >= c_hi) {
+        if (gp >= ge) return false;
+        if (gp >= c_hi) {
           do {
             ++head;
             c_lo = c_hi;
@@ -287,17 +230,16 @@ __global__ void __launch_bounds__(kQ4Threads, MINB)
         const int lp = gp - c_lo;
         int np = pps;
         if (c_hi - gp < np) np = c_hi - gp;
-        if (seg_end - gp < np) np = seg_end - gp;
+        if (ge - gp < np) np = ge - gp;
         nx_head = head;
         nx_np = np;
         const int left = c_len - (lp << log2_bs);
         nx_tok = left < np << log2_bs ? left : np << log2_bs;
-        // 1: the head's first stage in the segment, 2: its last, 4: the whole
-        // head is in the segment
-        nx_flags = (gp == c_lo || gp == seg_start ? 1 : 0) |
-                   (gp + np == c_hi || gp + np == seg_end ? 2 : 0) |
-                   (c_lo >= seg_start && c_hi <= seg_end ? 4 : 0);
-        if (nx_flags & 2) nx_slot = head + segment_of_page(gp, total, W, sm_m, sm_k);
+        // 1: the head's first stage in the range, 2: its last, 4: the whole head
+        // is in the range
+        nx_flags = (gp == c_lo || gp == gs ? 1 : 0) |
+                   (gp + np == c_hi || gp + np == ge ? 2 : 0) |
+                   (c_lo >= gs && c_hi <= ge ? 4 : 0);
         nx_add = static_cast<int64_t>(c_h) * p.bt_add;
         if (lane < np) nx_raw = c_bt[static_cast<int64_t>(lp + lane) * p.bt_si];
         gp += np;
@@ -308,7 +250,7 @@ __global__ void __launch_bounds__(kQ4Threads, MINB)
       bool more = prepare();
       while (more) {
         const int np = nx_np;
-        int4 rec = make_int4(nx_head, nx_tok, nx_flags, nx_slot);
+        int4 rec = make_int4(nx_head, nx_tok, nx_flags, 0);
         const int64_t pid = static_cast<int64_t>(nx_raw) * p.bt_mul + nx_add;
         const bool ok = lane < np && pid >= 0 && pid < p.num_pages;
         const uint32_t bad = __ballot_sync(0xffffffffu, lane < np && !ok);
@@ -386,7 +328,7 @@ __global__ void __launch_bounds__(kQ4Threads, MINB)
     // did (the end record's slot was waited for above).
     for (int j = max(issued - depth + (ended ? 1 : 0), 0); j < issued; ++j)
       mbar_wait(full + (j % depth) * 8, (j / depth) & 1, kWaitLimitNs);
-    wait_plan();  // the planner has reset the status word
+    grid_dependency_wait();  // the planner has reset the status word
     if (lane == 0 && (bad_seen || timeout))
       atomicOr(p.status, (bad_seen ? kStatusBadPage : 0u) | (timeout ? kStatusTimeout : 0u));
     return;
@@ -528,9 +470,10 @@ __global__ void __launch_bounds__(kQ4Threads, MINB)
   auto deposit = [&](bool last) -> bool {
     if (!emptied && !__all_sync(0xffffffffu, mbar_wait(drained, (joins & 1) ^ 1, kWaitLimitNs)))
       return false;
-    // codes entered as c 2^-24 (even registers of a word) or c 2^-20 (odd ones)
-    const float down = kHalf ? 1.f : __uint_as_float((254u << 23) - __float_as_uint(nu)) * 1048576.f;
-    const float w0 = kHalf ? 1.f : down * 16.f, w1 = down;
+    // Codes entered as c 2^-24 (even registers of a word) or c 2^-20 (odd ones).
+    // Undone in two steps, as 2^24 / nu passes fp32's range for the largest scales.
+    const float down = kHalf ? 1.f : __uint_as_float((254u << 23) - __float_as_uint(nu));
+    const float w0 = kHalf ? 1.f : 16777216.f, w1 = kHalf ? 1.f : 1048576.f;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -551,10 +494,10 @@ __global__ void __launch_bounds__(kQ4Threads, MINB)
           // accumulator (tile 4 gi + m, register e + 2 j): element 64 gi + 8 lr + 2 m + j
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
-            float4 x = make_float4(fmaf(acc[gi * 4 + 2 * half][nt][e], w0, v),
-                                   fmaf(acc[gi * 4 + 2 * half][nt][e + 2], w0, v),
-                                   fmaf(acc[gi * 4 + 2 * half + 1][nt][e], w1, v),
-                                   fmaf(acc[gi * 4 + 2 * half + 1][nt][e + 2], w1, v));
+            float4 x = make_float4(fmaf(acc[gi * 4 + 2 * half][nt][e] * w0, down, v),
+                                   fmaf(acc[gi * 4 + 2 * half][nt][e + 2] * w0, down, v),
+                                   fmaf(acc[gi * 4 + 2 * half + 1][nt][e] * w1, down, v),
+                                   fmaf(acc[gi * 4 + 2 * half + 1][nt][e + 2] * w1, down, v));
             float4* at = reinterpret_cast<float4*>(row + gi * 64 + half * 4);
             if (g < G) {
               if (emptied) {
@@ -867,7 +810,7 @@ __global__ void __launch_bounds__(kQ4Threads, MINB)
       code_at -= depth * STAGE_BYTES;
       pair_at -= depth * STAGE_BYTES;
     }
-    if ((rec.z & 2) && !finish_head(rec.x, (rec.z & 4) != 0, rec.w)) {
+    if ((rec.z & 2) && !finish_head(rec.x, (rec.z & 4) != 0, rec.x + u)) {
       timeout = true;
       break;
     }

@@ -507,11 +507,9 @@ int make_plan_int4(const pab200_decode_args* a, Plan* pl) {
   pl->W = pl->grid = W;
   pl->unit_pages = pab::kQ4Stage / a->block_size;
   pl->slot_floats = (pl->G * D + 2 * pl->G + 3) & ~3;
-  // The CTAs of an SM do not get equal shares of its issue slots (64 x 4096
-  // tokens: they end between 65 and 88 us without tail chunks).
-  int m_max = env_int("PAB200_STEAL_M", 0);
-  lay_out_workspace(pl, m_max < 0 ? 0 : m_max, SIZE_MAX);
-  pl->steal_min_stages = env_int("PAB200_STEAL_MIN_STAGES", 2);
+  // Ranges without tail chunks (measured in int4_decode.cuh).
+  lay_out_workspace(pl, 0, SIZE_MAX);
+  pl->steal_min_stages = 1;
   return PAB200_OK;
 }
 

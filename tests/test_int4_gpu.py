@@ -263,6 +263,31 @@ def test_read_ranges(cuda_device):
         assert (err <= (half_step(dt) + 2.0 ** -23) * want.abs() + 1e-8).all()
 
 
+@pytest.mark.parametrize("cu,N", [([5, 12, 12, 20], 40), ([0, 0, 0, 0], 9), ([9, 9, 9, 9], 9),
+                                  ([3, 4, 70, 71], 71)])
+def test_read_rows_of_no_sequence(cuda_device, cu, N):
+    """Fresh outputs are zero before the first sequence's rows and behind the last's."""
+    dt, D, bs, Hkv = BF, 64, 8, 3
+    g = torch.Generator().manual_seed(4)
+    lens = torch.tensor([70, 70, 70], dtype=torch.int32)
+    bt, pool = tables(lens, bs)
+    kp = random_pages(pool * Hkv, D, bs, dt, g, False)
+    vp = random_pages(pool * Hkv, D, bs, dt, g, True)
+    kcd, vcd = (torch.from_numpy(p).view(pool, Hkv, -1).to(cuda_device) for p in (kp, vp))
+    torch.full((2, N, Hkv, D), 7.0, dtype=dt, device=cuda_device)  # freed: the memory is not zero
+    k, v = pa.kv_read_int4(kcd, vcd, bt.to(cuda_device), lens.to(cuda_device), bs, D, dt,
+                           cu_out=torch.tensor(cu, dtype=torch.int32, device=cuda_device), num_tokens=N)
+    for got, pages, value in ((k, kp, False), (v, vp, True)):
+        vals = op.get_rows(pages, D, bs, dt, value)
+        want = torch.zeros((N, Hkv, D), dtype=torch.float64)
+        for s in range(3):
+            for j in range(cu[s + 1] - cu[s]):
+                for h in range(Hkv):
+                    want[cu[s] + j, h] = torch.from_numpy(vals[int(bt[s, j // bs]) * Hkv + h, j % bs])
+        err = (got.cpu().double() - want).abs()
+        assert (err <= (half_step(dt) + 2.0 ** -23) * want.abs() + 1e-8).all()
+
+
 # --------------------------------------------------------------- attention
 
 def check_attention(got, q, kp, vp, bt, lens, scale, bs, Hkv, dt, per_head_pages=False):
@@ -362,6 +387,73 @@ def test_attention_matches_64_bits(cuda_device, dt, D, G, Hkv, bs, lens):
     again = torch.empty_like(out)
     pa.paged_attention_int4(again, q.to(cuda_device), *args, scale, bs)
     assert torch.equal(again, out)
+
+
+# Binary exponents of the values' standard deviation, page by page.
+UP = list(range(-96, 100, 4))
+SCALES = [(BF, [UP, UP[::-1], [-118] * 40, [117] * 12, [0, 60, -20, 30, -60, 100] * 6]),
+          (HF, [list(range(-6, 11)) * 2, list(range(10, -7, -1)) * 2, [-7] * 40, [12] * 40])]
+
+
+@pytest.mark.parametrize("dt,exps", SCALES)
+@pytest.mark.parametrize("D,G,bs", [(64, 8, 8), (128, 4, 16), (128, 20, 8)])
+def test_attention_values_of_many_scales(cuda_device, dt, exps, D, G, bs):
+    """Values whose size jumps from page to page, tiny and huge ones."""
+    g = torch.Generator().manual_seed(9)
+    lens = torch.tensor([len(e) * bs - 3 for e in exps], dtype=torch.int32)
+    bt, pool = tables(lens, bs)
+    mul = torch.ones((pool, 1, 1))
+    for s, es in enumerate(exps):
+        for i, e in enumerate(es):
+            mul[int(bt[s, i])] = 2.0 ** e
+    kp = random_pages(pool, D, bs, dt, g, False)
+    vp = random_pages(pool, D, bs, dt, g, True, mul)
+    q = (torch.randn((len(exps), G, D), generator=g) * 0.5).to(dt)
+    out = torch.empty_like(q).to(cuda_device)
+    for splits in (0, 2):
+        pa.paged_attention_int4(out, q.to(cuda_device),
+                                *(torch.from_numpy(p).view(pool, 1, -1).to(cuda_device)
+                                  for p in (kp, vp)), bt.to(cuda_device), lens.to(cuda_device),
+                                0.1, bs, num_splits=splits)
+        check_attention(out, q, kp, vp, bt, lens, 0.1, bs, 1, dt)
+
+
+@pytest.mark.parametrize("dt,D,G,bs", [(BF, 128, 2, 16), (BF, 64, 32, 8), (BF, 256, 4, 64),
+                                       (HF, 128, 2, 16)])
+def test_attention_long_range_of_one_cta(cuda_device, dt, D, G, bs):
+    """20,001 tokens over two CTAs: hundreds of stages of one head per CTA."""
+    g = torch.Generator().manual_seed(10)
+    L, pages = 20001, 48
+    bt = torch.randint(0, pages, (1, (L + bs - 1) // bs), generator=g, dtype=torch.int32)
+    kp = random_pages(pages, D, bs, dt, g, False)
+    vp = random_pages(pages, D, bs, dt, g, True)
+    q = torch.randn((1, G, D), generator=g).to(dt)
+    out = torch.empty_like(q).to(cuda_device)
+    lens = torch.tensor([L], dtype=torch.int32)
+    pa.paged_attention_int4(out, q.to(cuda_device), *(torch.from_numpy(p).view(pages, 1, -1).to(cuda_device)
+                                                      for p in (kp, vp)),
+                            bt.to(cuda_device), lens.to(cuda_device), 0.05, bs, num_splits=2)
+    check_attention(out, q, kp, vp, bt, lens, 0.05, bs, 1, dt)
+
+
+@pytest.mark.parametrize("dt", [BF, HF])
+def test_attention_many_heads(cuda_device, dt):
+    """1,200 (sequence, kv head) pairs, many of them empty or of one token."""
+    D, G, Hkv, bs, B = 64, 2, 4, 8, 300
+    g = torch.Generator().manual_seed(11)
+    lens = torch.randint(0, 60, (B, Hkv), generator=g, dtype=torch.int32)
+    lens[::7] = 0
+    lens[::11] = 1
+    bt, pool = tables(lens, bs)
+    kp = random_pages(pool, D, bs, dt, g, False)
+    vp = random_pages(pool, D, bs, dt, g, True)
+    q = torch.randn((B, G * Hkv, D), generator=g).to(dt)
+    out = torch.full_like(q, 5.0).to(cuda_device)
+    pa.paged_attention_int4(out, q.to(cuda_device), torch.from_numpy(kp).to(cuda_device),
+                            torch.from_numpy(vp).to(cuda_device), bt.to(cuda_device),
+                            lens.to(cuda_device), 0.125, bs)
+    assert pa.read_status() == 0
+    check_attention(out, q, kp, vp, bt, lens, 0.125, bs, Hkv, dt, per_head_pages=True)
 
 
 def test_attention_per_head_pages_and_bad_ids(cuda_device):
