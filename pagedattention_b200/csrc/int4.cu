@@ -14,33 +14,52 @@ struct Int4AppendParams {
   int64_t r_st, r_sh;      // strides of the new rows (elements)
   int32_t vec;             // rows may be read in 16-byte units
   int32_t increment;
+  int32_t log2_run;        // tokens a warp takes: one 8-token tile, or two of a page
 };
 
 // Codes of a group whose scale is below T's normal numbers (rounded coarsely,
-// so that quotients pass 15), as in int4_quantise; lo and s of the group.
+// so that quotients pass 15), 0 or NaN (no codes), as in int4_codes_of.
 template <typename T>
-__device__ __noinline__ uint32_t int4_quantise_tiny(uint4 x, float lo, float s) {
+__device__ __noinline__ uint32_t int4_quantise_tiny(uint4 x, uint32_t pair) {
   const uint32_t v[4] = {x.x, x.y, x.z, x.w};
+  const float2 sl = unpack2<T>(pair);
   uint32_t word = 0;
-  for (int i = 0; i < 8 && s > 0.f; ++i) {
+  for (int i = 0; i < 8 && sl.x > 0.f; ++i) {
     const float2 f = unpack2<T>(v[i / 2]);
-    const float q = rintf(__fdiv_rn((i & 1 ? f.y : f.x) - lo, s));
+    const float q = rintf(__fdiv_rn((i & 1 ? f.y : f.x) - sl.y, sl.x));
     word |= static_cast<uint32_t>(fminf(q, 15.f)) << (4 * (i / 2 + 4 * (i % 2)));
   }
   return word;
 }
 
 // (minimum, -maximum) of the 64 elements of a group, 8 in each of 8 consecutive
-// lanes, in every lane: one comparison per step (a 16-bit float changes sign by
-// its top bit).
-template <typename T>
-__device__ __forceinline__ uint32_t group_range(const uint4& x) {
-  const uint32_t lo = min2_nan<T>(min2_nan<T>(x.x, x.y), min2_nan<T>(x.z, x.w));
-  const uint32_t hi = max2_nan<T>(max2_nan<T>(x.x, x.y), max2_nan<T>(x.z, x.w)) ^ 0x80008000u;
-  uint32_t both = min2_nan<T>(__byte_perm(lo, hi, 0x5410), __byte_perm(lo, hi, 0x7632));
+// lanes, of the rows of N rounds: lane o of the 8 gets round o % N.  A 16-bit
+// float changes sign by its top bit, so one comparison serves both; a step
+// across lanes also halves the rounds that a lane goes on with.
+template <typename T, int N>
+__device__ __forceinline__ uint32_t group_ranges(const uint4 (&x)[N], int o) {
+  uint32_t v[N];
 #pragma unroll
-  for (int o = 1; o < 8; o <<= 1) both = min2_nan<T>(both, __shfl_xor_sync(0xffffffffu, both, o));
-  return both;
+  for (int i = 0; i < N; ++i) {
+    const uint32_t lo = min2_nan<T>(min2_nan<T>(x[i].x, x[i].y), min2_nan<T>(x[i].z, x[i].w));
+    const uint32_t hi = max2_nan<T>(max2_nan<T>(x[i].x, x[i].y), max2_nan<T>(x[i].z, x[i].w)) ^ 0x80008000u;
+    v[i] = min2_nan<T>(__byte_perm(lo, hi, 0x5410), __byte_perm(lo, hi, 0x7632));
+  }
+#pragma unroll
+  for (int b = 1; b < 8; b <<= 1) {
+    const bool up = o & b;
+#pragma unroll
+    for (int j = 0; 2 * j < N / b; ++j) {
+      if (N / b > 1) {
+        const uint32_t got = __shfl_xor_sync(0xffffffffu, up ? v[2 * j] : v[2 * j + 1], b);
+        v[j] = min2_nan<T>(up ? v[2 * j + 1] : v[2 * j], got);
+      } else {
+        v[0] = min2_nan<T>(v[0], __shfl_xor_sync(0xffffffffu, v[0], b));
+      }
+    }
+    if (N / b == 0) v[0] = min2_nan<T>(v[0], __shfl_xor_sync(0xffffffffu, v[0], b));
+  }
+  return v[0];
 }
 
 // Smallest scale whose quotients stay at 15 (1 + 2^-8) at most: the normal
@@ -72,8 +91,8 @@ __device__ __forceinline__ uint32_t int4_scale(uint32_t both, float* inv) {
 // inputs, stay ties; adding 1.5 * 2^23 rounds it.
 template <typename T>
 __device__ __forceinline__ uint32_t int4_codes_of(const uint4& x, uint32_t pair, float inv) {
+  if (inv == 0.f) return int4_quantise_tiny<T>(x, pair);
   const float2 sl = unpack2<T>(pair);
-  if (inv == 0.f) return int4_quantise_tiny<T>(x, sl.y, sl.x);  // no code if s is 0 or NaN
   constexpr float kMagic = 12582912.f;  // 1.5 * 2^23
   const uint32_t v[4] = {x.x, x.y, x.z, x.w};
   uint32_t c[8];  // 0x4b400000 + code
@@ -146,14 +165,8 @@ __device__ __forceinline__ void append_tile(const Int4AppendParams& p, int64_t o
 #pragma unroll
   for (int kv = 0; kv < 2; ++kv) {
     uint8_t* page = p.cache[kv] + off;
-    uint32_t mine = 0u;
-#pragma unroll
-    for (int i = 0; i < ROUNDS; ++i) {
-      const uint32_t both = group_range<T>(x[kv][i]);
-      if (o % ROUNDS == i) mine = both;
-    }
     float inv;
-    const uint32_t pair = int4_scale<T>(mine, &inv);
+    const uint32_t pair = int4_scale<T>(group_ranges<T, ROUNDS>(x[kv], o), &inv);
     const int mr = o % ROUNDS * RP + rr;  // the row this lane has scaled
     if (o < ROUNDS && (FULL || (mr >= r0 && mr < r1)))
       *reinterpret_cast<uint32_t*>(page + int4_pair(D, bs, tile + mr, g)) = pair;
@@ -184,41 +197,52 @@ __device__ __forceinline__ void append_tile(const Int4AppendParams& p, int64_t o
   }
 }
 
-// Ragged runs of tokens: one warp per (8-token tile, kv head).
+// Ragged runs of tokens: one warp per (run of 8 or 16 positions, kv head).
+//
+// Reads 2 bytes per element and writes 9/16: 29,000 tokens of 8 kv heads, D 128,
+// move 151 MB, 23 us at a copy's 6.55 TB/s.  It takes 43 (3.5 TB/s): issue binds
+// it (73 % of the slots), about 1,190 warp instructions per 8-token tile; without
+// any arithmetic the same loads and stores take 29, the ranges and the codes about
+// 7 each.  64 registers (4 CTAs per SM, a few spilled) 42.8, 80 registers 44.4.
 template <typename T, int D>
-__global__ void __launch_bounds__(256, 4) int4_append_kernel(const Int4AppendParams p, int warps) {
+__global__ void __launch_bounds__(256, D == 256 ? 2 : 4) int4_append_kernel(const Int4AppendParams p, int warps) {
   const TokenMap& m = p.map;
   const int wid = blockIdx.x * 8 + (threadIdx.x >> 5);
   if (wid >= warps) return;
   const int slot = wid / m.Hkv, h = wid - slot * m.Hkv;
-  const TokenRun t = find_run(m, slot, 3);
+  const int k = p.log2_run;
+  const TokenRun t = find_run(m, slot, k);
   if (t.n == 0) return;
   const int L = p.lens[t.s * m.l_sb + h * m.l_sh];
   uint32_t flags = 0;
   if (L < 0) {
     flags = kStatusNegative;
   } else {
-    const int64_t pos0 = ((static_cast<int64_t>(L) >> 3) + t.run) << 3;  // the tile's position
-    const int64_t a = L > pos0 ? L - pos0 : 0;
-    const int64_t end = static_cast<int64_t>(L) + t.n - pos0;
-    if (end <= 0) return;
+    const int64_t pos0 = ((static_cast<int64_t>(L) >> k) + t.run) << k;  // the run's position
+    const int64_t over = static_cast<int64_t>(L) + t.n - pos0;
+    if (over <= 0) return;
+    const int a = L > pos0 ? static_cast<int>(L - pos0) : 0;  // its new rows: [a, end)
+    const int end = over < (1 << k) ? static_cast<int>(over) : 1 << k;
     const int64_t pid = find_page(m, t.s, h, pos0 >> m.log2_bs, &flags);
     if (pid >= 0) {
-      const int64_t src0 = (t.t0 + pos0 - L) * p.r_st + h * p.r_sh;
       const int64_t off = pid * (static_cast<int64_t>(m.bs) * int4_row_bytes(D));
       const int tile = static_cast<int>(pos0) & (m.bs - 1);
-      if (a == 0 && end >= 8 && p.vec)
-        append_tile<T, D, true>(p, off, tile, 0, 8, src0);
-      else
-        append_tile<T, D, false>(p, off, tile, static_cast<int>(a),
-                                 end < 8 ? static_cast<int>(end) : 8, src0);
+      int64_t src0 = (t.t0 + pos0 - L) * p.r_st + h * p.r_sh;
+#pragma unroll 1
+      for (int r = 0; r < end; r += 8, src0 += 8 * p.r_st) {
+        if (a <= r && end >= r + 8 && p.vec)
+          append_tile<T, D, true>(p, off, tile + r, 0, 8, src0);
+        else if (a < r + 8)
+          append_tile<T, D, false>(p, off, tile + r, a - r, end - r, src0);
+      }
     }
   }
   if (flags && p.status && (threadIdx.x & 31) == 0) atomicOr(p.status, flags);
 }
 
 // One token per sequence: one CTA per sequence, a warp per kv head, and the
-// length, which every warp has read by then, in the same launch.
+// length, which every warp has read by then, in the same launch.  A chain of
+// dependent loads (length, table, row): 4.4 us for 64 sequences of 8 kv heads.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) int4_append_step_kernel(const Int4AppendParams p) {
   const TokenMap& m = p.map;
@@ -301,6 +325,7 @@ struct Int4ReadParams {
   uint32_t* status;
   int64_t o_st, o_sh, start_sb;
   int32_t zero_rest;       // rows of no sequence become zeros
+  int32_t log2_run;        // as in Int4AppendParams
 };
 
 // lo + s c of 8 elements: c, s and lo are exact in T, so one packed fma rounds
@@ -317,68 +342,85 @@ __device__ __forceinline__ uint4 int4_values(uint32_t word, uint32_t pair) {
   return make_uint4(r[0], r[1], r[2], r[3]);
 }
 
-// One warp per (8-token tile, kv head), lanes as in append_tile.
+// One warp per (run of 8 or 16 positions, kv head), lanes as in append_tile: the
+// rounds of a tile of which every row is wanted differ by constant offsets.
+// 29,000 tokens of 8 kv heads, D 128 (151 MB, 23 us at a copy's rate): 31.8 us,
+// 4.7 TB/s; waits for loads, 58 % of the issue slots busy.  More CTAs per SM with
+// fewer registers: 32.6 to 34.3.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) int4_read_kernel(const Int4ReadParams p, int warps) {
   constexpr int LR = D / 8, RP = 32 / LR, ROUNDS = 8 / RP;
   const TokenMap& m = p.map;
   const int wid = blockIdx.x * 8 + (threadIdx.x >> 5);
   if (wid >= warps) return;
-  const int slot = wid / m.Hkv, h = wid - slot * m.Hkv;
+  const int slot = wid / m.Hkv, h = wid - slot * m.Hkv, k = p.log2_run, run = 1 << k;
   const int lane = threadIdx.x & 31, e = lane % LR, rr = lane / LR, g = e / 8, o = e % 8;
-  auto put = [&](int64_t row, int kv, const uint4& v) {
-    *reinterpret_cast<uint4*>(static_cast<T*>(p.out[kv]) + row * p.o_st + h * p.o_sh + e * 8) = v;
-  };
+  const int64_t column = h * p.o_sh + e * 8;
   if (p.zero_rest && m.cu) {
     // Slots past the last sequence's: rows from cu[B]; the slots before the
     // first sequence's: rows up to cu[0].
     const int first = m.cu[0], last = max(m.cu[m.B], 0);
-    const int past = slot - ((last >> 3) + 2 * m.B);
-    const int64_t z0 = past >= 0 ? last + 8 * static_cast<int64_t>(past) : 8 * static_cast<int64_t>(slot);
+    const int past = slot - ((last >> k) + 2 * m.B);
+    const int64_t z0 = (past >= 0 ? last : 0) + (static_cast<int64_t>(past >= 0 ? past : slot) << k);
     const int64_t z1 = past >= 0 ? m.num_tokens : min(first, m.num_tokens);
-    if (past >= 0 || z0 < z1)
-      for (int64_t r = z0 + rr; r < z1 && r < z0 + 8; r += RP) {
-        put(r, 0, make_uint4(0u, 0u, 0u, 0u));
-        put(r, 1, make_uint4(0u, 0u, 0u, 0u));
-      }
+    for (int64_t r = z0 + rr; r < z1 && r < z0 + run; r += RP)
+#pragma unroll
+      for (int kv = 0; kv < 2; ++kv)
+        *reinterpret_cast<uint4*>(static_cast<T*>(p.out[kv]) + r * p.o_st + column) =
+            make_uint4(0u, 0u, 0u, 0u);
     if (past >= 0) return;
   }
-  const TokenRun t = find_run(m, slot, 3);
+  const TokenRun t = find_run(m, slot, k);
   if (t.n == 0) return;
   const int L = p.lens[t.s * m.l_sb + h * m.l_sh];
   const int64_t start = p.starts ? p.starts[t.s * p.start_sb] : 0;
-  const int64_t pos0 = ((start >> 3) + t.run) << 3;  // the tile's position (start may be < 0)
-  const int64_t a = start > pos0 ? start - pos0 : 0, end = start + t.n - pos0;
-  if (end <= 0) return;
-  const int r0 = static_cast<int>(a), r1 = end < 8 ? static_cast<int>(end) : 8;
+  const int64_t pos0 = ((start >> k) + t.run) << k;  // the run's position (start may be < 0)
+  const int64_t over = start + t.n - pos0;
+  if (over <= 0) return;
+  const int a = start > pos0 ? static_cast<int>(start - pos0) : 0;  // its rows: [a, end)
+  const int end = over < run ? static_cast<int>(over) : run;
+  const int64_t left = L - pos0;
+  const int have = left < end ? static_cast<int>(left) : end;  // rows from here on hold no token
   uint32_t flags = 0;
   int64_t pid = -1;
-  if (pos0 >= 0 && pos0 + r0 < L) {
+  if (pos0 >= 0 && a < have) {
     pid = find_page(m, t.s, h, pos0 >> m.log2_bs, &flags);
     if (flags && p.status && lane == 0)
       atomicOr(p.status, flags & kStatusAppendFull ? kStatusClamp : flags);
   }
-  const int64_t left = L - pos0;  // rows of the tile that hold a token
-  const int tile = static_cast<int>(pos0) & (m.bs - 1);
+  const int tile = (static_cast<int>(pos0) & (m.bs - 1)) + rr;  // this lane's first row of the page
   const int64_t off = pid * (static_cast<int64_t>(m.bs) * int4_row_bytes(D));
+  int64_t to = (t.t0 + pos0 - start + rr) * p.o_st + column;
+#pragma unroll 1
+  for (int r = 0; r < end; r += 8, to += 8 * p.o_st) {
+    if (a >= r + 8) continue;
+    uint32_t w[2][ROUNDS], pr[2][ROUNDS];
+    const bool full = pid >= 0 && a <= r && have >= r + 8;
 #pragma unroll
-  for (int kv = 0; kv < 2; ++kv) {
-    uint32_t w[ROUNDS], pr[ROUNDS];
+    for (int kv = 0; kv < 2; ++kv) {
+      const uint8_t* page = p.cache[kv] + off;
+      const uint8_t* code = page + (kv ? int4_value_word(D, tile + r, g, o) : int4_key_word(D, tile + r, g, o));
+      const uint8_t* pairs = page + int4_pair(D, m.bs, tile + r, g);
 #pragma unroll
-    for (int i = 0; i < ROUNDS; ++i) {
-      const int r = i * RP + rr;
-      w[i] = pr[i] = 0u;
-      if (pid >= 0 && r >= r0 && r < r1 && r < left) {
-        const uint8_t* page = p.cache[kv] + off;
-        w[i] = __ldg(reinterpret_cast<const uint32_t*>(
-            page + (kv ? int4_value_word(D, tile + r, g, o) : int4_key_word(D, tile + r, g, o))));
-        pr[i] = __ldg(reinterpret_cast<const uint32_t*>(page + int4_pair(D, m.bs, tile + r, g)));
+      for (int i = 0; i < ROUNDS; ++i) {
+        const int row = r + i * RP + rr;
+        w[kv][i] = pr[kv][i] = 0u;
+        if (full || (pid >= 0 && row >= a && row < have)) {
+          // a round's rows lie RP further: 128 bytes of keys, 16 of values and pairs
+          w[kv][i] = __ldg(reinterpret_cast<const uint32_t*>(code + i * (kv ? 16 : 128)));
+          pr[kv][i] = __ldg(reinterpret_cast<const uint32_t*>(pairs + i * 16));
+        }
       }
     }
 #pragma unroll
-    for (int i = 0; i < ROUNDS; ++i) {
-      const int r = i * RP + rr;
-      if (r >= r0 && r < r1) put(t.t0 + pos0 + r - start, kv, int4_values<T>(w[i], pr[i]));
+    for (int kv = 0; kv < 2; ++kv) {
+      T* out = static_cast<T*>(p.out[kv]) + to;
+#pragma unroll
+      for (int i = 0; i < ROUNDS; ++i, out += RP * p.o_st) {
+        const int row = r + i * RP + rr;
+        if (full || (row >= a && row < end))
+          *reinterpret_cast<uint4*>(out) = int4_values<T>(w[kv][i], pr[kv][i]);
+      }
     }
   }
 }
@@ -447,12 +489,18 @@ bool rows_vec(const pab200_int4_rows_args* a) {
          a->row_stride_h % 8 == 0;
 }
 
-// Warps of a kernel over (8-token tile, kv head) pairs.
-int tile_warps(const pab200_int4_rows_args* a) {
+// Positions a warp takes (log2): two tiles of a page where there are pages of two,
+// which shares the search for the run and its page (29,000 tokens of 8 kv heads,
+// D 128, pages of 16: append 50 us with one tile per warp, 44 with two at 80
+// registers; read-back 34 and 32).
+int log2_run(const pab200_int4_rows_args* a) { return a->block_size >= 16 ? 4 : 3; }
+
+// Warps of a kernel over (run, kv head) pairs.
+int run_warps(const pab200_int4_rows_args* a, int k) {
   // two slots more: the read-back's rows behind the last sequence
   const int more = a->cu_tokens ? 2 : 0;
   return static_cast<int>(
-      (pab::num_slots(a->num_tokens, a->num_seqs, a->cu_tokens != nullptr, 3) + more) *
+      (pab::num_slots(a->num_tokens, a->num_seqs, a->cu_tokens != nullptr, k) + more) *
       a->num_kv_heads);
 }
 
@@ -509,11 +557,12 @@ PAB200_EXPORT int pab200_kv_append_int4(const pab200_int4_rows_args* a, int32_t 
   p.r_sh = a->row_stride_h;
   p.vec = rows_vec(a);
   p.increment = increment ? 1 : 0;
+  p.log2_run = log2_run(a);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (a->dtype == PAB200_DTYPE_BF16)
-    launch_append_d<__nv_bfloat16>(p, a->head_size, tile_warps(a), s);
+    launch_append_d<__nv_bfloat16>(p, a->head_size, run_warps(a, p.log2_run), s);
   else
-    launch_append_d<__half>(p, a->head_size, tile_warps(a), s);
+    launch_append_d<__half>(p, a->head_size, run_warps(a, p.log2_run), s);
   cudaError_t e = cudaGetLastError();
   if (e == cudaSuccess && increment && a->cu_tokens) {
     // scheduled while the rows' kernel drains; waits for it before any length
@@ -541,11 +590,12 @@ PAB200_EXPORT int pab200_kv_read_int4(const pab200_int4_rows_args* a, const int3
   p.status = a->status;
   p.o_st = a->row_stride_t;
   p.o_sh = a->row_stride_h;
+  p.log2_run = log2_run(a);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (a->dtype == PAB200_DTYPE_BF16)
-    launch_read<__nv_bfloat16>(p, a->head_size, tile_warps(a), s);
+    launch_read<__nv_bfloat16>(p, a->head_size, run_warps(a, p.log2_run), s);
   else
-    launch_read<__half>(p, a->head_size, tile_warps(a), s);
+    launch_read<__half>(p, a->head_size, run_warps(a, p.log2_run), s);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? PAB200_OK : pabh::cuda_fail(e, "4-bit read launch");
 }

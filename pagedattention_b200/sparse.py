@@ -159,7 +159,8 @@ def paged_attention_sparse(out, query, key_cache, value_cache, page_bounds, bloc
     ``out`` and returns the (tables, lens) it attended to.
 
     Arguments as for ``paged_attention`` (16-bit caches of either layout) and
-    ``select_pages``; ``out`` must not overlap ``query``.
+    ``select_pages``, whose ranking takes ``scale`` for positive; ``out`` must not
+    overlap ``query``.
     """
     args, device, keep = _paged_args(query, key_cache, value_cache, block_tables, context_lens,
                                      scale, block_size, kv_layout, num_splits)
