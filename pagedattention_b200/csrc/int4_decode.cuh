@@ -25,7 +25,7 @@
 //     |x|, not by s c, about the group's range: the output keeps fp16's 11 bits.
 //     bf16: as they stand, like the keys': an fp16 p s is eight times finer than
 //     the bf16 output needs, and than a bf16 p s (error against 64 bits 0.0017,
-//     0.0023 with bf16 c - 8; 4 contexts of 32768 to 131072 tokens 111 -> 108 us).
+//     0.0023 with bf16 c - 8; 4 contexts of 32768 to 131072 tokens 3 us less of 111).
 //     Its scales reach past fp16, so they carry a power of two that follows the
 //     largest scale seen (values whose scale lies more than 2^27 below that lose
 //     bits); and since sums of codes >= 0 only grow, and the tensor cores cut
@@ -38,13 +38,15 @@
 // for the reduce kernels of decode.cuh.
 //
 // Measured (bf16, 8 kv heads of 4 query heads, D 128, pages of 16): 64 sequences
-// of 4096 tokens 82 us, 3.7 TB/s of the 6.55 a copy reaches.  About 618 warp
-// instructions per 32 tokens and head keep the issue slots 52 % and the ALU pipe
-// 55 % busy; the copies alone take 59 us, the arithmetic alone 77.  Without a
-// producing warp (the last warp of a stage refills its slot) 97, with 4 CTAs per
-// SM at 96 registers (which spill) 94.  Handing CTAs that end early the last
-// chunks of others, as decode.cuh does, costs one more join per chunk: 82.3 to
-// 90 us with 1 to 4 chunks, so the ranges are fixed.
+// of 4096 tokens (303 MB) 76 us, 4.0 TB/s of the 6.55 a copy reaches.  About 618
+// warp instructions per 32 tokens and head keep the issue slots a good half and
+// the ALU pipe 55 to 60 % busy; the copies alone take 59 us, the arithmetic alone
+// 70 to 77.  Without a producing warp (the last warp of a stage refills its slot)
+// 15 us more, with 4 CTAs per SM at 96 registers (which spill) 12 more.  Handing
+// CTAs that end early the last chunks of others, as decode.cuh does, costs one more
+// join per chunk and instructions that the producer has to fetch: 5 us with that
+// code in place but unused, 6 to 13 with 1 to 4 chunks.  One copy of the emptying
+// and of the join in the loop instead of two: 77.3 -> 76.1.
 #pragma once
 
 #include <type_traits>
@@ -514,10 +516,9 @@ __global__ void __launch_bounds__(kQ4Threads, MINB)
       }
     return true;
   };
-  // Joins the parts' states of head hd and writes the output (whole) or the
+  // Joins the deposited states of head hd and writes the output (whole) or the
   // partial state of this CTA's segment.
   auto finish_head = [&](int hd, bool whole, int slot) -> bool {
-    if (!deposit(true)) return false;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -788,18 +789,7 @@ __global__ void __launch_bounds__(kQ4Threads, MINB)
           }
         }
       }
-      if constexpr (!kHalf) {
-        if (++chunks == kFlush) {
-          chunks = 0;
-          if (!deposit(false)) {
-            timeout = true;
-            break;
-          }
-          emptied = true;
-        }
-      }
     }
-    if (timeout) break;
     __syncwarp();
     if (lane == 0) mbar_arrive(empty + slot * 8);  // the slot may be refilled
     code_at += STAGE_BYTES;
@@ -810,9 +800,15 @@ __global__ void __launch_bounds__(kQ4Threads, MINB)
       code_at -= depth * STAGE_BYTES;
       pair_at -= depth * STAGE_BYTES;
     }
-    if ((rec.z & 2) && !finish_head(rec.x, (rec.z & 4) != 0, rec.x + u)) {
-      timeout = true;
-      break;
+    const bool last = (rec.z & 2) != 0;
+    chunks += PT / 32;
+    if (last || (!kHalf && chunks >= kFlush)) {
+      if (!deposit(last) || (last && !finish_head(rec.x, (rec.z & 4) != 0, rec.x + u))) {
+        timeout = true;
+        break;
+      }
+      chunks = 0;
+      emptied = !kHalf;  // (a last deposit: start_head resets it)
     }
   }
   grid_dependency_wait();  // the reduce kernel follows the planner too
