@@ -93,13 +93,18 @@ __device__ __forceinline__ void int4_raw_pairs(uint32_t w, uint32_t (&r)[4]) {
 }
 
 // Nibble m of both 16-bit halves of w as the fp16 pair r[m] of c - 8 (CENTRED;
-// -8..7, exact) or as it stands.  A nibble OR-ed into the low mantissa bits of
+// -8..7, exact), or the nibbles as they stand: an odd one then together with the
+// even one below it, c * 2^-20 + c' * 2^-24 (exact too), which saves an instruction
+// of five; sums of the two differ by what the odd one contributes.  A nibble OR-ed into the low mantissa bits of
 // 1024 reads as 1024 + c, at bits 4..7 as 1024 + 16 c: subtracting 1032 from the
 // one, and 1/16 of the other minus 72, are exact.
 template <bool CENTRED>
 __device__ __forceinline__ void int4_value_pairs(uint32_t w, uint32_t (&r)[4]) {
   if constexpr (!CENTRED) {
-    int4_raw_pairs(w, r);
+    r[0] = w & 0x000f000fu;
+    r[1] = w & 0x00ff00ffu;
+    r[3] = __byte_perm(w, 0u, 0x4341);
+    r[2] = r[3] & 0x000f000fu;
     return;
   }
   const uint32_t v = w >> 8;

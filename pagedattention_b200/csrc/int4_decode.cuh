@@ -472,8 +472,8 @@ __global__ void __launch_bounds__(kQ4Threads, MINB)
   auto deposit = [&](bool last) -> bool {
     if (!emptied && !__all_sync(0xffffffffu, mbar_wait(drained, (joins & 1) ^ 1, kWaitLimitNs)))
       return false;
-    // Codes entered as c 2^-24 (even registers of a word) or c 2^-20 (odd ones).
-    // Undone in two steps, as 2^24 / nu passes fp32's range for the largest scales.
+    // Codes entered as c 2^-24 (even registers of a word), or c 2^-20 and the even
+    // one's code besides (odd ones).  Undone in two steps, as 2^24 / nu passes fp32's range for the largest scales.
     const float down = kHalf ? 1.f : __uint_as_float((254u << 23) - __float_as_uint(nu));
     const float w0 = kHalf ? 1.f : 16777216.f, w1 = kHalf ? 1.f : 1048576.f;
 #pragma unroll
@@ -496,6 +496,10 @@ __global__ void __launch_bounds__(kQ4Threads, MINB)
           // accumulator (tile 4 gi + m, register e + 2 j): element 64 gi + 8 lr + 2 m + j
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
+            if constexpr (!kHalf) {
+              acc[gi * 4 + 2 * half + 1][nt][e] -= acc[gi * 4 + 2 * half][nt][e];
+              acc[gi * 4 + 2 * half + 1][nt][e + 2] -= acc[gi * 4 + 2 * half][nt][e + 2];
+            }
             float4 x = make_float4(fmaf(acc[gi * 4 + 2 * half][nt][e] * w0, down, v),
                                    fmaf(acc[gi * 4 + 2 * half][nt][e + 2] * w0, down, v),
                                    fmaf(acc[gi * 4 + 2 * half + 1][nt][e] * w1, down, v),
