@@ -92,12 +92,12 @@ __device__ __forceinline__ void int4_raw_pairs(uint32_t w, uint32_t (&r)[4]) {
   r[3] = v & 0x00f000f0u;
 }
 
-// Nibble m of both 16-bit halves of w as the fp16 pair r[m] of c - 8 (CENTRED;
-// -8..7, exact), or the nibbles as they stand: an odd one then together with the
-// even one below it, c * 2^-20 + c' * 2^-24 (exact too), which saves an instruction
-// of five; sums of the two differ by what the odd one contributes.  A nibble OR-ed into the low mantissa bits of
-// 1024 reads as 1024 + c, at bits 4..7 as 1024 + 16 c: subtracting 1032 from the
-// one, and 1/16 of the other minus 72, are exact.
+// Nibble m of both 16-bit halves of w as the fp16 pair r[m], the odd nibbles with
+// the even ones below them, which saves an instruction of five; sums of the two
+// differ by what the odd one contributes.  Everything here is exact.
+//   plain    even c 2^-24; odd c 2^-20 + c' 2^-24
+//   CENTRED  even c - 8; odd (c - 8) + (c' - 8) / 16.  A byte OR-ed under the
+//            exponent of 1024 reads as 1024 + c' + 16 c.
 template <bool CENTRED>
 __device__ __forceinline__ void int4_value_pairs(uint32_t w, uint32_t (&r)[4]) {
   if constexpr (!CENTRED) {
@@ -107,11 +107,13 @@ __device__ __forceinline__ void int4_value_pairs(uint32_t w, uint32_t (&r)[4]) {
     r[2] = r[3] & 0x000f000fu;
     return;
   }
-  const uint32_t v = w >> 8;
   const __half2 base = __float2half2_rn(1032.f);
-  const __half2 sixteenth = __float2half2_rn(0.0625f), off = __float2half2_rn(-72.f);
-  const uint32_t t[4] = {and_or(w, 0x000f000fu, 0x64006400u), and_or(w, 0x00f000f0u, 0x64006400u),
-                         and_or(v, 0x000f000fu, 0x64006400u), and_or(v, 0x00f000f0u, 0x64006400u)};
+  const __half2 sixteenth = __float2half2_rn(0.0625f), off = __float2half2_rn(-72.5f);
+  uint32_t t[4];
+  t[0] = and_or(w, 0x000f000fu, 0x64006400u);
+  t[1] = and_or(w, 0x00ff00ffu, 0x64006400u);
+  t[3] = __byte_perm(w, 0x64646464u, 0x4341);
+  t[2] = t[3] & 0xff0fff0fu;
 #pragma unroll
   for (int m = 0; m < 4; ++m) {
     const __half2 x = *reinterpret_cast<const __half2*>(&t[m]);

@@ -38,10 +38,11 @@
 // for the reduce kernels of decode.cuh.
 //
 // Measured (bf16, 8 kv heads of 4 query heads, D 128, pages of 16): 64 sequences
-// of 4096 tokens (303 MB) 76 us, 4.0 TB/s of the 6.55 a copy reaches.  About 618
+// of 4096 tokens (303 MB) 75 us, 4.0 TB/s of the 6.55 a copy reaches.  About 600
 // warp instructions per 32 tokens and head keep the issue slots a good half and
 // the ALU pipe 55 to 60 % busy; the copies alone take 59 us, the arithmetic alone
-// 70 to 77.  Without a producing warp (the last warp of a stage refills its slot)
+// about 70.  The pairs of int4_value_pairs cost 4 instructions instead of 5: 76.3
+// -> 74.8.  Without a producing warp (the last warp of a stage refills its slot)
 // 15 us more, with 4 CTAs per SM at 96 registers (which spill) 12 more.  Handing
 // CTAs that end early the last chunks of others, as decode.cuh does, costs one more
 // join per chunk and instructions that the producer has to fetch: 5 us with that
@@ -472,8 +473,8 @@ __global__ void __launch_bounds__(kQ4Threads, MINB)
   auto deposit = [&](bool last) -> bool {
     if (!emptied && !__all_sync(0xffffffffu, mbar_wait(drained, (joins & 1) ^ 1, kWaitLimitNs)))
       return false;
-    // Codes entered as c 2^-24 (even registers of a word), or c 2^-20 and the even
-    // one's code besides (odd ones).  Undone in two steps, as 2^24 / nu passes fp32's range for the largest scales.
+    // Codes entered as c 2^-24 (even ones of a word) or c 2^-20 (odd ones).  Undone in
+    // two steps, as 2^24 / nu passes fp32's range for the largest scales.
     const float down = kHalf ? 1.f : __uint_as_float((254u << 23) - __float_as_uint(nu));
     const float w0 = kHalf ? 1.f : 16777216.f, w1 = kHalf ? 1.f : 1048576.f;
 #pragma unroll
@@ -496,7 +497,11 @@ __global__ void __launch_bounds__(kQ4Threads, MINB)
           // accumulator (tile 4 gi + m, register e + 2 j): element 64 gi + 8 lr + 2 m + j
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
-            if constexpr (!kHalf) {
+            // odd codes entered with the even ones below them
+            if constexpr (kHalf) {
+              acc[gi * 4 + 2 * half + 1][nt][e] -= 0.0625f * acc[gi * 4 + 2 * half][nt][e];
+              acc[gi * 4 + 2 * half + 1][nt][e + 2] -= 0.0625f * acc[gi * 4 + 2 * half][nt][e + 2];
+            } else {
               acc[gi * 4 + 2 * half + 1][nt][e] -= acc[gi * 4 + 2 * half][nt][e];
               acc[gi * 4 + 2 * half + 1][nt][e + 2] -= acc[gi * 4 + 2 * half][nt][e + 2];
             }
