@@ -680,8 +680,11 @@ __global__ void __launch_bounds__(kMaxWarpsPerCta * 32, (PAIR && D == 64 && !TC)
     tbase = *reinterpret_cast<volatile uint32_t*>(tail0 + tc_slot_offset(upc));
   }
   // The reduce grid may be scheduled at once: it waits for this grid to
-  // complete before it reads anything.
-  grid_launch_dependents();
+  // complete before it reads anything.  But the next call's planner may follow
+  // the reduce grid's start and read its lengths before it waits: where this call
+  // writes lengths and tables itself (a selection), only once they are there.
+  const bool selected = p.lens != p.plan_lens;
+  if (!selected) grid_launch_dependents();
   // Heads of length 0 get zeros (an empty state in state mode), matching
   // softmax over zero keys times an empty V in src/kernel_eager.py:51-53.
   // The planner lists them; this runs after the wait for the planner.
@@ -759,6 +762,7 @@ __global__ void __launch_bounds__(kMaxWarpsPerCta * 32, (PAIR && D == 64 && !TC)
     // are independent loads, issued together (wstart has total_warps
     // entries, so the read is in bounds even for a warp that then exits).
     grid_dependency_wait();
+    if (selected) grid_launch_dependents();
     W = *p.weff;  // min(total_warps, total pages), set by the planner
     // Total pages < 2^31 (checked on the host), so page indices are 32-bit.
     total = p.cum[n_heads];

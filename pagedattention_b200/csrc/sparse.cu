@@ -118,6 +118,7 @@ struct SelectParams {
   uint32_t* status;
   int64_t q_sb, q_sh, l_sb, l_sh, bt_sb, bt_sh, bt_si, num_pages;
   int32_t bt_mul, bt_add, B, Hkv, G, bs, maxb, keep, sink, recent, chunk;
+  int32_t chained;     // the decode grid of the same call follows
 };
 
 __device__ __forceinline__ int clamped_length(const SelectParams& p, int s, int h) {
@@ -351,7 +352,9 @@ __global__ void __launch_bounds__(NTH) select_pages_kernel(const SelectParams p)
   __shared__ float sh_size[32];
   __shared__ uint32_t sh_key;
   __shared__ int sh_bin, sh_rank, sh_count, sh_listed;
-  grid_launch_dependents();
+  // The decode grid of the same call waits for the tables; whatever follows a
+  // selection on its own may read its lengths first, so that has to start later.
+  if (p.chained) grid_launch_dependents();
   const int u = blockIdx.x, s = u / p.Hkv, h = u - s * p.Hkv;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int L = clamped_length(p, s, h);
@@ -655,8 +658,8 @@ cudaError_t launch_selection(const pab::SelectParams& p, int D, bool small,
   }
 }
 
-// `pdl`: programmatically dependent on the kernel before it (the planner).
-int launch_select(const pab200_select_args* a, void* scores, bool pdl, cudaStream_t s) {
+// `chained`: between the planner and the decode grid of one call.
+int launch_select(const pab200_select_args* a, void* scores, bool chained, cudaStream_t s) {
   pab::SelectParams p{};
   p.q = a->q;
   p.bounds = a->page_bounds;
@@ -684,6 +687,7 @@ int launch_select(const pab200_select_args* a, void* scores, bool pdl, cudaStrea
   p.keep = a->num_selected;
   p.sink = a->num_sink;
   p.recent = a->num_recent;
+  p.chained = chained;
   const unsigned units = static_cast<unsigned>(p.B * p.Hkv);
   const bool scored = p.maxb > p.keep;
   if (scored) {
@@ -695,7 +699,7 @@ int launch_select(const pab200_select_args* a, void* scores, bool pdl, cudaStrea
     const int chunk = each < 64 ? 64 : (each > 512 ? 512 : static_cast<int>(each));
     p.chunk = chunk;
     const dim3 grid((p.maxb + chunk - 1) / chunk, units);
-    pabh::LaunchCfg sc(grid, dim3(256), 0, s, pdl);
+    pabh::LaunchCfg sc(grid, dim3(256), 0, s, chained);
     const cudaError_t e = a->dtype == PAB200_DTYPE_BF16
                               ? launch_scores<__nv_bfloat16>(p, a->head_size, &sc.cfg)
                               : launch_scores<__half>(p, a->head_size, &sc.cfg);
@@ -705,7 +709,7 @@ int launch_select(const pab200_select_args* a, void* scores, bool pdl, cudaStrea
   // 256 threads while 8 registers hold a thread's keys, so that several units
   // share an SM.
   const bool small = p.maxb <= 2048;
-  pabh::LaunchCfg lc(dim3(units), dim3(small ? 256 : 1024), 0, s, scored || pdl);
+  pabh::LaunchCfg lc(dim3(units), dim3(small ? 256 : 1024), 0, s, scored || chained);
   const cudaError_t err = a->dtype == PAB200_DTYPE_BF16
                               ? launch_selection<__nv_bfloat16>(p, a->head_size, small, &lc.cfg)
                               : launch_selection<__half>(p, a->head_size, small, &lc.cfg);

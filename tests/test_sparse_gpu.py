@@ -371,6 +371,45 @@ def test_captured_ragged_and_sparse_calls(cuda_device):
         assert ((out.float() - full.float()).abs() <= tol).all()
 
 
+def test_selections_used_by_the_next_call(cuda_device):
+    """Tables and lengths of a selection, read by a decode call that follows it at
+    once in a graph, are this replay's, not the last one's."""
+    dt, D, G, Hkv, bs, B, keep = BF, 128, 4, 4, 16, 8, 16
+    g = torch.Generator().manual_seed(13)
+    lens = torch.tensor([900, 16, 0, 333, 1000, 50, 700, 257], dtype=torch.int32)
+    bt, pool = tables(torch.full((B,), 1000, dtype=torch.int32), bs)
+    k, v = (torch.randn((pool, Hkv, bs, D), generator=g).to(dt).to(cuda_device) for _ in range(2))
+    bounds = torch.stack((k.amin(2), k.amax(2)), 2).contiguous()
+    q, ld, btd = torch.zeros((B, G * Hkv, D), dtype=dt, device=cuda_device), lens.to(cuda_device), bt.to(cuda_device)
+    out1, out2, out3 = (torch.empty_like(q) for _ in range(3))
+    res = {}
+
+    def step():
+        res["a"] = pa.select_pages(q, bounds, btd, ld, bs, keep)
+        pa.paged_attention(out1, q, k, v, *res["a"], 0.1, bs)
+        res["b"] = pa.paged_attention_sparse(out2, q, k, v, bounds, btd, ld, 0.1, bs, keep)
+        pa.paged_attention(out3, q, k, v, *res["b"], 0.1, bs)
+
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for i in range(6):
+        qn = torch.randn((B, G * Hkv, D), generator=g).to(dt)
+        q.copy_(qn)
+        lens = lens.roll(1)
+        ld.copy_(lens)
+        graph.replay()
+        torch.cuda.synchronize()
+        want, wl = expect_select(qn, bounds.cpu().view(-1, 2, D), bt, lens, bs, keep, 1, 1, Hkv, False)
+        for t, n in res.values():
+            assert torch.equal(t.cpu(), want) and torch.equal(n.cpu(), wl)
+        full = torch.empty_like(q)
+        pa.paged_attention(full, q, k, v, want.to(cuda_device), wl.to(cuda_device), 0.1, bs)
+        assert torch.equal(out1, full) and torch.equal(out3, full)
+
+
 def test_serving_steps_together(cuda_device):
     """Prompts and steps: bounds, 4-bit append, selection and 4-bit attention
     over the selection, eager and then replayed from a graph."""
