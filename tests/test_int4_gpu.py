@@ -456,6 +456,59 @@ def test_attention_many_heads(cuda_device, dt):
     check_attention(out, q, kp, vp, bt, lens, 0.125, bs, Hkv, dt, per_head_pages=True)
 
 
+@pytest.mark.parametrize("dt", [BF, HF])
+def test_states_of_two_ranges(cuda_device, dt):
+    """The C entry's state outputs: attention and log-sum-exp of a range; two
+    ranges of a context merge to the whole."""
+    D, G, Hkv, bs, B, scale = 128, 4, 2, 16, 3, 0.08
+    g = torch.Generator().manual_seed(14)
+    lens = torch.tensor([3000, 0, 40], dtype=torch.int32)
+    bt, pool = tables(lens, bs)
+    kp = random_pages(pool * Hkv, D, bs, dt, g, False)
+    vp = random_pages(pool * Hkv, D, bs, dt, g, True)
+    q = torch.randn((B, G * Hkv, D), generator=g).to(dt)
+    qd = q.to(cuda_device)
+    kc, vc = (torch.from_numpy(p).view(pool, Hkv, -1).to(cuda_device) for p in (kp, vp))
+    lib = _lib.load()
+    cut = 32                                     # pages of the first range
+    parts = [(bt[:, :cut].contiguous(), lens.clamp(max=cut * bs)),
+             (bt[:, cut:].contiguous(), (lens - cut * bs).clamp(min=0))]
+    rows, states = B * G * Hkv, []
+    for table, ln in parts:
+        td, ld = table.to(cuda_device), ln.to(cuda_device)
+        o = torch.full((rows, D), 9.0, device=cuda_device)
+        lse = torch.full((rows,), 9.0, device=cuda_device)
+        a = _lib.DecodeArgs(
+            None, qd.data_ptr(), kc.data_ptr(), vc.data_ptr(), ld.data_ptr(), td.data_ptr(),
+            0 if dt == BF else 1, _lib.LAYOUT_PAGES, B, G * Hkv, Hkv, D, bs, table.shape[1],
+            pool * Hkv, G * Hkv * D, D, 0, 0, 1, 0, table.shape[1], 0, 1, Hkv, 1, scale, 0)
+        a.state_o, a.state_lse = o.data_ptr(), lse.data_ptr()
+        need = lib.pab200_decode_int4_workspace_size(a)
+        ws = torch.empty(need, dtype=torch.uint8, device=cuda_device)
+        st = torch.cuda.current_stream().cuda_stream
+        assert lib.pab200_decode_int4(a, ws.data_ptr(), need, st) == 0
+        states.append((o.view(B, G * Hkv, D), lse.view(B, G * Hkv)))
+        torch.cuda.synchronize()
+        check_attention(states[-1][0], q, kp, vp, table, ln, scale, bs, Hkv, dt)
+        kv = op.get_rows(kp, D, bs, dt, False)
+        for s in range(B):
+            for h in range(G * Hkv):
+                n = int(ln[s])
+                got = float(states[-1][1][s, h])
+                if n == 0:
+                    assert got == -math.inf
+                    continue
+                k = np.concatenate([kv[int(e) * Hkv + h // G] for e in table[s, :(n + bs - 1) // bs]])[:n]
+                sc = k @ q[s, h].double().numpy() * scale
+                want = sc.max() + math.log(np.exp(sc - sc.max()).sum())
+                # scores: as in check_attention; the sum and its logarithm: 2^-18
+                size = np.abs(q[s, h].double().numpy()) @ np.abs(k).max(0) * scale
+                assert abs(got - want) <= 128 * 2.0 ** -24 * 2 * size + 2.0 ** -18 * (1 + abs(want))
+    out = pa.merge_states(torch.stack([o for o, _ in states]), torch.stack([l for _, l in states]),
+                          out_dtype=dt)
+    check_attention(out.view_as(q), q, kp, vp, bt, lens, scale, bs, Hkv, dt)
+
+
 def test_attention_per_head_pages_and_bad_ids(cuda_device):
     """Reference page layout with lengths per head; pages out of range read as zeros."""
     dt, D, G, Hkv, bs = BF, 128, 4, 3, 16

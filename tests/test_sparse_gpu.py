@@ -295,6 +295,12 @@ def test_sparse_attention(cuda_device, dt, D, G, Hkv, bs, lens, keep, layout):
     assert ((out.float() - full.float()).abs() <= tol).all()
 
 
+def test_sparse_attention_on_the_tcgen05_kernel(cuda_device, monkeypatch):
+    """The opt-in decode kernel takes a selection's tables too."""
+    monkeypatch.setenv("PAB200_TC", "1")
+    test_sparse_attention(cuda_device, BF, 64, 32, 1, 16, [900, 0, 40, 333], 12, "HND")
+
+
 def test_captured_ragged_and_sparse_calls(cuda_device):
     """A chunk of a prompt (bounds, append, read-back) and a page-sparse decode in
     two graphs, replayed in turn on two streams while their inputs change."""
