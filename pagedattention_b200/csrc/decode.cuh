@@ -768,6 +768,7 @@ __global__ void __launch_bounds__(kMaxWarpsPerCta * 32, (PAIR && D == 64 && !TC)
     total = p.cum[n_heads];
     first_head = gw < p.total_warps ? p.wstart[gw] : 0;
     const int4 steal = *reinterpret_cast<const int4*>(p.steal);
+    if (gw >= W) first_head = 0;  // the planner wrote nothing there
     sm_m = steal.x;
     sm_k = steal.y;
     zero_empty_heads();

@@ -298,6 +298,8 @@ def test_sparse_attention(cuda_device, dt, D, G, Hkv, bs, lens, keep, layout):
 def test_sparse_attention_on_the_tcgen05_kernel(cuda_device, monkeypatch):
     """The opt-in decode kernel takes a selection's tables too."""
     monkeypatch.setenv("PAB200_TC", "1")
+    # freed: workspaces that come from here are not zero
+    torch.full((64 << 20,), 0x7f, dtype=torch.uint8, device=cuda_device)
     test_sparse_attention(cuda_device, BF, 64, 32, 1, 16, [900, 0, 40, 333], 12, "HND")
 
 
