@@ -461,8 +461,8 @@ __global__ void __launch_bounds__(NTH) select_pages_kernel(const SelectParams p)
       __syncthreads();
       rank = sh_rank;
       lo += static_cast<uint32_t>(sh_bin) << shift;
-      const uint32_t last = lo + ((1u << shift) - 1u);
-      hi = last < hi ? last : hi;
+      const uint32_t span = (1u << shift) - 1u;  // lo + span may pass the largest key
+      if (hi - lo > span) hi = lo + span;
       const int count = sh_count;
       if (lo < hi && count <= NTH) {
         walk([&](uint32_t x) {
@@ -579,7 +579,8 @@ __global__ void __launch_bounds__(NTH) select_pages_kernel(const SelectParams p)
         take = y > lo || (y == lo && ties-- > 0);
       }
     }
-    if (take) out[p.sink + at++] = bt[(c0 + i) * p.bt_si];
+    // exactly k are taken; the bound keeps a unit inside its table all the same
+    if (take && at < k) out[p.sink + at++] = bt[(c0 + i) * p.bt_si];
   }
 }
 

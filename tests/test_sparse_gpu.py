@@ -178,6 +178,72 @@ def test_select_ties_nan_and_bad_pages(cuda_device):
         assert torch.equal(out.cpu(), wl) and torch.equal(tabs.cpu(), want)
 
 
+def select_within_guards(cuda_device, q, bounds, bt, lens, bs, keep, Hkv):
+    """The C entry's tables and lengths, with words before and behind them that
+    no unit may touch."""
+    B, Hq, D = q.shape
+    lib = _lib.load()
+    qd, bd, btd, ld = (x.to(cuda_device) for x in (q, bounds, bt, lens))
+    units, guard = B * Hkv, 4096
+    tabs = torch.full((units * keep + 2 * guard,), 77, dtype=torch.int32, device=cuda_device)
+    out = torch.full((units + 2 * guard,), 77, dtype=torch.int32, device=cuda_device)
+    status = torch.zeros(1, dtype=torch.int32, device=cuda_device)
+    a = _lib.SelectArgs(
+        qd.data_ptr(), bd.data_ptr(), ld.data_ptr(), btd.data_ptr(), tabs[guard:].data_ptr(),
+        out[guard:].data_ptr(), status.data_ptr(), 0 if q.dtype == BF else 1, B, Hq, Hkv, D, bs,
+        bt.shape[1], keep, 1, 1, bounds.shape[0], Hq * D, D, 1, 0, bt.shape[1], 0, 1, Hkv, 1)
+    need = lib.pab200_select_pages_workspace_size(a)
+    ws = torch.empty(need, dtype=torch.uint8, device=cuda_device)
+    assert lib.pab200_select_pages(a, ws.data_ptr(), need, torch.cuda.current_stream().cuda_stream) == 0
+    tabs, out = tabs.cpu(), out.cpu()
+    for x in (tabs, out):
+        assert (x[:guard] == 77).all() and (x[-guard:] == 77).all()
+    return tabs[guard:-guard].view(B, Hkv, keep), out[guard:-guard].view(B, Hkv), int(status[0])
+
+
+@pytest.mark.parametrize("n,nans,keep", [
+    (300, 100, 32),        # more NaN pages than places
+    (300, 299, 32), (700, 500, 64),
+    (2500, 1000, 256),     # 1,024 threads: more open pages than are compared directly
+    (2500, 2, 4), (700, 65, 64),
+])
+def test_select_many_nan_pages(cuda_device, n, nans, keep):
+    """NaN pages beyond the free places: the earlier ones are kept, and neither the
+    recent pages nor another unit's table nor anything behind the last is written."""
+    dt, D, G, Hkv, bs, B = BF, 64, 2, 2, 8, 3
+    g = torch.Generator().manual_seed(n + nans)
+    pool = B * n
+    x = torch.randn((pool * Hkv, 2, D), generator=g).to(dt)
+    bounds = torch.stack((x.amin(1), x.amax(1)), 1)
+    bt = torch.randperm(pool, generator=g).to(torch.int32).view(B, n)
+    for s in range(B - 1):                        # the last sequence has none
+        for h in range(Hkv):
+            at = torch.randperm(n, generator=g)[:nans]
+            bounds[bt[s, at].long() * Hkv + h, :, 3] = float("nan")
+    q = torch.randn((B, G * Hkv, D), generator=g).to(dt)
+    lens = torch.full((B,), n * bs - 1, dtype=torch.int32)
+    tabs, out, status = select_within_guards(cuda_device, q, bounds, bt, lens, bs, keep, Hkv)
+    want, wl = expect_select(q, bounds, bt, lens, bs, keep, 1, 1, Hkv, False)
+    assert status == 0 and torch.equal(out, wl) and torch.equal(tabs, want)
+
+
+@pytest.mark.parametrize("n,keep", [(300, 32), (2500, 256)])
+def test_select_nan_query_and_a_bad_page(cuda_device, n, keep):
+    """A NaN in the query makes every page NaN but the one whose id is out of range."""
+    dt, D, G, Hkv, bs, B = HF, 64, 2, 1, 8, 2
+    g = torch.Generator().manual_seed(n)
+    x = torch.randn((B * n, 2, D), generator=g).to(dt)
+    bounds = torch.stack((x.amin(1), x.amax(1)), 1)
+    bt = torch.randperm(B * n, generator=g).to(torch.int32).view(B, n)
+    bt[0, 5] = -1
+    q = torch.randn((B, G, D), generator=g).to(dt)
+    q[0, 1, 7] = float("nan")
+    lens = torch.full((B,), n * bs, dtype=torch.int32)
+    tabs, out, status = select_within_guards(cuda_device, q, bounds, bt, lens, bs, keep, Hkv)
+    want, wl = expect_select(q, bounds, bt, lens, bs, keep, 1, 1, Hkv, False)
+    assert status == _lib.STATUS_BAD_PAGE_ID and torch.equal(out, wl) and torch.equal(tabs, want)
+
+
 @pytest.mark.parametrize("dt,n,keep,spread", [
     (BF, 3000, 700, 0.0),      # all alike but one page in seven: only the order decides
     (HF, 5000, 1200, 2.0 ** -22), (BF, 9000, 40, 2.0 ** -20), (HF, 600, 300, 2.0 ** -24)])
