@@ -297,6 +297,13 @@ __device__ __forceinline__ float key_score(uint32_t k) {
   return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k);
 }
 
+// The larger of two numbers, NaN if either is.
+__device__ __forceinline__ float fmax_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
 // Sums of x.x and of x.y over the block's threads before this one, and the
 // totals (`warp_sum` is free again after the next barrier).
 template <int NTH>
@@ -398,12 +405,11 @@ __global__ void __launch_bounds__(NTH) select_pages_kernel(const SelectParams p)
     if (i < kHeld) keys[i + (i >> 5)] = key;
     lo = min(lo, key);
     hi = max(hi, key);
-    size = x.y <= size ? size : x.y;  // a NaN is kept
+    size = fmax_nan(size, x.y);
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
-    const float z = __shfl_xor_sync(0xffffffffu, size, o);
-    size = z <= size ? size : z;
+    size = fmax_nan(size, __shfl_xor_sync(0xffffffffu, size, o));
   }
   if (lane == 0) sh_size[warp] = size;
   // This thread's pages, in order, with their keys.
@@ -488,7 +494,7 @@ __global__ void __launch_bounds__(NTH) select_pages_kernel(const SelectParams p)
       }
     }
     if (exact) break;
-    for (int w = 0; w < NTH / 32; ++w) size = sh_size[w] <= size ? size : sh_size[w];
+    for (int w = 0; w < NTH / 32; ++w) size = fmax_nan(size, sh_size[w]);
     const float t = key_score(lo), e2 = 2.f * (size * kScoreError + 1e-37f);
     sure = e2 <= 3e38f && t == t;
     if (sure) {

@@ -244,6 +244,28 @@ def test_select_nan_query_and_a_bad_page(cuda_device, n, keep):
     assert status == _lib.STATUS_BAD_PAGE_ID and torch.equal(out, wl) and torch.equal(tabs, want)
 
 
+@pytest.mark.parametrize("threads", [256, 1024])
+def test_select_nan_pages_after_large_terms(cuda_device, threads):
+    """Scores that only 64 bits tell apart (large terms that cancel), read before
+    NaN pages and those before small ones: the NaNs hide none of the sizes."""
+    dt, D, G, bs = BF, 64, 1, 8
+    g = torch.Generator().manual_seed(threads)
+    n, keep = 3 * threads + 2, threads + threads // 2 + 2
+    rows = torch.zeros((n, D))
+    first = rows[1:1 + threads]
+    first[:, 0], first[:, 63] = 4096.0, -4096.0
+    first[:, 1:63] = torch.randint(-64, 65, (threads, 62), generator=g) * 2.0 ** -18
+    rows[1 + threads:1 + 2 * threads] = float("nan")
+    rows[1 + 2 * threads:-1, 0] = -1.0
+    bounds = rows[:, None].expand(n, 2, D).to(dt).contiguous()
+    q = torch.ones((1, G, D), dtype=dt)
+    bt = torch.arange(n, dtype=torch.int32)[None].contiguous()
+    lens = torch.tensor([n * bs], dtype=torch.int32)
+    tabs, out, _ = select_within_guards(cuda_device, q, bounds, bt, lens, bs, keep, 1)
+    want, wl = expect_select(q, bounds, bt, lens, bs, keep, 1, 1, 1, False)
+    assert torch.equal(out, wl) and torch.equal(tabs, want)
+
+
 @pytest.mark.parametrize("dt,n,keep,spread", [
     (BF, 3000, 700, 0.0),      # all alike but one page in seven: only the order decides
     (HF, 5000, 1200, 2.0 ** -22), (BF, 9000, 40, 2.0 ** -20), (HF, 600, 300, 2.0 ** -24)])
