@@ -480,7 +480,7 @@ typedef struct pab200_select_args {
  * the highest score
  *   u(page) = sum_g sum_d max(q[g, d] * min[d], q[g, d] * max[d]),
  * g over the kv head's query group: no token of the page has a larger sum of
- * raw scores.  Scores are those of a sum in 64 bits, rounded to fp32; equal scores
+ * raw scores (0 times an infinite bound is NaN).  Scores are those of a sum in 64 bits, rounded to fp32; equal scores
  * go to the lower page, a score that is NaN ranks first, a page id out of range
  * last.  tables[s, h] receives the block-table entries of the kept pages in
  * ascending page order (-1 behind them) and selected_lens[s, h] the number of

@@ -127,9 +127,10 @@ __device__ __forceinline__ int clamped_length(const SelectParams& p, int s, int 
   return L < 0 ? 0 : (L > cap ? static_cast<int>(cap) : L);
 }
 
-// A page's score is the sum over the head elements of max * (sum of the group's
-// positive query parts) + min * (sum of the negative ones), the upper bound of
-// the group's summed scores; by definition in 64 bits, rounded to fp32.  Which
+// A page's score is the sum over the group and the head elements of max(q * min,
+// q * max), the upper bound of the group's summed scores; by definition in 64 bits,
+// rounded to fp32.  Where nothing is infinite that is the sum over the elements of
+// max * (sum of the group's positive query parts) + min * (sum of the negative ones).  Which
 // pages rank next to the border must not hang on the order of an fp32 sum, but
 // 64-bit conversions and sums bound the kernel (24,400 pages of 8 kv heads, D
 // 128: 100 MB of bounds, 15 us at a copy's rate; 36 to 40 us in 64 bits, 26 as
@@ -270,10 +271,33 @@ __global__ void __launch_bounds__(256, 4) page_scores_kernel(const SelectParams 
   grid_dependency_wait();
 }
 
-// The score of page `pid` by its definition, in every lane of a warp; `qs`: the
-// query's parts in 64 bits.
+// Sum over the lanes of a warp, in every lane.
+__device__ __forceinline__ double warp_sum(double a) {
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
+  return a;
+}
+
+// The score of bounds `b` term by term, for infinities: the query's parts would
+// multiply an infinite bound that the maximum leaves aside by 0.  NaN where a
+// query element of 0 meets an infinite bound.
 template <typename T, int D>
-__device__ __forceinline__ float exact_score(const SelectParams& p, int64_t pid, const double* qs) {
+__device__ __noinline__ float term_score(const SelectParams& p, const T* q, const T* b) {
+  double a = 0.0;
+  for (int d = threadIdx.x & 31; d < D; d += 32)
+    for (int g = 0; g < p.G; ++g) {
+      const double x = static_cast<float>(q[g * p.q_sh + d]);
+      const double u = x * static_cast<float>(b[d]), v = x * static_cast<float>(b[D + d]);
+      a += u != u || v != v ? u + v : (u > v ? u : v);
+    }
+  return static_cast<float>(warp_sum(a));
+}
+
+// The score of page `pid` by its definition, in every lane of a warp; `q`: the
+// group's queries, `qs`: their parts in 64 bits.
+template <typename T, int D>
+__device__ __forceinline__ float exact_score(const SelectParams& p, int64_t pid, const T* q,
+                                             const double* qs) {
   if (pid < 0 || pid >= p.num_pages) return -INFINITY;
   const T* b = static_cast<const T*>(p.bounds) + pid * (2 * D);
   double a = 0.0;
@@ -281,8 +305,9 @@ __device__ __forceinline__ float exact_score(const SelectParams& p, int64_t pid,
     a = fma(static_cast<double>(static_cast<float>(b[D + d])), qs[d], a);
     a = fma(static_cast<double>(static_cast<float>(b[d])), qs[D + d], a);
   }
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
+  a = warp_sum(a);
+  // finite 16-bit bounds and queries have a sum far inside 64 bits' range
+  if (!(fabs(a) <= 1e300)) return term_score<T, D>(p, q, b);
   return static_cast<float>(a);
 }
 
@@ -370,8 +395,8 @@ __global__ void __launch_bounds__(NTH) select_pages_kernel(const SelectParams p)
   const int32_t* bt = p.bt + s * p.bt_sb + h * p.bt_sh;
   int32_t* out = p.tables + static_cast<int64_t>(u) * p.keep;
   hist[tid] = 0;
+  const T* q = static_cast<const T*>(p.q) + s * p.q_sb + static_cast<int64_t>(h) * p.G * p.q_sh;
   if (n > p.keep) {  // the query's parts, while the scores are still summed
-    const T* q = static_cast<const T*>(p.q) + s * p.q_sb + static_cast<int64_t>(h) * p.G * p.q_sh;
     for (int d = tid; d < D; d += NTH) {
       const double2 x = query_parts<T>(p, q, d);
       qs[d] = x.x;
@@ -528,7 +553,7 @@ __global__ void __launch_bounds__(NTH) select_pages_kernel(const SelectParams p)
       if (opened > NTH && !open(key_of(i))) continue;
       const int64_t pid = static_cast<int64_t>(bt[(c0 + i) * p.bt_si]) * p.bt_mul +
                           static_cast<int64_t>(h) * p.bt_add;
-      const float x = exact_score<T, D>(p, pid, qs);
+      const float x = exact_score<T, D>(p, pid, q, qs);
       if (lane == 0) {
         if (few)
           list[kFew + j] = score_key(x);

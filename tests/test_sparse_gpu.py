@@ -310,6 +310,38 @@ def test_select_infinite_bounds(cuda_device):
     assert torch.equal(out.cpu(), wl) and torch.equal(tabs.cpu(), want)
 
 
+@pytest.mark.parametrize("n", [300, 2500])
+@pytest.mark.parametrize("dt", [BF, HF])
+def test_select_infinite_bounds_by_definition(cuda_device, dt, n):
+    """max(q min, q max) of an infinite bound: the finite product where the infinite
+    one is the smaller, NaN only where the query is 0."""
+    D, bs, G, keep = 64, 8, 3, 40
+    g = torch.Generator().manual_seed(n)
+    x = torch.randn((n, 2, D), generator=g).to(dt)
+    bounds = torch.stack((x.amin(1), x.amax(1)), 1)
+    inf = float("inf")
+    q = torch.randn((4, G, D), generator=g).to(dt)
+    q[:, :, 5], q[:, :, 6] = q[:, :, 5].abs() + 0.1, -q[:, :, 6].abs() - 0.1
+    q[1, 1, 5] = 0.0                              # 0 * inf
+    q[2, :, 5] = torch.tensor([inf, 1.0, 2.0])    # an infinite query
+    q[3, 1, 9] = -0.0
+    for i in range(20, 40):
+        bounds[i, 0, 5] = -inf
+        bounds[i + 50, 1, 6] = inf
+    bounds[100, 1, 5] = inf                       # ranks first
+    bounds[101, 0, 6] = -inf
+    bounds[102, :, 5] = -inf                      # ranks last
+    bounds[103, 0, 9] = -inf
+    bounds[104, 1, 9] = 0.0
+    bt = torch.randperm(n, generator=g).to(torch.int32)[None].expand(4, n).contiguous()
+    lens = torch.full((4,), n * bs - 1, dtype=torch.int32)
+    tabs, out, _ = select_within_guards(cuda_device, q, bounds, bt, lens, bs, keep, 1)
+    with np.errstate(invalid="ignore"):          # 0 * inf, inf - inf
+        want, wl = expect_select(q, bounds, bt, lens, bs, keep, 1, 1, 1, False)
+    for s in range(4):
+        assert torch.equal(out[s], wl[s]) and torch.equal(tabs[s], want[s]), s
+
+
 def test_select_lengths_out_of_range(cuda_device):
     dt, D, bs = HF, 64, 8
     g = torch.Generator().manual_seed(0)
