@@ -358,8 +358,8 @@ __global__ void __launch_bounds__(256) int4_read_kernel(const Int4ReadParams p, 
   const int64_t column = h * p.o_sh + e * 8;
   if (p.zero_rest && m.cu) {
     // Slots past the last sequence's: rows from cu[B]; the slots before the
-    // first sequence's: rows up to cu[0].
-    const int first = m.cu[0], last = max(m.cu[m.B], 0);
+    // first sequence's: rows up to cu[0].  Without sequences all rows lie behind.
+    const int first = m.cu[0], last = m.B > 0 ? max(m.cu[m.B], 0) : 0;
     const int past = slot - ((last >> k) + 2 * m.B);
     const int64_t z0 = (past >= 0 ? last : 0) + (static_cast<int64_t>(past >= 0 ? past : slot) << k);
     const int64_t z1 = past >= 0 ? m.num_tokens : min(first, m.num_tokens);
@@ -432,8 +432,13 @@ namespace {
 using pabh::aligned;
 using pabh::fail;
 
+// Whether a call has rows to write; `rest`: rows of no sequence too.
+bool any_rows(const pab200_int4_rows_args* a, bool rest) {
+  return a->num_tokens > 0 && (a->num_seqs > 0 || rest);
+}
+
 // The checks that append and read-back share; fills the token map.
-int check_int4(const pab200_int4_rows_args* a, pab::TokenMap* m) {
+int check_int4(const pab200_int4_rows_args* a, pab::TokenMap* m, bool rest) {
   if (!a) return fail(PAB200_ERR_INVALID_ARGUMENT, "args is null");
   if (a->dtype != PAB200_DTYPE_BF16 && a->dtype != PAB200_DTYPE_F16)
     return fail(PAB200_ERR_UNSUPPORTED, "dtype %d: rows must be bf16 or f16", a->dtype);
@@ -455,10 +460,11 @@ int check_int4(const pab200_int4_rows_args* a, pab::TokenMap* m) {
           (int64_t(1) << 31))
     return fail(PAB200_ERR_UNSUPPORTED,
                 "max_blocks*block_size, or num_tokens*num_kv_heads/8, too large (>= 2^31)");
-  if (a->num_seqs == 0 || a->num_tokens == 0) return PAB200_OK;
-  if (!a->k_rows || !a->v_rows || !a->seqlens)
+  if (!any_rows(a, rest)) return PAB200_OK;
+  const bool seqs = a->num_seqs > 0;
+  if (!a->k_rows || !a->v_rows || (seqs && !a->seqlens))
     return fail(PAB200_ERR_INVALID_ARGUMENT, "k_rows, v_rows or seqlens is null");
-  if (a->max_blocks > 0 && a->num_pages > 0 && (!a->k_cache || !a->v_cache || !a->block_table))
+  if (seqs && a->max_blocks > 0 && a->num_pages > 0 && (!a->k_cache || !a->v_cache || !a->block_table))
     return fail(PAB200_ERR_INVALID_ARGUMENT, "k_cache, v_cache or block_table is null");
   if (!aligned(a->k_cache, 16) || !aligned(a->v_cache, 16))
     return fail(PAB200_ERR_ALIGNMENT, "k_cache and v_cache must be 16-byte aligned");
@@ -545,8 +551,8 @@ PAB200_EXPORT size_t pab200_int4_page_bytes(int32_t head_size, int32_t block_siz
 PAB200_EXPORT int pab200_kv_append_int4(const pab200_int4_rows_args* a, int32_t increment,
                                         void* stream) {
   pab::Int4AppendParams p{};
-  const int rc = check_int4(a, &p.map);
-  if (rc || a->num_seqs == 0 || a->num_tokens == 0) return rc;
+  const int rc = check_int4(a, &p.map, false);
+  if (rc || !any_rows(a, false)) return rc;
   p.cache[0] = static_cast<uint8_t*>(a->k_cache);
   p.cache[1] = static_cast<uint8_t*>(a->v_cache);
   p.rows[0] = a->k_rows;
@@ -575,8 +581,8 @@ PAB200_EXPORT int pab200_kv_append_int4(const pab200_int4_rows_args* a, int32_t 
 PAB200_EXPORT int pab200_kv_read_int4(const pab200_int4_rows_args* a, const int32_t* starts,
                                       int64_t starts_stride, int32_t zero_rest, void* stream) {
   pab::Int4ReadParams p{};
-  const int rc = check_int4(a, &p.map);
-  if (rc || a->num_seqs == 0 || a->num_tokens == 0) return rc;
+  const int rc = check_int4(a, &p.map, zero_rest != 0);
+  if (rc || !any_rows(a, zero_rest != 0)) return rc;
   if (!rows_vec(a))
     return fail(PAB200_ERR_ALIGNMENT, "rows must be 16-byte aligned with strides that are multiples of 8");
   p.cache[0] = static_cast<const uint8_t*>(a->k_cache);

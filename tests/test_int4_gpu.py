@@ -288,6 +288,24 @@ def test_read_rows_of_no_sequence(cuda_device, cu, N):
         assert (err <= (half_step(dt) + 2.0 ** -23) * want.abs() + 1e-8).all()
 
 
+@pytest.mark.parametrize("N,first", [(1, 0), (9, 0), (70, 3), (70, 70)])
+@pytest.mark.parametrize("bs", [8, 16])
+def test_read_of_an_empty_batch(cuda_device, N, first, bs):
+    """Without sequences every row is a row of no sequence."""
+    dt, D, Hkv = BF, 64, 3
+    kc, vc = pa.int4_cache(2, Hkv, bs, D, device=cuda_device)
+    lens = torch.zeros(0, dtype=torch.int32, device=cuda_device)
+    bt = torch.zeros((0, 4), dtype=torch.int32, device=cuda_device)
+    cu = torch.full((1,), first, dtype=torch.int32, device=cuda_device)
+    x = torch.full((2, N, Hkv, D), 7.0, dtype=dt, device=cuda_device)
+    del x                                          # freed: the memory is not zero
+    k, v = pa.kv_read_int4(kc, vc, bt, lens, bs, D, dt, cu_out=cu, num_tokens=N)
+    assert k.shape == v.shape == (N, Hkv, D) and not k.any() and not v.any()
+    out = tuple(torch.full((N, Hkv, D), 7.0, dtype=dt, device=cuda_device) for _ in range(2))
+    pa.kv_read_int4(kc, vc, bt, lens, bs, D, dt, cu_out=cu, out=out)
+    assert (out[0] == 7.0).all() and (out[1] == 7.0).all()
+
+
 # --------------------------------------------------------------- attention
 
 def check_attention(got, q, kp, vp, bt, lens, scale, bs, Hkv, dt, per_head_pages=False):
