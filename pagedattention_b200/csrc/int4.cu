@@ -380,7 +380,7 @@ __global__ void __launch_bounds__(256) int4_read_kernel(const Int4ReadParams p, 
   const int a = start > pos0 ? static_cast<int>(start - pos0) : 0;  // its rows: [a, end)
   const int end = over < run ? static_cast<int>(over) : run;
   const int64_t left = L - pos0;
-  const int have = left < end ? static_cast<int>(left) : end;  // rows from here on hold no token
+  const int have = left < 0 ? 0 : (left < end ? static_cast<int>(left) : end);  // rows from here on hold no token
   uint32_t flags = 0;
   int64_t pid = -1;
   if (pos0 >= 0 && a < have) {

@@ -306,6 +306,23 @@ def test_read_of_an_empty_batch(cuda_device, N, first, bs):
     assert (out[0] == 7.0).all() and (out[1] == 7.0).all()
 
 
+@pytest.mark.parametrize("length,start", [(-2 ** 31, 16), (-1, 0), (0, 2 ** 31 - 8), (24, 2 ** 31 - 8)])
+def test_read_lengths_and_starts_at_the_ends_of_int32(cuda_device, length, start):
+    """Positions past every length read as zeros, however far."""
+    dt, D, bs, Hkv = HF, 64, 8, 1
+    g = torch.Generator().manual_seed(5)
+    kc, vc = (torch.from_numpy(random_pages(4, D, bs, dt, g, val)).view(4, 1, -1).to(cuda_device)
+              for val in (False, True))
+    bt = torch.arange(4, dtype=torch.int32, device=cuda_device)[None]
+
+    def mk(*x):
+        return torch.tensor(x, dtype=torch.int32, device=cuda_device)
+
+    k, v = pa.kv_read_int4(kc, vc, bt, mk(length), bs, D, dt, starts=mk(start), cu_out=mk(0, 24),
+                           num_tokens=24)
+    assert not k.any() and not v.any()
+
+
 # --------------------------------------------------------------- attention
 
 def check_attention(got, q, kp, vp, bt, lens, scale, bs, Hkv, dt, per_head_pages=False):
