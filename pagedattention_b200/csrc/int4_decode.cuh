@@ -16,21 +16,23 @@
 //   * Keys enter the MMA as fp16 subnormals, the nibbles as they stand (one
 //     mask per pair); the query is brought to fp16 by a power of two per head,
 //     which loses nothing of a bf16 or fp16 query that matters, and the score is
-//     scaled back in fp32.  Values are widened to c - 8 in T.
+//     scaled back in fp32.
 //   * Scales and minima never touch the codes: the keys' multiply the partial
 //     scores of their group, the values' scale multiplies the probability, which
 //     is rounded to fp16 once, and the rest of the value is summed apart in fp32.
+//     The scales carry a power of two that follows the largest scale seen, so that
+//     the fp16 product keeps its bits for small values and unlikely tokens, and
+//     stays in range for bf16's scales (products of probability and scale more than
+//     2^24 below the largest scale lose bits).
 //     How the values' codes enter depends on T.
 //     fp16: as c - 8, so that the rounding of p s is multiplied by s (c - 8), about
 //     |x|, not by s c, about the group's range: the output keeps fp16's 11 bits.
 //     bf16: as they stand, like the keys': an fp16 p s is eight times finer than
 //     the bf16 output needs, and than a bf16 p s (error against 64 bits 0.0017,
 //     0.0023 with bf16 c - 8; 4 contexts of 32768 to 131072 tokens 3 us less of 111).
-//     Its scales reach past fp16, so they carry a power of two that follows the
-//     largest scale seen (values whose scale lies more than 2^27 below that lose
-//     bits); and since sums of codes >= 0 only grow, and the tensor cores cut
-//     their fp32 sums short, the accumulators are emptied into shared memory every
-//     kFlush chunks of 32 tokens.
+//     Since sums of codes >= 0 only grow, and the tensor cores cut their fp32 sums
+//     short, the accumulators are emptied into shared memory every kFlush chunks of
+//     32 tokens.
 //   * The softmax's reference point moves only when a score exceeds it by
 //     kRaise (log2 units): no shuffles or rescaling in most stages.
 // At the end of a head (or of the CTA's part of it) the consumers' states are
@@ -86,11 +88,10 @@ __global__ void __launch_bounds__(kQ4Threads, MINB)
   constexpr int MT = 2;                        // 16-token tiles per chunk
   constexpr int STAGE_BYTES = q4_stage_bytes(D), KV_BYTES = STAGE_BYTES / 2;
   // Probability x scale must stay below 65504, a probability stays below
-  // 2^kRaise = 7.46.  fp16: scales reach 2 * 65504 / 15, and the reference point
-  // lies kBelow under the maximum it was set to, a few binades further above
-  // fp16's subnormals for small scales.  bf16: scales are brought to 2^13 at most.
+  // 2^kRaise = 7.46, and scales are brought to 2^13 at most (fp16's largest, 2 *
+  // 65504 / 15, stay as they are).
   constexpr bool kHalf = std::is_same<T, __half>::value;
-  constexpr float kBelow = kHalf ? 1.4f : 0.f, kRaise = 2.9f;
+  constexpr float kRaise = 2.9f;
   constexpr int kFlush = 32;  // bf16: chunks between two emptyings of the accumulators
   // Reference point of an empty state: below every score, and finite, so that
   // a score of -inf has probability 0.
@@ -375,8 +376,8 @@ __global__ void __launch_bounds__(kQ4Threads, MINB)
   float qsum[NT][NG][2];   // scale_log2 x sum of the query over a group, heads 2 lc + e
   float qmul[NT][2];       // what a sum of (query x code) products is multiplied by
   float acc[KS][NT][4], mid[NT][NG][2], m_ref[NT][2], l_sum[NT][2];
-  // bf16: the scales' power of two, the largest scale it allows; chunks since the
-  // accumulators were emptied, and the reference points then (`emptied`: there
+  // The scales' power of two and the largest scale it allows.  bf16: chunks since
+  // the accumulators were emptied, and the reference points then (`emptied`: there
   // is something in shared memory).
   float nu = 1.f, s_lim = -1.f, m_then[NT][2];
   int chunks = 0;
@@ -473,9 +474,9 @@ __global__ void __launch_bounds__(kQ4Threads, MINB)
   auto deposit = [&](bool last) -> bool {
     if (!emptied && !__all_sync(0xffffffffu, mbar_wait(drained, (joins & 1) ^ 1, kWaitLimitNs)))
       return false;
-    // Codes entered as c 2^-24 (even ones of a word) or c 2^-20 (odd ones).  Undone in
-    // two steps, as 2^24 / nu passes fp32's range for the largest scales.
-    const float down = kHalf ? 1.f : __uint_as_float((254u << 23) - __float_as_uint(nu));
+    // bf16: codes entered as c 2^-24 (even ones of a word) or c 2^-20 (odd ones).
+    // Undone in two steps, as 2^24 / nu passes fp32's range for the largest scales.
+    const float down = __uint_as_float((254u << 23) - __float_as_uint(nu));
     const float w0 = kHalf ? 1.f : 16777216.f, w1 = kHalf ? 1.f : 1048576.f;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
@@ -688,7 +689,7 @@ __global__ void __launch_bounds__(kQ4Threads, MINB)
             m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
             m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
             m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
-            const float mn = fmaxf(m_ref[nt][e], m - kBelow);
+            const float mn = fmaxf(m_ref[nt][e], m);
             const float alpha = fast_exp2(m_ref[nt][e] - mn);
             m_ref[nt][e] = mn;
             l_sum[nt][e] *= alpha;
@@ -729,7 +730,7 @@ __global__ void __launch_bounds__(kQ4Threads, MINB)
           }
         }
       }
-      if constexpr (!kHalf) {
+      {
         uint32_t big = ma[0][0];  // pairs (scale, minimum): the low half counts
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
@@ -742,12 +743,13 @@ __global__ void __launch_bounds__(kQ4Threads, MINB)
         if (__any_sync(0xffffffffu, s_max > s_lim)) {
           // Scales are >= 0 (or NaN, which stays out): their bits order them.
           const uint32_t bits = __reduce_max_sync(0xffffffffu, s_max > 0.f ? __float_as_uint(s_max) : 0u);
-          // four times the power of two above the largest becomes 2^13
-          uint32_t ex = min(max((bits >> 23) + 3u, 16u), 255u);
+          // four times the power of two above the largest becomes 2^13; fp16: none
+          // shrinks, as 2^kRaise times its largest scale is still in range
+          const uint32_t ex = min(max((bits >> 23) + 3u, 16u), kHalf ? 140u : 255u);
           const float nu_new = __uint_as_float((267u - ex) << 23);
           const float f = s_lim < 0.f ? 0.f : nu_new * __uint_as_float((254u << 23) - __float_as_uint(nu));
           nu = nu_new;
-          s_lim = __uint_as_float(ex << 23);
+          s_lim = kHalf && ex == 140u ? INFINITY : __uint_as_float(ex << 23);
 #pragma unroll
           for (int dt = 0; dt < KS; ++dt)
 #pragma unroll
@@ -769,10 +771,8 @@ __global__ void __launch_bounds__(kQ4Threads, MINB)
           // (scale, value of the code that enters as 0)
           float2 fa = kHalf ? int4_centre<T>(ma[mt][gi]) : unpack2<T>(ma[mt][gi]);
           float2 fb = kHalf ? int4_centre<T>(mb[mt][gi]) : unpack2<T>(mb[mt][gi]);
-          if (!kHalf) {
-            fa.x *= nu;
-            fb.x *= nu;
-          }
+          fa.x *= nu;
+          fb.x *= nu;
           uint32_t pg[NT][2];
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {

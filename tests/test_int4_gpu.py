@@ -453,6 +453,68 @@ def test_attention_values_of_many_scales(cuda_device, dt, exps, D, G, bs):
         check_attention(out, q, kp, vp, bt, lens, 0.1, bs, 1, dt)
 
 
+def flat_values(D, L, bs, dt, g, size, sink):
+    """Keys and values of one head: a first token with a score of `sink` and values
+    of 0, and L - 1 like tokens with scores of 0 and values of one size, whose codes
+    lie at the top but for one element of each group."""
+    base = torch.randn(D, generator=g)
+    k = torch.zeros((L, D))
+    k[0] = base * sink / (base @ base)
+    v = torch.full((L, D), size) * (1 - 0.02 * torch.rand(D, generator=g))
+    v[:, ::64] = 0.0
+    v[0] = 0.0
+    return base, k.to(dt), v.to(dt)
+
+
+def pages_of(x, bs, dt, value):
+    L, D = x.shape
+    n = (L + bs - 1) // bs
+    pad = torch.zeros((n * bs, D), dtype=dt)
+    pad[:L] = x
+    c, s, lo = op.quantise(pad.view(n, bs, D))
+    out = np.zeros((n, op.page_bytes(D, bs)), np.uint8)
+    for p in range(n):
+        for r in range(bs):
+            op.put_row(out[p], bs, r, c[p, r], s[p, r], lo[p, r], value)
+    return out
+
+
+@pytest.mark.parametrize("D,G,bs,sink", [(64, 1, 8, 8.0), (128, 4, 16, 10.0), (64, 32, 8, 10.0),
+                                         (256, 2, 16, 12.0)])
+@pytest.mark.parametrize("size", [1.0, 0.1, 0.02, 0.005])
+def test_attention_small_values_beside_a_dominating_token(cuda_device, D, G, bs, sink, size):
+    """fp16 values whose probability x scale lies far below fp16's normal numbers."""
+    dt, L = HF, 1025
+    g = torch.Generator().manual_seed(D + G)
+    base, k, v = flat_values(D, L, bs, dt, g, size, sink)
+    q = base.expand(1, G, D).to(dt)
+    kp, vp = pages_of(k, bs, dt, False), pages_of(v, bs, dt, True)
+    n = kp.shape[0]
+    bt = torch.arange(n, dtype=torch.int32)[None]
+    out = torch.empty_like(q).to(cuda_device)
+    for splits in (0, 2):
+        pa.paged_attention_int4(out, q.to(cuda_device),
+                                *(torch.from_numpy(p).view(n, 1, -1).to(cuda_device) for p in (kp, vp)),
+                                bt.to(cuda_device), torch.tensor([L], dtype=torch.int32, device=cuda_device),
+                                1.0, bs, num_splits=splits)
+        kv, vv = (op.get_rows(p, D, bs, dt, val).reshape(-1, D)[:L] for p, val in ((kp, False), (vp, True)))
+        sc = torch.from_numpy(np.ascontiguousarray(vp[:, bs * D // 2:])).view(dt).double()
+        sc = sc.view(-1, D // 64, 2)[:L, :, 0].repeat_interleave(64, -1).numpy()   # scales
+        qq = q[0].double().numpy()
+        w = np.exp(qq @ kv.T - (qq @ kv.T).max(1, keepdims=True))
+        w /= w.sum(1, keepdims=True)
+        want, u = w @ vv, half_step(dt)
+        size_ = (np.abs(qq) @ np.abs(kv).T).max(1)[:, None]
+        # The output's rounding; each probability x scale rounded once, times codes
+        # of at most 8; below fp16's normal numbers, that is 2^24 under the largest
+        # scale, 2^-35 of that scale per token; the scores' sums as in
+        # check_attention, against the mean size of the values.
+        tol = u * np.abs(want) + torch.finfo(dt).smallest_normal * u + u * 8 * (w @ sc) \
+            + L * 8 * 2.0 ** -35 * sc.max() + 2 * (2.0 ** -18 + 256 * 2.0 ** -24 * size_) * (w @ np.abs(vv))
+        err = np.abs(out[0].double().cpu().numpy() - want)
+        assert (err <= tol).all()
+
+
 @pytest.mark.parametrize("dt,D,G,bs", [(BF, 128, 2, 16), (BF, 64, 32, 8), (BF, 256, 4, 64),
                                        (HF, 128, 2, 16)])
 def test_attention_long_range_of_one_cta(cuda_device, dt, D, G, bs):
