@@ -96,6 +96,7 @@ __global__ void __launch_bounds__(kQ4Threads, MINB)
   // Reference point of an empty state: below every score, and finite, so that
   // a score of -inf has probability 0.
   constexpr float kNoScore = -3e38f;
+  constexpr float kFar = 9.094947017729282e-13f;  // 2^-40
 
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_addr = smem_addr(smem_raw);
@@ -375,6 +376,9 @@ __global__ void __launch_bounds__(kQ4Threads, MINB)
   uint32_t qb[KS][NT][2];
   float qsum[NT][NG][2];   // scale_log2 x sum of the query over a group, heads 2 lc + e
   float qmul[NT][2];       // what a sum of (query x code) products is multiplied by
+  // Tokens of a chunk from which on its scores are taken as they are: 32.  Where a
+  // head tile's scores are in units of 1 / kFar, more than any, with bit nt set.
+  int whole = 32;
   float acc[KS][NT][4], mid[NT][NG][2], m_ref[NT][2], l_sum[NT][2];
   // The scales' power of two and the largest scale it allows.  bf16: chunks since
   // the accumulators were emptied, and the reference points then (`emptied`: there
@@ -388,6 +392,7 @@ __global__ void __launch_bounds__(kQ4Threads, MINB)
   // at bits 0..3 are 16 times larger), and a fresh state.
   auto start_head = [&](int hd) {
     const int s = hd / Hkv, h = hd - s * Hkv;
+    whole = 32;
     const T* qp = static_cast<const T*>(p.q) + s * p.q_sb + static_cast<int64_t>(h) * G * p.q_sh;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -404,16 +409,9 @@ __global__ void __launch_bounds__(kQ4Threads, MINB)
       }
       float big = 0.f, sum[NG];
 #pragma unroll
-      for (int gi = 0; gi < NG; ++gi) {
-        sum[gi] = 0.f;
-#pragma unroll
-        for (int ks = 4 * gi; ks < 4 * gi + 4; ++ks) {
-          const float2 a = unpack2<T>(raw[ks][0]), b = unpack2<T>(raw[ks][1]);
-          big = fmaxf(fmaxf(big, fmaxf(fabsf(a.x), fabsf(a.y))), fmaxf(fabsf(b.x), fabsf(b.y)));
-          sum[gi] += (a.x + a.y) + (b.x + b.y);
-        }
-        sum[gi] += __shfl_xor_sync(0xffffffffu, sum[gi], 1);
-        sum[gi] += __shfl_xor_sync(0xffffffffu, sum[gi], 2);
+      for (int ks = 0; ks < KS; ++ks) {
+        const float2 a = unpack2<T>(raw[ks][0]), b = unpack2<T>(raw[ks][1]);
+        big = fmaxf(fmaxf(big, fmaxf(fabsf(a.x), fabsf(a.y))), fmaxf(fabsf(b.x), fabsf(b.y)));
       }
       big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
       big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
@@ -422,17 +420,30 @@ __global__ void __launch_bounds__(kQ4Threads, MINB)
       if (big == 0.f || ex > 127) ex = 10;
       if (ex < -110) ex = -110;
       const float up = __uint_as_float(static_cast<uint32_t>(137 - ex) << 23);      // 2^(10 - ex)
-      // 2^(ex - 10) x 2^20 (the codes' weight), in two factors that stay normal
-      const float down = __uint_as_float(static_cast<uint32_t>(117 + ex > 0 ? 117 + ex : 1) << 23) * 1048576.f;
+      // 2^(ex - 10), what the scaled query's sums and products are multiplied by;
+      // where a head's largest element passes 2^64, 2^-40 of it for all of the tile
+      // (that keeps it, the codes' weight and the sums inside fp32).
+      const bool is_far = !kHalf && __any_sync(0xffffffffu, ex > 64);
+      if (is_far) whole |= 0x7ffffff0 | 1 << nt;
+      const float down = __uint_as_float(static_cast<uint32_t>(117 + ex) << 23) * (is_far ? kFar : 1.f);
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) {
-        const float2 a = unpack2<T>(raw[ks][0]), b = unpack2<T>(raw[ks][1]);
-        qb[ks][nt][0] = pack2<__half>(a.x * up * 16.f, a.y * up * 16.f);
-        qb[ks][nt][1] = pack2<__half>(b.x * up, b.y * up);
+      for (int gi = 0; gi < NG; ++gi) {
+        sum[gi] = 0.f;
+#pragma unroll
+        for (int ks = 4 * gi; ks < 4 * gi + 4; ++ks) {
+          const float2 a = unpack2<T>(raw[ks][0]), b = unpack2<T>(raw[ks][1]);
+          qb[ks][nt][0] = pack2<__half>(a.x * up * 16.f, a.y * up * 16.f);
+          qb[ks][nt][1] = pack2<__half>(b.x * up, b.y * up);
+          sum[gi] += (a.x * up + a.y * up) + (b.x * up + b.y * up);
+        }
+        sum[gi] += __shfl_xor_sync(0xffffffffu, sum[gi], 1);
+        sum[gi] += __shfl_xor_sync(0xffffffffu, sum[gi], 2);
+        sum[gi] *= down;
       }
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        qmul[nt][e] = __shfl_sync(0xffffffffu, down, lc * 8 + e * 4) * p.scale_log2;
+        // 2^20: the codes' weight
+        qmul[nt][e] = __shfl_sync(0xffffffffu, down * 1048576.f, lc * 8 + e * 4) * p.scale_log2;
         m_ref[nt][e] = kNoScore;
         l_sum[nt][e] = 0.f;
 #pragma unroll
@@ -657,15 +668,17 @@ __global__ void __launch_bounds__(kQ4Threads, MINB)
 #pragma unroll
           for (int i = 0; i < 4; ++i) sc[mt][nt][i] = fmaf(t[nt][i], qmul[nt][i & 1], z[nt][i]);
       }
-      const bool ragged = ntok < 32;
+      const bool ragged = ntok < whole;
       if (ragged) {
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+            for (int i = 0; i < 4; ++i) {
+              if (!kHalf && whole >> nt & 1) sc[mt][nt][i] *= 1.f / kFar;
               if (mt * 16 + lr + (i >> 1) * 8 >= ntok) sc[mt][nt][i] = -INFINITY;
+            }
       }
       // The reference point of the softmax.
       float mx[NT][2];

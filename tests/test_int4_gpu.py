@@ -515,6 +515,28 @@ def test_attention_small_values_beside_a_dominating_token(cuda_device, D, G, bs,
         assert (err <= tol).all()
 
 
+@pytest.mark.parametrize("D,G", [(64, 8), (128, 4), (128, 20), (256, 2)])
+@pytest.mark.parametrize("e,same", [(60, False), (108, False), (118, False), (124, False), (126, True)])
+def test_attention_queries_near_the_largest(cuda_device, D, G, e, same):
+    """bf16 queries up to the type's largest; `same`: sums of a group's elements pass it."""
+    dt, bs, L = BF, 16, 333
+    g = torch.Generator().manual_seed(e + G)
+    lens = torch.tensor([L, 1], dtype=torch.int32)
+    bt, pool = tables(lens, bs)
+    kp = random_pages(pool, D, bs, dt, g, False, 2.0 ** -60)
+    vp = random_pages(pool, D, bs, dt, g, True)
+    q = torch.rand((2, G, D), generator=g) + 0.5 if same else torch.randn((2, G, D), generator=g)
+    q[:, 0] *= 2.0 ** -4                           # heads of other sizes beside the largest
+    q = (q * 2.0 ** e).clamp(-torch.finfo(dt).max, torch.finfo(dt).max).to(dt)
+    scale = 2.0 ** (60 - e) / math.sqrt(D)
+    out = torch.empty_like(q).to(cuda_device)
+    pa.paged_attention_int4(out, q.to(cuda_device),
+                            *(torch.from_numpy(p).view(pool, 1, -1).to(cuda_device) for p in (kp, vp)),
+                            bt.to(cuda_device), lens.to(cuda_device), scale, bs)
+    assert torch.isfinite(out).all()
+    check_attention(out, q, kp, vp, bt, lens, scale, bs, 1, dt)
+
+
 @pytest.mark.parametrize("dt,D,G,bs", [(BF, 128, 2, 16), (BF, 64, 32, 8), (BF, 256, 4, 64),
                                        (HF, 128, 2, 16)])
 def test_attention_long_range_of_one_cta(cuda_device, dt, D, G, bs):
