@@ -498,6 +498,11 @@ size_t pab200_decode_sparse_workspace_size(const pab200_decode_args* args,
 int pab200_decode_sparse(const pab200_decode_args* args, const pab200_select_args* sel,
                          void* workspace, size_t workspace_bytes, void* stream);
 
+/* The current device's word for the status bits of append calls (their `status`),
+ * zero when the library is loaded on the device and never freed.  Valid inside a
+ * stream capture.  Null on failure. */
+uint32_t* pab200_append_status_word(void);
+
 /* Copy the device status word of `workspace` (the PAB200_STATUS_* bits raised
  * by the most recent pab200_decode call on it) to *status_out.  Synchronises
  * `stream`. */

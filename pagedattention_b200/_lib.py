@@ -69,6 +69,7 @@ EXPORTED_SYMBOLS = (
     "pab200_select_pages",
     "pab200_decode_sparse_workspace_size",
     "pab200_decode_sparse",
+    "pab200_append_status_word",
     "pab200_read_status",
     "pab200_strerror",
     "pab200_last_error",
@@ -255,6 +256,7 @@ def load() -> ctypes.CDLL:
     V, Z, I32, I64 = ctypes.c_void_p, ctypes.c_size_t, ctypes.c_int32, ctypes.c_int64
     R, S = ctypes.POINTER(Int4RowsArgs), ctypes.POINTER(SelectArgs)
     for name, res, args in (
+            ("pab200_append_status_word", V, []),
             ("pab200_int4_page_bytes", Z, [I32, I32]),
             ("pab200_kv_append_int4", ctypes.c_int, [R, I32, V]),
             ("pab200_kv_read_int4", ctypes.c_int, [R, V, I64, I32, V]),

@@ -1260,6 +1260,17 @@ PAB200_EXPORT int pab200_decode_append(const pab200_decode_args* a, const pab200
   return decode_impl(a, pl, empty ? nullptr : &p, workspace, workspace_bytes, stream);
 }
 
+// Not an allocation of a caller's first append, which may be inside a capture: its
+// memory and its zeroing would be the graph's.
+static __device__ uint32_t g_append_status;
+
+PAB200_EXPORT uint32_t* pab200_append_status_word(void) {
+  void* p = nullptr;
+  const cudaError_t e = cudaGetSymbolAddress(&p, g_append_status);
+  if (e != cudaSuccess) cuda_fail(e, "cudaGetSymbolAddress(append status)");
+  return e == cudaSuccess ? static_cast<uint32_t*>(p) : nullptr;
+}
+
 PAB200_EXPORT int pab200_read_status(const void* workspace, uint32_t* status_out, void* stream) {
   if (!workspace || !status_out) return fail(PAB200_ERR_INVALID_ARGUMENT, "null pointer");
   cudaStream_t s = static_cast<cudaStream_t>(stream);

@@ -607,10 +607,23 @@ def default_scale(head_size: int) -> float:
 _append_status: dict[int, torch.Tensor] = {}
 
 
+class _DeviceWord:
+    """One int32 of device memory, as torch.as_tensor takes it."""
+
+    def __init__(self, ptr):
+        self.__cuda_array_interface__ = {"shape": (1,), "typestr": "<i4", "data": (ptr, False),
+                                         "version": 2}
+
+
 def _append_status_word(device) -> torch.Tensor:
     w = _append_status.get(device.index)
     if w is None:
-        w = torch.zeros(1, dtype=torch.int32, device=device)
+        lib = _lib.load()
+        with torch.cuda.device(device):
+            ptr = lib.pab200_append_status_word()
+        if not ptr:
+            raise RuntimeError(f"pab200_append_status_word: {lib.pab200_last_error().decode()}")
+        w = torch.as_tensor(_DeviceWord(ptr), device=device)
         _append_status[device.index] = w
     return w
 

@@ -8,7 +8,7 @@ import torch
 
 import pagedattention_b200 as pa
 from oracle import pages as op
-from pagedattention_b200 import _lib
+from pagedattention_b200 import _lib, kernel_b200
 from tests.test_int4_gpu import check_attention, half_step, tables
 
 pytestmark = pytest.mark.gpu
@@ -611,3 +611,28 @@ def test_serving_steps_together(cuda_device):
         qn = fill()
         graph.replay()
         check(qn)
+
+
+def test_append_status_word_is_not_a_graphs(cuda_device):
+    """A first call inside a capture: the bits outlive the graph's replays."""
+    dt, D, bs = BF, 64, 8
+    bounds = torch.zeros((2, 1, 2, D), dtype=dt, device=cuda_device)
+    k = torch.zeros((1, 1, D), dtype=dt, device=cuda_device)
+    lens = torch.zeros(1, dtype=torch.int32, device=cuda_device)
+    good = torch.zeros((1, 1), dtype=torch.int32, device=cuda_device)
+    bad = good - 5
+    pa.update_page_bounds(bounds, k, lens, good, bs)
+    pa.kv_append_status()
+    torch.cuda.synchronize()
+    old = dict(kernel_b200._append_status)
+    kernel_b200._append_status.clear()
+    try:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            pa.update_page_bounds(bounds, k, lens, good, bs)
+        assert pa.kv_append_status(reset=False) == 0
+        pa.update_page_bounds(bounds, k, lens, bad, bs)
+        graph.replay()
+        assert pa.kv_append_status() == _lib.STATUS_BAD_PAGE_ID
+    finally:
+        kernel_b200._append_status.update(old)
