@@ -100,9 +100,8 @@ def _select_args(query, page_bounds, block_tables, context_lens, block_size, num
         raise ValueError("need num_sink >= 0, num_recent >= 1 and "
                          "num_sink + num_recent <= num_selected")
     B, Hq, D = shape
-    if B < 1 or Hq % num_kv_heads != 0:
-        raise ValueError(f"num_q_heads {Hq} is not a multiple of num_kv_heads {num_kv_heads}, "
-                         "or there is no sequence")
+    if Hq % num_kv_heads != 0:
+        raise ValueError(f"num_q_heads {Hq} is not a multiple of num_kv_heads {num_kv_heads}")
     bt, num_pages, mul, add, maxb, bts = _check_bounds(page_bounds, block_tables, B, num_kv_heads, D,
                                                        query.dtype)
     lens = _as_int32(context_lens, "context_lens")
@@ -142,7 +141,8 @@ def select_pages(query, page_bounds, block_tables, context_lens, block_size, num
     a, device, tables, lens, keep = _select_args(query, page_bounds, block_tables, context_lens,
                                                  block_size, num_selected, num_sink, num_recent,
                                                  heads)
-    _on_device(device, _run_select, a, device)
+    if a.num_seqs:
+        _on_device(device, _run_select, a, device)
     del keep
     return tables, lens
 
@@ -179,7 +179,8 @@ def paged_attention_sparse(out, query, key_cache, value_cache, page_bounds, bloc
                                                 args.num_kv_heads)
     if dev != device:
         raise ValueError(f"page_bounds must be on {device}")
-    _on_device(device, _run_sparse, args, sel, device)
+    if args.num_seqs:
+        _on_device(device, _run_sparse, args, sel, device)
     del keep, kept
     return tables, lens
 

@@ -415,6 +415,25 @@ def test_sparse_attention(cuda_device, dt, D, G, Hkv, bs, lens, keep, layout):
     assert ((out.float() - full.float()).abs() <= tol).all()
 
 
+def test_empty_batch(cuda_device):
+    """No sequences: empty results, like the other calls of a step."""
+    dt, D, Hkv, bs = BF, 64, 2, 8
+    q = torch.zeros((0, 4, D), dtype=dt, device=cuda_device)
+    lens = torch.zeros(0, dtype=torch.int32, device=cuda_device)
+    bt = torch.zeros((0, 5), dtype=torch.int32, device=cuda_device)
+    pool = torch.zeros((3, Hkv, bs, D), dtype=dt, device=cuda_device)
+    bounds = torch.zeros((3, Hkv, 2, D), dtype=dt, device=cuda_device)
+    for tabs, sl in (pa.select_pages(q, bounds, bt, lens, bs, 4),
+                     pa.paged_attention_sparse(q.clone(), q, pool, pool, bounds, bt, lens, 0.1, bs, 4)):
+        assert tabs.shape == (0, Hkv, 4) and sl.shape == (0, Hkv)
+        assert tabs.dtype == sl.dtype == torch.int32
+    kc, vc = pa.int4_cache(3, Hkv, bs, D, device=cuda_device)
+    x = torch.zeros((0, Hkv, D), dtype=dt, device=cuda_device)
+    pa.update_page_bounds(bounds, x, lens, bt, bs)
+    pa.kv_append_int4(kc, vc, x, x, lens, bt, bs)
+    pa.paged_attention_int4(q.clone(), q, kc, vc, bt, lens, 0.1, bs)
+
+
 def test_sparse_attention_on_the_tcgen05_kernel(cuda_device, monkeypatch):
     """The opt-in decode kernel takes a selection's tables too."""
     monkeypatch.setenv("PAB200_TC", "1")
