@@ -406,8 +406,9 @@ typedef struct pab200_int4_rows_args {
  * sequence's tokens that come before the first without a place (no page slot:
  * PAB200_STATUS_APPEND_FULL; a page id out of range: PAB200_STATUS_BAD_PAGE_ID;
  * a negative length: PAB200_STATUS_NEG_SEQLEN, nothing is written), a length
- * shared by the heads (seqlens_stride_h == 0) by the least of theirs.  Tokens
- * outside every [cu[s], cu[s+1]) are not read. */
+ * shared by the heads (seqlens_stride_h == 0) by the least of theirs; sequences
+ * may not share one (seqlens_stride_b == 0).  Tokens outside every [cu[s],
+ * cu[s+1]) are not read. */
 int pab200_kv_append_int4(const pab200_int4_rows_args* args, int32_t increment, void* stream);
 
 /* Read rows back: k_rows / v_rows token j of sequence s becomes lo + s * c,

@@ -553,6 +553,9 @@ PAB200_EXPORT int pab200_kv_append_int4(const pab200_int4_rows_args* a, int32_t 
   pab::Int4AppendParams p{};
   const int rc = check_int4(a, &p.map, false);
   if (rc || !any_rows(a, false)) return rc;
+  if (increment && a->num_seqs > 1 && a->seqlens_stride_b == 0)
+    return fail(PAB200_ERR_INVALID_ARGUMENT,
+                "sequences share a length (seqlens_stride_b is 0): it cannot be advanced for each");
   p.cache[0] = static_cast<uint8_t*>(a->k_cache);
   p.cache[1] = static_cast<uint8_t*>(a->v_cache);
   p.rows[0] = a->k_rows;

@@ -102,6 +102,15 @@ def test_rows_refusals(field, value, code):
     assert lib.pab200_last_error() != b""
 
 
+def test_append_refuses_a_length_of_many_sequences():
+    """An expanded length would be advanced once per sequence, in any order."""
+    lib = _lib.load()
+    a = _rows()
+    a.seqlens_stride_b = 0
+    assert lib.pab200_kv_append_int4(ctypes.byref(a), 1, None) == _lib.ERR_INVALID_ARGUMENT
+    assert b"share a length" in lib.pab200_last_error()
+
+
 def test_rows_edge_calls():
     lib = _lib.load()
     assert lib.pab200_kv_append_int4(None, 1, None) == _lib.ERR_INVALID_ARGUMENT
