@@ -114,9 +114,12 @@ def _rows_args(key_cache, value_cache, k, v, lens, block_table, cu, block_size, 
     code = _DTYPES.get(k.dtype)
     if code is None or v.dtype != k.dtype:
         raise TypeError(f"{what} must share one dtype, bfloat16 or float16")
-    if st[2] != 1 or v.stride() != st:
-        raise ValueError(f"{what} must share strides, contiguous in head_size")
     N, Hkv, D = shape
+    vst = v.stride()
+    # the stride of a dimension of one element means nothing
+    st_t, st_h = (st[0] if N > 1 else 0), (st[1] if Hkv > 1 else 0)
+    if (st[2] != 1 or vst[2] != 1 or (N > 1 and vst[0] != st_t) or (Hkv > 1 and vst[1] != st_h)):
+        raise ValueError(f"{what} must share strides, contiguous in head_size")
     B = lens.shape[0]
     bt, num_pages, _, mul, add, maxb, bts = _check_caches(key_cache, value_cache, block_table, D,
                                                           block_size, B, Hkv)
@@ -130,7 +133,7 @@ def _rows_args(key_cache, value_cache, k, v, lens, block_table, cu, block_size, 
     args = _lib.Int4RowsArgs(
         key_cache.data_ptr(), value_cache.data_ptr(), k.data_ptr(), v.data_ptr(), lens.data_ptr(),
         bt.data_ptr(), None if cu is None else cu.data_ptr(), _append_status_ptr(device), code, B, Hkv,
-        D, block_size, maxb, num_pages, N, st[0], st[1], lsb, lsh, *bts, mul, add)
+        D, block_size, maxb, num_pages, N, st_t, st_h, lsb, lsh, *bts, mul, add)
     return args, device, bt
 
 

@@ -169,6 +169,31 @@ def test_append_bytes(cuda_device, dt, D, bs, Hkv, lens, new, per_head, per_len,
         assert (got[M:] == 7.0).all()
 
 
+def test_append_and_read_one_row_of_any_stride(cuda_device):
+    """Strides of dimensions of one element mean nothing: neither their agreement
+    nor their alignment is asked for."""
+    dt, D, bs = BF, 64, 8
+    g = torch.Generator().manual_seed(2)
+    x = torch.randn((2, 1, 1, D), generator=g).to(dt)
+    xd = x.to(cuda_device)
+    k, v = xd[0].as_strided((1, 1, D), (D, D, 1)), xd[1].as_strided((1, 1, D), (7, 3, 1))
+    kc, vc = pa.int4_cache(1, 1, bs, D, device=cuda_device)
+    lens = torch.zeros(1, dtype=torch.int32, device=cuda_device)
+    bt = torch.zeros((1, 1), dtype=torch.int32, device=cuda_device)
+    pa.kv_append_int4(kc, vc, k, v, lens, bt, bs)
+    out = torch.full((2, D), 7.0, dtype=dt, device=cuda_device)
+    start = torch.zeros(1, dtype=torch.int32, device=cuda_device)
+    k2, v2 = pa.kv_read_int4(kc, vc, bt, lens, bs, D, dt, starts=start,
+                             out=(out[0].as_strided((1, 1, D), (1, 5, 1)),
+                                  out[1].as_strided((1, 1, D), (2, 3, 1))))
+    for got, src in ((k2, x[0]), (v2, x[1])):
+        c, s, lo = op.quantise(src)
+        want = (lo.double()[..., None] + s.double()[..., None] * c.unflatten(-1, (-1, 64)).double())
+        want = want.flatten(-2)
+        # the one rounding of lo + s c
+        assert ((got.cpu().double() - want).abs() <= half_step(dt) * want.abs()).all()
+
+
 def test_append_places_that_do_not_exist(cuda_device):
     """A full table, bad page ids and a negative length: nothing else is
     touched, lengths stop before the first token without a place."""
