@@ -449,6 +449,22 @@ def test_attention_matches_64_bits(cuda_device, dt, D, G, Hkv, bs, lens):
     assert torch.equal(again, out)
 
 
+@pytest.mark.parametrize("dt,D,G,Hkv,bs,lens", ATTEND)
+@pytest.mark.parametrize("splits", [0, 1, 4])
+def test_attention_is_finite(cuda_device, dt, D, G, Hkv, bs, lens, splits):
+    """No NaN or infinity comes out of finite rows (a comparison with a bound
+    would let a NaN pass)."""
+    g = torch.Generator().manual_seed(D + G + splits)
+    lens = torch.tensor(lens, dtype=torch.int32)
+    bt, pool = tables(lens, bs)
+    kp, vp = (random_pages(pool * Hkv, D, bs, dt, g, value) for value in (False, True))
+    q = torch.randn((lens.numel(), G * Hkv, D), generator=g).to(dt).to(cuda_device)
+    out = torch.full_like(q, float("nan"))
+    pa.paged_attention_int4(out, q, *(torch.from_numpy(p).view(pool, Hkv, -1).to(cuda_device) for p in (kp, vp)),
+                            bt.to(cuda_device), lens.to(cuda_device), 0.1, bs, num_splits=splits)
+    assert torch.isfinite(out).all()
+
+
 # Binary exponents of the values' standard deviation, page by page.
 UP = list(range(-96, 100, 4))
 SCALES = [(BF, [UP, UP[::-1], [-118] * 40, [117] * 12, [0, 60, -20, 30, -60, 100] * 6]),
@@ -560,6 +576,48 @@ def test_attention_queries_near_the_largest(cuda_device, D, G, e, same):
                             bt.to(cuda_device), lens.to(cuda_device), scale, bs)
     assert torch.isfinite(out).all()
     check_attention(out, q, kp, vp, bt, lens, scale, bs, 1, dt)
+
+
+@pytest.mark.parametrize("dt", [BF, HF])
+@pytest.mark.parametrize("D,G,bs", [(64, 8, 8), (128, 4, 16), (128, 20, 64), (256, 2, 16)])
+def test_attention_nan_in_a_group_or_a_query(cuda_device, dt, D, G, bs):
+    """A NaN group of values makes its 64 elements NaN, one of keys or a NaN in a
+    query the heads that read it; everything else stays what it is."""
+    g = torch.Generator().manual_seed(D)
+    lens = torch.tensor([200, 200, 200, 77], dtype=torch.int32)
+    bt, pool = tables(lens, bs)
+    kp = random_pages(pool, D, bs, dt, g, False)
+    vp = random_pages(pool, D, bs, dt, g, True)
+    q = torch.randn((4, G, D), generator=g).to(dt)
+
+    def run(kp, vp, q):
+        out = torch.empty_like(q).to(cuda_device)
+        pa.paged_attention_int4(out, q.to(cuda_device),
+                                *(torch.from_numpy(p).view(pool, 1, -1).to(cuda_device) for p in (kp, vp)),
+                                bt.to(cuda_device), lens.to(cuda_device), 0.1, bs)
+        return out.cpu()
+
+    clean, clean_q = run(kp, vp, q), q
+    clean_kp, clean_vp = kp, vp
+    assert torch.isfinite(clean).all()
+    bad = torch.zeros(clean.shape, dtype=torch.bool)
+    nan = torch.full((1, D), float("nan")).to(dt)
+    kp, vp, q = kp.copy(), vp.copy(), q.clone()
+    at = bs * D // 2 + 5 * (D // 64) * 4           # pairs of row 5
+    vp[int(bt[0, 1]), at:at + 4] = nan.view(torch.uint8).numpy()[0, :4]
+    bad[0, :, :64] = True
+    kp[int(bt[1, 0]), at + (D // 64 - 1) * 4:at + (D // 64) * 4] = nan.view(torch.uint8).numpy()[0, :4]
+    bad[1] = True
+    q[2, G - 1, 9] = float("nan")
+    bad[2, G - 1] = True
+    q[3, 0, 3] = float("inf")
+    bad[3, 0] = True
+    got = run(kp, vp, q)
+    assert torch.isnan(got[bad]).all()
+    assert torch.isfinite(got[~bad]).all()
+    # not bit for bit: a head whose scores are infinite makes its warp take new
+    # reference points, which moves the roundings of the warp's other heads
+    check_attention(torch.where(bad, clean, got), clean_q, clean_kp, clean_vp, bt, lens, 0.1, bs, 1, dt)
 
 
 @pytest.mark.parametrize("dt,D,G,bs", [(BF, 128, 2, 16), (BF, 64, 32, 8), (BF, 256, 4, 64),

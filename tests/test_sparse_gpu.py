@@ -342,6 +342,21 @@ def test_select_infinite_bounds_by_definition(cuda_device, dt, n):
         assert torch.equal(out[s], wl[s]) and torch.equal(tabs[s], want[s]), s
 
 
+@pytest.mark.parametrize("width", [2000, 9000])
+def test_select_wide_tables(cuda_device, width):
+    """Tables far wider than the contexts; what lies behind a context is not read."""
+    dt, D, G, Hkv, bs, keep = BF, 128, 2, 2, 16, 20
+    g = torch.Generator().manual_seed(width)
+    lens = torch.tensor([3000, 0, 5000, 17], dtype=torch.int32)
+    bt, pool = tables(lens, bs, maxb=width)
+    x = torch.randn((pool * Hkv, 2, D), generator=g).to(dt)
+    bounds = torch.stack((x.amin(1), x.amax(1)), 1)
+    q = torch.randn((4, G * Hkv, D), generator=g).to(dt)
+    tabs, out, status = select_within_guards(cuda_device, q, bounds, bt, lens, bs, keep, Hkv)
+    want, wl = expect_select(q, bounds, bt, lens, bs, keep, 1, 1, Hkv, False)
+    assert status == 0 and torch.equal(out, wl) and torch.equal(tabs, want)
+
+
 def test_select_lengths_out_of_range(cuda_device):
     dt, D, bs = HF, 64, 8
     g = torch.Generator().manual_seed(0)
