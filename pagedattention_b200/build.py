@@ -21,8 +21,8 @@ CSRC = PKG_DIR / "csrc"
 LIB_PATH = PKG_DIR / "libpab200.so"
 OBJ_DIR = PKG_DIR / "build"
 SOURCES = [CSRC / "pab200.cu", CSRC / "int4_decode.cu", CSRC / "int4.cu", CSRC / "sparse.cu"]
-HEADERS = [CSRC / "decode.cuh", CSRC / "int4.cuh", CSRC / "int4_decode.cuh", CSRC / "ptx.cuh", CSRC / "tokens.cuh",
-           CSRC / "host.h", REPO_DIR / "include" / "pab200.h"]
+HEADERS = [CSRC / "append.cuh", CSRC / "decode.cuh", CSRC / "int4.cuh", CSRC / "int4_decode.cuh",
+           CSRC / "ptx.cuh", CSRC / "tokens.cuh", CSRC / "host.h", REPO_DIR / "include" / "pab200.h"]
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 

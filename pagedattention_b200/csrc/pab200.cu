@@ -17,6 +17,7 @@
 #include <cstring>
 #include <mutex>
 
+#include "append.cuh"
 #include "host.h"
 #include "int4_decode.cuh"
 
