@@ -282,9 +282,11 @@ __device__ __forceinline__ double warp_sum(double a) {
 // multiply an infinite bound that the maximum leaves aside by 0.  NaN where a
 // query element of 0 meets an infinite bound.
 template <typename T, int D>
-__device__ __noinline__ float term_score(const SelectParams& p, const T* q, const T* b) {
+__device__ __forceinline__ float term_score(const SelectParams& p, const T* q, const T* b) {
   double a = 0.0;
+#pragma unroll 1
   for (int d = threadIdx.x & 31; d < D; d += 32)
+#pragma unroll 1
     for (int g = 0; g < p.G; ++g) {
       const double x = static_cast<float>(q[g * p.q_sh + d]);
       const double u = x * static_cast<float>(b[d]), v = x * static_cast<float>(b[D + d]);
