@@ -19,7 +19,7 @@ import torch
 
 from . import _lib
 from .kernel_b200 import (_DTYPES, _append_status_word, _as_int32, _call_with_workspace,
-                          _check_device, _keep_workspace, _on_device, _raise_for)
+                          _check_device, _keep_workspace, _on_device, _raise_for, _take_events)
 
 _HEAD_SIZES = (64, 128, 256)
 _BLOCK_SIZES = (8, 16, 32, 64)
@@ -256,6 +256,7 @@ def paged_attention_int4(out, query, key_cache, value_cache, block_tables, conte
 
 
 def _run_int4(args, device, stream):
+    _take_events(args)
     ws = _call_with_workspace(
         _lib.load(), "pab200_decode_int4", device,
         (args.dtype, args.num_seqs, args.num_q_heads, args.num_kv_heads, args.head_size,

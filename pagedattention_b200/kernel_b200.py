@@ -128,12 +128,17 @@ def kernel_events(before: torch.cuda.Event, after: torch.cuda.Event):
         _tls.events = prev
 
 
-def _run_decode(args: _lib.DecodeArgs, device: torch.device, append=None, exchange=None) -> None:
-    lib = _lib.load()
+def _take_events(args: _lib.DecodeArgs) -> None:
+    """The events of an enclosing ``kernel_events`` block."""
     ev = getattr(_tls, "events", None)
     if ev is not None:
         args.event_before = ev[0].cuda_event
         args.event_after = ev[1].cuda_event
+
+
+def _run_decode(args: _lib.DecodeArgs, device: torch.device, append=None, exchange=None) -> None:
+    lib = _lib.load()
+    _take_events(args)
     if torch.cuda.current_device() == device.index:
         rc = _launch(lib, args, device, append, exchange)
     else:

@@ -15,7 +15,7 @@ import torch
 from . import _lib
 from .int4 import _append_status_ptr, _check_offsets, _check_table, _length_strides
 from .kernel_b200 import (_DTYPES, _as_int32, _call_with_workspace, _check_device,
-                          _keep_workspace, _on_device, _paged_args, _raise_for)
+                          _keep_workspace, _on_device, _paged_args, _raise_for, _take_events)
 
 
 def _check_bounds(page_bounds, block_table, num_seqs, num_kv_heads, head_size, dtype):
@@ -186,6 +186,7 @@ def paged_attention_sparse(out, query, key_cache, value_cache, page_bounds, bloc
 
 
 def _run_sparse(args, sel, device, stream):
+    _take_events(args)
     ws = _call_with_workspace(
         _lib.load(), "pab200_decode_sparse", device,
         (args.dtype, args.num_seqs, args.num_q_heads, args.num_kv_heads, args.head_size,

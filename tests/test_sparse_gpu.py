@@ -449,6 +449,29 @@ def test_empty_batch(cuda_device):
     pa.paged_attention_int4(q.clone(), q, kc, vc, bt, lens, 0.1, bs)
 
 
+@pytest.mark.parametrize("int4", [False, True])
+def test_kernel_events_of_the_new_decode_calls(cuda_device, int4):
+    """Events set around the decode kernel of every decode call are recorded by
+    the 4-bit and the page-sparse calls too."""
+    dt, D, Hkv, bs = BF, 64, 2, 8
+    q = torch.zeros((2, 4, D), dtype=dt, device=cuda_device)
+    lens = torch.full((2,), 300, dtype=torch.int32, device=cuda_device)
+    bt = torch.zeros((2, 40), dtype=torch.int32, device=cuda_device)
+    pool = torch.zeros((3, Hkv, bs, D), dtype=dt, device=cuda_device)
+    bounds = torch.zeros((3, Hkv, 2, D), dtype=dt, device=cuda_device)
+    kc, vc = pa.int4_cache(3, Hkv, bs, D, device=cuda_device)
+    before, after, mark = (torch.cuda.Event(enable_timing=True) for _ in range(3))
+    for e in (before, after, mark):
+        e.record()
+    with kernel_b200.kernel_events(before, after):
+        if int4:
+            pa.paged_attention_int4(q.clone(), q, kc, vc, bt, lens, 0.1, bs)
+        else:
+            pa.paged_attention_sparse(q.clone(), q, pool, pool, bounds, bt, lens, 0.1, bs, 4)
+    torch.cuda.synchronize()
+    assert mark.elapsed_time(before) > 0 and before.elapsed_time(after) > 0
+
+
 def test_sparse_attention_on_the_tcgen05_kernel(cuda_device, monkeypatch):
     """The opt-in decode kernel takes a selection's tables too."""
     monkeypatch.setenv("PAB200_TC", "1")
