@@ -388,7 +388,9 @@ typedef struct pab200_int4_rows_args {
   int32_t* seqlens;
   const int32_t* block_table;
   const int32_t* cu_tokens;  /* [num_seqs + 1]: tokens cu[s] .. cu[s+1] - 1 are
-                                sequence s's; null: one token per sequence      */
+                                sequence s's; null: one token per sequence.
+                                Ascending, in 0 .. num_tokens; a sequence whose
+                                offsets are not is left out                     */
   uint32_t* status;          /* device word: PAB200_STATUS_* bits ORed in; may be null */
 
   int32_t dtype;             /* of the rows, and of the scales in the pages    */

@@ -130,9 +130,9 @@ struct DecodeParams {
   int32_t bt_mul, bt_add;
   int32_t B, Hkv, G, D, bs, maxb;
   int64_t num_pages;
-  const uint8_t* k_pages;  // 4-bit caches: the pages (no tensor map)
+  const uint8_t* k_pages;  // 4-bit caches: the pages, for copies without a tensor map
   const uint8_t* v_pages;
-  int32_t gather;       // four pages per copy, through the tensor maps
+  int32_t gather;       // 4-bit pages of up to 2 KB: four per copy, through tensor maps
   int32_t unit_pages;   // fewest pages per range where there are enough: fewer ranges otherwise
   int32_t head_in_map;  // NHD layout: kv head is the tensor map's y coordinate
   float scale_log2;     // softmax_scale * log2(e)

@@ -199,8 +199,8 @@ __device__ __forceinline__ void append_tile(const Int4AppendParams& p, int64_t o
 
 // Ragged runs of tokens: one warp per (run of 8 or 16 positions, kv head).
 //
-// Reads 2 bytes per element and writes 9/16: 29,000 tokens of 8 kv heads, D 128,
-// move 151 MB, 23 us at a copy's 6.55 TB/s.  It takes 43 (3.5 TB/s): issue binds
+// Reads 2 bytes per element and writes 9/16: 32,375 tokens of 8 kv heads, D 128,
+// move 170 MB, 26 us at a copy's 6.55 TB/s.  It takes 43 (4.0 TB/s): issue binds
 // it (73 % of the slots), about 1,190 warp instructions per 8-token tile; without
 // any arithmetic the same loads and stores take 29, the ranges and the codes about
 // 7 each.  64 registers (4 CTAs per SM, a few spilled) 42.8, 80 registers 44.4.
@@ -344,8 +344,8 @@ __device__ __forceinline__ uint4 int4_values(uint32_t word, uint32_t pair) {
 
 // One warp per (run of 8 or 16 positions, kv head), lanes as in append_tile: the
 // rounds of a tile of which every row is wanted differ by constant offsets.
-// 29,000 tokens of 8 kv heads, D 128 (151 MB, 23 us at a copy's rate): 31.8 us,
-// 4.7 TB/s; waits for loads, 58 % of the issue slots busy.  More CTAs per SM with
+// 32,375 tokens of 8 kv heads, D 128 (170 MB, 26 us at a copy's rate): 32 us,
+// 5.3 TB/s; waits for loads, 58 % of the issue slots busy.  More CTAs per SM with
 // fewer registers: 32.6 to 34.3.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) int4_read_kernel(const Int4ReadParams p, int warps) {
@@ -496,7 +496,7 @@ bool rows_vec(const pab200_int4_rows_args* a) {
 }
 
 // Positions a warp takes (log2): two tiles of a page where there are pages of two,
-// which shares the search for the run and its page (29,000 tokens of 8 kv heads,
+// which shares the search for the run and its page (32,375 tokens of 8 kv heads,
 // D 128, pages of 16: append 50 us with one tile per warp, 44 with two at 80
 // registers; read-back 34 and 32).
 int log2_run(const pab200_int4_rows_args* a) { return a->block_size >= 16 ? 4 : 3; }

@@ -8,7 +8,8 @@ namespace {
 // MINB: resident CTAs per SM the registers are held to.  A CTA's 5 warps share 4
 // register files, so 2 CTAs leave 168 registers a thread, 3 leave 128 and 4 leave
 // 96.  State per thread grows with D/16 x NT: 24 accumulator and query registers
-// fit 4 CTAs, 48 fit 3, 96 fit 2 (with some spills).
+// fit 4 CTAs, 48 fit 3, 96 fit 2 (with spills of 0.1 to 0.3 KB a thread).  Other
+// counts were timed at D 128 with groups of up to 8 and D 64 with 32 heads.
 template <typename T, int D, int NT, int HS, int MINB>
 void take(pabh::Int4Kernel* o) {
   o->ops = pabh::kernel_ops<&pab::decode_int4_kernel<T, D, NT, HS, MINB>>();

@@ -40,11 +40,11 @@
 // for the reduce kernels of decode.cuh.
 //
 // Measured (bf16, 8 kv heads of 4 query heads, D 128, pages of 16): 64 sequences
-// of 4096 tokens (303 MB) 75 us, 4.0 TB/s of the 6.55 a copy reaches.  About 600
-// warp instructions per 32 tokens and head keep the issue slots a good half and
-// the ALU pipe 55 to 60 % busy; the copies alone take 59 us, the arithmetic alone
-// about 70.  The pairs of int4_value_pairs cost 4 instructions instead of 5: 76.3
-// -> 74.8.  Without a producing warp (the last warp of a stage refills its slot)
+// of 4096 tokens (303 MB) 75.5 us, 4.0 TB/s of the 6.55 a copy reaches (pages of 32
+// and 64, which take bulk copies: 75.8 and 74.6).  About 600 warp instructions per 32
+// tokens and head keep the issue slots a good half and the ALU pipe 55 to 60 % busy;
+// the copies alone take 59 us, the arithmetic alone about 70.  The pairs of
+// int4_value_pairs cost 4 instructions instead of 5: 76.3 -> 74.8.  Without a producing warp (the last warp of a stage refills its slot)
 // 15 us more, with 4 CTAs per SM at 96 registers (which spill) 12 more.  Handing
 // CTAs that end early the last chunks of others, as decode.cuh does, costs one more
 // join per chunk and instructions that the producer has to fetch: 5 us with that

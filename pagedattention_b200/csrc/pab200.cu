@@ -782,8 +782,8 @@ int decode_impl(const pab200_decode_args* a, const Plan& pl, const pab::AppendPa
     if ((rc = encode_cache_map(a, a->k_cache, &kmap))) return rc;
     if ((rc = encode_cache_map(a, a->v_cache, &vmap))) return rc;
   } else {
-    // 4-bit pages are copied without maps.  No pages: every sequence is
-    // empty, and the decode kernel exits before touching the maps.
+    // 4-bit pages of more than 2 KB are copied without maps.  No pages: every
+    // sequence is empty, and the decode kernel exits before touching the maps.
     kmap = CUtensorMap{};
     vmap = CUtensorMap{};
   }

@@ -19,9 +19,9 @@ struct BoundsParams {
 // One warp per (page, kv head): the minimum and maximum of the page's new rows,
 // D/8 lanes per row and 256/D rows at a time, joined with the page's bounds when
 // it began before.  Comparisons work on the 16-bit pairs as they are.  Bound by
-// reading the rows: 29,000 tokens of 8 kv heads, D 128 (59 MB, and 7 MB of bounds
-// to write): 12.2 us from L2, 20 with the launch; one token each of 64 sequences
-// 2.7 us, a chain of dependent loads.
+// reading the rows: 32,375 tokens of 8 kv heads, D 128 (66 MB, and 8 MB of bounds
+// to write): 12.3 us from L2, 19 from HBM; one token each of 64 sequences 2.7 us, a
+// chain of dependent loads.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) page_bounds_kernel(const BoundsParams p, int warps) {
   constexpr int LR = D / 8, RP = 32 / LR;
@@ -740,8 +740,8 @@ int launch_select(const pab200_select_args* a, void* scores, bool chained, cudaS
     if (e != cudaSuccess) return pabh::cuda_fail(e, "page scores launch");
   }
   // Scheduled while the scores drain; waits for them before it reads any.
-  // 256 threads while 8 registers hold a thread's keys, so that several units
-  // share an SM.
+  // 256 threads while shared memory holds all of their keys (8 per thread), so that
+  // several units share an SM.
   const bool small = p.maxb <= 2048;
   pabh::LaunchCfg lc(dim3(units), dim3(small ? 256 : 1024), 0, s, scored || chained);
   const cudaError_t err = a->dtype == PAB200_DTYPE_BF16

@@ -143,11 +143,13 @@ def kv_append_int4(key_cache, value_cache, k_new, v_new, cache_seqlens, block_ta
 
     The 4-bit form of ``kv_append``, for one token per sequence or for ragged
     runs of them (prompts).  k_new, v_new: (num_tokens, num_kv_heads,
-    head_size), bfloat16 or float16.  ``cu_new``: int32 (num_seqs + 1,), tokens
-    cu_new[s] .. cu_new[s+1] - 1 belong to sequence s; None: one token per
+    head_size), bfloat16 or float16.  ``cu_new``: int32 (num_seqs + 1,), ascending
+    in 0 .. num_tokens, tokens cu_new[s] .. cu_new[s+1] - 1 belong to sequence s
+    (one whose offsets are out of order or range is left out); None: one token per
     sequence.  cache_seqlens: int32 (num_seqs,) or (num_seqs, num_kv_heads), the
     lengths L before the call; token j goes to position L + j and, with
-    ``increment``, L grows in place by the tokens written.  Tokens from the
+    ``increment``, L grows in place by the tokens written (sequences may not share
+    one length).  Tokens from the
     first one without a page slot or with an invalid page id are not counted,
     and a bit read by ``kv_append_status`` is set.
     """
@@ -170,7 +172,8 @@ def kv_read_int4(key_cache, value_cache, block_table, cache_seqlens, block_size,
     Returns (k, v), each (num_tokens, num_kv_heads, head_size) of ``dtype``, the
     type the tokens were appended in.  Rows cu_out[s] .. cu_out[s+1] - 1 are
     positions starts[s], starts[s] + 1, ... of sequence s (``starts`` None: from
-    0); ``cu_out`` int32 (num_seqs + 1,) with ``num_tokens`` rows in all, or
+    0); ``cu_out`` int32 (num_seqs + 1,), ascending in 0 .. ``num_tokens``, the
+    rows in all (rows of a sequence whose offsets are not are not written), or
     None: one row per sequence.  Positions at or past cache_seqlens and pages
     with an invalid id read as zeros, and so do rows of no sequence.  ``out``: a
     (k, v) pair to fill; its rows of no sequence are left as they were.

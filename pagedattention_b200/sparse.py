@@ -131,7 +131,8 @@ def select_pages(query, page_bounds, block_tables, context_lens, block_size, num
     others those with the highest score: the sum over the kv head's query group
     and the head elements of max(q * min, q * max), which no token of the page
     exceeds.  Scores are those of a sum in 64 bits, rounded to fp32; ties go to the
-    earlier page, a NaN score ranks first, an invalid page id last (it, and a
+    earlier page, a NaN score (a NaN in the query or the bounds, 0 times an
+    infinite bound) ranks first, an invalid page id last (it, and a
     length out of range, set bits read by ``kv_append_status``).  At most 65,535
     (sequence, kv head) pairs.  query: (num_seqs, num_q_heads,
     head_size); page_bounds as kept by ``update_page_bounds``; block_tables,
